@@ -41,6 +41,10 @@ class WeightsInfo(C.Structure):
                 ("code_bytes", u64), ("scale_bytes", u64)]
 
 
+class Kv4Shape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seq", "n_kv_heads", "head_dim", "dv", "capacity")]
+
+
 class HwProfile(C.Structure):
     _fields_ = [("name", C.c_char_p), ("cbuf_banks", C.c_int), ("cbuf_bank_size", C.c_int),
                 ("max_tile", C.c_int), ("kgroup_2b", C.c_int), ("kgroup_4b", C.c_int),
@@ -188,6 +192,14 @@ PROTOS = {
     "rocket_i4_weights_save": (i32, [vp, vp, vp, C.c_char_p]),
     "rocket_i8_weights_load": (vp, [vp, C.c_char_p, vp]),
     "rocket_i4_weights_load": (vp, [vp, C.c_char_p, vp]),
+    # rocket_serve.h
+    "rocket_qk_norm_rope_fp16": (i32, [i32] * 8 + [fl, vp, i64, vp, i64] + [vp] * 6),
+    "rocket_qk_norm_rope_f32in": (i32, [i32] * 8 + [fl, vp, i64, vp, i64] + [vp] * 6),
+    "rocket_kv4_bytes": (sz, [C.POINTER(Kv4Shape)]),
+    "rocket_kv4_append_fp16": (i32, [i32, C.POINTER(Kv4Shape), vp, i32, i32, i32, vp, i64, i64, i64, vp, i64, i64, i64, vp]),
+    "rocket_kv4_read_fp16": (i32, [i32, C.POINTER(Kv4Shape), vp, i32, i32, i32, vp, vp, vp]),
+    "rocket_kv4_attn_fp16": (i32, [i32, C.POINTER(Kv4Shape), vp] + [i32] * 5 + [fl, fl, i32, i32, vp, vp, vp]),
+    "rocket_flash_attn_window_fp16": (i32, [i32] * 8 + [fl, fl, i32, i32] + [vp] * 4),
     # rocket_quant.h
     "rocket_quantize_rows_int8": (i32, [i32, i32, i32, vp, vp, vp]),
     "rocket_matmul_int4_prepacked_gw_f32in_noalloc": (i32, [vp, i32, i32, i32, vp, vp, vp, vp]),
@@ -202,6 +214,9 @@ PROTOS = {
 
 # rocket_activation.h
 ROCKET_ACTIVATION_SILU, ROCKET_ACTIVATION_TANH, ROCKET_ACTIVATION_GELU = 3, 4, 5
+
+# rocket_serve.h
+ROCKET_ROPE_HALVES, ROCKET_ROPE_PAIRS = 0, 1
 
 # data objects exported by the headers (not functions)
 DATA_SYMBOLS = ("rocket_hw_mi355x", "rocket_hw_rk3588", "rocket_hw_rk3576")

@@ -1,0 +1,481 @@
+"""rocket_serve.h on the GPU against numpy in 64 bits (serveforms.py, which derives each bound): every head
+size, one token to long prompts, lengths that end inside every tile, windows and sinks at their edges, rows
+that see no key, memory behind and between the visible keys that holds NaN, batches with idle places, captured
+calls that are replayed with other lengths, and the operators in a row as a layer calls them."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import rocketnpu as R
+import serveforms as F
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def rng(seed):
+    return np.random.default_rng(0x52434D80 + seed)
+
+
+def dev(x):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x)).to(DEV)
+
+
+def near(got, want, tol):
+    got = got.astype(np.float64)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:3].tolist(), got[bad][:3], want[bad][:3], tol[bad][:3])
+
+
+# ---- norms and rotation ----------------------------------------------------------------
+
+ROPE = [  # sequences, tokens, query heads, key heads, dim, rotated, pairs, eps, weights, spare columns
+    (1, 1, 1, 1, 32, 32, False, 1e-6, True, 0), (5, 1, 16, 8, 256, 256, False, 1e-6, True, 8), (1, 67, 10, 2, 96, 64, True, 1e-5, True, 192),
+    (3, 9, 5, 1, 160, 80, False, 1e-6, False, 0), (2, 33, 32, 8, 128, 128, True, -1.0, False, 1024), (1, 40, 3, 3, 224, 8, False, 1e-6, True, 0),
+    (1, 7, 4, 4, 64, 0, False, 0.0, True, 0), (2, 3, 7, 5, 192, 184, True, 1e-6, True, 16), (1, 130, 40, 8, 128, 64, False, 1e-6, True, 0),
+]
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("case", ROPE)
+def test_qk_norm_rope(lib, fd, case, f32):
+    n_seq, T, nq, nk, d, rot, pairs, eps, weighted, spare = case
+    print("rope", case, f32, flush=True)
+    g = rng(1)
+    rows = n_seq * T
+    x = (g.standard_normal((rows, (nq + nk) * d + spare)) * 3).astype(np.float32 if f32 else np.float16)
+    w = F.f16(1 + 0.3 * g.standard_normal((2, d))) if weighted else (None, None)
+    freq = (10000.0 ** (-np.arange(max(4, rot // 2)) / max(1, rot // 2))).astype(np.float32)
+    pos = g.integers(0, 1 << 20, rows).astype(np.int32)
+    pos[: min(rows, 4)] = np.array([0, -3, 2 ** 31 - 1, -2 ** 31])[: min(rows, 4)]
+    qo, ko = np.empty((n_seq, nq, T, d), np.float16), np.empty((n_seq, nk, T, d), np.float16)
+    fn = lib.rocket_qk_norm_rope_f32in if f32 else lib.rocket_qk_norm_rope_fp16
+    assert fn(fd, n_seq, T, nq, nk, d, rot, int(pairs), eps, R.ptr(x), x.shape[1], R.ptr(x.ctypes.data + nq * d * x.itemsize), x.shape[1],
+              R.ptr(w[0]), R.ptr(w[1]), R.ptr(freq), R.ptr(pos), R.ptr(qo), R.ptr(ko)) == 0
+    freq = freq[:rot // 2]
+    near(qo, *F.rope(x, nq, d, rot, pairs, eps, w[0], freq, pos, n_seq))
+    near(ko, *F.rope(x[:, nq * d:], nk, d, rot, pairs, eps, w[1], freq, pos, n_seq))
+
+
+# ---- the cache -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n_seq,seq0,places,H,dk,dv,cap,T,lens", [
+    (1, 0, 1, 1, 32, 32, 1, 1, [1]), (3, 1, 2, 2, 96, 160, 45, 5, [45, 3]), (4, 0, 4, 8, 128, 128, 300, 1, [300, 0, 17, 1]),
+    (1, 0, 1, 2, 256, 64, 700, 613, [613]), (2, 0, 2, 3, 64, 224, 64, 70, [64, 33]),
+])
+def test_cache(lib, fd, n_seq, seq0, places, H, dk, dv, cap, T, lens):
+    """Every byte of the cache after an append, with what was there kept, and the values read back: exactly."""
+    print("cache", n_seq, H, dk, dv, cap, T, lens, flush=True)
+    g = rng(2)
+    c = F.Cache(n_seq, H, dk, dv, cap)
+    c.buf[:] = g.integers(0, 256, c.buf.size)
+    mem = dev(c.buf)
+    K, V = F.f16(g.standard_normal((places, T, H, dk)) * 4), F.f16(g.standard_normal((places, H, T, dv)) * 1000)
+    K[0, -1, 0, :32] = 2.25
+    V[0, 0, -1, :32] = np.where(np.arange(32) % 2, 6e-8, -6e-8)      # a range of subnormals
+    V[0, -1, -1, -32:] = np.linspace(-65504, 65504, 32)
+    L = np.array(lens, np.int32)
+    for s in range(places):
+        for t in range(T):
+            j = L[s] - T + t
+            if 0 <= j < cap:
+                for h in range(H):
+                    c.put(seq0 + s, h, j, K[s, t, h], V[s, h, t])
+    sh = R.Kv4Shape(*c.dims)
+    put = lib.rocket_kv4_append_fp16
+    dK, dV, dL = dev(K), dev(V), dev(L)
+    assert put(fd, C.byref(sh), R.ptr(mem), seq0, places, T, R.ptr(dK), T * H * dk, dk, H * dk, R.ptr(dV), H * T * dv, T * dv, dv, R.ptr(dL)) == 0
+    assert np.array_equal(mem.cpu().numpy(), c.buf)
+    if max(lens) <= cap:   # and from host operands
+        mem2 = dev(c.buf)
+        assert put(fd, C.byref(sh), R.ptr(mem2), seq0, places, T, R.ptr(K), T * H * dk, dk, H * dk, R.ptr(V), H * T * dv, T * dv, dv, R.ptr(L)) == 0
+        assert np.array_equal(mem2.cpu().numpy(), c.buf)
+    k, v = c.rows()
+    Ko, Vo = np.full((places, H, T, dk), 7, np.float16), np.full((places, H, T, dv), 7, np.float16)
+    assert lib.rocket_kv4_read_fp16(fd, C.byref(sh), R.ptr(mem), seq0, places, T, R.ptr(L), R.ptr(Ko), R.ptr(Vo)) == 0
+    for s in range(places):
+        at = L[s] - T + np.arange(T)
+        ok = (at >= 0) & (at < cap)
+        assert np.array_equal(Ko[s][:, ok], F.f16(k[seq0 + s][:, at[ok]])) and np.array_equal(Vo[s][:, ok], F.f16(v[seq0 + s][:, at[ok]]))
+        assert not Ko[s][:, ~ok].any() and not Vo[s][:, ~ok].any()
+    V2 = np.full_like(Vo, 7)
+    assert lib.rocket_kv4_read_fp16(fd, C.byref(sh), R.ptr(mem), seq0, places, T, R.ptr(L), None, R.ptr(V2)) == 0
+    assert np.array_equal(V2, Vo)
+
+
+def test_cache_lengths_past_the_capacity(lib, fd):
+    """Device lengths that no capacity holds, or far negative: the tokens are dropped, nothing else is touched."""
+    c = F.Cache(3, 1, 32, 32, 40, fill=0x5A)
+    mem, K = dev(c.buf), dev(F.f16(np.ones((3, 2, 32))))
+    L = dev(np.array([43, 2 ** 31 - 1, -2 ** 31], np.int32))
+    sh = R.Kv4Shape(*c.dims)
+    assert lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), 0, 3, 2, R.ptr(K), 64, 0, 32, R.ptr(K), 64, 0, 32, R.ptr(L)) == 0
+    assert np.array_equal(mem.cpu().numpy(), c.buf)
+    assert lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(c.buf), 0, 3, 2, R.ptr(K), 64, 0, 32, R.ptr(K), 64, 0, 32, R.ptr(L)) == R.ROCKET_E_SHAPE
+
+
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+def test_cache_holds_finite_values(lib, fd, what):
+    K = F.f16(rng(3).standard_normal((1, 1, 1, 64)))
+    K[..., 5] = what
+    c = F.Cache(1, 1, 64, 64, 8)
+    sh, mem, L = R.Kv4Shape(*c.dims), dev(c.buf), np.array([1], np.int32)
+    assert lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, 1, R.ptr(K), 0, 0, 0, R.ptr(K), 0, 0, 0, R.ptr(L)) == 0
+    x = K[0, 0, 0].copy()
+    x[5] = {np.inf: 65504, -np.inf: -65504}.get(what, 0)
+    c.put(0, 0, 0, x, x)
+    assert np.array_equal(mem.cpu().numpy(), c.buf)
+
+
+# ---- attention over the cache ----------------------------------------------------------
+
+KV4 = [  # heads, kv heads, dk, dv, tokens, lengths (the largest is max_kv), window, sinks, softcap
+    (1, 1, 32, 32, 1, [1], 0, 0, 0.0), (2, 1, 64, 64, 1, [31, 32, 33], 0, 0, 0.0), (8, 2, 64, 96, 1, [257, 0, 5, 64], 0, 0, 0.0),
+    (16, 8, 256, 256, 1, [1000], 0, 0, 0.0), (32, 8, 128, 128, 1, [700, 127, 128, 1, 0], 0, 0, 0.0), (5, 1, 96, 32, 3, [130, 2], 0, 0, 0.0),
+    (4, 4, 160, 224, 2, [333], 0, 0, 30.0), (2, 2, 192, 128, 16, [100, 17], 0, 0, 0.0), (4, 2, 128, 128, 7, [300, 200], 0, 0, 0.0),
+    (4, 2, 128, 64, 17, [300, 40], 0, 0, 0.0), (2, 1, 256, 256, 70, [200], 0, 0, 0.0), (8, 8, 64, 64, 130, [130, 300, 77], 0, 0, 0.0),
+    (6, 2, 96, 160, 200, [900], 0, 0, 50.0), (4, 1, 128, 128, 129, [64, 513], 0, 0, 0.0),
+    # windows: inside a chunk, across chunks, one key, more than the keys; sinks that meet the window, and that lie past it
+    (4, 2, 64, 64, 1, [500, 20], 64, 4, 0.0), (4, 2, 128, 128, 5, [411, 3, 70], 33, 1, 0.0), (2, 2, 256, 128, 1, [1025], 1, 0, 0.0),
+    (8, 2, 128, 128, 40, [600, 90], 100, 5, 0.0), (2, 1, 64, 64, 300, [1000], 129, 70, 0.0), (3, 1, 64, 64, 33, [200, 100], 1000, 1000, 20.0),
+    (2, 1, 128, 128, 300, [310], 64, 300, 0.0), (1, 1, 64, 64, 130, [4000], 17, 3, 0.0), (4, 1, 256, 256, 1, [4003], 1500, 33, 0.0),
+]
+
+
+def kv4_case(seed, heads, kvh, dk, dv, T, lens, uniform=False, spare=9):
+    """A cache of random rows behind which (and in whose unused places) every byte is 0xFF: codes of 15, NaN scales."""
+    g = rng(seed)
+    cap = max(lens) + spare
+    c = F.Cache(len(lens) + 2, kvh, dk, dv, cap, fill=0xFF)
+    for s, n in enumerate(lens):
+        if n:
+            # dims of their own offset, as keys have after a rotation
+            c.put_all(s + 1, F.f16(g.standard_normal((kvh, n, dk)) + 0.5 * g.standard_normal(dk)), F.f16(g.standard_normal((kvh, n, dv))))
+    Q = F.f16(np.zeros((len(lens), heads, T, dk)) if uniform else g.standard_normal((len(lens), heads, T, dk)) * 1.5)
+    return c, Q
+
+
+def kv4_want(c, Q, lens, window, sinks, scale, cap):
+    k, v = c.rows()
+    T = Q.shape[2]
+    for s, n in enumerate(lens):
+        yield F.attend(Q[s], k[s + 1, :, :max(1, n)], v[s + 1, :, :max(1, n)], F.visible(n, T, window, sinks, max(1, n)), scale, cap, True)
+
+
+@pytest.mark.parametrize("uniform", [False, True])
+@pytest.mark.parametrize("case", KV4)
+def test_kv4_attn(lib, fd, case, uniform):
+    """Random queries; and queries of zero, whose results are the plain means of the visible values: a key too many or
+    too few would show. Rows of other places and keys behind the lengths hold NaN scales."""
+    heads, kvh, dk, dv, T, lens, window, sinks, cap = case
+    print("kv4", case, uniform, flush=True)
+    c, Q = kv4_case(10, heads, kvh, dk, dv, T, lens, uniform)
+    scale = dk ** -0.5
+    mem, dQ, dL = dev(c.buf), dev(Q), dev(np.array(lens, np.int32))
+    out = dev(np.full((len(lens), heads, T, dv), 7, np.float16))
+    sh = R.Kv4Shape(*c.dims)
+    call = lambda o: lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 1, len(lens), T, max(lens), heads, scale, cap, window, sinks,  # noqa: E731
+                                              R.ptr(dQ), R.ptr(dL), R.ptr(o))
+    assert call(out) == 0
+    got = out.cpu().numpy()
+    for s, (want, tol) in enumerate(kv4_want(c, Q, lens, window, sinks, scale, cap)):
+        near(got[s], want, tol)
+        empty = ~F.visible(lens[s], T, window, sinks, max(1, lens[s])).any(1)
+        assert not got[s][:, empty].any()
+    again = dev(np.full((len(lens), heads, T, dv), 7, np.float16))
+    assert call(again) == 0
+    assert np.array_equal(again.cpu().numpy(), got)
+
+
+def test_kv4_attn_larger_bound_and_host_operands(lib, fd):
+    """max_kv above every length, lengths above max_kv (idle), host Q, lengths and results."""
+    lens = [50, 7, 90]
+    c, Q = kv4_case(11, 4, 2, 128, 128, 2, lens, spare=400)
+    out = np.full((3, 4, 2, 128), 7, np.float16)
+    L = np.array(lens, np.int32)
+    sh, mem = R.Kv4Shape(*c.dims), dev(c.buf)
+    call = lib.rocket_kv4_attn_fp16
+    assert call(fd, C.byref(sh), R.ptr(mem), 1, 3, 2, 490, 4, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+    for s, (want, tol) in enumerate(kv4_want(c, Q, lens, 0, 0, 0.1, 0.0)):
+        near(out[s], want, tol)
+    assert call(fd, C.byref(sh), R.ptr(mem), 1, 3, 2, 60, 4, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == R.ROCKET_E_SHAPE
+    first = out.copy()
+    dL = dev(L)
+    assert call(fd, C.byref(sh), R.ptr(mem), 1, 3, 2, 60, 4, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(dL), R.ptr(out)) == 0
+    assert not out[2].any()
+    for s, (want, tol) in list(enumerate(kv4_want(c, Q, lens, 0, 0, 0.1, 0.0)))[:2]:
+        near(out[s], want, tol)
+    assert first.any()
+
+
+def test_kv4_attn_large_scores(lib, fd):
+    """Scores in the thousands, growing and falling along the keys: the running maximum moves in every tile."""
+    for T in (1, 40):
+        for flip in (False, True):
+            heads, kvh, d, n = 4, 2, 128, 600
+            g = rng(12)
+            c = F.Cache(3, kvh, d, d, n, fill=0xFF)
+            up = np.linspace(0.1, 8, n)[::-1 if flip else 1]
+            c.put_all(1, F.f16(np.abs(g.standard_normal((kvh, n, d))) * up[None, :, None]), F.f16(g.standard_normal((kvh, n, d))))
+            Q = F.f16(np.abs(g.standard_normal((1, heads, T, d))) * 3)
+            out, sh = np.full((1, heads, T, d), 7, np.float16), R.Kv4Shape(*c.dims)
+            assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, 1, T, n, heads, d ** -0.5, 0.0, 0, 0, R.ptr(Q),
+                                            R.ptr(np.array([n], np.int32)), R.ptr(out)) == 0
+            (want, tol), = kv4_want(c, Q, [n], 0, 0, d ** -0.5, 0.0)
+            near(out[0], want, tol)
+
+
+# ---- windowed attention over fp16 keys -------------------------------------------------
+
+WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
+    (1, 1, 32, 16, 1, 1, 1, 0, 0, 0.0), (4, 2, 64, 64, 1, 63, 64, 0, 0, 0.0), (8, 2, 128, 128, 1, 1000, 1000, 0, 0, 0.0), (16, 8, 256, 256, 1, 777, 800, 0, 0, 0.0),
+    (4, 4, 96, 80, 3, 130, 131, 0, 0, 30.0), (4, 2, 64, 64, 1, 500, 500, 64, 4, 0.0), (2, 2, 256, 128, 1, 1025, 1030, 1, 0, 0.0), (8, 2, 128, 128, 5, 411, 416, 33, 1, 0.0),
+    (4, 1, 160, 224, 4, 600, 600, 100, 40, 0.0), (2, 1, 64, 64, 17, 300, 300, 0, 0, 0.0), (2, 1, 64, 64, 130, 130, 130, 0, 0, 0.0), (4, 2, 128, 128, 200, 512, 512, 0, 0, 0.0),
+    (2, 2, 256, 256, 129, 1000, 1001, 0, 0, 20.0), (4, 2, 64, 64, 300, 1000, 1024, 129, 70, 0.0), (2, 1, 128, 64, 257, 900, 904, 64, 3, 0.0), (3, 1, 192, 192, 140, 1111, 1111, 100, 0, 0.0),
+    (2, 1, 128, 128, 300, 310, 310, 64, 300, 0.0), (2, 1, 64, 48, 200, 90, 96, 0, 0, 0.0), (2, 1, 64, 64, 150, 100, 100, 20, 2, 0.0), (1, 1, 64, 64, 130, 4000, 4000, 17, 3, 0.0),
+    (4, 1, 256, 256, 1, 4003, 4003, 1500, 33, 0.0), (2, 1, 128, 128, 40, 5, 7, 3, 1, 0.0), (2, 1, 64, 64, 20, 3000, 3000, 2000, 1, 0.0),
+]
+
+
+def win_case(seed, heads, kvh, dk, dv, T, n, stride, window, sinks, uniform=False):
+    g = rng(seed)
+    Q = F.f16(np.zeros((heads, T, dk)) if uniform else g.standard_normal((heads, T, dk)) * 1.5)
+    K, V = F.f16(g.standard_normal((kvh, stride, dk))), F.f16(g.standard_normal((kvh, dv, stride)))
+    see = F.visible(n, T, window, sinks, stride)
+    see[:, n:] = False
+    return Q, K, V, see
+
+
+def win_want(Q, K, V, see, scale, cap):
+    return F.attend(Q, K.astype(np.float64), V.astype(np.float64).transpose(0, 2, 1), see, scale, cap, False)
+
+
+@pytest.mark.parametrize("kind", ["random", "uniform", "nan"])
+@pytest.mark.parametrize("case", WIN)
+def test_window_attn(lib, fd, case, kind):
+    """Random queries; queries of zero, whose results are plain means of the visible values; and NaN and infinities in
+    every key and value that no token sees."""
+    heads, kvh, dk, dv, T, n, stride, window, sinks, cap = case
+    print("window", case, kind, flush=True)
+    Q, K, V, see = win_case(20, heads, kvh, dk, dv, T, n, stride, window, sinks, kind == "uniform")
+    if kind == "nan":
+        dead = ~see.any(0)
+        K[:, dead], V[:, :, dead] = np.nan, np.inf
+        V[:, ::2, dead] = np.nan
+    scale = dk ** -0.5
+    dQ, dK, dV = dev(Q), dev(K), dev(V)
+    outs = []
+    for _ in range(2):
+        out = dev(np.full((heads, T, dv), 7, np.float16))
+        assert lib.rocket_flash_attn_window_fp16(fd, T, n, stride, dk, dv, heads, kvh, scale, cap, window, sinks, R.ptr(dQ), R.ptr(dK), R.ptr(dV), R.ptr(out)) == 0
+        outs.append(out.cpu().numpy())
+    near(outs[0], *win_want(Q, K, V, see, scale, cap))
+    assert not outs[0][:, ~see.any(1)].any()
+    assert np.array_equal(*outs)
+
+
+@pytest.mark.parametrize("T,n,window,sinks", [(5, 200, 30, 2), (130, 400, 50, 3), (20, 333, 0, 0)])
+def test_window_attn_values_that_some_tokens_see(lib, fd, T, n, window, sinks):
+    """An infinite value reaches the tokens that see its key, and no other (0 times it would be NaN)."""
+    heads, kvh, d = 2, 1, 64
+    Q, K, V, see = win_case(21, heads, kvh, d, d, T, n, n, window, sinks)
+    j = n - T + T // 2   # the middle token's own position
+    V[0, 3, j] = np.inf
+    out = np.full((heads, T, d), 7, np.float16)
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, 0.125, 0.0, window, sinks, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(out)) == 0
+    hit = see[:, j]
+    assert np.isposinf(out[:, hit, 3]).all()
+    V[0, 3, j] = 0
+    want, tol = win_want(Q, K, V, see, 0.125, 0.0)
+    keep = np.ones((T, d), bool)
+    keep[hit, 3] = False
+    near(out[:, keep], want[:, keep], tol[:, keep])
+
+
+def test_window_attn_is_the_masked_one(lib, fd):
+    """The library's masked attention under the same visibility, as a causal mask of 0 and -infinity: its scores are
+    clamped at -30000, so hidden keys weigh 0 there too wherever a token sees one."""
+    heads, kvh, d, T, n = 4, 2, 128, 70, 500
+    Q, K, V, see = win_case(22, heads, kvh, d, d, T, n, n, 90, 3)
+    mask = F.f16(np.where(see, 0.0, -np.inf))
+    a, b = np.empty((heads, T, d), np.float16), np.empty((heads, T, d), np.float16)
+    scale = d ** -0.5
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, 0.0, 90, 3, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(a)) == 0
+    assert lib.rocket_flash_attn_fp16(fd, T, n, d, d, heads, kvh, scale, 0.0, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(mask), R.ptr(b)) == 0
+    want, tol = win_want(Q, K, V, see, scale, 0.0)
+    near(a, want, tol)
+    near(b, want, tol)
+
+
+# ---- together, and as programs call them -----------------------------------------------
+
+def _handle(lib, stream):
+    fd = lib.rocket_open()
+    assert fd >= 0
+    assert lib.rocket_hip_set_stream(fd, R.ptr(stream.cuda_stream)) == 0
+    assert lib.rocket_hip_set_mode(fd, R.ROCKET_HIP_ASYNC | R.ROCKET_HIP_DEVICE_OPERANDS) == 0
+    return fd
+
+
+class Layer:
+    """A serving layer's attention over a batch: rows of a fused product -> rotated heads -> cache -> attention, on
+    buffers that stay where they are, so that a captured step can be replayed."""
+
+    def __init__(self, lib, n_seq, nq, nk, d, cap, window=0, sinks=0):
+        import torch
+        self.lib, self.dims, self.win = lib, (n_seq, nq, nk, d, cap), (window, sinks)
+        self.c = F.Cache(n_seq, nk, d, d, cap, fill=0xFF)
+        self.sh = R.Kv4Shape(*self.c.dims)
+        self.mem = dev(self.c.buf)
+        self.freq = (10000.0 ** (-np.arange(d // 2) / (d // 2))).astype(np.float32)
+        self.w = F.f16(1 + 0.2 * rng(30).standard_normal((2, d)))
+        self.dfreq, self.dw = dev(self.freq), dev(self.w)
+        self.torch = torch
+
+    def buffers(self, T):
+        n_seq, nq, nk, d, _ = self.dims
+        new = lambda *s: self.torch.zeros(s, dtype=self.torch.float16, device=DEV)  # noqa: E731
+        i = lambda *s: self.torch.zeros(s, dtype=self.torch.int32, device=DEV)  # noqa: E731
+        return dict(x=new(n_seq * T, (nq + 2 * nk) * d), pos=i(n_seq * T), lens=i(n_seq), q=new(n_seq, nq, T, d), k=new(n_seq, nk, T, d), out=new(n_seq, nq, T, d), T=T)
+
+    def step(self, fd, b):
+        n_seq, nq, nk, d, cap = self.dims
+        lib, T, W, sh = self.lib, b["T"], b["x"].shape[1], C.byref(self.sh)
+        at = lambda h: R.ptr(b["x"].data_ptr() + 2 * h * d)  # noqa: E731
+        assert lib.rocket_qk_norm_rope_fp16(fd, n_seq, T, nq, nk, d, d, R.ROCKET_ROPE_HALVES, 1e-6, at(0), W, at(nq), W, R.ptr(self.dw[0]), R.ptr(self.dw[1]),
+                                            R.ptr(self.dfreq), R.ptr(b["pos"]), R.ptr(b["q"]), R.ptr(b["k"])) == 0
+        assert lib.rocket_kv4_append_fp16(fd, sh, R.ptr(self.mem), 0, n_seq, T, R.ptr(b["k"]), nk * T * d, T * d, d, at(nq + nk), T * W, d, W, R.ptr(b["lens"])) == 0
+        assert lib.rocket_kv4_attn_fp16(fd, sh, R.ptr(self.mem), 0, n_seq, T, cap, nq, d ** -0.5, 0.0, *self.win, R.ptr(b["q"]), R.ptr(b["lens"]), R.ptr(b["out"])) == 0
+
+    def feed(self, b, x, lens):
+        T = b["T"]
+        pos = (np.array(lens)[:, None] - T + np.arange(T)).astype(np.int32).reshape(-1)
+        b["x"].copy_(dev(x))
+        b["pos"].copy_(dev(pos))
+        b["lens"].copy_(dev(np.array(lens, np.int32)))
+        return pos
+
+    def check(self, b, x, pos, lens):
+        """This step's results from the GPU's own rotated rows (checked first) and the cache built so far."""
+        n_seq, nq, nk, d, cap = self.dims
+        T = b["T"]
+        q, k, out = (b[n].cpu().numpy() for n in ("q", "k", "out"))
+        near(q, *F.rope(x, nq, d, d, False, 1e-6, self.w[0], self.freq, pos, n_seq))
+        near(k, *F.rope(x[:, nq * d:], nk, d, d, False, 1e-6, self.w[1], self.freq, pos, n_seq))
+        v = x[:, (nq + nk) * d:].reshape(n_seq, T, nk, d)
+        for s, n in enumerate(lens):
+            for t in range(T):
+                if 0 <= n - T + t < cap:
+                    for h in range(nk):
+                        self.c.put(s, h, n - T + t, k[s, h, t], v[s, t, h])
+        assert np.array_equal(self.mem.cpu().numpy(), self.c.buf)
+        K, V = self.c.rows()
+        for s, n in enumerate(lens):
+            see = F.visible(n, T, *self.win, max(1, n))
+            near(out[s], *F.attend(q[s], K[s, :, :max(1, n)], V[s, :, :max(1, n)], see, d ** -0.5, 0.0, True))
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (24, 3)])
+def test_layer_prompt_then_steps(lib, window, sinks):
+    """A ragged prompt (padded in front), then single tokens, then drafts of three: eager, on a stream of the caller's."""
+    import torch
+    stream = torch.cuda.Stream()
+    fd = _handle(lib, stream)
+    g = rng(31)
+    with torch.cuda.stream(stream):
+        L = Layer(lib, 3, 4, 2, 64, 120, window, sinks)
+        lens = np.array([40, 17, 0])
+        for T, grow in ((40, [0, 0, 0]), (1, [1, 1, 0]), (1, [1, 1, 1]), (3, [3, 3, 3])):
+            lens = lens + grow
+            b = L.buffers(T)
+            x = F.f16(g.standard_normal(b["x"].shape))
+            pos = L.feed(b, x, lens)
+            L.step(fd, b)
+            stream.synchronize()
+            L.check(b, x, pos, lens)
+    lib.rocket_close(fd)
+
+
+def test_layer_captured(lib):
+    """One step captured into a graph and replayed with growing lengths, eager work between the replays: every replay
+    is checked. Two graphs of two handles run side by side."""
+    import torch
+    g = rng(32)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    fds = [_handle(lib, s) for s in streams]
+    layers, bufs, graphs, lens = [], [], [], [np.array([4, 0, 30]), np.array([1, 63, 64])]
+    for i in range(2):
+        with torch.cuda.stream(streams[i]):
+            L = Layer(lib, 3, 8, 2, 128, 400)
+            for s, n in enumerate(lens[i]):   # what the sequences hold already
+                if n:
+                    L.c.put_all(s, F.f16(g.standard_normal((2, n, 128))), F.f16(g.standard_normal((2, n, 128))))
+            L.mem.copy_(dev(L.c.buf))
+            b = L.buffers(1)
+            x = F.f16(g.standard_normal(b["x"].shape))
+            lens[i] = lens[i] + 1
+            pos = L.feed(b, x, lens[i])
+            L.step(fds[i], b)   # eager first: the kernels' one-time set-up and the handle's scratch
+            streams[i].synchronize()
+            L.check(b, x, pos, lens[i])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[i]):
+            L.step(fds[i], b)
+        layers.append(L)
+        bufs.append(b)
+        graphs.append(graph)
+    for rep in range(4):
+        state = []
+        for i in range(2):
+            lens[i] = lens[i] + (1 if rep < 3 else [1, 300, 0])
+            with torch.cuda.stream(streams[i]):
+                if rep == 3:   # a long jump: rows put in by hand
+                    old = lens[i] - [1, 300, 0]
+                    n = int(lens[i][1]) - 1
+                    L = layers[i]
+                    L.c.put_all(1, F.f16(g.standard_normal((2, n, 128))), F.f16(g.standard_normal((2, n, 128))))
+                    assert old[1] <= n
+                    L.mem.copy_(dev(L.c.buf))
+                x = F.f16(g.standard_normal(bufs[i]["x"].shape))
+                state.append((x, layers[i].feed(bufs[i], x, lens[i])))
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            layers[i].check(bufs[i], *state[i], lens[i])
+    del graphs
+    for fd in fds:
+        lib.rocket_close(fd)
+
+
+@pytest.mark.parametrize("T,n", [(1, 700), (150, 700)])
+def test_window_attn_captured(lib, T, n):
+    import torch
+    heads, kvh, d, window, sinks = 4, 2, 128, 200, 4
+    stream = torch.cuda.Stream()
+    fd = _handle(lib, stream)
+    with torch.cuda.stream(stream):
+        Q, K, V, see = win_case(33, heads, kvh, d, d, T, n, n + 4, window, sinks)
+        dQ, dK, dV = dev(Q), dev(K), dev(V)
+        out = dev(np.full((heads, T, d), 7, np.float16))
+        call = lambda: lib.rocket_flash_attn_window_fp16(fd, T, n, n + 4, d, d, heads, kvh, 0.1, 0.0, window, sinks, R.ptr(dQ), R.ptr(dK), R.ptr(dV), R.ptr(out))  # noqa: E731
+        assert call() == 0
+        stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        rc = call()
+    assert rc == 0
+    for rep in range(3):
+        Q = win_case(34 + rep, heads, kvh, d, d, T, n, n + 4, window, sinks)[0]
+        with torch.cuda.stream(stream):
+            dQ.copy_(dev(Q))
+            out.fill_(7)
+            graph.replay()
+        stream.synchronize()
+        near(out.cpu().numpy(), *win_want(Q, K, V, see, 0.1, 0.0))
+    del graph
+    lib.rocket_close(fd)
