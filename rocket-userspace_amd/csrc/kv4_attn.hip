@@ -80,8 +80,11 @@ __global__ __launch_bounds__(256) void k_serve_row(const ServeAttn a)
 
 }  // namespace
 
+size_t serve_attn_ws(const ServeAttn &a) { return !a.Kf && kv4_few_rows(a) ? kv4_rows_ws(a) : 0; }
+
 hipError_t serve_attn(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
 {
+    if (!a.Kf && kv4_few_rows(a)) return kv4_rows(a, s, blocks);
     if (a.n_seq > 65535) return hipErrorInvalidValue;
     hipLaunchKernelGGL(k_serve_row, dim3((unsigned)a.n_tokens, (unsigned)a.n_head, (unsigned)a.n_seq), dim3(256), 0, s, a);
     *blocks = (uint64_t)a.n_tokens * a.n_head * a.n_seq;

@@ -1,0 +1,432 @@
+// kv4_rows.hip — attention of few query rows (decode steps, drafts) over the 4-bit cache.
+//
+// What bounds it is how fast the codes arrive, and then the VALU that widens them: about two
+// operations a value, whatever the number of query rows. So all rows of a KV head (its query heads'
+// tokens, at most 16) share one widening. A workgroup owns a place of the batch, a KV head and a range
+// of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
+// they lie in the cache, the next chunk's while this one's are widened.
+//
+// Scores are transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16, K the first operand): lane (c, q) =
+// (l % 16, l / 16) holds query c and keys 8 q .. 8 q + 7 of the chunk, as the second product takes them.
+// The order of the summed dims is free as long as Q has the same: quarter q takes whole groups, so a
+// lane's sixteen bytes of a key share one scale. In O^T += V^T P^T the rows (dims) are free: lane c
+// takes a word of eight dims of each of its eight keys, product j their nibbles j, which two byte permutes
+// and a shift bring side by side as pairs of keys. A code c becomes the half 1024 + c by or-ing bits in,
+// less 1024 (exact), times scale plus minimum (one rounding): the values that rocket_kv4_read_fp16 gives.
+#include "lds_optin.h"
+#include "serve.h"
+
+#include <algorithm>
+#include <atomic>
+
+namespace rk {
+namespace {
+
+typedef int      i32x2 __attribute__((ext_vector_type(2)));
+typedef int      i32x4 __attribute__((ext_vector_type(4)));
+typedef float    f32x2 __attribute__((ext_vector_type(2)));
+typedef float    f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kRows = 16, kChunk = 32, kWaves = 4, kMaxSplit = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Kv4RowArgs {
+    ServeAttn a;
+    int nsplit, cps;   // workgroups a place and KV head, chunks a workgroup
+    float *part;       // [place][split][head][token][dv] outputs, then (max, sum) pairs
+};
+
+// The chunks of a sequence of n keys that some of its last T tokens sees: those of the sinks, then from the
+// first window's on. v -> the v-th of them.
+struct Chunks {
+    int first, sinks, ns, skip, count;
+    __device__ Chunks(const ServeAttn &a, int n)
+    {
+        first = a.window ? max(0, n - a.n_tokens - a.window + 1) : 0;   // (n and n_tokens below 2^24)
+        sinks = min(a.sinks, first);
+        ns = (sinks + kChunk - 1) / kChunk;
+        const int f = max(first / kChunk, ns);
+        skip = f - ns;
+        count = ns + (n - 1) / kChunk - f + 1;
+    }
+    __device__ int at(int v) const { return v < ns ? v : v + skip; }
+};
+
+// Eight codes of a word as halves in the order 0 4 1 5 2 6 3 7, times scale plus minimum.
+__device__ __forceinline__ f16x2 widen2(int nibbles, f16x2 s, f16x2 m)
+{
+    const f16x2 c = __builtin_bit_cast(f16x2, (nibbles & 0x000F000F) | 0x64006400) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
+    return __builtin_elementwise_fma(c, s, m);
+}
+__device__ __forceinline__ f16x8 widen8(int w, f16x2 sm)
+{
+    const f16x2 s = {sm[0], sm[0]}, m = {sm[1], sm[1]};
+    f16x8 r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const f16x2 x = widen2(w >> (4 * e), s, m);
+        r[2 * e] = x[0];
+        r[2 * e + 1] = x[1];
+    }
+    return r;
+}
+
+// D: head sizes up to this (64, 128, 256). FULL: dk and dv are D.
+template <int D, bool CAP, bool FULL>
+__global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
+{
+    const ServeAttn &a = ra.a;
+    constexpr int U = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4, KS = U * KW;   // key words of a lane: U runs of KW
+    constexpr int NJ = D == 64 ? 4 : 8, VB = U * NJ, LROW = D + 4;          // output blocks of 16 dims; LDS row (floats)
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x, zs = blockIdx.y, s = blockIdx.z;
+    const int T = a.n_tokens, R = a.gqa * T;
+    const int n = a.seq_len[s];
+    const bool served = n >= 1 && n <= a.max_kv;
+    const Chunks list(a, served ? n : 1);
+    const int count = served ? list.count : 0;
+    if (zs > 0 && zs * ra.cps >= count) return;   // (the merge knows)
+    const int hg = c / T, t = c - hg * T;         // this lane's query: head hk gqa + hg, token t
+    const bool qok = c < R;
+    const int pos = n - T + t;                    // its position
+    const int p_lo = n - T, p_hi = n - 1;
+
+    const size_t hr = (size_t)s * a.c.heads + hk;
+    const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;   // row of the first query
+    f16x8 qf[KS];
+    {
+        const _Float16 *qrow = a.Q + (head0 + (qok ? c : 0)) * a.dk;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int d = D == 64 ? 16 * q + 8 * i : 128 * (i / 4) + 32 * q + 8 * (i % 4);
+            f16x8 x = {};
+            if (qok && (FULL || d < a.dk)) x = *reinterpret_cast<const f16x8 *>(qrow + d);
+            qf[i] = __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
+        }
+    }
+
+    const int dk = FULL ? D : a.dk, dv = FULL ? D : a.dv;
+    const char *const kc = a.c.kc + hr * a.c.cap * (dk / 2), *const ks = a.c.ks + hr * a.c.cap * (dk / 8);
+    const char *const vc = a.c.vc + hr * a.c.cap * (dv / 2), *const vs = a.c.vs + hr * a.c.cap * (dv / 8);
+    int kw[2][KS];        // block b's key of this lane: 8 (c / 4) + 4 b + c % 4
+    f16x2 ksm[2][U];
+    i32x4 vw[U][2];       // a word of each of the keys 8 q .. 8 q + 7
+    i32x4 vsm[U][2];      // their (scale, minimum)
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int i = 0; i < KW; i++) kw[b][u * KW + i] = 0;
+            ksm[b][u] = f16x2{};
+            vw[u][b] = vsm[u][b] = i32x4{};
+        }
+    auto load_k = [&](int key0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const uint32_t key = key0 + 8 * (c >> 2) + 4 * b + (c & 3);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int g = D == 64 ? q >> 1 : 4 * u + q;   // the run's group
+                if (!FULL && (D == 64 ? 16 * q : 32 * g) >= dk) continue;
+                if constexpr (D == 64) {
+                    const i32x2 x = *reinterpret_cast<const i32x2 *>(kc + (size_t)key * (dk / 2) + 8 * q);
+                    kw[b][0] = x[0];
+                    kw[b][1] = x[1];
+                } else {
+                    const i32x4 x = *reinterpret_cast<const i32x4 *>(kc + (size_t)key * (dk / 2) + 16 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) kw[b][4 * u + i] = x[i];
+                }
+                ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (size_t)key * (dk / 8) + 4 * g);
+            }
+        }
+    };
+    auto load_v = [&](int key0) __attribute__((always_inline)) {
+        const uint32_t block = key0 / 8 + q;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int w = D == 64 ? c >> 1 : 16 * u + c;   // the lane's word: dims 8 w .. 8 w + 7
+            if (!FULL && 8 * w >= dv) continue;
+            const char *p = vc + ((size_t)block * (dv / 8) + w) * 32, *m = vs + ((size_t)block * (dv / 32) + w / 4) * 32;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                vw[u][i] = *reinterpret_cast<const i32x4 *>(p + 16 * i);
+                vsm[u][i] = *reinterpret_cast<const i32x4 *>(m + 16 * i);
+            }
+        }
+    };
+
+    float m_run = -1e30f, l_run = 0.f;
+    f32x4 O[VB];
+#pragma unroll
+    for (int j = 0; j < VB; j++) O[j] = f32x4{};
+    const int c1 = min(count, (zs + 1) * ra.cps);
+    int ch = zs * ra.cps + wave;
+    if (ch < c1) {
+        load_k(list.at(ch) * kChunk);
+        load_v(list.at(ch) * kChunk);
+    }
+    for (; ch < c1; ch += kWaves) {
+        const int key0 = list.at(ch) * kChunk;
+        f32x4 S[2] = {};
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+                S[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kw[b][i], ksm[b][i / KW]), qf[i], S[b], 0, 0, 0);
+        const bool more = ch + kWaves < c1;
+        const int next = list.at(more ? ch + kWaves : ch) * kChunk;
+        if (more) load_k(next);
+        // every row sees every key of the chunk, or the rows differ (uniform)
+        const bool whole = key0 + kChunk - 1 <= p_lo && (!a.window || key0 > p_hi - a.window || key0 + kChunk <= a.sinks);
+        float v[8], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float x = S[i >> 2][i & 3];
+            if constexpr (CAP) v[i] = a.softcap * tanhf(x * a.scale / a.softcap) * kLog2e;
+            else v[i] = x * (a.scale * kLog2e);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int key = key0 + 8 * q + i;
+                if (key > pos || (a.window && key <= pos - a.window && key >= a.sinks)) v[i] = -INFINITY;
+            }
+            // keys that no row sees: their values count as 0, whatever the memory holds
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int key = key0 + 8 * q + i;
+                    if (key > p_hi || (key < list.first && key >= list.sinks)) vsm[u][i >> 2][i & 3] = 0;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (__any(mx > m_run)) {
+            const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int j = 0; j < VB; j++) O[j] *= alpha;
+        }
+        f16x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float e = __builtin_amdgcn_exp2f(v[i] - m_run);
+            l_run += e;
+            p[i] = (_Float16)e;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int x[2][4];      // low and high halves of the words of two keys each
+            f16x2 sc[4], mi[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const unsigned w0 = vw[u][k >> 1][2 * (k & 1)], w1 = vw[u][k >> 1][2 * (k & 1) + 1];
+                const unsigned s0 = vsm[u][k >> 1][2 * (k & 1)], s1 = vsm[u][k >> 1][2 * (k & 1) + 1];
+                if constexpr (D == 64) {   // lane c has the low or the high half of its word
+                    x[0][k] = (int)__builtin_amdgcn_perm(w1, w0, c & 1 ? 0x07060302u : 0x05040100u);
+                } else {
+                    x[0][k] = (int)__builtin_amdgcn_perm(w1, w0, 0x05040100u);
+                    x[1][k] = (int)__builtin_amdgcn_perm(w1, w0, 0x07060302u);
+                }
+                sc[k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
+                mi[k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                f16x8 f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const f16x2 y = widen2(x[j >> 2][k] >> (4 * (j & 3)), sc[k], mi[k]);
+                    f[2 * k] = y[0];
+                    f[2 * k + 1] = y[1];
+                }
+                O[u * NJ + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, O[u * NJ + j], 0, 0, 0);
+            }
+        }
+        if (more) load_v(next);
+    }
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+
+    // merge the waves: [wave][row][LROW] outputs, then [wave][row] (max, sum)
+    float *const Ol = reinterpret_cast<float *>(smem);
+    f32x2 *const ml = reinterpret_cast<f32x2 *>(Ol + kWaves * R * LROW);
+    if (qok) {
+        float *const row = Ol + (wave * R + c) * LROW;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)   // block row 4 q + e: dims NJ (4 q + e) + j
+#pragma unroll
+                for (int j = 0; j < NJ; j += 4)
+                    *reinterpret_cast<f32x4 *>(row + 128 * u + NJ * (4 * q + e) + j) =
+                        f32x4{O[u * NJ + j][e], O[u * NJ + j + 1][e], O[u * NJ + j + 2][e], O[u * NJ + j + 3][e]};
+        if (q == 0) ml[wave * R + c] = f32x2{m_run, l_run};
+    }
+    __syncthreads();
+    const int dq = dv / 4;
+    for (int i = tid; i < R * dq; i += kWaves * 64) {
+        const int r = i / dq, d0 = (i - r * dq) * 4;
+        float m = -1e30f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) m = fmaxf(m, ml[w * R + r][0]);
+        float l = 0.f;
+        f32x4 o = {};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const f32x2 x = ml[w * R + r];
+            const float f = __builtin_amdgcn_exp2f(x[0] - m);
+            l += f * x[1];
+            o += f * *reinterpret_cast<const f32x4 *>(Ol + (w * R + r) * LROW + d0);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing; NaN stays)
+        if (ra.nsplit > 1) {
+            const size_t row = ((size_t)s * ra.nsplit + zs) * a.n_head * T + (size_t)hk * R + r;
+            *reinterpret_cast<f32x4 *>(ra.part + row * dv + d0) = o * inv;
+            if (d0 == 0) reinterpret_cast<f32x2 *>(ra.part + (size_t)a.n_seq * ra.nsplit * a.n_head * T * dv)[row] = f32x2{m, l};
+        } else {
+            f16x4 out;
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[e] = (_Float16)(o[e] * inv);
+            *reinterpret_cast<f16x4 *>(a.out + (head0 + r) * dv + d0) = out;
+        }
+    }
+}
+
+// Merges the splits that a sequence's length has, one (head, token) row of a place a workgroup: out = sum_s
+// w_s On_s / sum_s w_s with w_s = 2^(m_s - m) l_s, outputs in fp32 (a rounding of each to fp16 would be a third
+// one beside the probabilities' and the result's).
+__global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
+{
+    const ServeAttn &a = ra.a;
+    __shared__ float wt[kMaxSplit], sum[8 * 256];
+    const int tid = threadIdx.x, row = blockIdx.x, s = blockIdx.y, dv = a.dv;
+    const int n = a.seq_len[s];
+    const int count = n >= 1 && n <= a.max_kv ? Chunks(a, n).count : 0;
+    const int nsplit = max(1, min(ra.nsplit, (count + ra.cps - 1) / ra.cps));
+    const size_t rows = (size_t)a.n_head * a.n_tokens, base = (size_t)s * ra.nsplit * rows + row;
+    const int dq = dv / 8, sg = tid / dq, d0 = (tid - sg * dq) * 8, ng = min(8, 256 / dq);   // dv <= 256: 8
+    f32x4 os[8][2];
+    if (sg < ng)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int sp = sg + i * ng;
+            if (sp < nsplit)
+#pragma unroll
+                for (int j = 0; j < 2; j++) os[i][j] = reinterpret_cast<const f32x4 *>(ra.part + (base + sp * rows) * dv + d0)[j];
+        }
+    if (tid < 64) {
+        const f32x2 x = tid < nsplit ? reinterpret_cast<const f32x2 *>(ra.part + (size_t)a.n_seq * ra.nsplit * rows * dv)[base + tid * rows]
+                                     : f32x2{-1e30f, 0.f};
+        float m = x[0];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float w = __builtin_amdgcn_exp2f(x[0] - m) * x[1];
+        float l = w;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+        wt[tid] = l == 0.f ? 0.f : w / l;
+    }
+    __syncthreads();
+    if (sg < ng) {
+        float acc[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int sp = sg + i * ng;
+            if (sp < nsplit)
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc[e] += wt[sp] * os[i][e >> 2][e & 3];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum[sg * dv + d0 + e] = acc[e];
+    }
+    __syncthreads();
+    for (int d = tid; d < dv; d += 256) {
+        float o = 0.f;
+        for (int sp = 0; sp < ng; sp++) o += sum[sp * dv + d];
+        a.out[((size_t)s * rows + row) * dv + d] = (_Float16)o;
+    }
+}
+
+template <int D, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
+{
+    auto kern = k_kv4_rows<D, CAP, FULL>;
+    const ServeAttn &a = ra.a;
+    const int R = a.gqa * a.n_tokens;
+    const size_t lds = (size_t)kWaves * R * ((D + 4) * 4 + 8);
+    if (lds > 64 * 1024) {
+        static std::atomic<uint64_t> opted{0};
+        if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), 80 * 1024, opted)) return e;
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)a.c.heads, (unsigned)ra.nsplit, (unsigned)a.n_seq), dim3(kWaves * 64), lds, s, ra);
+    return hipGetLastError();
+}
+template <int D> hipError_t launch(const Kv4RowArgs &ra, hipStream_t s)
+{
+    const bool cap = ra.a.softcap != 0.f;
+    if (ra.a.dk == D && ra.a.dv == D) return cap ? launch_f<D, true, true>(ra, s) : launch_f<D, false, true>(ra, s);
+    return cap ? launch_f<D, true, false>(ra, s) : launch_f<D, false, false>(ra, s);
+}
+
+// Chunks that a sequence of up to max_kv keys may have to visit.
+int most_chunks(const ServeAttn &a)
+{
+    const int all = (a.max_kv + kChunk - 1) / kChunk;
+    if (!a.window) return all;
+    const long seen = (std::min<long>(a.sinks, a.max_kv) + kChunk - 1) / kChunk + ((long)a.n_tokens + a.window - 2) / kChunk + 2;
+    return (int)std::min<long>(all, seen);
+}
+
+void split_of(const ServeAttn &a, int *nsplit, int *cps)
+{
+    const int chunks = most_chunks(a);
+    const long wgs = (long)a.c.heads * a.n_seq;
+    const int n = (int)std::max<long>(1, std::min<long>({(chunks + kWaves - 1) / kWaves, 1024 / wgs, kMaxSplit}));
+    *cps = (chunks + n - 1) / n;
+    *nsplit = (chunks + *cps - 1) / *cps;
+}
+
+}  // namespace
+
+bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= kRows; }
+
+size_t kv4_rows_ws(const ServeAttn &a)
+{
+    int n, cps;
+    split_of(a, &n, &cps);
+    return n > 1 ? (size_t)a.n_seq * n * a.n_head * a.n_tokens * (a.dv + 2) * sizeof(float) : 0;
+}
+
+hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
+{
+    if (a.n_seq > 65535) return hipErrorInvalidValue;
+    Kv4RowArgs ra;
+    ra.a = a;
+    split_of(a, &ra.nsplit, &ra.cps);
+    if (ra.nsplit > 1 && (!a.ws || a.ws_bytes < kv4_rows_ws(a))) {
+        ra.nsplit = 1;
+        ra.cps = most_chunks(a);
+    }
+    ra.part = a.ws;
+    const int d = std::max(a.dk, a.dv);
+    const hipError_t e = d <= 64 ? launch<64>(ra, s) : d <= 128 ? launch<128>(ra, s) : launch<256>(ra, s);
+    *blocks = (uint64_t)a.c.heads * ra.nsplit * a.n_seq;
+    if (e != hipSuccess || ra.nsplit == 1) return e;
+    const unsigned rows = (unsigned)(a.n_head * a.n_tokens);
+    hipLaunchKernelGGL(k_kv4_merge, dim3(rows, (unsigned)a.n_seq), dim3(256), 0, s, ra);
+    *blocks += (uint64_t)rows * a.n_seq;
+    return hipGetLastError();
+}
+
+}  // namespace rk

@@ -76,8 +76,17 @@ struct ServeAttn {
     const int32_t *seq_len = nullptr;   // null: max_kv
     int n_seq = 1, n_tokens = 0, n_head = 0, gqa = 1, dk = 0, dv = 0, max_kv = 0, window = 0, sinks = 0;
     float scale = 1.f, softcap = 0.f;
+    // workspace for splits of the key axis (serve_attn_ws); without it a workgroup walks every key
+    float *ws = nullptr;
+    size_t ws_bytes = 0;
 };
+size_t serve_attn_ws(const ServeAttn &a);
 hipError_t serve_attn(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
+
+// At most 16 query rows a KV head over the cache (kv4_rows.hip).
+bool kv4_few_rows(const ServeAttn &a);
+size_t kv4_rows_ws(const ServeAttn &a);
+hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 
 // The fp64 host paths (fd < 0); false where host memory runs out.
 bool qk_norm_rope_ref(const RopeLaunch &L);

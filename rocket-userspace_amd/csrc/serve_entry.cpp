@@ -6,6 +6,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <new>
 
 using namespace rk;
@@ -280,7 +281,7 @@ int rocket_kv4_attn_fp16(int fd, const rocket_kv4_shape *shape, const void *cach
         ServeAttn a;
         a.c = kv4_view(*shape, l, const_cast<void *>(cache), seq0, n_seq);
         a.n_seq = n_seq; a.n_tokens = n_tokens; a.n_head = n_head; a.gqa = n_head / shape->n_kv_heads; a.dk = shape->head_dim; a.dv = shape->dv;
-        a.max_kv = max_kv; a.window = window; a.sinks = sinks; a.scale = scale; a.softcap = softcap;
+        a.max_kv = max_kv; a.window = std::min(window, kServeMaxCap); a.sinks = std::min(sinks, kServeMaxCap); a.scale = scale; a.softcap = softcap;
         if (fd < 0) {
             if (!lens_ok(seq_len, n_seq, max_kv)) return bad(who, "a length above max_kv");
             a.Q = Q; a.out = out; a.seq_len = seq_len;
@@ -294,7 +295,10 @@ int rocket_kv4_attn_fp16(int fd, const rocket_kv4_shape *shape, const void *cach
         c.want(Q, qb);
         c.want(seq_len, nb);
         c.want(out, ob);
+        const size_t ws = c.want_optional(serve_attn_ws(a), max_kv >= 512);
         if (int rc = c.begin()) return rc;
+        a.ws = static_cast<float *>(c.optional(ws));
+        a.ws_bytes = a.ws ? ws : 0;
         a.Q = static_cast<const _Float16 *>(c.in(Q, qb));
         a.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb));
         a.out = static_cast<_Float16 *>(c.out(out, ob));
@@ -320,7 +324,7 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
         if (overlap(out, ob, Q, qb) || overlap(out, ob, K, kb) || overlap(out, ob, V, vb)) return bad(who, "results over operands");
         ServeAttn a;
         a.n_tokens = n_tokens; a.n_head = n_head; a.gqa = n_head / n_kv_heads; a.dk = head_dim; a.dv = dv; a.stride = kv_stride;
-        a.max_kv = n_kv; a.window = window; a.sinks = sinks; a.scale = scale; a.softcap = softcap;
+        a.max_kv = n_kv; a.window = std::min(window, kServeMaxCap); a.sinks = std::min(sinks, kServeMaxCap); a.scale = scale; a.softcap = softcap;
         if (fd < 0) {
             a.Q = Q; a.Kf = K; a.Vf = V; a.out = out;
             return serve_attn_ref(a) ? ROCKET_OK : ROCKET_E_NOMEM;

@@ -140,7 +140,8 @@ KV4 = [  # heads, kv heads, dk, dv, tokens, lengths (the largest is max_kv), win
     # windows: inside a chunk, across chunks, one key, more than the keys; sinks that meet the window, and that lie past it
     (4, 2, 64, 64, 1, [500, 20], 64, 4, 0.0), (4, 2, 128, 128, 5, [411, 3, 70], 33, 1, 0.0), (2, 2, 256, 128, 1, [1025], 1, 0, 0.0),
     (8, 2, 128, 128, 40, [600, 90], 100, 5, 0.0), (2, 1, 64, 64, 300, [1000], 129, 70, 0.0), (3, 1, 64, 64, 33, [200, 100], 1000, 1000, 20.0),
-    (2, 1, 128, 128, 300, [310], 64, 300, 0.0), (1, 1, 64, 64, 130, [4000], 17, 3, 0.0), (4, 1, 256, 256, 1, [4003], 1500, 33, 0.0),
+    (2, 1, 128, 128, 300, [310], 64, 300, 0.0), (1, 1, 64, 64, 130, [4000], 17, 3, 0.0),
+    (2, 1, 64, 64, 2, [70, 9], 2 ** 31 - 1, 2 ** 31 - 1, 0.0), (4, 1, 256, 256, 1, [4003], 1500, 33, 0.0),
 ]
 
 
@@ -235,7 +236,7 @@ WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
     (4, 1, 160, 224, 4, 600, 600, 100, 40, 0.0), (2, 1, 64, 64, 17, 300, 300, 0, 0, 0.0), (2, 1, 64, 64, 130, 130, 130, 0, 0, 0.0), (4, 2, 128, 128, 200, 512, 512, 0, 0, 0.0),
     (2, 2, 256, 256, 129, 1000, 1001, 0, 0, 20.0), (4, 2, 64, 64, 300, 1000, 1024, 129, 70, 0.0), (2, 1, 128, 64, 257, 900, 904, 64, 3, 0.0), (3, 1, 192, 192, 140, 1111, 1111, 100, 0, 0.0),
     (2, 1, 128, 128, 300, 310, 310, 64, 300, 0.0), (2, 1, 64, 48, 200, 90, 96, 0, 0, 0.0), (2, 1, 64, 64, 150, 100, 100, 20, 2, 0.0), (1, 1, 64, 64, 130, 4000, 4000, 17, 3, 0.0),
-    (4, 1, 256, 256, 1, 4003, 4003, 1500, 33, 0.0), (2, 1, 128, 128, 40, 5, 7, 3, 1, 0.0), (2, 1, 64, 64, 20, 3000, 3000, 2000, 1, 0.0),
+    (2, 1, 64, 64, 20, 70, 72, 2 ** 31 - 1, 2 ** 31 - 1, 0.0), (4, 1, 256, 256, 1, 4003, 4003, 1500, 33, 0.0), (2, 1, 128, 128, 40, 5, 7, 3, 1, 0.0), (2, 1, 64, 64, 20, 3000, 3000, 2000, 1, 0.0),
 ]
 
 
