@@ -1,5 +1,5 @@
 // serve.h — launches behind rocket_serve.h: head norms with rotation (rope.hip), the 4-bit key / value
-// cache (kv4.hip) and attention over it (kv4_attn.hip).
+// cache (kv4.hip) and attention over it or under a window (serve_attn.cpp).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -70,7 +70,7 @@ hipError_t kv4_read(const Kv4View &c, const Kv4Rows &r, hipStream_t s, uint64_t 
 struct ServeAttn {
     Kv4View c{};
     const _Float16 *Kf = nullptr, *Vf = nullptr;
-    long stride = 0;
+    long stride = 0, k_hs = 0;               // keys a V^T row holds (a multiple of 8); elements a head's keys take
     const _Float16 *Q = nullptr;
     _Float16 *out = nullptr;
     const int32_t *seq_len = nullptr;   // null: max_kv
@@ -87,6 +87,10 @@ hipError_t serve_attn(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 bool kv4_few_rows(const ServeAttn &a);
 size_t kv4_rows_ws(const ServeAttn &a);
 hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
+
+// More rows, or fp16 keys (serve_tiles.hip).
+size_t serve_tiles_ws(const ServeAttn &a);
+hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 
 // The fp64 host paths (fd < 0); false where host memory runs out.
 bool qk_norm_rope_ref(const RopeLaunch &L);

@@ -1,5 +1,6 @@
 // serve_entry.cpp — rocket_serve.h: argument checks, staging and launches of the head norms with
 // rotation (rope.hip), the 4-bit cache (kv4.hip) and attention over it or under a window.
+#include "attn.h"
 #include "internal.h"
 #include "ops.h"
 #include "serve.h"
@@ -147,7 +148,7 @@ int attn_args(const char *who, int n_tokens, int n_head, int kv_heads, float sca
     if (n_head < 1 || n_head > 65535 || kv_heads < 1 || n_head % kv_heads) return bad(who, "n_head is not a multiple of the KV heads, or too large");
     if (window < 0 || sinks < 0 || (!window && sinks)) return bad(who, "window and sinks are not negative, and sinks need a window");
     if (isnan(scale) || isnan(softcap)) return bad(who, "scale or softcap is NaN");
-    if ((long)n_tokens * n_head > ((long)1 << 31) - 1) return bad(who, "too many rows");
+    if ((long)n_tokens * n_head > (long)1 << 30) return bad(who, "too many rows");
     return ROCKET_OK;
 }
 
@@ -275,7 +276,7 @@ int rocket_kv4_attn_fp16(int fd, const rocket_kv4_shape *shape, const void *cach
         if (!Q || !out) return bad(who, "null operand");
         if (max_kv < 1 || max_kv > shape->capacity) return bad(who, "max_kv outside [1, capacity]");
         const size_t rows = (size_t)n_seq * n_head * n_tokens, nb = (size_t)n_seq * sizeof(int32_t);
-        if (rows > ((size_t)1 << 31) - 1) return bad(who, "too many rows");
+        if (rows > (size_t)1 << 30) return bad(who, "too many rows");
         const size_t qb = h16(rows * shape->head_dim), ob = h16(rows * shape->dv);
         if (overlap(out, ob, Q, qb) || overlap(out, ob, cache, l.bytes) || overlap(out, ob, seq_len, nb)) return bad(who, "results over operands");
         ServeAttn a;
@@ -313,7 +314,7 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
 {
     static const char *who = "rocket_flash_attn_window_fp16";
     return guarded(who, [&]() -> int {
-        if (n_tokens < 1 || n_kv < 1 || kv_stride < n_kv || n_tokens > kServeMaxCap || kv_stride > kServeMaxCap / 2)
+        if (n_tokens < 1 || n_kv < 1 || kv_stride < n_kv || n_tokens > kServeMaxCap || kv_stride > kServeMaxCap / 2 - 64)
             return bad(who, "n_tokens or n_kv below 1, kv_stride below n_kv, or one too large");
         if (int rc = attn_args(who, n_tokens, n_head, n_kv_heads, scale, softcap, window, sinks)) return rc;
         if (head_dim < 32 || head_dim % 32 || head_dim > kServeMaxDim || dv < 16 || dv % 16 || dv > kServeMaxDim)
@@ -323,7 +324,7 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
         const size_t kb = h16((size_t)n_kv_heads * kv_stride * head_dim), vb = h16((size_t)n_kv_heads * kv_stride * dv);
         if (overlap(out, ob, Q, qb) || overlap(out, ob, K, kb) || overlap(out, ob, V, vb)) return bad(who, "results over operands");
         ServeAttn a;
-        a.n_tokens = n_tokens; a.n_head = n_head; a.gqa = n_head / n_kv_heads; a.dk = head_dim; a.dv = dv; a.stride = kv_stride;
+        a.n_tokens = n_tokens; a.n_head = n_head; a.gqa = n_head / n_kv_heads; a.dk = head_dim; a.dv = dv; a.stride = kv_stride; a.k_hs = (long)kv_stride * head_dim;
         a.max_kv = n_kv; a.window = std::min(window, kServeMaxCap); a.sinks = std::min(sinks, kServeMaxCap); a.scale = scale; a.softcap = softcap;
         if (fd < 0) {
             a.Q = Q; a.Kf = K; a.Vf = V; a.out = out;
@@ -336,6 +337,12 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
         c.want(K, kb);
         c.want(V, vb);
         c.want(out, ob);
+        // V^T rows that are no whole 16-byte chunks are copied into ones that are
+        const int padded = kv_stride % 8 ? (kv_stride + 63) / 64 * 64 : kv_stride;
+        const size_t pb = padded != kv_stride ? h16((size_t)n_kv_heads * dv * padded) : 0;
+        if (pb) c.want_scratch(pb);
+        a.Kf = K;
+        const size_t ws = c.want_optional(serve_attn_ws(a), n_kv >= 512);
         if (int rc = c.begin()) return rc;
         a.Q = static_cast<const _Float16 *>(c.in(Q, qb));
         a.Kf = static_cast<const _Float16 *>(c.in(K, kb));
@@ -343,6 +350,17 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
         a.out = static_cast<_Float16 *>(c.out(out, ob));
         if (!a.Q || !a.Kf || !a.Vf || !a.out) return c.finish();
         uint64_t blocks = 0;
+        if (pb) {
+            _Float16 *const vp = static_cast<_Float16 *>(c.scratch(pb));
+            if (!vp) return c.finish();
+            if (pad_cols_f16(a.Vf, vp, (long)n_kv_heads * dv, nullptr, nullptr, 0, kv_stride, padded, c.stream(), &blocks) != hipSuccess)
+                return launched(c, hipErrorInvalidValue, 0);
+            count_launch(blocks);
+            a.Vf = vp;
+            a.stride = padded;
+        }
+        a.ws = static_cast<float *>(c.optional(ws));
+        a.ws_bytes = a.ws ? ws : 0;
         return launched(c, serve_attn(a, c.stream(), &blocks), blocks);
     });
 }

@@ -173,7 +173,7 @@ try {
                     if (!sees(j)) continue;
                     double x = 0;
                     for (int i = 0; i < a.dk; i++)
-                        x += (double)q[i] * (a.Kf ? (double)a.Kf[((size_t)(h / a.gqa) * a.stride + j) * a.dk + i] : value(key_group(a.c, hr, j, i / 32), i % 32));
+                        x += (double)q[i] * (a.Kf ? (double)a.Kf[(size_t)(h / a.gqa) * a.k_hs + (size_t)j * a.dk + i] : value(key_group(a.c, hr, j, i / 32), i % 32));
                     x *= (double)a.scale;
                     if (a.softcap != 0.f) x = (double)a.softcap * tanh(x / (double)a.softcap);
                     p[j] = x;

@@ -1,0 +1,639 @@
+// serve_tiles.hip — attention of many query rows over the 4-bit cache, and over fp16 keys under a window.
+//
+// One workgroup = 4 waves = 128 query rows of a KV head (the tokens of all its query heads in a row, so
+// that they share each tile), a wave 32 rows. The key axis goes by tiles of 64 keys, those alone that some
+// row sees: the sinks' tiles, then from the first window's to the last token's. K tiles [64][D] and V^T
+// tiles [D][64] lie in LDS as halves, two of each. fp16 keys arrive by buffer-load DMA. Codes arrive in
+// registers a tile ahead and are widened between the MFMAs (two VALU operations a value, shared by the
+// 128 rows), then written to LDS.
+//
+// The loop is software-pipelined: an iteration runs the previous tile's PV products with this tile's
+// score arithmetic between them, then the next tile's QK products with this tile's exponentials between
+// them; K runs a tile ahead of V^T. Scores are transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so a lane
+// holds one row's scores and P stays in registers: rounded to fp16 and swapped between the half-waves
+// it is the second product's operand. O is rescaled only when some running maximum grows by more than 8.
+#include "attn.h"
+#include "lds_optin.h"
+#include "serve.h"
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+namespace rk {
+namespace {
+
+typedef int      i32x2  __attribute__((ext_vector_type(2)));
+typedef int      i32x4  __attribute__((ext_vector_type(4)));
+typedef float    f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2  __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4  __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8  __attribute__((ext_vector_type(8)));
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+
+constexpr uint32_t kOOB = 0x80000000u;   // an offset past every range: loads return 0
+constexpr int BQ = 128, BK = 64, NW = 4;
+
+[[maybe_unused]] __device__ __forceinline__ Rsrc rsrc(const void *base, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ void wait_vm0()
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));
+#endif
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+struct TileArgs {
+    ServeAttn a;
+    int nsplit, nqb;   // shares of the key tiles; row blocks of BQ
+    void *part;        // [split][row][dv] fp16 outputs (divided by the split's sum), then [split][row] (max, sum)
+};
+
+// D: 64, 128 or 256. 16-byte chunk c of an LDS row lies at slot c ^ x(row): the sixteen lanes that one
+// LDS cycle serves (consecutive rows, one chunk) hit all banks once.
+template <int D> struct Cfg {
+    static constexpr int KC = D / 16;            // score MFMA steps
+    static constexpr int KCPR = D / 8;           // 16-byte chunks a K row
+    static constexpr int KINS = D / 32, VINS = D / 32;   // DMA instructions a wave and tile
+    static constexpr int KBYTES = BK * D * 2, VBYTES = D * BK * 2, STAGE = KBYTES + VBYTES;
+    static constexpr int DB = D / 32;            // 32-row blocks of output dims
+    static constexpr int LDS = 2 * STAGE + 16;   // + the flag of a tile with non-finite values
+    // 4-bit: a thread's runs of a tile's key codes and value codes, and the 16-byte writes they make
+    static constexpr int ITEMS = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4, VD = D == 64 ? 2 : 4;
+    static constexpr int KU = ITEMS * KW, VU = ITEMS * VD;
+    __device__ static int kx(int row) { return (D * 2) % 256 == 0 ? (row & 15) : ((row >> 1) & 7); }
+};
+__device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T rows: 128 bytes
+
+// Two codes (bits 0-3 and 16-19) as halves: 1024 + c by or-ing bits in, less 1024, times scale plus minimum
+// (one rounding).
+__device__ __forceinline__ f16x2 widen2(int nibbles, f16x2 s, f16x2 m)
+{
+    const f16x2 c = __builtin_bit_cast(f16x2, (nibbles & 0x000F000F) | 0x64006400) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
+    return __builtin_elementwise_fma(c, s, m);
+}
+
+template <int D, bool C4, bool CAP>
+__global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
+{
+    const ServeAttn &a = ta.a;
+    using CF = Cfg<D>;
+    constexpr int KC = CF::KC, KCPR = CF::KCPR, DB = CF::DB;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *const bad_tile = reinterpret_cast<int *>(smem + 2 * CF::STAGE);
+
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int T = a.n_tokens, R = a.gqa * T, kvh = a.n_head / a.gqa;
+    // Workgroup w runs on XCD w % 8; each XCD gets a contiguous range of logical ids, and consecutive ids are
+    // the row blocks that read the same keys.
+    int qb, hk, zs, s;
+    {
+        const int total = (int)gridDim.x, w = (int)blockIdx.x;
+        const int xcd = w % 8, idx = w / 8, per = total / 8, rem = total % 8;
+        int lid = xcd * per + (xcd < rem ? xcd : rem) + idx;
+        qb = ta.nqb - 1 - lid % ta.nqb;   // the last rows, which see the most keys, first
+        lid /= ta.nqb;
+        zs = lid % ta.nsplit;
+        lid /= ta.nsplit;
+        hk = lid % kvh;
+        s = lid / kvh;
+    }
+    const int n = a.seq_len ? a.seq_len[s] : a.max_kv;
+    const bool served = n >= 1 && n <= a.max_kv;
+    // the block's rows: head r / T of the KV head, token r % T; the lane's row and its position
+    const int r = qb * BQ + wave * 32 + l32;
+    const bool qok = r < R;
+    const int r0 = qb * BQ, r1 = min(R, r0 + BQ) - 1;
+    const bool one = r0 / T == r1 / T;
+    const int p_lo = n - T + (one ? r0 % T : 0), p_hi = n - T + (one ? r1 % T : T - 1);
+    const int pos = n - T + r % T;
+    const size_t row0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;
+
+    // the tiles that some row of the block sees, v -> tile: the sinks', then from the first window's on
+    const int first = a.window ? max(0, p_lo - a.window + 1) : 0, sinks = min(a.sinks, first);
+    const int ns = (sinks + BK - 1) / BK, f0 = max(first / BK, ns);
+    const int count = served && p_hi >= 0 ? ns + p_hi / BK - f0 + 1 : 0;
+    const int tps = (count + ta.nsplit - 1) / ta.nsplit;
+    const int kb0 = min(zs * tps, count), kb1 = min(count, kb0 + tps);
+    auto key_of = [&](int kb) __attribute__((always_inline)) { return (kb < ns ? kb : kb - ns + f0) * BK; };
+    // every row of the block sees every key of the tile
+    auto whole = [&](int key0) __attribute__((always_inline)) {
+        return key0 + BK - 1 <= p_lo && (!a.window || key0 > p_hi - a.window || key0 + BK <= a.sinks);
+    };
+    // no row of the block sees the key
+    auto dead = [&](int key) __attribute__((always_inline)) { return key > p_hi || (key < first && key >= sinks); };
+    auto sees = [&](int key) __attribute__((always_inline)) { return key <= pos && (!a.window || key > pos - a.window || key < a.sinks); };
+
+    // the lane's query row as the B operand of the score MFMAs: step c takes dims 16 c + 8 hh .. + 8 (in the order in
+    // which widened codes lie)
+    f16x8 qf[KC];
+    {
+        const _Float16 *qrow = a.Q + (row0 + (qok ? r : 0)) * a.dk;
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            f16x8 x = {};
+            if (qok && 16 * c + 8 * hh < a.dk) x = *reinterpret_cast<const f16x8 *>(qrow + 16 * c + 8 * hh);
+            qf[c] = C4 ? __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7) : x;
+        }
+    }
+
+    // ---- tiles into LDS: K tile at smem + slot * STAGE, V^T tile right behind it ----
+    // fp16: DMA. Lane slot g of a tile -> (row, chunk), the global chunk the swizzled one; an instruction moves
+    // 256 / KCPR rows on where those are a multiple of the swizzle's period.
+    constexpr bool KSEP = 256 % KCPR == 0 && (256 / KCPR) % 16 == 0;
+    constexpr int KN = KSEP ? 1 : CF::KINS;
+    [[maybe_unused]] uint32_t kvo[KN], vvo = 0, kstep = 0, vstep = 0;
+    [[maybe_unused]] int vkey = 0;
+    [[maybe_unused]] const _Float16 *Kh = nullptr, *Vh = nullptr;
+    if constexpr (!C4) {
+#pragma unroll
+        for (int i = 0; i < KN; i++) {
+            const int g = (i * NW + wave) * 64 + lane, row = g / KCPR, lc = (g % KCPR) ^ CF::kx(row);
+            kvo[i] = lc * 8 < a.dk ? (uint32_t)(row * a.dk + lc * 8) * 2u : kOOB;
+        }
+        const int g = wave * 64 + lane, row = g >> 3, lc = (g & 7) ^ vx(row);
+        vvo = (uint32_t)((long)row * a.stride + lc * 8) * 2u;
+        vkey = lc * 8;
+        kstep = (uint32_t)((256 / KCPR) * a.dk * 2);
+        vstep = (uint32_t)(32 * a.stride * 2);
+        Kh = a.Kf + (size_t)hk * a.k_hs;
+        Vh = a.Vf + (size_t)hk * a.dv * a.stride;
+    }
+    auto dma_k = [&](int kb, int slot) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const int k0 = key_of(kb);
+        const Rsrc rk = rsrc(Kh + (size_t)k0 * a.dk, (uint32_t)((long)max(n - k0, 0) * a.dk * 2));
+        char *ks = smem + slot * CF::STAGE;
+#pragma unroll
+        for (int i = 0; i < CF::KINS; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void *)(ks + (i * NW + wave) * 1024), 16,
+                                                     KSEP ? kvo[0] + i * kstep : kvo[i < KN ? i : 0], 0, 0, 0);
+#else
+        (void)kb; (void)slot;
+#endif
+    };
+    auto dma_v = [&](int kb, int slot) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const int k0 = key_of(kb);
+        const Rsrc rv = rsrc(Vh + k0, (uint32_t)((long)a.dv * a.stride * 2 - (long)k0 * 2));
+        char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+        const uint32_t past = k0 + vkey < a.stride ? 0u : kOOB;   // past a row's end lies the next row
+#pragma unroll
+        for (int i = 0; i < CF::VINS; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void *)(vs + (i * NW + wave) * 1024), 16,
+                                                     (vvo + i * vstep) | past, 0, 0, 0);
+#else
+        (void)kb; (void)slot;
+#endif
+    };
+    // 4-bit: a thread's runs of codes. Keys: key tid / 4, words 4 g + i of run g (D 64: 2 (tid % 4) + i). Values: block
+    // tid % 8 of eight keys, VD nibbles of word w.
+    [[maybe_unused]] int kw[CF::ITEMS][CF::KW] = {};
+    [[maybe_unused]] f16x2 ksm[CF::ITEMS] = {};
+    [[maybe_unused]] i32x4 vw[CF::ITEMS][2] = {}, vsm[CF::ITEMS][2] = {};
+    [[maybe_unused]] int vp[CF::ITEMS][4] = {};           // pairs of keys, the thread's nibbles lowest
+    [[maybe_unused]] f16x2 vsc[CF::ITEMS][4] = {}, vmi[CF::ITEMS][4] = {};
+    [[maybe_unused]] const int vpart = D == 64 ? (tid >> 3) & 3 : (tid >> 3) & 1, vword = D == 64 ? tid >> 5 : tid >> 4;
+    [[maybe_unused]] const size_t hr = C4 ? (size_t)s * a.c.heads + hk : 0;
+    auto load_k = [&](int kb) __attribute__((always_inline)) {
+        const size_t row = hr * a.c.cap + key_of(kb) + (tid >> 2);
+        if (key_of(kb) + (tid >> 2) >= a.c.cap) return;   // (a tile may end 32 keys past the capacity's end)
+#pragma unroll
+        for (int i = 0; i < CF::ITEMS; i++) {
+            const int p = tid & 3, d = D == 64 ? 16 * p : 32 * (p + 4 * i);
+            if (d >= a.dk) continue;
+            const char *src = a.c.kc + row * (a.dk / 2) + d / 2;
+            if constexpr (D == 64) {
+                const i32x2 x = *reinterpret_cast<const i32x2 *>(src);
+                kw[i][0] = x[0];
+                kw[i][1] = x[1];
+            } else {
+                const i32x4 x = *reinterpret_cast<const i32x4 *>(src);
+#pragma unroll
+                for (int e = 0; e < 4; e++) kw[i][e] = x[e];
+            }
+            ksm[i] = *reinterpret_cast<const f16x2 *>(a.c.ks + row * (a.dk / 8) + d / 32 * 4);
+        }
+    };
+    auto load_v = [&](int kb) __attribute__((always_inline)) {
+        const int key = key_of(kb) + 8 * (tid & 7);
+        if (key >= a.c.cap) return;
+        const size_t block = hr * (a.c.cap / 8) + key / 8;
+#pragma unroll
+        for (int i = 0; i < CF::ITEMS; i++) {
+            const int w = vword + 16 * i;
+            if (8 * w >= a.dv) continue;
+            const char *p = a.c.vc + (block * (a.dv / 8) + w) * 32, *m = a.c.vs + (block * (a.dv / 32) + w / 4) * 32;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                vw[i][e] = *reinterpret_cast<const i32x4 *>(p + 16 * e);
+                vsm[i][e] = *reinterpret_cast<const i32x4 *>(m + 16 * e);
+            }
+        }
+    };
+    // unit u of a thread's key words: eight dims of its key, one 16-byte write
+    auto put_k = [&](int slot, int u) __attribute__((always_inline)) {
+        const int i = u / CF::KW, w = u % CF::KW, key = tid >> 2;
+        const int chunk = D == 64 ? 2 * (tid & 3) + w : 4 * ((tid & 3) + 4 * i) + w;
+        const f16x2 sc = {ksm[i][0], ksm[i][0]}, mi = {ksm[i][1], ksm[i][1]};
+        f16x8 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const f16x2 y = widen2(kw[i][w] >> (4 * e), sc, mi);
+            x[2 * e] = y[0];
+            x[2 * e + 1] = y[1];
+        }
+        *reinterpret_cast<f16x8 *>(smem + slot * CF::STAGE + key * (D * 2) + ((chunk ^ CF::kx(key)) << 4)) = x;
+    };
+    // pairs of keys of the thread's value words; keys that no row sees get scale and minimum 0
+    auto pair_v = [&](int kb) __attribute__((always_inline)) {
+        const int key0 = key_of(kb);
+        if (!whole(key0)) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (dead(key0 + 8 * (tid & 7) + e))
+#pragma unroll
+                    for (int i = 0; i < CF::ITEMS; i++) vsm[i][e >> 2][e & 3] = 0;
+        }
+        const unsigned half = D == 64 ? vpart >> 1 : vpart;
+        const unsigned sel = half ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int i = 0; i < CF::ITEMS; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const unsigned w0 = vw[i][k >> 1][2 * (k & 1)], w1 = vw[i][k >> 1][2 * (k & 1) + 1];
+                const unsigned s0 = vsm[i][k >> 1][2 * (k & 1)], s1 = vsm[i][k >> 1][2 * (k & 1) + 1];
+                vp[i][k] = (int)__builtin_amdgcn_perm(w1, w0, sel) >> (D == 64 ? 8 * (vpart & 1) : 0);
+                vsc[i][k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
+                vmi[i][k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
+            }
+    };
+    // unit u: eight keys of one dim, one 16-byte write
+    auto put_v = [&](int slot, int u) __attribute__((always_inline)) {
+        const int i = u / CF::VD, j = u % CF::VD, d = 8 * (vword + 16 * i) + CF::VD * vpart + j;
+        f16x8 x;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const f16x2 y = widen2(vp[i][k] >> (4 * j), vsc[i][k], vmi[i][k]);
+            x[2 * k] = y[0];
+            x[2 * k + 1] = y[1];
+        }
+        *reinterpret_cast<f16x8 *>(smem + slot * CF::STAGE + CF::KBYTES + d * 128 + (((tid & 7) ^ vx(d)) << 4)) = x;
+    };
+
+    float m_run = -1e30f, l_run = 0.f;   // (finite: a row may see nothing of a tile)
+    f32x16 O[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++) O[d] = f32x16{};
+
+    // S^T for the 64 keys of the K tile in slot `slot`: two 32-key blocks; fragments are read two steps ahead
+    auto qk = [&](int slot, f32x16 (&Sx)[2], auto &&beside) __attribute__((always_inline)) {
+        const char *ks = smem + slot * CF::STAGE;
+        Sx[0] = f32x16{};
+        Sx[1] = f32x16{};
+        auto kfrag = [&](int c, int sb) __attribute__((always_inline)) {
+            const int row = 32 * sb + l32, lc = 2 * c + hh;
+            return *reinterpret_cast<const f16x8 *>(ks + row * (D * 2) + ((lc ^ CF::kx(row)) << 4));
+        };
+        f16x8 kf[3][2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            kf[c][0] = kfrag(c, 0);
+            kf[c][1] = kfrag(c, 1);
+        }
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            if (c + 2 < KC) {
+                kf[(c + 2) % 3][0] = kfrag(c + 2, 0);
+                kf[(c + 2) % 3][1] = kfrag(c + 2, 1);
+            }
+#pragma unroll
+            for (int sb = 0; sb < 2; sb++) {
+                Sx[sb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c % 3][sb], qf[c], Sx[sb], 0, 0, 0);
+                beside(2 * c + sb);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    // scores in log2 units, so that p = 2^(v - m) is one v_exp_f32
+    auto transform1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
+        constexpr float L2E = 1.4426950408889634f;
+        const float v = Sx[e >> 4][e & 15];
+        if constexpr (CAP) Sx[e >> 4][e & 15] = a.softcap * tanhf(v * a.scale / a.softcap) * L2E;
+        else Sx[e >> 4][e & 15] = v * (a.scale * L2E);
+    };
+    auto finish = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
+        const int key0 = key_of(kb);
+        if (!whole(key0)) {
+#pragma unroll
+            for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (!sees(key0 + 32 * sb + 8 * (e >> 2) + 4 * hh + (e & 3))) Sx[sb][e] = -INFINITY;
+        }
+        float mloc = -INFINITY;
+#pragma unroll
+        for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) mloc = fmaxf(mloc, Sx[sb][e]);
+        return fmaxf(mloc, __shfl_xor(mloc, 32, 64));
+    };
+    // the running maximum moves when some row's scores pass it by more than 8 (11.5 in log2 units: p stays far inside
+    // fp16); the division by the sum makes the result independent of it
+    auto grow = [&](float mloc) __attribute__((always_inline)) {
+        float alpha = 1.f;
+        if (__builtin_expect(__any(mloc > m_run + 11.5f), 0)) {
+            const float m_new = fmaxf(m_run, mloc);
+            alpha = exp2f(m_run - m_new);
+            m_run = m_new;
+#pragma unroll
+            for (int d = 0; d < DB; d++) O[d] *= alpha;
+        }
+        return alpha;
+    };
+    auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float &psum, int e) __attribute__((always_inline)) {
+        const int sb = e >> 4, i = e & 15;
+        const float p = __builtin_amdgcn_exp2f(Sx[sb][i] - m_run);
+        psum += p;
+        pb[sb][i >> 3][i & 7] = (_Float16)p;
+    };
+    // P to natural key order: of 16 keys, half-wave 0 holds 0-3 and 8-11 and takes 0-7
+    auto reorder = [&](f16x8 (&pb)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                i32x4 w = __builtin_bit_cast(i32x4, pb[sb][t]);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const auto x = __builtin_amdgcn_permlane32_swap((unsigned)w[e], (unsigned)w[2 + e], false, false);
+                    w[e] = (int)x[0];
+                    w[2 + e] = (int)x[1];
+                }
+                pb[sb][t] = __builtin_bit_cast(f16x8, w);
+            }
+    };
+    // O^T += V^T P^T for the V^T tile in slot `slot`
+    auto pv = [&](int slot, const f16x8 (&pb)[2][2], auto &&beside) __attribute__((always_inline)) {
+        const char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+        auto vfrag = [&](int j, int db) __attribute__((always_inline)) {   // keys 16 j + 8 hh .. + 8
+            const int d = 32 * db + l32;
+            return *reinterpret_cast<const f16x8 *>(vs + d * 128 + (((2 * j + hh) ^ vx(d)) << 4));
+        };
+        f16x8 vf[2][DB];
+#pragma unroll
+        for (int db = 0; db < DB; db++) vf[0][db] = vfrag(0, db);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                if (j + 1 < 4) vf[(j + 1) & 1][db] = vfrag(j + 1, db);
+                O[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j & 1][db], pb[j >> 1][j & 1], O[db], 0, 0, 0);
+                beside(j * DB + db);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    // fp16 values of a tile that is not seen whole, before its products (0 times an infinity or a NaN would reach rows
+    // that do not see its key): dead keys become 0; where a key that some rows see holds a non-finite value, the rows
+    // that see it take it here, and the products take 0.
+    auto clean_v = [&](int kb, int slot) __attribute__((always_inline)) {
+        if constexpr (!C4) {
+            const int key0 = key_of(kb);
+            if (whole(key0)) return;
+            char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+            auto each = [&](bool finite) __attribute__((always_inline)) {
+                bool bad = false;
+                for (int g = tid; g < D * 8; g += 256) {
+                    const int d = g >> 3, key = key0 + 8 * ((g & 7) ^ vx(d));
+                    i32x4 *const p = reinterpret_cast<i32x4 *>(vs + g * 16);
+                    i32x4 x = *p;
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int m = 0xFFFF << (16 * (e & 1)), inf = 0x7C00 << (16 * (e & 1));
+                        const bool out = dead(key + e), nf = (x[e >> 1] & inf) == inf;
+                        bad |= nf && !out;
+                        if (out || (finite && nf)) {
+                            x[e >> 1] &= ~m;
+                            any = true;
+                        }
+                    }
+                    if (any) *p = x;
+                }
+                return bad;
+            };
+            if (each(false)) *bad_tile = kb;
+            lds_barrier();
+            if (__builtin_expect(*bad_tile == kb, 0)) {
+#pragma unroll 1
+                for (int i = 0; i < DB * 16; i++) {   // (rolled, and the register picked by comparison: this is rare)
+                    const int d = 32 * (i >> 4) + 8 * (i >> 2 & 3) + 4 * hh + (i & 3);
+                    float x = 0.f;
+#pragma unroll 1
+                    for (int j = 0; j < BK; j++) {
+                        const int w = *reinterpret_cast<const uint16_t *>(vs + d * 128 + (((j >> 3) ^ vx(d)) << 4) + 2 * (j & 7));
+                        if ((w & 0x7C00) == 0x7C00 && sees(key0 + j)) x += (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+                    }
+#pragma unroll
+                    for (int db = 0; db < DB; db++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) O[db][e] = i == 16 * db + e ? O[db][e] + x : O[db][e];
+                }
+                lds_barrier();
+                each(true);
+                lds_barrier();
+            }
+        }
+    };
+
+    // One iteration (kb): PV of tile kb - 1, scores of tile kb finished, QK of tile kb + 1. K tile kb + 2 goes into the K
+    // slot that tile kb left, V^T tile kb into the V^T slot that tile kb - 2 left; both are read an iteration on.
+    constexpr int QKM = 2 * KC, PVM = 4 * DB;
+    auto none = [](int) {};
+    f32x16 S[2];
+    f16x8 P[2][2];
+    float psum = 0.f;
+    if (kb0 < kb1) {
+        if constexpr (C4) {
+            load_k(kb0);
+#pragma unroll
+            for (int u = 0; u < CF::KU; u++) put_k(0, u);
+            if (kb0 + 1 < kb1) {
+                load_k(kb0 + 1);
+#pragma unroll
+                for (int u = 0; u < CF::KU; u++) put_k(1, u);
+            }
+            if (kb0 + 2 < kb1) load_k(kb0 + 2);
+            load_v(kb0);
+        } else {
+            if (tid == 0) *bad_tile = -1;
+            dma_k(kb0, 0);
+            wait_vm0();
+        }
+        lds_barrier();
+        if constexpr (!C4) {
+            if (kb0 + 1 < kb1) dma_k(kb0 + 1, 1);
+        }
+        qk(0, S, none);
+        auto body = [&](auto FIRST, auto LAST, int kb) __attribute__((always_inline)) {
+            const int cur = (kb - kb0) & 1;
+            if constexpr (!C4) wait_vm0();
+            lds_barrier();
+            if constexpr (C4) {
+                pair_v(kb);
+                if (!decltype(LAST)::value) load_v(kb + 1);
+            } else {
+                if (kb + 2 < kb1) dma_k(kb + 2, cur);
+                dma_v(kb, cur);
+            }
+            if constexpr (decltype(FIRST)::value) {
+#pragma unroll
+                for (int e = 0; e < 32; e++) transform1(S, e);
+                if constexpr (C4) {
+#pragma unroll
+                    for (int u = 0; u < CF::VU; u++) put_v(cur, u);
+                }
+            } else {
+                clean_v(kb - 1, cur ^ 1);
+                pv(cur ^ 1, P, [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = m * 32 / PVM; e < (m + 1) * 32 / PVM; e++) transform1(S, e);
+                    if constexpr (C4) {
+#pragma unroll
+                        for (int u = m * CF::VU / PVM; u < (m + 1) * CF::VU / PVM; u++) put_v(cur, u);
+                    }
+                });
+            }
+            const float alpha = grow(finish(kb, S));
+            psum = 0.f;
+            if constexpr (decltype(LAST)::value) {
+#pragma unroll
+                for (int e = 0; e < 32; e++) prob1(S, P, psum, e);
+            } else {
+                const bool ahead = kb + 2 < kb1;
+                f32x16 Sn[2];
+                qk(cur ^ 1, Sn, [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = m * 32 / QKM; e < (m + 1) * 32 / QKM; e++) prob1(S, P, psum, e);
+                    if constexpr (C4) {
+                        if (ahead) {
+#pragma unroll
+                            for (int u = m * CF::KU / QKM; u < (m + 1) * CF::KU / QKM; u++) put_k(cur, u);
+                        }
+                    }
+                });
+                if constexpr (C4) {
+                    if (kb + 3 < kb1) load_k(kb + 3);
+                }
+                S[0] = Sn[0];
+                S[1] = Sn[1];
+            }
+            reorder(P);
+            l_run = l_run * alpha + psum;
+        };
+        using T_ = std::true_type;
+        using F_ = std::false_type;
+        if (kb1 - kb0 == 1) {
+            body(T_{}, T_{}, kb0);
+        } else {
+            body(T_{}, F_{}, kb0);
+#pragma unroll 1
+            for (int kb = kb0 + 1; kb < kb1 - 1; kb++) body(F_{}, F_{}, kb);
+            body(F_{}, T_{}, kb1 - 1);
+        }
+        if constexpr (!C4) wait_vm0();
+        lds_barrier();
+        clean_v(kb1 - 1, (kb1 - 1 - kb0) & 1);
+        pv((kb1 - 1 - kb0) & 1, P, none);
+    }
+
+    // lane holds dims 32 db + 8 b + 4 hh + c of its row
+    const float l = l_run + __shfl_xor(l_run, 32, 64);
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing; NaN stays)
+    if (!qok) return;
+    const size_t rows = (size_t)a.n_seq * a.n_head * T;
+    _Float16 *orow;
+    if (ta.nsplit > 1) {
+        orow = static_cast<_Float16 *>(ta.part) + (zs * rows + row0 + r) * a.dv;
+        if (hh == 0) {
+            float *pml = reinterpret_cast<float *>(static_cast<_Float16 *>(ta.part) + ta.nsplit * rows * a.dv) + 2 * (zs * rows + row0 + r);
+            pml[0] = m_run;
+            pml[1] = l;
+        }
+    } else {
+        orow = a.out + (row0 + r) * a.dv;
+    }
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const int d0 = 32 * db + 8 * b + 4 * hh;
+            if (d0 < a.dv) {
+                f16x4 v;
+#pragma unroll
+                for (int c = 0; c < 4; c++) v[c] = (_Float16)(O[db][4 * b + c] * inv);
+                *reinterpret_cast<f16x4 *>(orow + d0) = v;
+            }
+        }
+}
+
+template <int D, bool C4, bool CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
+{
+    auto kern = k_serve_tiles<D, C4, CAP>;
+    static_assert(Cfg<D>::LDS <= 160 * 1024, "LDS budget");
+    static std::atomic<uint64_t> opted{0};
+    if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), Cfg<D>::LDS, opted)) return e;
+    hipLaunchKernelGGL(kern, dim3(wgs), dim3(256), Cfg<D>::LDS, s, ta);
+    return hipGetLastError();
+}
+template <int D> hipError_t launch(const TileArgs &ta, unsigned wgs, hipStream_t s)
+{
+    const bool cap = ta.a.softcap != 0.f;
+    if (ta.a.Kf) return cap ? launch_c<D, false, true>(ta, wgs, s) : launch_c<D, false, false>(ta, wgs, s);
+    return cap ? launch_c<D, true, true>(ta, wgs, s) : launch_c<D, true, false>(ta, wgs, s);
+}
+
+long row_blocks(const ServeAttn &a) { return ((long)a.gqa * a.n_tokens + BQ - 1) / BQ; }
+
+int splits(const ServeAttn &a)
+{
+    // enough workgroups for every CU (256), each split keeping at least 4 of the tiles that a block may see
+    const long wgs = row_blocks(a) * (a.n_head / a.gqa) * a.n_seq;
+    long tiles = (a.max_kv + BK - 1) / BK;
+    if (a.window) tiles = std::min<long>(tiles, (std::min(a.sinks, a.max_kv) + BK - 1) / BK + ((long)std::min(a.n_tokens, BQ) + a.window - 2) / BK + 2);
+    return (int)std::max<long>(1, std::min<long>({(256 + wgs - 1) / wgs, tiles / 4, 16}));
+}
+
+}  // namespace
+
+size_t serve_tiles_ws(const ServeAttn &a)
+{
+    const int ns = splits(a);
+    return ns > 1 ? (size_t)ns * a.n_seq * a.n_head * a.n_tokens * (a.dv * sizeof(_Float16) + 2 * sizeof(float)) : 0;
+}
+
+hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
+{
+    TileArgs ta;
+    ta.a = a;
+    ta.nsplit = a.ws && a.ws_bytes >= serve_tiles_ws(a) ? splits(a) : 1;
+    ta.part = a.ws;
+    const long nqb = row_blocks(a), wgs = nqb * (a.n_head / a.gqa) * a.n_seq * ta.nsplit;
+    if (wgs > 0x7FFFFFFFL) return hipErrorInvalidValue;
+    ta.nqb = (int)nqb;
+    const int d = std::max(a.dk, a.dv);
+    const hipError_t e = d <= 64 ? launch<64>(ta, (unsigned)wgs, s) : d <= 128 ? launch<128>(ta, (unsigned)wgs, s) : launch<256>(ta, (unsigned)wgs, s);
+    *blocks = (uint64_t)wgs;
+    if (e != hipSuccess || ta.nsplit == 1) return e;
+    uint64_t more = 0;
+    const int rows = a.n_seq * a.n_head * a.n_tokens;
+    const hipError_t e2 = flash_attn_combine(ta.part, a.out, 0, a.dv, 1, rows, a.dv, ta.nsplit, s, &more);
+    *blocks += more;
+    return e2;
+}
+
+}  // namespace rk
