@@ -21,6 +21,10 @@ struct FaLaunch {
     long q_hs = 0, q_rs = 0, k_hs = 0, k_rs = 0, v_hs = 0, v_rs = 0, o_hs = 0, o_rs = 0, m_rs = 0;
     int T = 0, n_kv = 0, dk = 0, dv = 0, n_head = 0, gqa = 1;
     float scale = 1.f, softcap = 0.f;
+    // few rows only: in place of the mask and the clamp, token t sees the keys up to its own position (n_kv - T +
+    // t) that lie in its window (0: all) or below sinks
+    bool win = false;
+    int window = 0, sinks = 0;
     // workspace for key-axis splits (flash_attn_ws_bytes); without it one workgroup walks
     // every key of its queries
     float *ws = nullptr;

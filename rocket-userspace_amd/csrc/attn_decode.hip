@@ -22,6 +22,7 @@
 //   8 x 3000 keys, 16 / 8 heads of 256    33.5 -> 14.2     (with a mask)
 #include "attn.h"
 #include "lds_optin.h"
+#include "softcap.h"
 
 #include <algorithm>
 #include <atomic>
@@ -58,6 +59,9 @@ struct RowArgs {
     float scale, softcap;
     int nsplit, cps;   // workgroups a KV head, chunks a workgroup
     float *part;       // [split][head][T][dv] outputs, then [split][head][T] (max, sum)
+    // WIN: the chunks that some token sees, v -> v below ns, v + skip from there on, count of them; keys
+    // [sinks, first) are seen by none
+    int window, sinks, first, ns, skip, count;
 };
 
 // Halves key .. key + 8 of a row of n (n >= 8), zeros past the row: the last eight are loaded
@@ -135,8 +139,10 @@ __global__ __launch_bounds__(256) void k_fa_merge(const float *__restrict__ part
 }
 
 // D: head sizes up to this (64, 128, 256); dk a multiple of 32, dv of 16. FULL: both are D, so
-// that no load or product carries a test of its dims.
-template <int D, bool CAP, bool FULL>
+// that no load or product carries a test of its dims. WIN: token t sees the keys up to its own, n_kv - T + t, that
+// lie in its window or among the sinks; no mask and no clamp. There a row may see nothing of a chunk (a
+// finite first maximum), and values of keys that a row does not see must not reach it as 0 times an infinity.
+template <int D, bool CAP, bool FULL, bool WIN>
 __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 {
     constexpr int KS = D / 32, VB = D / 16, LROW = D + 4;   // score steps, output blocks, LDS row (floats)
@@ -157,7 +163,12 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
     }
     const Rsrc rk = rsrc(a.K + (size_t)hk * a.k_hs, (uint32_t)((long)a.n_kv * a.k_rs * 2));   // keys past n_kv: zeros
     const _Float16 *const Vh = a.Vt + (size_t)hk * a.v_hs + (size_t)c * a.v_rs;              // rows 16 j + c
-    const _Float16 *const mrow = a.mask ? a.mask + (size_t)t * a.m_rs : nullptr;
+    const _Float16 *const mrow = !WIN && a.mask ? a.mask + (size_t)t * a.m_rs : nullptr;
+    const int pos = a.n_kv - a.T + t;
+    auto key_of = [&](int ch) __attribute__((always_inline)) { return (WIN && ch >= a.ns ? ch + a.skip : ch) * kChunk; };
+    // (no short circuits: a branch a score takes longer, and the compiler lost a lane's mask among them)
+    const int behind = a.window ? pos - a.window : -1;   // the last key behind the token's window
+    auto sees = [&](int key) __attribute__((always_inline)) { return (bool)((key <= pos) & ((key > behind) | (key < a.sinks))); };
 
     i32x4 kf[2][KS], vf[VB];
     const uint32_t ko = (uint32_t)((8 * (c >> 2) + (c & 3)) * a.k_rs + 8 * q) * 2u, k4 = (uint32_t)(4 * a.k_rs) * 2u;
@@ -183,19 +194,19 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
         }
     };
 
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run = WIN ? -1e30f : -INFINITY, l_run = 0.f;
     f32x4 O[VB];
 #pragma unroll
     for (int j = 0; j < VB; j++) O[j] = f32x4{};
-    const int chunks = (a.n_kv + kChunk - 1) / kChunk;
+    const int chunks = WIN ? a.count : (a.n_kv + kChunk - 1) / kChunk;
     const int c1 = min(chunks, (zs + 1) * a.cps);
     int ch = zs * a.cps + wave;
     if (ch < c1) {
-        load_k(ch * kChunk);
-        load_v(ch * kChunk);
+        load_k(key_of(ch));
+        load_v(key_of(ch));
     }
     for (; ch < c1; ch += kWaves) {
-        const int key0 = ch * kChunk;
+        const int key0 = key_of(ch);
         f32x4 S[2] = {};
 #pragma unroll
         for (int s = 0; s < KS; s++)
@@ -206,7 +217,10 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
                                                                   S[b], 0, 0, 0);
             }
         const bool more = ch + kWaves < c1;
-        if (more) load_k(key0 + kWaves * kChunk);
+        const int next = WIN ? key_of(more ? ch + kWaves : ch) : key0 + kWaves * kChunk;
+        if (more) load_k(next);
+        // every row sees every key of the chunk (uniform)
+        [[maybe_unused]] const bool whole = key0 + kChunk <= a.n_kv - a.T + 1 && (!a.window || key0 > a.n_kv - 1 - a.window || key0 + kChunk <= a.sinks);
         // the reference's score steps in log2 units; lane holds keys key0 + 8 q + 4 b + e
         i32x4 mw = {0, 0, 0, 0};
         if (mrow) mw = row8(mrow, key0 + 8 * q, a.n_kv);
@@ -215,19 +229,73 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float x = S[i >> 2][i & 3];
-            if constexpr (CAP) v[i] = fmaxf(a.softcap * tanhf(x * a.scale / a.softcap) + (float)mv[i], -30000.f) * kLog2e;
+            if constexpr (WIN) v[i] = CAP ? softcap_log2(x, a.scale, a.softcap) : x * (a.scale * kLog2e);
+            else if constexpr (CAP) v[i] = fmaxf(a.softcap * tanhf(x * a.scale / a.softcap) + (float)mv[i], -30000.f) * kLog2e;
             else v[i] = fmaxf(fmaf((float)mv[i], kLog2e, x * (a.scale * kLog2e)), -30000.f * kLog2e);
-            if (key0 + 8 * q + i >= a.n_kv) v[i] = -INFINITY;   // weighs 0
-            mx = fmaxf(mx, v[i]);
+            if constexpr (!WIN) {
+                if (key0 + 8 * q + i >= a.n_kv) v[i] = -INFINITY;   // weighs 0
+                mx = fmaxf(mx, v[i]);
+            }
+        }
+        if constexpr (WIN) {
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = sees(key0 + 8 * q + i) ? v[i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (__any(mx > m_run)) {   // (a chunk has a key below n_kv, so the new maximum is finite)
+        if (__any(mx > m_run)) {   // (a chunk has a key below n_kv, so without a window the new maximum is finite)
             const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= alpha;
 #pragma unroll
             for (int j = 0; j < VB; j++) O[j] *= alpha;
+        }
+        if constexpr (WIN) {
+            if (!whole) {
+                // keys that no row sees: their values count as 0
+                i32x4 live = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int key = key0 + 8 * q + i;
+                    if (key < a.n_kv && !(key < a.first && key >= a.sinks)) live[i >> 1] |= 0xFFFF << (16 * (i & 1));
+                }
+#pragma unroll
+                for (int j = 0; j < VB; j++) vf[j] &= live;
+                // a non-finite value of a key that some rows see: those take it here, the products take 0
+                if (a.T > 1) {
+                    bool bad = false;
+#pragma unroll
+                    for (int j = 0; j < VB; j++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) bad |= (vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
+                    if (__builtin_expect(__any(bad), 0)) {
+                        const uint16_t *const vr = reinterpret_cast<const uint16_t *>(a.Vt + (size_t)hk * a.v_hs);
+#pragma unroll 1
+                        for (int i = 0; i < VB * 4; i++) {   // (rolled, and the register picked by comparison: this is rare)
+                            const int d = 16 * (i >> 2) + 4 * q + (i & 3);
+                            float x = 0.f;
+#pragma unroll 1
+                            for (int j = 0; d < a.dv && j < kChunk && key0 + j < a.n_kv; j++) {
+                                const uint16_t w = vr[(size_t)d * a.v_rs + key0 + j];
+                                if ((w & 0x7C00) == 0x7C00 && sees(key0 + j)) x += (float)__builtin_bit_cast(_Float16, w);
+                            }
+#pragma unroll
+                            for (int j = 0; j < VB; j++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) O[j][e] = i == 4 * j + e ? O[j][e] + x : O[j][e];
+                        }
+#pragma unroll
+                        for (int j = 0; j < VB; j++)
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                if ((vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00) vf[j][i >> 1] &= 0xFFFF << (16 * (~i & 1));
+                    }
+                }
+            }
         }
         f16x8 p;
 #pragma unroll
@@ -239,7 +307,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 #pragma unroll
         for (int j = 0; j < VB; j++)
             if (FULL || 16 * j < a.dv) O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vf[j]), p, O[j], 0, 0, 0);
-        if (more) load_v(key0 + kWaves * kChunk);
+        if (more) load_v(next);
     }
     l_run += __shfl_xor(l_run, 16, 64);
     l_run += __shfl_xor(l_run, 32, 64);
@@ -285,9 +353,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
     }
 }
 
-template <int D, bool CAP, bool FULL> hipError_t launch_rows_f(const RowArgs &a, int kv_heads, hipStream_t s)
+template <int D, bool CAP, bool FULL, bool WIN> hipError_t launch_rows_f(const RowArgs &a, int kv_heads, hipStream_t s)
 {
-    auto kern = k_fa_rows<D, CAP, FULL>;
+    auto kern = k_fa_rows<D, CAP, FULL, WIN>;
     const int R = a.gqa * a.T;
     const size_t lds = (size_t)kWaves * R * ((D + 4) * 4 + 8);
     if (lds > 64 * 1024) {
@@ -298,11 +366,30 @@ template <int D, bool CAP, bool FULL> hipError_t launch_rows_f(const RowArgs &a,
     return hipGetLastError();
 }
 
-template <int D> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
+template <int D, bool WIN> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
 {
     const bool cap = a.softcap != 0.f;
-    if (a.dk == D && a.dv == D) return cap ? launch_rows_f<D, true, true>(a, kv_heads, s) : launch_rows_f<D, false, true>(a, kv_heads, s);
-    return cap ? launch_rows_f<D, true, false>(a, kv_heads, s) : launch_rows_f<D, false, false>(a, kv_heads, s);
+    if (a.dk == D && a.dv == D)
+        return cap ? launch_rows_f<D, true, true, WIN>(a, kv_heads, s) : launch_rows_f<D, false, true, WIN>(a, kv_heads, s);
+    return cap ? launch_rows_f<D, true, false, WIN>(a, kv_heads, s) : launch_rows_f<D, false, false, WIN>(a, kv_heads, s);
+}
+template <bool WIN> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
+{
+    const int d = std::max(a.dk, a.dv);
+    return d <= 64 ? launch_rows<64, WIN>(a, kv_heads, s) : d <= 128 ? launch_rows<128, WIN>(a, kv_heads, s) : launch_rows<256, WIN>(a, kv_heads, s);
+}
+
+// The chunks to visit: all, or those that some token sees.
+int chunk_list(const FaLaunch &L, RowArgs *a)
+{
+    const int all = (L.n_kv + kChunk - 1) / kChunk;
+    const int first = L.win && L.window ? std::max(0, L.n_kv - L.T - L.window + 1) : 0, sinks = std::min(L.sinks, first);
+    const int ns = (sinks + kChunk - 1) / kChunk, f = std::max(first / kChunk, ns), count = all - (f - ns);
+    if (a) {
+        a->window = L.window; a->sinks = L.sinks; a->first = first;
+        a->ns = ns; a->skip = f - ns; a->count = count;
+    }
+    return count;
 }
 
 // Workgroups a KV head: one chunk a wave while the workgroups stay near three a CU; one workgroup for
@@ -314,7 +401,7 @@ template <int D> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStrea
 // and 12.8, 255 keys 18.8 and 14.6).
 void split_of(const FaLaunch &L, int *nsplit, int *cps)
 {
-    const int kvh = L.n_head / L.gqa, chunks = (L.n_kv + kChunk - 1) / kChunk;
+    const int kvh = L.n_head / L.gqa, chunks = chunk_list(L, nullptr);
     const int d = std::max(L.dk, L.dv), odd = L.n_kv & 1;
     const int whole = d <= 64 ? (odd ? 10 : 16) : d <= 128 ? (odd ? 8 : 10) : odd ? 5 : 8;
     const int n = chunks <= whole ? 1 : std::min({(chunks + kWaves - 1) / kWaves, std::max(1, 768 / kvh), 64});
@@ -327,6 +414,7 @@ void split_of(const FaLaunch &L, int *nsplit, int *cps)
 bool flash_attn_few_rows(const FaLaunch &L)
 {
     if ((long)L.gqa * L.T > kRows || L.n_kv < 8 || L.dk % 32 || L.dv % 16) return false;
+    if (L.win) return true;
     // One query head a KV head and long caches: the tiled kernel reads V^T in whole 128-byte lines (64
     // keys a tile, 32 here), and where its workgroups fill the CUs and nothing has to be padded it is the
     // faster one while the cache is not far larger than the memory-side cache (heads of 256, 16 x 8192
@@ -356,12 +444,12 @@ hipError_t flash_attn_rows(const FaLaunch &L, hipStream_t s, uint64_t *blocks)
     split_of(L, &a.nsplit, &a.cps);
     if (a.nsplit > 1 && (!L.ws || L.ws_bytes < flash_attn_rows_ws(L))) {
         a.nsplit = 1;
-        a.cps = (L.n_kv + kChunk - 1) / kChunk;
+        a.cps = chunk_list(L, nullptr);
     }
+    (void)chunk_list(L, &a);
     a.part = L.ws;
     const int kvh = L.n_head / L.gqa;
-    const int d = std::max(L.dk, L.dv);
-    const hipError_t e = d <= 64 ? launch_rows<64>(a, kvh, s) : d <= 128 ? launch_rows<128>(a, kvh, s) : launch_rows<256>(a, kvh, s);
+    const hipError_t e = L.win ? launch_rows<true>(a, kvh, s) : launch_rows<false>(a, kvh, s);
     if (blocks) *blocks = (uint64_t)kvh * a.nsplit;
     if (e != hipSuccess || a.nsplit == 1) return e;
     const unsigned rows = (unsigned)(L.n_head * L.T);

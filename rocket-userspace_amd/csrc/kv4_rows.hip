@@ -15,6 +15,7 @@
 // less 1024 (exact), times scale plus minimum (one rounding): the values that rocket_kv4_read_fp16 gives.
 #include "lds_optin.h"
 #include "serve.h"
+#include "softcap.h"
 
 #include <algorithm>
 #include <atomic>
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const int hg = c / T, t = c - hg * T;         // this lane's query: head hk gqa + hg, token t
     const bool qok = c < R;
     const int pos = n - T + t;                    // its position
-    const int p_lo = n - T, p_hi = n - 1;
+    const int p_lo = n - T, p_hi = n - 1, behind = a.window ? pos - a.window : -1;   // (the last key behind its window)
 
     const size_t hr = (size_t)s * a.c.heads + hk;
     const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;   // row of the first query
@@ -189,14 +190,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float x = S[i >> 2][i & 3];
-            if constexpr (CAP) v[i] = a.softcap * tanhf(x * a.scale / a.softcap) * kLog2e;
+            if constexpr (CAP) v[i] = softcap_log2(x, a.scale, a.softcap);
             else v[i] = x * (a.scale * kLog2e);
         }
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int key = key0 + 8 * q + i;
-                if (key > pos || (a.window && key <= pos - a.window && key >= a.sinks)) v[i] = -INFINITY;
+                v[i] = (bool)((key <= pos) & ((key > behind) | (key < a.sinks))) ? v[i] : -INFINITY;
             }
             // keys that no row sees: their values count as 0, whatever the memory holds
 #pragma unroll
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int key = key0 + 8 * q + i;
-                    if (key > p_hi || (key < list.first && key >= list.sinks)) vsm[u][i >> 2][i & 3] = 0;
+                    if ((bool)((key > p_hi) | ((key < list.first) & (key >= list.sinks)))) vsm[u][i >> 2][i & 3] = 0;
                 }
         }
 #pragma unroll

@@ -80,6 +80,7 @@ struct ServeAttn {
     float *ws = nullptr;
     size_t ws_bytes = 0;
 };
+bool serve_few_rows(const ServeAttn &a);
 size_t serve_attn_ws(const ServeAttn &a);
 hipError_t serve_attn(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 

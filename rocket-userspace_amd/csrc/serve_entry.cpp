@@ -337,11 +337,11 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
         c.want(K, kb);
         c.want(V, vb);
         c.want(out, ob);
-        // V^T rows that are no whole 16-byte chunks are copied into ones that are
-        const int padded = kv_stride % 8 ? (kv_stride + 63) / 64 * 64 : kv_stride;
+        // V^T rows that are no whole 16-byte chunks are copied into ones that are, for the tiles
+        a.Kf = K;
+        const int padded = kv_stride % 8 && !serve_few_rows(a) ? (kv_stride + 63) / 64 * 64 : kv_stride;
         const size_t pb = padded != kv_stride ? h16((size_t)n_kv_heads * dv * padded) : 0;
         if (pb) c.want_scratch(pb);
-        a.Kf = K;
         const size_t ws = c.want_optional(serve_attn_ws(a), n_kv >= 512);
         if (int rc = c.begin()) return rc;
         a.Q = static_cast<const _Float16 *>(c.in(Q, qb));

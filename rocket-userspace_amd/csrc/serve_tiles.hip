@@ -15,6 +15,7 @@
 #include "attn.h"
 #include "lds_optin.h"
 #include "serve.h"
+#include "softcap.h"
 
 #include <algorithm>
 #include <atomic>
@@ -125,8 +126,9 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
         return key0 + BK - 1 <= p_lo && (!a.window || key0 > p_hi - a.window || key0 + BK <= a.sinks);
     };
     // no row of the block sees the key
-    auto dead = [&](int key) __attribute__((always_inline)) { return key > p_hi || (key < first && key >= sinks); };
-    auto sees = [&](int key) __attribute__((always_inline)) { return key <= pos && (!a.window || key > pos - a.window || key < a.sinks); };
+    auto dead = [&](int key) __attribute__((always_inline)) { return (bool)((key > p_hi) | ((key < first) & (key >= sinks))); };
+    const int behind = a.window ? pos - a.window : -1;   // the last key behind the row's window
+    auto sees = [&](int key) __attribute__((always_inline)) { return (bool)((key <= pos) & ((key > behind) | (key < a.sinks))); };
 
     // the lane's query row as the B operand of the score MFMAs: step c takes dims 16 c + 8 hh .. + 8 (in the order in
     // which widened codes lie)
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
     auto transform1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
         constexpr float L2E = 1.4426950408889634f;
         const float v = Sx[e >> 4][e & 15];
-        if constexpr (CAP) Sx[e >> 4][e & 15] = a.softcap * tanhf(v * a.scale / a.softcap) * L2E;
+        if constexpr (CAP) Sx[e >> 4][e & 15] = softcap_log2(v, a.scale, a.softcap);
         else Sx[e >> 4][e & 15] = v * (a.scale * L2E);
     };
     auto finish = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
             for (int sb = 0; sb < 2; sb++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    if (!sees(key0 + 32 * sb + 8 * (e >> 2) + 4 * hh + (e & 3))) Sx[sb][e] = -INFINITY;
+                    Sx[sb][e] = sees(key0 + 32 * sb + 8 * (e >> 2) + 4 * hh + (e & 3)) ? Sx[sb][e] : -INFINITY;
         }
         float mloc = -INFINITY;
 #pragma unroll
