@@ -19,7 +19,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 namespace rk {
 namespace {
@@ -78,7 +77,7 @@ __device__ __forceinline__ f16x2 widen2(int nibbles, f16x2 s, f16x2 m)
 }
 
 template <int D, bool C4, bool CAP>
-__global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const TileArgs ta)
 {
     const ServeAttn &a = ta.a;
     using CF = Cfg<D>;
@@ -138,7 +137,8 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             f16x8 x = {};
-            if (qok && 16 * c + 8 * hh < a.dk) x = *reinterpret_cast<const f16x8 *>(qrow + 16 * c + 8 * hh);
+            if (qok && 16 * c + 8 * hh < a.dk && a.scale != 0.f) x = *reinterpret_cast<const f16x8 *>(qrow + 16 * c + 8 * hh);
+            if (a.scale < 0.f) x = -x;
             qf[c] = C4 ? __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7) : x;
         }
     }
@@ -321,28 +321,33 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
             }
         }
     };
-    // scores in log2 units, so that p = 2^(v - m) is one v_exp_f32
-    auto transform1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
-        constexpr float L2E = 1.4426950408889634f;
-        const float v = Sx[e >> 4][e & 15];
-        if constexpr (CAP) Sx[e >> 4][e & 15] = softcap_log2(v, a.scale, a.softcap);
-        else Sx[e >> 4][e & 15] = v * (a.scale * L2E);
+    // Soft-capped scores are made in log2 units; the others stay products, and the factor to log2 units joins the
+    // exponential's subtraction (Q carries the scale's sign, so that the largest product is the largest score).
+    // (a scale of 0: Q is 0 and the factor 1, so that hidden keys' -infinity stays one)
+    const float unit = CAP || a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    auto cap1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
+        if constexpr (CAP) Sx[e >> 4][e & 15] = softcap_log2(Sx[e >> 4][e & 15], fabsf(a.scale), a.softcap);
     };
     auto finish = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
         const int key0 = key_of(kb);
         if (!whole(key0)) {
+            // (negative where the row does not see the key: bits, as comparisons became a branch each)
+            const int k0 = key0 + 4 * hh, after = pos - k0, before = k0 - behind - 1, sink = a.sinks - 1 - k0;
 #pragma unroll
             for (int sb = 0; sb < 2; sb++)
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    Sx[sb][e] = sees(key0 + 32 * sb + 8 * (e >> 2) + 4 * hh + (e & 3)) ? Sx[sb][e] : -INFINITY;
+                for (int e = 0; e < 16; e++) {
+                    const int k = 32 * sb + 8 * (e >> 2) + (e & 3);
+                    const int hid = (after - k) | ((before + k) & (sink - k));
+                    Sx[sb][e] = hid < 0 ? -INFINITY : Sx[sb][e];
+                }
         }
         float mloc = -INFINITY;
 #pragma unroll
         for (int sb = 0; sb < 2; sb++)
 #pragma unroll
             for (int e = 0; e < 16; e++) mloc = fmaxf(mloc, Sx[sb][e]);
-        return fmaxf(mloc, __shfl_xor(mloc, 32, 64));
+        return fmaxf(mloc, __shfl_xor(mloc, 32, 64)) * unit;
     };
     // the running maximum moves when some row's scores pass it by more than 8 (11.5 in log2 units: p stays far inside
     // fp16); the division by the sum makes the result independent of it
@@ -359,9 +364,10 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
     };
     auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float &psum, int e) __attribute__((always_inline)) {
         const int sb = e >> 4, i = e & 15;
-        const float p = __builtin_amdgcn_exp2f(Sx[sb][i] - m_run);
-        psum += p;
+        const float p = __builtin_amdgcn_exp2f(fmaf(Sx[sb][i], unit, -m_run));
         pb[sb][i >> 3][i & 7] = (_Float16)p;
+        // the sum of the rounded weights, two at a time, in fp32: weights and their sum round alike
+        if (i & 1) psum = __builtin_amdgcn_fdot2(f16x2{pb[sb][i >> 3][(i & 7) - 1], pb[sb][i >> 3][i & 7]}, f16x2{(_Float16)1.f, (_Float16)1.f}, psum, false);
     };
     // P to natural key order: of 16 keys, half-wave 0 holds 0-3 and 8-11 and takes 0-7
     auto reorder = [&](f16x8 (&pb)[2][2]) __attribute__((always_inline)) {
@@ -452,105 +458,98 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
         }
     };
 
-    // One iteration (kb): PV of tile kb - 1, scores of tile kb finished, QK of tile kb + 1. K tile kb + 2 goes into the K
-    // slot that tile kb left, V^T tile kb into the V^T slot that tile kb - 2 left; both are read an iteration on.
+    // Iteration kb: PV of tile kb - 1 beside the score arithmetic of tile kb, then QK of tile kb + 1 beside the
+    // exponentials of tile kb. K tile kb + 2 goes into the K slot that tile kb left, V^T tile kb into the V^T slot that tile
+    // kb - 2 left; both are read an iteration on. The first iteration (kb0 - 1) has the first QK alone and the last
+    // (kb1) the last PV: one copy of the products' code, since a workgroup runs through few tiles and its first run
+    // through each line of code waits for the instruction cache (peeled first and last iterations took 22 us of a
+    // call's 83 outside its 16 tiles). Codes are loaded a whole iteration before they are widened, keys beside PV and
+    // values beside QK.
     constexpr int QKM = 2 * KC, PVM = 4 * DB;
-    auto none = [](int) {};
-    f32x16 S[2];
-    f16x8 P[2][2];
-    float psum = 0.f;
+    f32x16 S[2] = {};
+    f16x8 P[2][2] = {};
     if (kb0 < kb1) {
         if constexpr (C4) {
             load_k(kb0);
+            load_v(kb0);
 #pragma unroll
             for (int u = 0; u < CF::KU; u++) put_k(0, u);
-            if (kb0 + 1 < kb1) {
-                load_k(kb0 + 1);
-#pragma unroll
-                for (int u = 0; u < CF::KU; u++) put_k(1, u);
-            }
-            if (kb0 + 2 < kb1) load_k(kb0 + 2);
-            load_v(kb0);
+            if (kb0 + 1 < kb1) load_k(kb0 + 1);
         } else {
-            if (tid == 0) *bad_tile = -1;
             dma_k(kb0, 0);
-            wait_vm0();
+            if (tid == 0) *bad_tile = -1;
         }
-        lds_barrier();
-        if constexpr (!C4) {
-            if (kb0 + 1 < kb1) dma_k(kb0 + 1, 1);
-        }
-        qk(0, S, none);
-        auto body = [&](auto FIRST, auto LAST, int kb) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int kb = kb0 - 1;; kb++) {
             const int cur = (kb - kb0) & 1;
+            const bool puts_k = kb + 2 < kb1, tile = kb >= kb0 && kb < kb1;
             if constexpr (!C4) wait_vm0();
             lds_barrier();
-            if constexpr (C4) {
-                pair_v(kb);
-                if (!decltype(LAST)::value) load_v(kb + 1);
-            } else {
-                if (kb + 2 < kb1) dma_k(kb + 2, cur);
-                dma_v(kb, cur);
+            if constexpr (!C4) {
+                if (puts_k) dma_k(kb + 2, cur);
+                if (tile) dma_v(kb, cur);
             }
-            if constexpr (decltype(FIRST)::value) {
-#pragma unroll
-                for (int e = 0; e < 32; e++) transform1(S, e);
-                if constexpr (C4) {
-#pragma unroll
-                    for (int u = 0; u < CF::VU; u++) put_v(cur, u);
-                }
-            } else {
+            if (kb > kb0) {
                 clean_v(kb - 1, cur ^ 1);
                 pv(cur ^ 1, P, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = m * 32 / PVM; e < (m + 1) * 32 / PVM; e++) transform1(S, e);
+                    for (int e = m * 32 / PVM; e < (m + 1) * 32 / PVM; e++) cap1(S, e);
                     if constexpr (C4) {
+                        if (puts_k) {
 #pragma unroll
-                        for (int u = m * CF::VU / PVM; u < (m + 1) * CF::VU / PVM; u++) put_v(cur, u);
+                            for (int u = m * CF::KU / PVM; u < (m + 1) * CF::KU / PVM; u++) put_k(cur, u);
+                        }
                     }
                 });
-            }
-            const float alpha = grow(finish(kb, S));
-            psum = 0.f;
-            if constexpr (decltype(LAST)::value) {
-#pragma unroll
-                for (int e = 0; e < 32; e++) prob1(S, P, psum, e);
+                if (kb == kb1) break;
             } else {
-                const bool ahead = kb + 2 < kb1;
+#pragma unroll
+                for (int e = 0; e < 32; e++) cap1(S, e);
+                if constexpr (C4) {
+                    if (puts_k) {
+#pragma unroll
+                        for (int u = 0; u < CF::KU; u++) put_k(cur, u);
+                    }
+                }
+            }
+            if constexpr (C4) {
+                if (kb + 3 < kb1) load_k(kb + 3);
+            }
+            float alpha = 1.f, psum = 0.f;
+            if (tile) {
+                alpha = grow(finish(kb, S));
+                if constexpr (C4) pair_v(kb);
+            }
+            if (kb + 1 < kb1) {
                 f32x16 Sn[2];
                 qk(cur ^ 1, Sn, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
                     for (int e = m * 32 / QKM; e < (m + 1) * 32 / QKM; e++) prob1(S, P, psum, e);
                     if constexpr (C4) {
-                        if (ahead) {
+                        if (tile) {
 #pragma unroll
-                            for (int u = m * CF::KU / QKM; u < (m + 1) * CF::KU / QKM; u++) put_k(cur, u);
+                            for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(cur, u);
                         }
                     }
                 });
-                if constexpr (C4) {
-                    if (kb + 3 < kb1) load_k(kb + 3);
-                }
                 S[0] = Sn[0];
                 S[1] = Sn[1];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e++) prob1(S, P, psum, e);
+                if constexpr (C4) {
+#pragma unroll
+                    for (int u = 0; u < CF::VU; u++) put_v(cur, u);
+                }
             }
-            reorder(P);
-            l_run = l_run * alpha + psum;
-        };
-        using T_ = std::true_type;
-        using F_ = std::false_type;
-        if (kb1 - kb0 == 1) {
-            body(T_{}, T_{}, kb0);
-        } else {
-            body(T_{}, F_{}, kb0);
-#pragma unroll 1
-            for (int kb = kb0 + 1; kb < kb1 - 1; kb++) body(F_{}, F_{}, kb);
-            body(F_{}, T_{}, kb1 - 1);
+            if (tile) {
+                reorder(P);
+                l_run = l_run * alpha + psum;
+                if constexpr (C4) {
+                    if (kb + 1 < kb1) load_v(kb + 1);
+                }
+            }
         }
-        if constexpr (!C4) wait_vm0();
-        lds_barrier();
-        clean_v(kb1 - 1, (kb1 - 1 - kb0) & 1);
-        pv((kb1 - 1 - kb0) & 1, P, none);
     }
 
     // lane holds dims 32 db + 8 b + 4 hh + c of its row
@@ -574,7 +573,7 @@ __global__ __launch_bounds__(256) void k_serve_tiles(const TileArgs ta)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             const int d0 = 32 * db + 8 * b + 4 * hh;
-            if (d0 < a.dv) {
+            if (32 * db + 8 * b < a.dv) {   // (dv is a multiple of 16: the same for both half-waves)
                 f16x4 v;
 #pragma unroll
                 for (int c = 0; c < 4; c++) v[c] = (_Float16)(O[db][4 * b + c] * inv);
@@ -603,11 +602,11 @@ long row_blocks(const ServeAttn &a) { return ((long)a.gqa * a.n_tokens + BQ - 1)
 
 int splits(const ServeAttn &a)
 {
-    // enough workgroups for every CU (256), each split keeping at least 4 of the tiles that a block may see
-    const long wgs = row_blocks(a) * (a.n_head / a.gqa) * a.n_seq;
+    // enough workgroups for every CU (256; heads of up to 128 run two on one), each split keeping at least 4 of the tiles that a block may see
+    const long wgs = row_blocks(a) * (a.n_head / a.gqa) * a.n_seq, want = std::max(a.dk, a.dv) <= 128 ? 512 : 256;
     long tiles = (a.max_kv + BK - 1) / BK;
     if (a.window) tiles = std::min<long>(tiles, (std::min(a.sinks, a.max_kv) + BK - 1) / BK + ((long)std::min(a.n_tokens, BQ) + a.window - 2) / BK + 2);
-    return (int)std::max<long>(1, std::min<long>({(256 + wgs - 1) / wgs, tiles / 4, 16}));
+    return (int)std::max<long>(1, std::min<long>({(want + wgs - 1) / wgs, tiles / 4, 16}));
 }
 
 }  // namespace

@@ -228,6 +228,23 @@ def test_kv4_attn_large_scores(lib, fd):
             near(out[0], want, tol)
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, -0.0])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("T", [2, 40])
+def test_attn_scale_not_positive(lib, fd, T, cap, scale):
+    """A negative scale, and none (plain means of the visible values), over the cache and over fp16 keys."""
+    heads, kvh, d, n, window, sinks = 4, 2, 64, 150, 70, 3
+    c, Q = kv4_case(13, heads, kvh, d, d, T, [n])
+    out, sh = np.full((1, heads, T, d), 7, np.float16), R.Kv4Shape(*c.dims)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, 1, T, n, heads, scale, cap, window, sinks, R.ptr(Q),
+                                    R.ptr(np.array([n], np.int32)), R.ptr(out)) == 0
+    (want, tol), = kv4_want(c, Q, [n], window, sinks, scale, cap)
+    near(out[0], want, tol)
+    Q, K, V, see = win_case(14, heads, kvh, d, d, T, n, n, window, sinks)
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, cap, window, sinks, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(out)) == 0
+    near(out[0], *win_want(Q, K, V, see, scale, cap))
+
+
 # ---- windowed attention over fp16 keys -------------------------------------------------
 
 WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
