@@ -330,17 +330,17 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     };
     auto finish = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
         const int key0 = key_of(kb);
-        if (!whole(key0)) {
-            // (negative where the row does not see the key: bits, as comparisons became a branch each)
-            const int k0 = key0 + 4 * hh, after = pos - k0, before = k0 - behind - 1, sink = a.sinks - 1 - k0;
+        const int k0 = key0 + 4 * hh, after = pos - k0, before = behind - k0;
+        auto hide = [&](auto &&hidden) __attribute__((always_inline)) {
 #pragma unroll
             for (int sb = 0; sb < 2; sb++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int k = 32 * sb + 8 * (e >> 2) + (e & 3);
-                    const int hid = (after - k) | ((before + k) & (sink - k));
-                    Sx[sb][e] = hid < 0 ? -INFINITY : Sx[sb][e];
-                }
+                for (int e = 0; e < 16; e++) Sx[sb][e] = hidden(32 * sb + 8 * (e >> 2) + (e & 3)) ? -INFINITY : Sx[sb][e];
+        };
+        if (key0 + BK - 1 > p_lo) hide([&](int k) __attribute__((always_inline)) { return k > after; });
+        if (a.window && key0 <= p_hi - a.window) {
+            if (key0 >= a.sinks) hide([&](int k) __attribute__((always_inline)) { return k <= before; });
+            else if (key0 + BK > a.sinks) hide([&](int k) __attribute__((always_inline)) { return ((k - before - 1) & (a.sinks - 1 - k0 - k)) < 0; });
         }
         float mloc = -INFINITY;
 #pragma unroll
@@ -413,26 +413,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
             const int key0 = key_of(kb);
             if (whole(key0)) return;
             char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+            // an exponent of all ones carries into the sign's place
+            auto not_finite = [](unsigned w) __attribute__((always_inline)) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; };
             auto each = [&](bool finite) __attribute__((always_inline)) {
-                bool bad = false;
+                unsigned bad = 0;
+#pragma unroll 1
                 for (int g = tid; g < D * 8; g += 256) {
                     const int d = g >> 3, key = key0 + 8 * ((g & 7) ^ vx(d));
                     i32x4 *const p = reinterpret_cast<i32x4 *>(vs + g * 16);
                     i32x4 x = *p;
-                    bool any = false;
+                    const bool edge = key + 7 > p_hi || (key < first && key + 7 >= sinks);
+                    if (edge) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int m = 0xFFFF << (16 * (e & 1)), inf = 0x7C00 << (16 * (e & 1));
-                        const bool out = dead(key + e), nf = (x[e >> 1] & inf) == inf;
-                        bad |= nf && !out;
-                        if (out || (finite && nf)) {
-                            x[e >> 1] &= ~m;
-                            any = true;
-                        }
+                        for (int e = 0; e < 8; e++)
+                            if (dead(key + e)) x[e >> 1] &= 0xFFFF << (16 * (~e & 1));
                     }
-                    if (any) *p = x;
+                    unsigned nf[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) nf[i] = not_finite(x[i]);
+                    bad |= (nf[0] | nf[1]) | (nf[2] | nf[3]);
+                    if (finite)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[i] &= ~(int)((nf[i] >> 15) * 0xFFFFu);
+                    if (edge || finite) *p = x;
                 }
-                return bad;
+                return bad != 0;
             };
             if (each(false)) *bad_tile = kb;
             lds_barrier();
