@@ -2,7 +2,7 @@
 //
 // What bounds it is how fast the codes arrive, and then the VALU that widens them: about two
 // operations a value, whatever the number of query rows. So all rows of a KV head (its query heads'
-// tokens, at most 16) share one widening. A workgroup owns a place of the batch, a KV head and a range
+// tokens, at most 32, in blocks of 16) share one widening. A workgroup owns a place of the batch, a KV head and a range
 // of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
 // they lie in the cache, the next chunk's while this one's are widened.
 //
@@ -31,7 +31,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kRows = 16, kChunk = 32, kWaves = 4, kMaxSplit = 64;
+constexpr int kRows = 32, kChunk = 32, kWaves = 4, kMaxSplit = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4RowArgs {
@@ -75,8 +75,8 @@ __device__ __forceinline__ f16x8 widen8(int w, f16x2 sm)
     return r;
 }
 
-// D: head sizes up to this (64, 128, 256). FULL: dk and dv are D.
-template <int D, bool CAP, bool FULL>
+// D: head sizes up to this (64, 128, 256). NQ: blocks of 16 rows. FULL: dk and dv are D.
+template <int D, int NQ, bool CAP, bool FULL>
 __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 {
     const ServeAttn &a = ra.a;
@@ -92,22 +92,30 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const Chunks list(a, served ? n : 1);
     const int count = served ? list.count : 0;
     if (zs > 0 && zs * ra.cps >= count) return;   // (the merge knows)
-    const int hg = c / T, t = c - hg * T;         // this lane's query: head hk gqa + hg, token t
-    const bool qok = c < R;
-    const int pos = n - T + t;                    // its position
-    const int p_lo = n - T, p_hi = n - 1, behind = a.window ? pos - a.window : -1;   // (the last key behind its window)
+    // this lane's queries: row 16 x + c of the KV head's (head r / T, token r % T), and its position
+    bool qok[NQ];
+    int pos[NQ], behind[NQ];                      // (the last key behind its window)
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        const int r = 16 * x + c;
+        qok[x] = r < R;
+        pos[x] = n - T + r % T;
+        behind[x] = a.window ? pos[x] - a.window : -1;
+    }
+    const int p_lo = n - T, p_hi = n - 1;
 
     const size_t hr = (size_t)s * a.c.heads + hk;
     const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;   // row of the first query
-    f16x8 qf[KS];
-    {
-        const _Float16 *qrow = a.Q + (head0 + (qok ? c : 0)) * a.dk;
+    f16x8 qf[NQ][KS];
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        const _Float16 *qrow = a.Q + (head0 + (qok[x] ? 16 * x + c : 0)) * a.dk;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             const int d = D == 64 ? 16 * q + 8 * i : 128 * (i / 4) + 32 * q + 8 * (i % 4);
-            f16x8 x = {};
-            if (qok && (FULL || d < a.dk)) x = *reinterpret_cast<const f16x8 *>(qrow + d);
-            qf[i] = __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
+            f16x8 y = {};
+            if (qok[x] && (FULL || d < a.dk)) y = *reinterpret_cast<const f16x8 *>(qrow + d);
+            qf[x][i] = __builtin_shufflevector(y, y, 0, 4, 1, 5, 2, 6, 3, 7);
         }
     }
 
@@ -163,10 +171,15 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
         }
     };
 
-    float m_run = -1e30f, l_run = 0.f;
-    f32x4 O[VB];
+    float m_run[NQ], l_run[NQ];
+    f32x4 O[NQ][VB];
 #pragma unroll
-    for (int j = 0; j < VB; j++) O[j] = f32x4{};
+    for (int x = 0; x < NQ; x++) {
+        m_run[x] = -1e30f;
+        l_run[x] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VB; j++) O[x][j] = f32x4{};
+    }
     const int c1 = min(count, (zs + 1) * ra.cps);
     int ch = zs * ra.cps + wave;
     if (ch < c1) {
@@ -175,30 +188,21 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     }
     for (; ch < c1; ch += kWaves) {
         const int key0 = list.at(ch) * kChunk;
-        f32x4 S[2] = {};
+        f32x4 S[NQ][2] = {};
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
-            for (int b = 0; b < 2; b++)
-                S[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kw[b][i], ksm[b][i / KW]), qf[i], S[b], 0, 0, 0);
+            for (int b = 0; b < 2; b++) {
+                const f16x8 kf = widen8(kw[b][i], ksm[b][i / KW]);
+#pragma unroll
+                for (int x = 0; x < NQ; x++) S[x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][i], S[x][b], 0, 0, 0);
+            }
         const bool more = ch + kWaves < c1;
         const int next = list.at(more ? ch + kWaves : ch) * kChunk;
         if (more) load_k(next);
         // every row sees every key of the chunk, or the rows differ (uniform)
         const bool whole = key0 + kChunk - 1 <= p_lo && (!a.window || key0 > p_hi - a.window || key0 + kChunk <= a.sinks);
-        float v[8], mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float x = S[i >> 2][i & 3];
-            if constexpr (CAP) v[i] = softcap_log2(x, a.scale, a.softcap);
-            else v[i] = x * (a.scale * kLog2e);
-        }
         if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int key = key0 + 8 * q + i;
-                v[i] = (bool)((key <= pos) & ((key > behind) | (key < a.sinks))) ? v[i] : -INFINITY;
-            }
             // keys that no row sees: their values count as 0, whatever the memory holds
 #pragma unroll
             for (int u = 0; u < U; u++)
@@ -208,23 +212,40 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
                     if ((bool)((key > p_hi) | ((key < list.first) & (key >= list.sinks)))) vsm[u][i >> 2][i & 3] = 0;
                 }
         }
+        f16x8 p[NQ];
 #pragma unroll
-        for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (__any(mx > m_run)) {
-            const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-            m_run = m_new;
-            l_run *= alpha;
+        for (int x = 0; x < NQ; x++) {
+            float v[8], mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < VB; j++) O[j] *= alpha;
-        }
-        f16x8 p;
+            for (int i = 0; i < 8; i++) {
+                const float y = S[x][i >> 2][i & 3];
+                if constexpr (CAP) v[i] = softcap_log2(y, a.scale, a.softcap);
+                else v[i] = y * (a.scale * kLog2e);
+            }
+            if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float e = __builtin_amdgcn_exp2f(v[i] - m_run);
-            l_run += e;
-            p[i] = (_Float16)e;
+                for (int i = 0; i < 8; i++) {
+                    const int key = key0 + 8 * q + i;
+                    v[i] = (bool)((key <= pos[x]) & ((key > behind[x]) | (key < a.sinks))) ? v[i] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(mx > m_run[x])) {
+                const float m_new = fmaxf(m_run[x], mx), alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
+                m_run[x] = m_new;
+                l_run[x] *= alpha;
+#pragma unroll
+                for (int j = 0; j < VB; j++) O[x][j] *= alpha;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float e = __builtin_amdgcn_exp2f(v[i] - m_run[x]);
+                l_run[x] += e;
+                p[x][i] = (_Float16)e;
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -252,19 +273,23 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
                     f[2 * k] = y[0];
                     f[2 * k + 1] = y[1];
                 }
-                O[u * NJ + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p, O[u * NJ + j], 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < NQ; b++)
+                    O[b][u * NJ + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[b], O[b][u * NJ + j], 0, 0, 0);
             }
         }
         if (more) load_v(next);
     }
-    l_run += __shfl_xor(l_run, 16, 64);
-    l_run += __shfl_xor(l_run, 32, 64);
 
     // merge the waves: [wave][row][LROW] outputs, then [wave][row] (max, sum)
     float *const Ol = reinterpret_cast<float *>(smem);
     f32x2 *const ml = reinterpret_cast<f32x2 *>(Ol + kWaves * R * LROW);
-    if (qok) {
-        float *const row = Ol + (wave * R + c) * LROW;
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        l_run[x] += __shfl_xor(l_run[x], 16, 64);
+        l_run[x] += __shfl_xor(l_run[x], 32, 64);
+        if (!qok[x]) continue;
+        float *const row = Ol + (wave * R + 16 * x + c) * LROW;
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -272,8 +297,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
                 for (int j = 0; j < NJ; j += 4)
                     *reinterpret_cast<f32x4 *>(row + 128 * u + NJ * (4 * q + e) + j) =
-                        f32x4{O[u * NJ + j][e], O[u * NJ + j + 1][e], O[u * NJ + j + 2][e], O[u * NJ + j + 3][e]};
-        if (q == 0) ml[wave * R + c] = f32x2{m_run, l_run};
+                        f32x4{O[x][u * NJ + j][e], O[x][u * NJ + j + 1][e], O[x][u * NJ + j + 2][e], O[x][u * NJ + j + 3][e]};
+        if (q == 0) ml[wave * R + 16 * x + c] = f32x2{m_run[x], l_run[x]};
     }
     __syncthreads();
     const int dq = dv / 4;
@@ -360,24 +385,30 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
     }
 }
 
-template <int D, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
+template <int D, int NQ, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
 {
-    auto kern = k_kv4_rows<D, CAP, FULL>;
+    auto kern = k_kv4_rows<D, NQ, CAP, FULL>;
     const ServeAttn &a = ra.a;
     const int R = a.gqa * a.n_tokens;
     const size_t lds = (size_t)kWaves * R * ((D + 4) * 4 + 8);
     if (lds > 64 * 1024) {
         static std::atomic<uint64_t> opted{0};
-        if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), 80 * 1024, opted)) return e;
+        constexpr int most = kWaves * 16 * NQ * ((D + 4) * 4 + 8);
+        static_assert(most <= 160 * 1024, "LDS budget");
+        if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), most, opted)) return e;
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)a.c.heads, (unsigned)ra.nsplit, (unsigned)a.n_seq), dim3(kWaves * 64), lds, s, ra);
     return hipGetLastError();
 }
-template <int D> hipError_t launch(const Kv4RowArgs &ra, hipStream_t s)
+template <int D, int NQ> hipError_t launch_q(const Kv4RowArgs &ra, hipStream_t s)
 {
     const bool cap = ra.a.softcap != 0.f;
-    if (ra.a.dk == D && ra.a.dv == D) return cap ? launch_f<D, true, true>(ra, s) : launch_f<D, false, true>(ra, s);
-    return cap ? launch_f<D, true, false>(ra, s) : launch_f<D, false, false>(ra, s);
+    if (ra.a.dk == D && ra.a.dv == D) return cap ? launch_f<D, NQ, true, true>(ra, s) : launch_f<D, NQ, false, true>(ra, s);
+    return cap ? launch_f<D, NQ, true, false>(ra, s) : launch_f<D, NQ, false, false>(ra, s);
+}
+template <int D> hipError_t launch(const Kv4RowArgs &ra, hipStream_t s)
+{
+    return ra.a.gqa * ra.a.n_tokens <= 16 ? launch_q<D, 1>(ra, s) : launch_q<D, 2>(ra, s);
 }
 
 // Chunks that a sequence of up to max_kv keys may have to visit.

@@ -362,9 +362,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
         }
         return alpha;
     };
-    auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float &psum, int e) __attribute__((always_inline)) {
+    auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float m, float &psum, int e) __attribute__((always_inline)) {
         const int sb = e >> 4, i = e & 15;
-        const float p = __builtin_amdgcn_exp2f(fmaf(Sx[sb][i], unit, -m_run));
+        const float p = __builtin_amdgcn_exp2f(fmaf(Sx[sb][i], unit, -m));
         pb[sb][i >> 3][i & 7] = (_Float16)p;
         // the sum of the rounded weights, two at a time, in fp32: weights and their sum round alike
         if (i & 1) psum = __builtin_amdgcn_fdot2(f16x2{pb[sb][i >> 3][(i & 7) - 1], pb[sb][i >> 3][i & 7]}, f16x2{(_Float16)1.f, (_Float16)1.f}, psum, false);
@@ -466,10 +466,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     // Iteration kb: PV of tile kb - 1 beside the score arithmetic of tile kb, then QK of tile kb + 1 beside the
     // exponentials of tile kb. K tile kb + 2 goes into the K slot that tile kb left, V^T tile kb into the V^T slot that tile
     // kb - 2 left; both are read an iteration on. The first iteration (kb0 - 1) has the first QK alone and the last
-    // (kb1) the last PV: one copy of the products' code, since a workgroup runs through few tiles and its first run
-    // through each line of code waits for the instruction cache (peeled first and last iterations took 22 us of a
-    // call's 83 outside its 16 tiles). Codes are loaded a whole iteration before they are widened, keys beside PV and
-    // values beside QK.
+    // (kb1) the last PV, so that there is one copy of the products' code. Codes are loaded a whole iteration before they are
+    // widened, keys beside PV and values beside QK.
     constexpr int QKM = 2 * KC, PVM = 4 * DB;
     f32x16 S[2] = {};
     f16x8 P[2][2] = {};
@@ -529,7 +527,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
                 f32x16 Sn[2];
                 qk(cur ^ 1, Sn, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = m * 32 / QKM; e < (m + 1) * 32 / QKM; e++) prob1(S, P, psum, e);
+                    for (int e = m * 32 / QKM; e < (m + 1) * 32 / QKM; e++) prob1(S, P, m_run, psum, e);
                     if constexpr (C4) {
                         if (tile) {
 #pragma unroll
@@ -540,8 +538,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
                 S[0] = Sn[0];
                 S[1] = Sn[1];
             } else {
+                float m = m_run;
+                asm("" : "+v"(m));   // (or the compiler takes both branches' subtractions out in front of the products)
 #pragma unroll
-                for (int e = 0; e < 32; e++) prob1(S, P, psum, e);
+                for (int e = 0; e < 32; e++) prob1(S, P, m, psum, e);
                 if constexpr (C4) {
 #pragma unroll
                     for (int u = 0; u < CF::VU; u++) put_v(cur, u);
