@@ -10,9 +10,9 @@
 // (l % 16, l / 16) holds query c and keys 8 q .. 8 q + 7 of the chunk, as the second product takes them.
 // The order of the summed dims is free as long as Q has the same: quarter q takes whole groups, so a
 // lane's sixteen bytes of a key share one scale. In O^T += V^T P^T the rows (dims) are free: lane c
-// takes a word of eight dims of each of its eight keys, product j their nibbles j, which two byte permutes
-// and a shift bring side by side as pairs of keys. A code c becomes the half 1024 + c by or-ing bits in,
-// less 1024 (exact), times scale plus minimum (one rounding): the values that rocket_kv4_read_fp16 gives.
+// takes a word of eight dims of each of its eight keys, product j their nibbles j, which a byte permute brings
+// side by side as pairs of keys.
+#include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
 #include "softcap.h"
@@ -27,9 +27,7 @@ typedef int      i32x2 __attribute__((ext_vector_type(2)));
 typedef int      i32x4 __attribute__((ext_vector_type(4)));
 typedef float    f32x2 __attribute__((ext_vector_type(2)));
 typedef float    f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 32, kChunk = 32, kWaves = 4, kMaxSplit = 64;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -55,25 +53,6 @@ struct Chunks {
     }
     __device__ int at(int v) const { return v < ns ? v : v + skip; }
 };
-
-// Eight codes of a word as halves in the order 0 4 1 5 2 6 3 7, times scale plus minimum.
-__device__ __forceinline__ f16x2 widen2(int nibbles, f16x2 s, f16x2 m)
-{
-    const f16x2 c = __builtin_bit_cast(f16x2, (nibbles & 0x000F000F) | 0x64006400) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
-    return __builtin_elementwise_fma(c, s, m);
-}
-__device__ __forceinline__ f16x8 widen8(int w, f16x2 sm)
-{
-    const f16x2 s = {sm[0], sm[0]}, m = {sm[1], sm[1]};
-    f16x8 r;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const f16x2 x = widen2(w >> (4 * e), s, m);
-        r[2 * e] = x[0];
-        r[2 * e + 1] = x[1];
-    }
-    return r;
-}
 
 // D: head sizes up to this (64, 128, 256). NQ: blocks of 16 rows. FULL: dk and dv are D.
 template <int D, int NQ, bool CAP, bool FULL>
@@ -171,6 +150,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
         }
     };
 
+    const Widen widen;
     float m_run[NQ], l_run[NQ];
     f32x4 O[NQ][VB];
 #pragma unroll
@@ -193,7 +173,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
         for (int i = 0; i < KS; i++)
 #pragma unroll
             for (int b = 0; b < 2; b++) {
-                const f16x8 kf = widen8(kw[b][i], ksm[b][i / KW]);
+                const f16x8 kf = widen.eight(kw[b][i], ksm[b][i / KW]);
 #pragma unroll
                 for (int x = 0; x < NQ; x++) S[x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][i], S[x][b], 0, 0, 0);
             }
@@ -269,7 +249,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
                 f16x8 f;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const f16x2 y = widen2(x[j >> 2][k] >> (4 * (j & 3)), sc[k], mi[k]);
+                    const f16x2 y = widen.at(x[j >> 2][k], j & 3, sc[k], mi[k]);
                     f[2 * k] = y[0];
                     f[2 * k + 1] = y[1];
                 }

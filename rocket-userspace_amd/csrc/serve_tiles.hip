@@ -4,8 +4,8 @@
 // that they share each tile), a wave 32 rows. The key axis goes by tiles of 64 keys, those alone that some
 // row sees: the sinks' tiles, then from the first window's to the last token's. K tiles [64][D] and V^T
 // tiles [D][64] lie in LDS as halves, two of each. fp16 keys arrive by buffer-load DMA. Codes arrive in
-// registers a tile ahead and are widened between the MFMAs (two VALU operations a value, shared by the
-// 128 rows), then written to LDS.
+// registers a tile ahead and are widened between the MFMAs (under two VALU operations a value, shared by
+// the 128 rows), then written to LDS.
 //
 // The loop is software-pipelined: an iteration runs the previous tile's PV products with this tile's
 // score arithmetic between them, then the next tile's QK products with this tile's exponentials between
@@ -13,6 +13,7 @@
 // holds one row's scores and P stays in registers: rounded to fp16 and swapped between the half-waves
 // it is the second product's operand. O is rescaled only when some running maximum grows by more than 8.
 #include "attn.h"
+#include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
 #include "softcap.h"
@@ -26,9 +27,7 @@ namespace {
 typedef int      i32x2  __attribute__((ext_vector_type(2)));
 typedef int      i32x4  __attribute__((ext_vector_type(4)));
 typedef float    f32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 f16x2  __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4  __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8  __attribute__((ext_vector_type(8)));
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 
 constexpr uint32_t kOOB = 0x80000000u;   // an offset past every range: loads return 0
@@ -67,14 +66,6 @@ template <int D> struct Cfg {
     __device__ static int kx(int row) { return (D * 2) % 256 == 0 ? (row & 15) : ((row >> 1) & 7); }
 };
 __device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T rows: 128 bytes
-
-// Two codes (bits 0-3 and 16-19) as halves: 1024 + c by or-ing bits in, less 1024, times scale plus minimum
-// (one rounding).
-__device__ __forceinline__ f16x2 widen2(int nibbles, f16x2 s, f16x2 m)
-{
-    const f16x2 c = __builtin_bit_cast(f16x2, (nibbles & 0x000F000F) | 0x64006400) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
-    return __builtin_elementwise_fma(c, s, m);
-}
 
 template <int D, bool C4, bool CAP>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const TileArgs ta)
@@ -197,9 +188,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     [[maybe_unused]] int kw[CF::ITEMS][CF::KW] = {};
     [[maybe_unused]] f16x2 ksm[CF::ITEMS] = {};
     [[maybe_unused]] i32x4 vw[CF::ITEMS][2] = {}, vsm[CF::ITEMS][2] = {};
-    [[maybe_unused]] int vp[CF::ITEMS][4] = {};           // pairs of keys, the thread's nibbles lowest
+    [[maybe_unused]] unsigned vp[CF::ITEMS][4] = {};      // pairs of keys, the thread's nibbles lowest
     [[maybe_unused]] f16x2 vsc[CF::ITEMS][4] = {}, vmi[CF::ITEMS][4] = {};
     [[maybe_unused]] const int vpart = D == 64 ? (tid >> 3) & 3 : (tid >> 3) & 1, vword = D == 64 ? tid >> 5 : tid >> 4;
+    [[maybe_unused]] const Widen widen;
     [[maybe_unused]] const size_t hr = C4 ? (size_t)s * a.c.heads + hk : 0;
     auto load_k = [&](int kb) __attribute__((always_inline)) {
         const size_t row = hr * a.c.cap + key_of(kb) + (tid >> 2);
@@ -241,14 +233,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     auto put_k = [&](int slot, int u) __attribute__((always_inline)) {
         const int i = u / CF::KW, w = u % CF::KW, key = tid >> 2;
         const int chunk = D == 64 ? 2 * (tid & 3) + w : 4 * ((tid & 3) + 4 * i) + w;
-        const f16x2 sc = {ksm[i][0], ksm[i][0]}, mi = {ksm[i][1], ksm[i][1]};
-        f16x8 x;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const f16x2 y = widen2(kw[i][w] >> (4 * e), sc, mi);
-            x[2 * e] = y[0];
-            x[2 * e + 1] = y[1];
-        }
+        const f16x8 x = widen.eight(kw[i][w], ksm[i]);
         *reinterpret_cast<f16x8 *>(smem + slot * CF::STAGE + key * (D * 2) + ((chunk ^ CF::kx(key)) << 4)) = x;
     };
     // pairs of keys of the thread's value words; keys that no row sees get scale and minimum 0
@@ -269,7 +254,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
             for (int k = 0; k < 4; k++) {
                 const unsigned w0 = vw[i][k >> 1][2 * (k & 1)], w1 = vw[i][k >> 1][2 * (k & 1) + 1];
                 const unsigned s0 = vsm[i][k >> 1][2 * (k & 1)], s1 = vsm[i][k >> 1][2 * (k & 1) + 1];
-                vp[i][k] = (int)__builtin_amdgcn_perm(w1, w0, sel) >> (D == 64 ? 8 * (vpart & 1) : 0);
+                vp[i][k] = __builtin_amdgcn_perm(w1, w0, sel) >> (D == 64 ? 8 * (vpart & 1) : 0);
                 vsc[i][k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
                 vmi[i][k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
             }
@@ -280,7 +265,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
         f16x8 x;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const f16x2 y = widen2(vp[i][k] >> (4 * j), vsc[i][k], vmi[i][k]);
+            const f16x2 y = widen.at(vp[i][k], j, vsc[i][k], vmi[i][k]);
             x[2 * k] = y[0];
             x[2 * k + 1] = y[1];
         }
