@@ -88,12 +88,12 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     f16x8 qf[NQ][KS];
 #pragma unroll
     for (int x = 0; x < NQ; x++) {
-        const _Float16 *qrow = a.Q + (head0 + (qok[x] ? 16 * x + c : 0)) * a.dk;
+        const _Float16 *qrow = a.Q + (head0 + min(16 * x + c, R - 1)) * a.dk;   // (rows behind the last repeat it)
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             const int d = D == 64 ? 16 * q + 8 * i : 128 * (i / 4) + 32 * q + 8 * (i % 4);
-            f16x8 y = {};
-            if (qok[x] && (FULL || d < a.dk)) y = *reinterpret_cast<const f16x8 *>(qrow + d);
+            f16x8 y = *reinterpret_cast<const f16x8 *>(qrow + (FULL ? d : min(d, a.dk - 8)));
+            if (!FULL && d >= a.dk) y = f16x8{};
             qf[x][i] = __builtin_shufflevector(y, y, 0, 4, 1, 5, 2, 6, 3, 7);
         }
     }
@@ -105,33 +105,26 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     f16x2 ksm[2][U];
     i32x4 vw[U][2];       // a word of each of the keys 8 q .. 8 q + 7
     i32x4 vsm[U][2];      // their (scale, minimum)
-#pragma unroll
-    for (int b = 0; b < 2; b++)
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-#pragma unroll
-            for (int i = 0; i < KW; i++) kw[b][u * KW + i] = 0;
-            ksm[b][u] = f16x2{};
-            vw[u][b] = vsm[u][b] = i32x4{};
-        }
     auto load_k = [&](int key0) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const uint32_t key = key0 + 8 * (c >> 2) + 4 * b + (c & 3);
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int g = D == 64 ? q >> 1 : 4 * u + q;   // the run's group
-                if (!FULL && (D == 64 ? 16 * q : 32 * g) >= dk) continue;
+                [[maybe_unused]] const int g = 4 * u + q;   // the run: a group (D 64: half of one)
+                // (past dk another run of the key: Q has those dims as 0)
+                const int run = FULL ? (D == 64 ? q : g) : D == 64 ? min(q, dk / 16 - 1) : min(g, dk / 32 - 1);
                 if constexpr (D == 64) {
-                    const i32x2 x = *reinterpret_cast<const i32x2 *>(kc + (size_t)key * (dk / 2) + 8 * q);
+                    const i32x2 x = *reinterpret_cast<const i32x2 *>(kc + (size_t)key * (dk / 2) + 8 * run);
                     kw[b][0] = x[0];
                     kw[b][1] = x[1];
+                    ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (size_t)key * (dk / 8) + 4 * (run >> 1));
                 } else {
-                    const i32x4 x = *reinterpret_cast<const i32x4 *>(kc + (size_t)key * (dk / 2) + 16 * g);
+                    const i32x4 x = *reinterpret_cast<const i32x4 *>(kc + (size_t)key * (dk / 2) + 16 * run);
 #pragma unroll
                     for (int i = 0; i < 4; i++) kw[b][4 * u + i] = x[i];
+                    ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (size_t)key * (dk / 8) + 4 * run);
                 }
-                ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (size_t)key * (dk / 8) + 4 * g);
             }
         }
     };
@@ -139,8 +132,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
         const uint32_t block = key0 / 8 + q;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int w = D == 64 ? c >> 1 : 16 * u + c;   // the lane's word: dims 8 w .. 8 w + 7
-            if (!FULL && 8 * w >= dv) continue;
+            const int word = D == 64 ? c >> 1 : 16 * u + c;   // the lane's word: dims 8 w .. 8 w + 7
+            const int w = FULL ? word : min(word, dv / 8 - 1);   // (results past dv are not stored)
             const char *p = vc + ((size_t)block * (dv / 8) + w) * 32, *m = vs + ((size_t)block * (dv / 32) + w / 4) * 32;
 #pragma unroll
             for (int i = 0; i < 2; i++) {

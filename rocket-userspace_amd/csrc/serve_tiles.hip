@@ -68,7 +68,7 @@ template <int D> struct Cfg {
 __device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T rows: 128 bytes
 
 template <int D, bool C4, bool CAP>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const TileArgs ta)
+__global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_serve_tiles(const TileArgs ta)
 {
     const ServeAttn &a = ta.a;
     using CF = Cfg<D>;
@@ -124,11 +124,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     // which widened codes lie)
     f16x8 qf[KC];
     {
-        const _Float16 *qrow = a.Q + (row0 + (qok ? r : 0)) * a.dk;
+        const _Float16 *qrow = a.Q + (row0 + min(r, R - 1)) * a.dk + 8 * hh;   // (rows behind the last repeat it)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
-            f16x8 x = {};
-            if (qok && 16 * c + 8 * hh < a.dk && a.scale != 0.f) x = *reinterpret_cast<const f16x8 *>(qrow + 16 * c + 8 * hh);
+            f16x8 x = *reinterpret_cast<const f16x8 *>(qrow + min(16 * c, a.dk - 16));
+            if (16 * c >= a.dk || a.scale == 0.f) x = f16x8{};
             if (a.scale < 0.f) x = -x;
             qf[c] = C4 ? __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7) : x;
         }
@@ -185,42 +185,41 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     };
     // 4-bit: a thread's runs of codes. Keys: key tid / 4, words 4 g + i of run g (D 64: 2 (tid % 4) + i). Values: block
     // tid % 8 of eight keys, VD nibbles of word w.
-    [[maybe_unused]] int kw[CF::ITEMS][CF::KW] = {};
-    [[maybe_unused]] f16x2 ksm[CF::ITEMS] = {};
-    [[maybe_unused]] i32x4 vw[CF::ITEMS][2] = {}, vsm[CF::ITEMS][2] = {};
-    [[maybe_unused]] unsigned vp[CF::ITEMS][4] = {};      // pairs of keys, the thread's nibbles lowest
-    [[maybe_unused]] f16x2 vsc[CF::ITEMS][4] = {}, vmi[CF::ITEMS][4] = {};
+    [[maybe_unused]] int kw[CF::ITEMS][CF::KW];
+    [[maybe_unused]] f16x2 ksm[CF::ITEMS];
+    [[maybe_unused]] i32x4 vw[CF::ITEMS][2], vsm[CF::ITEMS][2];
+    [[maybe_unused]] unsigned vp[CF::ITEMS][4];      // pairs of keys, the thread's nibbles lowest
+    [[maybe_unused]] f16x2 vsc[CF::ITEMS][4], vmi[CF::ITEMS][4];
     [[maybe_unused]] const int vpart = D == 64 ? (tid >> 3) & 3 : (tid >> 3) & 1, vword = D == 64 ? tid >> 5 : tid >> 4;
     [[maybe_unused]] const Widen widen;
     [[maybe_unused]] const size_t hr = C4 ? (size_t)s * a.c.heads + hk : 0;
+    // (No load stands under a condition: its registers would be copied, and so waited for, where the paths meet. Past the
+    // last tile the last one's loads are repeated; past the capacity, which a tile may end 32 keys behind, and past
+    // dk or dv others of the tile are loaded: hidden keys, dims that Q has as 0, rows that are not stored.)
     auto load_k = [&](int kb) __attribute__((always_inline)) {
-        const size_t row = hr * a.c.cap + key_of(kb) + (tid >> 2);
-        if (key_of(kb) + (tid >> 2) >= a.c.cap) return;   // (a tile may end 32 keys past the capacity's end)
+        const int key = min(key_of(min(kb, kb1 - 1)) + (tid >> 2), a.c.cap - 1);
+        const char *codes = a.c.kc + (hr * a.c.cap + key) * (a.dk / 2), *sms = a.c.ks + (hr * a.c.cap + key) * (a.dk / 8);
 #pragma unroll
         for (int i = 0; i < CF::ITEMS; i++) {
-            const int p = tid & 3, d = D == 64 ? 16 * p : 32 * (p + 4 * i);
-            if (d >= a.dk) continue;
-            const char *src = a.c.kc + row * (a.dk / 2) + d / 2;
+            const int p = tid & 3, d = D == 64 ? min(16 * p, a.dk - 16) : min(32 * (p + 4 * i), a.dk - 32);
             if constexpr (D == 64) {
-                const i32x2 x = *reinterpret_cast<const i32x2 *>(src);
+                const i32x2 x = *reinterpret_cast<const i32x2 *>(codes + d / 2);
                 kw[i][0] = x[0];
                 kw[i][1] = x[1];
             } else {
-                const i32x4 x = *reinterpret_cast<const i32x4 *>(src);
+                const i32x4 x = *reinterpret_cast<const i32x4 *>(codes + d / 2);
 #pragma unroll
                 for (int e = 0; e < 4; e++) kw[i][e] = x[e];
             }
-            ksm[i] = *reinterpret_cast<const f16x2 *>(a.c.ks + row * (a.dk / 8) + d / 32 * 4);
+            ksm[i] = *reinterpret_cast<const f16x2 *>(sms + d / 32 * 4);
         }
     };
     auto load_v = [&](int kb) __attribute__((always_inline)) {
-        const int key = key_of(kb) + 8 * (tid & 7);
-        if (key >= a.c.cap) return;
+        const int key = min(key_of(min(kb, kb1 - 1)) + 8 * (tid & 7), a.c.cap - 8);
         const size_t block = hr * (a.c.cap / 8) + key / 8;
 #pragma unroll
         for (int i = 0; i < CF::ITEMS; i++) {
-            const int w = vword + 16 * i;
-            if (8 * w >= a.dv) continue;
+            const int w = min(vword + 16 * i, a.dv / 8 - 1);
             const char *p = a.c.vc + (block * (a.dv / 8) + w) * 32, *m = a.c.vs + (block * (a.dv / 32) + w / 4) * 32;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -452,7 +451,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
     // exponentials of tile kb. K tile kb + 2 goes into the K slot that tile kb left, V^T tile kb into the V^T slot that tile
     // kb - 2 left; both are read an iteration on. The first iteration (kb0 - 1) has the first QK alone and the last
     // (kb1) the last PV, so that there is one copy of the products' code. Codes are loaded a whole iteration before they are
-    // widened, keys beside PV and values beside QK.
+    // widened, keys beside PV and values beside QK (also where there is no such tile: into slots that nothing reads again
+    // before they are written).
     constexpr int QKM = 2 * KC, PVM = 4 * DB;
     f32x16 S[2] = {};
     f16x8 P[2][2] = {};
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
             load_v(kb0);
 #pragma unroll
             for (int u = 0; u < CF::KU; u++) put_k(0, u);
-            if (kb0 + 1 < kb1) load_k(kb0 + 1);
+            load_k(kb0 + 1);
         } else {
             dma_k(kb0, 0);
             if (tid == 0) *bad_tile = -1;
@@ -470,11 +470,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
 #pragma unroll 1
         for (int kb = kb0 - 1;; kb++) {
             const int cur = (kb - kb0) & 1;
-            const bool puts_k = kb + 2 < kb1, tile = kb >= kb0 && kb < kb1;
+            const bool tile = kb >= kb0 && kb < kb1;
             if constexpr (!C4) wait_vm0();
             lds_barrier();
             if constexpr (!C4) {
-                if (puts_k) dma_k(kb + 2, cur);
+                if (kb + 2 < kb1) dma_k(kb + 2, cur);
                 if (tile) dma_v(kb, cur);
             }
             if (kb > kb0) {
@@ -483,10 +483,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
 #pragma unroll
                     for (int e = m * 32 / PVM; e < (m + 1) * 32 / PVM; e++) cap1(S, e);
                     if constexpr (C4) {
-                        if (puts_k) {
 #pragma unroll
-                            for (int u = m * CF::KU / PVM; u < (m + 1) * CF::KU / PVM; u++) put_k(cur, u);
-                        }
+                        for (int u = m * CF::KU / PVM; u < (m + 1) * CF::KU / PVM; u++) put_k(cur, u);
                     }
                 });
                 if (kb == kb1) break;
@@ -494,19 +492,16 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
 #pragma unroll
                 for (int e = 0; e < 32; e++) cap1(S, e);
                 if constexpr (C4) {
-                    if (puts_k) {
 #pragma unroll
-                        for (int u = 0; u < CF::KU; u++) put_k(cur, u);
-                    }
+                    for (int u = 0; u < CF::KU; u++) put_k(cur, u);
                 }
             }
-            if constexpr (C4) {
-                if (kb + 3 < kb1) load_k(kb + 3);
-            }
             float alpha = 1.f, psum = 0.f;
-            if (tile) {
-                alpha = grow(finish(kb, S));
-                if constexpr (C4) pair_v(kb);
+            if constexpr (C4) load_k(kb + 3);
+            if (tile) alpha = grow(finish(kb, S));
+            if constexpr (C4) {
+                pair_v(max(kb, kb0));
+                load_v(kb + 1);
             }
             if (kb + 1 < kb1) {
                 f32x16 Sn[2];
@@ -514,10 +509,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
 #pragma unroll
                     for (int e = m * 32 / QKM; e < (m + 1) * 32 / QKM; e++) prob1(S, P, m_run, psum, e);
                     if constexpr (C4) {
-                        if (tile) {
 #pragma unroll
-                            for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(cur, u);
-                        }
+                        for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(cur, u);
                     }
                 });
                 S[0] = Sn[0];
@@ -535,9 +528,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void k_serve_tiles(const Til
             if (tile) {
                 reorder(P);
                 l_run = l_run * alpha + psum;
-                if constexpr (C4) {
-                    if (kb + 1 < kb1) load_v(kb + 1);
-                }
             }
         }
     }
@@ -592,8 +582,10 @@ long row_blocks(const ServeAttn &a) { return ((long)a.gqa * a.n_tokens + BQ - 1)
 
 int splits(const ServeAttn &a)
 {
-    // enough workgroups for every CU (256; heads of up to 128 run two on one), each split keeping at least 4 of the tiles that a block may see
-    const long wgs = row_blocks(a) * (a.n_head / a.gqa) * a.n_seq, want = std::max(a.dk, a.dv) <= 128 ? 512 : 256;
+    // enough workgroups for every CU (256), and two on one where the registers allow it, each split keeping at least 4 of
+    // the tiles that a block may see
+    const int d = std::max(a.dk, a.dv);
+    const long wgs = row_blocks(a) * (a.n_head / a.gqa) * a.n_seq, want = d <= 64 || (d <= 128 && a.Kf) ? 512 : 256;
     long tiles = (a.max_kv + BK - 1) / BK;
     if (a.window) tiles = std::min<long>(tiles, (std::min(a.sinks, a.max_kv) + BK - 1) / BK + ((long)std::min(a.n_tokens, BQ) + a.window - 2) / BK + 2);
     return (int)std::max<long>(1, std::min<long>({(want + wgs - 1) / wgs, tiles / 4, 16}));
