@@ -144,7 +144,11 @@ hipError_t qk_norm_rope(const RopeLaunch &L, hipStream_t s, uint64_t *blocks)
     a.q = L.q; a.k = L.k; a.q_rs = L.q_rs; a.k_rs = L.k_rs; a.wq = L.wq; a.wk = L.wk; a.inv_freq = L.inv_freq; a.pos = L.pos;
     a.q_out = L.q_out; a.k_out = L.k_out; a.rows = L.n_seq * L.n_tokens; a.n_tokens = L.n_tokens; a.n_head = L.n_head; a.n_kv = L.n_kv;
     a.dim = L.dim; a.rot = L.rot; a.eps = L.eps; a.rdim = 1.f / (float)L.dim; a.norm = L.norm;
-    const int per = 256 / g, y = (L.n_head + L.n_kv + per - 1) / per;
+    // Workgroups of a row: as many as its heads fill, but no more than make about four a CU (1024): with more rows a
+    // lane takes several heads with one sine and cosine (4096 rows of 40 heads of 128: 27.0 us for three workgroups a
+    // row, 22.8 for one; 512 such rows 5.5 for three, 5.1 for two, 5.6 for one; 16 rows of 24 heads of 256 3.7 for three,
+    // 4.7 for one).
+    const int per = 256 / g, most = (L.n_head + L.n_kv + per - 1) / per, y = std::max(1, std::min(most, (1024 + a.rows - 1) / a.rows));
     a.step = y * per;
     const dim3 grid((unsigned)a.rows, (unsigned)y);
     *blocks = (uint64_t)a.rows * y;
