@@ -70,7 +70,7 @@ hipError_t kv4_read(const Kv4View &c, const Kv4Rows &r, hipStream_t s, uint64_t 
 struct ServeAttn {
     Kv4View c{};
     const _Float16 *Kf = nullptr, *Vf = nullptr;
-    long stride = 0, k_hs = 0;               // keys a V^T row holds (a multiple of 8); elements a head's keys take
+    long stride = 0, k_hs = 0;               // keys a V^T row holds; elements a head's keys take
     const _Float16 *Q = nullptr;
     _Float16 *out = nullptr;
     const int32_t *seq_len = nullptr;   // null: max_kv

@@ -337,9 +337,9 @@ int rocket_flash_attn_window_fp16(int fd, int n_tokens, int n_kv, int kv_stride,
         c.want(K, kb);
         c.want(V, vb);
         c.want(out, ob);
-        // V^T rows that are no whole 16-byte chunks are copied into ones that are, for the tiles
+        // (the tiles read chunks of eight keys: V^T rows of fewer are copied into longer ones)
         a.Kf = K;
-        const int padded = kv_stride % 8 && !serve_few_rows(a) ? (kv_stride + 63) / 64 * 64 : kv_stride;
+        const int padded = kv_stride < 8 && !serve_few_rows(a) ? 64 : kv_stride;
         const size_t pb = padded != kv_stride ? h16((size_t)n_kv_heads * dv * padded) : 0;
         if (pb) c.want_scratch(pb);
         const size_t ws = c.want_optional(serve_attn_ws(a), n_kv >= 512);

@@ -45,6 +45,9 @@ __device__ __forceinline__ void wait_vm0()
 }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// eight halves at any 2-byte address
+struct __attribute__((packed, aligned(2))) Halves8 { i32x4 v; };
+
 struct TileArgs {
     ServeAttn a;
     int nsplit, nqb;   // shares of the key tiles; row blocks of BQ
@@ -67,9 +70,14 @@ template <int D> struct Cfg {
 };
 __device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T rows: 128 bytes
 
-template <int D, bool C4, bool CAP>
-__global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_serve_tiles(const TileArgs ta)
+// Where keys and values come from: fp16 rows by DMA; the same with V^T rows that are no whole 16-byte chunks, whose values
+// go through registers; codes.
+enum Src { kHalves, kRagged, kCodes };
+
+template <int D, Src SRC, bool CAP>
+__global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1) void k_serve_tiles(const TileArgs ta)
 {
+    constexpr bool C4 = SRC == kCodes, RV = SRC == kRagged;
     const ServeAttn &a = ta.a;
     using CF = Cfg<D>;
     constexpr int KC = CF::KC, KCPR = CF::KCPR, DB = CF::DB;
@@ -140,7 +148,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_s
     constexpr bool KSEP = 256 % KCPR == 0 && (256 / KCPR) % 16 == 0;
     constexpr int KN = KSEP ? 1 : CF::KINS;
     [[maybe_unused]] uint32_t kvo[KN], vvo = 0, kstep = 0, vstep = 0;
-    [[maybe_unused]] int vkey = 0;
+    [[maybe_unused]] int vkey = 0, vrow = 0;
     [[maybe_unused]] const _Float16 *Kh = nullptr, *Vh = nullptr;
     if constexpr (!C4) {
 #pragma unroll
@@ -151,6 +159,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_s
         const int g = wave * 64 + lane, row = g >> 3, lc = (g & 7) ^ vx(row);
         vvo = (uint32_t)((long)row * a.stride + lc * 8) * 2u;
         vkey = lc * 8;
+        vrow = row;
         kstep = (uint32_t)((256 / KCPR) * a.dk * 2);
         vstep = (uint32_t)(32 * a.stride * 2);
         Kh = a.Kf + (size_t)hk * a.k_hs;
@@ -182,6 +191,36 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_s
 #else
         (void)kb; (void)slot;
 #endif
+    };
+    // Ragged V^T rows: the thread's chunks (those of its DMA slots) at any 2-byte address, a tile ahead; the last ones of a
+    // row lie at its last eight keys, and are moved into place, zeros behind them, on their way to LDS.
+    [[maybe_unused]] i32x4 rv[CF::VINS];
+    auto load_rv = [&](int kb) __attribute__((always_inline)) {
+        const int key = min(key_of(min(kb, kb1 - 1)) + vkey, (int)a.stride - 8);
+#pragma unroll
+        for (int i = 0; i < CF::VINS; i++)
+            rv[i] = reinterpret_cast<const Halves8 *>(Vh + (size_t)min(32 * i + vrow, a.dv - 1) * a.stride + key)->v;
+    };
+    auto put_rv = [&](int kb, int slot) __attribute__((always_inline)) {
+        const int past = key_of(kb) + vkey + 8 - (int)a.stride;   // halves of the chunk behind the row's end
+        char *vs = smem + slot * CF::STAGE + CF::KBYTES + (wave * 64 + lane) * 16;
+        if (key_of(kb) + BK > a.stride) {
+#pragma unroll
+            for (int i = 0; i < CF::VINS; i++) {
+                i32x4 x = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {   // half e of the chunk is half e + past of the eight that were loaded
+                    int h = 0;
+#pragma unroll
+                    for (int f = 0; f < 8; f++) h = f == e + max(past, 0) ? (rv[i][f >> 1] >> (16 * (f & 1))) & 0xFFFF : h;
+                    x[e >> 1] |= h << (16 * (e & 1));
+                }
+                *reinterpret_cast<i32x4 *>(vs + i * NW * 1024) = x;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CF::VINS; i++) *reinterpret_cast<i32x4 *>(vs + i * NW * 1024) = rv[i];
+        }
     };
     // 4-bit: a thread's runs of codes. Keys: key tid / 4, words 4 g + i of run g (D 64: 2 (tid % 4) + i). Values: block
     // tid % 8 of eight keys, VD nibbles of word w.
@@ -475,7 +514,12 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_s
             lds_barrier();
             if constexpr (!C4) {
                 if (kb + 2 < kb1) dma_k(kb + 2, cur);
-                if (tile) dma_v(kb, cur);
+                if constexpr (!RV) {
+                    if (tile) dma_v(kb, cur);
+                } else {
+                    if (tile) put_rv(kb, cur);
+                    load_rv(kb + 1);
+                }
             }
             if (kb > kb0) {
                 clean_v(kb - 1, cur ^ 1);
@@ -562,9 +606,9 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && !C4) ? 2 : 1) void k_s
         }
 }
 
-template <int D, bool C4, bool CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
+template <int D, Src SRC, bool CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
 {
-    auto kern = k_serve_tiles<D, C4, CAP>;
+    auto kern = k_serve_tiles<D, SRC, CAP>;
     static_assert(Cfg<D>::LDS <= 160 * 1024, "LDS budget");
     static std::atomic<uint64_t> opted{0};
     if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), Cfg<D>::LDS, opted)) return e;
@@ -574,8 +618,9 @@ template <int D, bool C4, bool CAP> hipError_t launch_c(const TileArgs &ta, unsi
 template <int D> hipError_t launch(const TileArgs &ta, unsigned wgs, hipStream_t s)
 {
     const bool cap = ta.a.softcap != 0.f;
-    if (ta.a.Kf) return cap ? launch_c<D, false, true>(ta, wgs, s) : launch_c<D, false, false>(ta, wgs, s);
-    return cap ? launch_c<D, true, true>(ta, wgs, s) : launch_c<D, true, false>(ta, wgs, s);
+    if (!ta.a.Kf) return cap ? launch_c<D, kCodes, true>(ta, wgs, s) : launch_c<D, kCodes, false>(ta, wgs, s);
+    if (ta.a.stride % 8) return cap ? launch_c<D, kRagged, true>(ta, wgs, s) : launch_c<D, kRagged, false>(ta, wgs, s);
+    return cap ? launch_c<D, kHalves, true>(ta, wgs, s) : launch_c<D, kHalves, false>(ta, wgs, s);
 }
 
 long row_blocks(const ServeAttn &a) { return ((long)a.gqa * a.n_tokens + BQ - 1) / BQ; }
@@ -601,6 +646,7 @@ size_t serve_tiles_ws(const ServeAttn &a)
 
 hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
 {
+    if (a.Kf && a.stride % 8 && a.stride < 8) return hipErrorInvalidValue;
     TileArgs ta;
     ta.a = a;
     ta.nsplit = a.ws && a.ws_bytes >= serve_tiles_ws(a) ? splits(a) : 1;

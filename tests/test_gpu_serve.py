@@ -254,6 +254,8 @@ WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
     (2, 2, 256, 256, 129, 1000, 1001, 0, 0, 20.0), (4, 2, 64, 64, 300, 1000, 1024, 129, 70, 0.0), (2, 1, 128, 64, 257, 900, 904, 64, 3, 0.0), (3, 1, 192, 192, 140, 1111, 1111, 100, 0, 0.0),
     (2, 1, 128, 128, 300, 310, 310, 64, 300, 0.0), (2, 1, 64, 48, 200, 90, 96, 0, 0, 0.0), (2, 1, 64, 64, 150, 100, 100, 20, 2, 0.0), (1, 1, 64, 64, 130, 4000, 4000, 17, 3, 0.0),
     (2, 1, 64, 64, 20, 70, 72, 2 ** 31 - 1, 2 ** 31 - 1, 0.0), (4, 1, 256, 256, 1, 4003, 4003, 1500, 33, 0.0), (2, 1, 128, 128, 40, 5, 7, 3, 1, 0.0), (2, 1, 64, 64, 20, 3000, 3000, 2000, 1, 0.0),
+    # V^T rows that end at every place of a chunk
+    *((2, 1, 64, 48, 33, n, n, 0, 0, 0.0) for n in range(185, 201)), (4, 2, 128, 128, 40, 203, 205, 64, 2, 0.0), (2, 1, 256, 192, 40, 195, 195, 0, 0, 0.0), (2, 1, 64, 64, 40, 9, 9, 0, 0, 0.0),
 ]
 
 
