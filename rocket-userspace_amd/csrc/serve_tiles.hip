@@ -50,7 +50,8 @@ struct __attribute__((packed, aligned(2))) Halves8 { i32x4 v; };
 
 struct TileArgs {
     ServeAttn a;
-    int nsplit, nqb;   // shares of the key tiles; row blocks of BQ
+    int nsplit, nqb;   // shares of the key tiles; row blocks of a KV head
+    int len, per;      // rows of a run that is cut into blocks of BQ: a head's T or all of a KV head's; blocks of a run
     void *part;        // [split][row][dv] fp16 outputs (divided by the split's sum), then [split][row] (max, sum)
 };
 
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int T = a.n_tokens, R = a.gqa * T, kvh = a.n_head / a.gqa;
+    const int T = a.n_tokens, kvh = a.n_head / a.gqa;
     // Workgroup w runs on XCD w % 8; each XCD gets a contiguous range of logical ids, and consecutive ids are
     // the row blocks that read the same keys.
     int qb, hk, zs, s;
@@ -103,10 +104,10 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     }
     const int n = a.seq_len ? a.seq_len[s] : a.max_kv;
     const bool served = n >= 1 && n <= a.max_kv;
-    // the block's rows: head r / T of the KV head, token r % T; the lane's row and its position
-    const int r = qb * BQ + wave * 32 + l32;
-    const bool qok = r < R;
-    const int r0 = qb * BQ, r1 = min(R, r0 + BQ) - 1;
+    // the block's rows r0 .. r1 of the KV head's (head r / T of it, token r % T); the lane's row and its position
+    const int run0 = qb / ta.per * ta.len, r0 = run0 + qb % ta.per * BQ, r1 = min(run0 + ta.len, r0 + BQ) - 1;
+    const int r = r0 + wave * 32 + l32;
+    const bool qok = r <= r1;
     const bool one = r0 / T == r1 / T;
     const int p_lo = n - T + (one ? r0 % T : 0), p_hi = n - T + (one ? r1 % T : T - 1);
     const int pos = n - T + r % T;
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     // which widened codes lie)
     f16x8 qf[KC];
     {
-        const _Float16 *qrow = a.Q + (row0 + min(r, R - 1)) * a.dk + 8 * hh;   // (rows behind the last repeat it)
+        const _Float16 *qrow = a.Q + (row0 + min(r, r1)) * a.dk + 8 * hh;   // (rows behind the last repeat it)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             f16x8 x = *reinterpret_cast<const f16x8 *>(qrow + min(16 * c, a.dk - 16));
@@ -623,17 +624,30 @@ template <int D> hipError_t launch(const TileArgs &ta, unsigned wgs, hipStream_t
     return cap ? launch_c<D, kHalves, true>(ta, wgs, s) : launch_c<D, kHalves, false>(ta, wgs, s);
 }
 
-long row_blocks(const ServeAttn &a) { return ((long)a.gqa * a.n_tokens + BQ - 1) / BQ; }
+// Row blocks of a KV head: its rows in a row, or each head's tokens by themselves, which takes more blocks where the
+// tokens are no multiple of one, but leaves none with rows of two heads, the first tokens of one and the last of the
+// other, which between them see every tile of the call: whichever has fewer tiles to visit.
+struct Blocks {
+    long len, per, all;
+};
+Blocks row_blocks(const ServeAttn &a)
+{
+    const long T = a.n_tokens, R = (long)a.gqa * T, w = a.window ? std::min(a.window, a.max_kv) : a.max_kv;
+    const long flat = (R + BQ - 1) / BQ, head = (T + BQ - 1) / BQ, mixed = T % BQ ? std::min<long>(a.gqa - 1, flat) : 0;
+    const long seen = a.window ? BQ + w : w;
+    if (a.window && T > BQ && head * a.gqa * seen < (flat - mixed) * seen + mixed * (T + w)) return {T, head, head * a.gqa};
+    return {R, flat, flat};
+}
 
 int splits(const ServeAttn &a)
 {
-    // enough workgroups for every CU (256), and two on one where the registers allow it, each split keeping at least 4 of
+    // enough workgroups for every CU (256), and two on one where the registers allow it, each split keeping at least 2 of
     // the tiles that a block may see
     const int d = std::max(a.dk, a.dv);
-    const long wgs = row_blocks(a) * (a.n_head / a.gqa) * a.n_seq, want = d <= 64 || (d <= 128 && a.Kf) ? 512 : 256;
+    const long wgs = row_blocks(a).all * (a.n_head / a.gqa) * a.n_seq, want = d <= 64 || (d <= 128 && a.Kf) ? 512 : 256;
     long tiles = (a.max_kv + BK - 1) / BK;
     if (a.window) tiles = std::min<long>(tiles, (std::min(a.sinks, a.max_kv) + BK - 1) / BK + ((long)std::min(a.n_tokens, BQ) + a.window - 2) / BK + 2);
-    return (int)std::max<long>(1, std::min<long>({(want + wgs - 1) / wgs, tiles / 4, 16}));
+    return (int)std::max<long>(1, std::min<long>({(want + wgs - 1) / wgs, tiles / 2, 16}));
 }
 
 }  // namespace
@@ -651,9 +665,12 @@ hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
     ta.a = a;
     ta.nsplit = a.ws && a.ws_bytes >= serve_tiles_ws(a) ? splits(a) : 1;
     ta.part = a.ws;
-    const long nqb = row_blocks(a), wgs = nqb * (a.n_head / a.gqa) * a.n_seq * ta.nsplit;
+    const Blocks b = row_blocks(a);
+    const long wgs = b.all * (a.n_head / a.gqa) * a.n_seq * ta.nsplit;
     if (wgs > 0x7FFFFFFFL) return hipErrorInvalidValue;
-    ta.nqb = (int)nqb;
+    ta.nqb = (int)b.all;
+    ta.len = (int)b.len;
+    ta.per = (int)b.per;
     const int d = std::max(a.dk, a.dv);
     const hipError_t e = d <= 64 ? launch<64>(ta, (unsigned)wgs, s) : d <= 128 ? launch<128>(ta, (unsigned)wgs, s) : launch<256>(ta, (unsigned)wgs, s);
     *blocks = (uint64_t)wgs;
