@@ -2,7 +2,7 @@
 //
 // What bounds it is how fast the codes arrive, and then the VALU that widens them: about two
 // operations a value, whatever the number of query rows. So all rows of a KV head (its query heads'
-// tokens, at most 32, in blocks of 16) share one widening. A workgroup owns a place of the batch, a KV head and a range
+// tokens, at most 64, in blocks of 16) share one widening. A workgroup owns a place of the batch, a KV head and a range
 // of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
 // they lie in the cache, the next chunk's while this one's are widened.
 //
@@ -29,7 +29,7 @@ typedef float    f32x2 __attribute__((ext_vector_type(2)));
 typedef float    f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 32, kChunk = 32, kWaves = 4, kMaxSplit = 64;
+constexpr int kChunk = 32, kWaves = 4, kMaxSplit = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4RowArgs {
@@ -358,6 +358,9 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
     }
 }
 
+// Blocks of 16 rows that a KV head's queries make.
+int row_blocks(const ServeAttn &a) { return (a.gqa * a.n_tokens + 15) / 16; }
+
 template <int D, int NQ, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
 {
     auto kern = k_kv4_rows<D, NQ, CAP, FULL>;
@@ -381,7 +384,11 @@ template <int D, int NQ> hipError_t launch_q(const Kv4RowArgs &ra, hipStream_t s
 }
 template <int D> hipError_t launch(const Kv4RowArgs &ra, hipStream_t s)
 {
-    return ra.a.gqa * ra.a.n_tokens <= 16 ? launch_q<D, 1>(ra, s) : launch_q<D, 2>(ra, s);
+    const int nq = row_blocks(ra.a);
+    if constexpr (D <= 128) {
+        if (nq > 2) return launch_q<D, 4>(ra, s);
+    }
+    return nq == 1 ? launch_q<D, 1>(ra, s) : launch_q<D, 2>(ra, s);
 }
 
 // Chunks that a sequence of up to max_kv keys may have to visit.
@@ -396,15 +403,23 @@ int most_chunks(const ServeAttn &a)
 void split_of(const ServeAttn &a, int *nsplit, int *cps)
 {
     const int chunks = most_chunks(a);
+    // As many workgroups as the CUs hold at once, a wave of each a SIMD: one more round, or a few workgroups of one, costs
+    // more than longer shares (1024 for all: 16 sequences of 4000 keys, heads of 256, one row 34.8 us, 512 30.9; 24 rows
+    // 66.9, 256 49.5; heads of 128, 20 rows 33.1, 512 29.3).
+    const int d = std::max(a.dk, a.dv), nq = row_blocks(a);
+    const long resident = 256 * (nq == 1 ? (d <= 128 ? 4 : 2) : nq == 2 ? (d <= 64 ? 3 : d <= 128 ? 2 : 1) : d <= 64 ? 2 : 1);
     const long wgs = (long)a.c.heads * a.n_seq;
-    const int n = (int)std::max<long>(1, std::min<long>({(chunks + kWaves - 1) / kWaves, 1024 / wgs, kMaxSplit}));
+    const int n = (int)std::max<long>(1, std::min<long>({(chunks + kWaves - 1) / kWaves, resident / wgs, kMaxSplit}));
     *cps = (chunks + n - 1) / n;
     *nsplit = (chunks + *cps - 1) / *cps;
 }
 
 }  // namespace
 
-bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= kRows; }
+// Up to 64 rows (heads of more than 128, whose outputs do not fit the registers, 32). In tiles of 128 rows, at 16000 keys of
+// one sequence, heads of 128: 20 rows 28.1 us, here 16.3; 64 rows 38.8 and 24.9; at 16 sequences of 4000 keys 63.5 and 29.3,
+// 66.0 and 61.2. (Short sequences of narrow heads, 64 rows: 32 of 1000 keys, 2 heads of 64, 15.4 and 21.1.)
+bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= (std::max(a.dk, a.dv) <= 128 ? 64 : 32); }
 
 size_t kv4_rows_ws(const ServeAttn &a)
 {

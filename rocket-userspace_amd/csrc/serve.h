@@ -84,7 +84,7 @@ bool serve_few_rows(const ServeAttn &a);
 size_t serve_attn_ws(const ServeAttn &a);
 hipError_t serve_attn(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 
-// At most 16 query rows a KV head over the cache (kv4_rows.hip).
+// Few query rows a KV head over the cache (kv4_rows.hip).
 bool kv4_few_rows(const ServeAttn &a);
 size_t kv4_rows_ws(const ServeAttn &a);
 hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks);

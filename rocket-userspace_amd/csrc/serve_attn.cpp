@@ -1,4 +1,4 @@
-// serve_attn.cpp — which kernel a serving attention call takes: few query rows a KV head (at most 16) run in
+// serve_attn.cpp — which kernel a serving attention call takes: few query rows a KV head run in
 // registers, over codes (kv4_rows.hip) or fp16 keys (attn_decode.hip), more in tiles (serve_tiles.hip).
 #include "attn.h"
 #include "serve.h"

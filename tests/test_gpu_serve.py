@@ -137,6 +137,8 @@ KV4 = [  # heads, kv heads, dk, dv, tokens, lengths (the largest is max_kv), win
     (4, 4, 160, 224, 2, [333], 0, 0, 30.0), (2, 2, 192, 128, 16, [100, 17], 0, 0, 0.0), (4, 2, 128, 128, 7, [300, 200], 0, 0, 0.0),
     (4, 2, 128, 64, 17, [300, 40], 0, 0, 0.0), (2, 1, 256, 256, 70, [200], 0, 0, 0.0), (8, 8, 64, 64, 130, [130, 300, 77], 0, 0, 0.0),
     (6, 2, 96, 160, 200, [900], 0, 0, 50.0), (4, 1, 128, 128, 129, [64, 513], 0, 0, 0.0),
+    (4, 1, 64, 64, 9, [500, 36, 35], 0, 0, 0.0), (8, 2, 128, 128, 16, [300, 15], 50, 3, 0.0), (4, 2, 96, 64, 32, [700], 0, 0, 20.0), (2, 1, 128, 32, 24, [65, 24, 7], 9, 2, 0.0),
+    (2, 1, 64, 64, 33, [300, 60], 0, 0, 0.0), (5, 1, 128, 128, 13, [400], 100, 0, 0.0), (2, 1, 160, 160, 16, [200, 31], 0, 0, 0.0), (2, 1, 256, 256, 17, [200, 31], 40, 4, 0.0),
     # windows: inside a chunk, across chunks, one key, more than the keys; sinks that meet the window, and that lie past it
     (4, 2, 64, 64, 1, [500, 20], 64, 4, 0.0), (4, 2, 128, 128, 5, [411, 3, 70], 33, 1, 0.0), (2, 2, 256, 128, 1, [1025], 1, 0, 0.0),
     (8, 2, 128, 128, 40, [600, 90], 100, 5, 0.0), (2, 1, 64, 64, 300, [1000], 129, 70, 0.0), (3, 1, 64, 64, 33, [200, 100], 1000, 1000, 20.0),
