@@ -141,8 +141,9 @@ __global__ __launch_bounds__(256) void k_fa_merge(const float *__restrict__ part
 // D: head sizes up to this (64, 128, 256); dk a multiple of 32, dv of 16. FULL: both are D, so
 // that no load or product carries a test of its dims. WIN: token t sees the keys up to its own, n_kv - T + t, that
 // lie in its window or among the sinks; no mask and no clamp. There a row may see nothing of a chunk (a
-// finite first maximum), and values of keys that a row does not see must not reach it as 0 times an infinity.
-template <int D, bool CAP, bool FULL, bool WIN>
+// finite first maximum), and values of keys that a row does not see must not reach it as 0 times an infinity. NQ:
+// blocks of 16 rows that share a chunk's fragments.
+template <int D, int NQ, bool CAP, bool FULL, bool WIN>
 __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 {
     constexpr int KS = D / 32, VB = D / 16, LROW = D + 4;   // score steps, output blocks, LDS row (floats)
@@ -151,24 +152,28 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x, zs = blockIdx.y;
     const int R = a.gqa * a.T;
-    const int hg = c / a.T, t = c - hg * a.T;               // this lane's query: head hk gqa + hg, token t
-    const bool qok = c < R;
-
-    i32x4 qf[KS];
-    {
-        const _Float16 *qrow = a.Q + (size_t)(hk * a.gqa + (qok ? hg : 0)) * a.q_hs + (size_t)(qok ? t : 0) * a.q_rs;
+    // this lane's queries: row 16 x + c, head hk gqa + row / T, token row % T
+    bool qok[NQ];
+    int t[NQ], pos[NQ], behind[NQ];                         // (position; the last key behind the token's window)
+    i32x4 qf[NQ][KS];
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        const int r = 16 * x + c, hg = r / a.T;
+        t[x] = r - hg * a.T;
+        qok[x] = r < R;
+        pos[x] = a.n_kv - a.T + t[x];
+        behind[x] = a.window ? pos[x] - a.window : -1;
+        const _Float16 *qrow = a.Q + (size_t)(hk * a.gqa + (qok[x] ? hg : 0)) * a.q_hs + (size_t)(qok[x] ? t[x] : 0) * a.q_rs;
 #pragma unroll
         for (int s = 0; s < KS; s++)
-            qf[s] = (qok && (FULL || 32 * s < a.dk)) ? *reinterpret_cast<const i32x4 *>(qrow + 32 * s + 8 * q) : i32x4{0, 0, 0, 0};
+            qf[x][s] = (qok[x] && (FULL || 32 * s < a.dk)) ? *reinterpret_cast<const i32x4 *>(qrow + 32 * s + 8 * q) : i32x4{0, 0, 0, 0};
     }
     const Rsrc rk = rsrc(a.K + (size_t)hk * a.k_hs, (uint32_t)((long)a.n_kv * a.k_rs * 2));   // keys past n_kv: zeros
     const _Float16 *const Vh = a.Vt + (size_t)hk * a.v_hs + (size_t)c * a.v_rs;              // rows 16 j + c
-    const _Float16 *const mrow = !WIN && a.mask ? a.mask + (size_t)t * a.m_rs : nullptr;
-    const int pos = a.n_kv - a.T + t;
+    const _Float16 *const mrow = !WIN && a.mask ? a.mask + (size_t)t[0] * a.m_rs : nullptr;
     auto key_of = [&](int ch) __attribute__((always_inline)) { return (WIN && ch >= a.ns ? ch + a.skip : ch) * kChunk; };
     // (no short circuits: a branch a score takes longer, and the compiler lost a lane's mask among them)
-    const int behind = a.window ? pos - a.window : -1;   // the last key behind the token's window
-    auto sees = [&](int key) __attribute__((always_inline)) { return (bool)((key <= pos) & ((key > behind) | (key < a.sinks))); };
+    auto sees = [&](int x, int key) __attribute__((always_inline)) { return (bool)((key <= pos[x]) & ((key > behind[x]) | (key < a.sinks))); };
 
     i32x4 kf[2][KS], vf[VB];
     const uint32_t ko = (uint32_t)((8 * (c >> 2) + (c & 3)) * a.k_rs + 8 * q) * 2u, k4 = (uint32_t)(4 * a.k_rs) * 2u;
@@ -194,10 +199,15 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
         }
     };
 
-    float m_run = WIN ? -1e30f : -INFINITY, l_run = 0.f;
-    f32x4 O[VB];
+    float m_run[NQ], l_run[NQ];
+    f32x4 O[NQ][VB];
 #pragma unroll
-    for (int j = 0; j < VB; j++) O[j] = f32x4{};
+    for (int x = 0; x < NQ; x++) {
+        m_run[x] = WIN ? -1e30f : -INFINITY;
+        l_run[x] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VB; j++) O[x][j] = f32x4{};
+    }
     const int chunks = WIN ? a.count : (a.n_kv + kChunk - 1) / kChunk;
     const int c1 = min(chunks, (zs + 1) * a.cps);
     int ch = zs * a.cps + wave;
@@ -207,14 +217,16 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
     }
     for (; ch < c1; ch += kWaves) {
         const int key0 = key_of(ch);
-        f32x4 S[2] = {};
+        f32x4 S[NQ][2] = {};
 #pragma unroll
         for (int s = 0; s < KS; s++)
             if (FULL || 32 * s < a.dk) {
 #pragma unroll
                 for (int b = 0; b < 2; b++)
-                    S[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[b][s]), __builtin_bit_cast(f16x8, qf[s]),
-                                                                  S[b], 0, 0, 0);
+#pragma unroll
+                    for (int x = 0; x < NQ; x++)
+                        S[x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[b][s]),
+                                                                         __builtin_bit_cast(f16x8, qf[x][s]), S[x][b], 0, 0, 0);
             }
         const bool more = ch + kWaves < c1;
         const int next = WIN ? key_of(more ? ch + kWaves : ch) : key0 + kWaves * kChunk;
@@ -225,35 +237,6 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
         i32x4 mw = {0, 0, 0, 0};
         if (mrow) mw = row8(mrow, key0 + 8 * q, a.n_kv);
         const f16x8 mv = __builtin_bit_cast(f16x8, mw);
-        float v[8], mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float x = S[i >> 2][i & 3];
-            if constexpr (WIN) v[i] = CAP ? softcap_log2(x, a.scale, a.softcap) : x * (a.scale * kLog2e);
-            else if constexpr (CAP) v[i] = fmaxf(a.softcap * tanhf(x * a.scale / a.softcap) + (float)mv[i], -30000.f) * kLog2e;
-            else v[i] = fmaxf(fmaf((float)mv[i], kLog2e, x * (a.scale * kLog2e)), -30000.f * kLog2e);
-            if constexpr (!WIN) {
-                if (key0 + 8 * q + i >= a.n_kv) v[i] = -INFINITY;   // weighs 0
-                mx = fmaxf(mx, v[i]);
-            }
-        }
-        if constexpr (WIN) {
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = sees(key0 + 8 * q + i) ? v[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (__any(mx > m_run)) {   // (a chunk has a key below n_kv, so without a window the new maximum is finite)
-            const float m_new = fmaxf(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-            m_run = m_new;
-            l_run *= alpha;
-#pragma unroll
-            for (int j = 0; j < VB; j++) O[j] *= alpha;
-        }
         if constexpr (WIN) {
             if (!whole) {
                 // keys that no row sees: their values count as 0
@@ -265,61 +248,104 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
                 }
 #pragma unroll
                 for (int j = 0; j < VB; j++) vf[j] &= live;
-                // a non-finite value of a key that some rows see: those take it here, the products take 0
-                if (a.T > 1) {
-                    bool bad = false;
+            }
+        }
+        f16x8 p[NQ];
 #pragma unroll
-                    for (int j = 0; j < VB; j++)
+        for (int x = 0; x < NQ; x++) {
+            float v[8], mx = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) bad |= (vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
-                    if (__builtin_expect(__any(bad), 0)) {
-                        const uint16_t *const vr = reinterpret_cast<const uint16_t *>(a.Vt + (size_t)hk * a.v_hs);
+            for (int i = 0; i < 8; i++) {
+                const float y = S[x][i >> 2][i & 3];
+                if constexpr (WIN) v[i] = CAP ? softcap_log2(y, a.scale, a.softcap) : y * (a.scale * kLog2e);
+                else if constexpr (CAP) v[i] = fmaxf(a.softcap * tanhf(y * a.scale / a.softcap) + (float)mv[i], -30000.f) * kLog2e;
+                else v[i] = fmaxf(fmaf((float)mv[i], kLog2e, y * (a.scale * kLog2e)), -30000.f * kLog2e);
+                if constexpr (!WIN) {
+                    if (key0 + 8 * q + i >= a.n_kv) v[i] = -INFINITY;   // weighs 0
+                    mx = fmaxf(mx, v[i]);
+                }
+            }
+            if constexpr (WIN) {
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = sees(x, key0 + 8 * q + i) ? v[i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(mx > m_run[x])) {   // (a chunk has a key below n_kv, so without a window the new maximum is finite)
+                const float m_new = fmaxf(m_run[x], mx), alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
+                m_run[x] = m_new;
+                l_run[x] *= alpha;
+#pragma unroll
+                for (int j = 0; j < VB; j++) O[x][j] *= alpha;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float e = __builtin_amdgcn_exp2f(v[i] - m_run[x]);
+                l_run[x] += e;
+                p[x][i] = (_Float16)e;
+            }
+        }
+        if constexpr (WIN) {
+            // a non-finite value of a key that some rows see: those take it here, the products take 0
+            if (!whole && a.T > 1) {
+                bool bad = false;
+#pragma unroll
+                for (int j = 0; j < VB; j++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) bad |= (vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
+                if (__builtin_expect(__any(bad), 0)) {
+                    const uint16_t *const vr = reinterpret_cast<const uint16_t *>(a.Vt + (size_t)hk * a.v_hs);
+#pragma unroll
+                    for (int x = 0; x < NQ; x++)
 #pragma unroll 1
                         for (int i = 0; i < VB * 4; i++) {   // (rolled, and the register picked by comparison: this is rare)
                             const int d = 16 * (i >> 2) + 4 * q + (i & 3);
-                            float x = 0.f;
+                            float y = 0.f;
 #pragma unroll 1
                             for (int j = 0; d < a.dv && j < kChunk && key0 + j < a.n_kv; j++) {
                                 const uint16_t w = vr[(size_t)d * a.v_rs + key0 + j];
-                                if ((w & 0x7C00) == 0x7C00 && sees(key0 + j)) x += (float)__builtin_bit_cast(_Float16, w);
+                                if ((w & 0x7C00) == 0x7C00 && sees(x, key0 + j)) y += (float)__builtin_bit_cast(_Float16, w);
                             }
 #pragma unroll
                             for (int j = 0; j < VB; j++)
 #pragma unroll
-                                for (int e = 0; e < 4; e++) O[j][e] = i == 4 * j + e ? O[j][e] + x : O[j][e];
+                                for (int e = 0; e < 4; e++) O[x][j][e] = i == 4 * j + e ? O[x][j][e] + y : O[x][j][e];
                         }
 #pragma unroll
-                        for (int j = 0; j < VB; j++)
+                    for (int j = 0; j < VB; j++)
 #pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                if ((vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00) vf[j][i >> 1] &= 0xFFFF << (16 * (~i & 1));
-                    }
+                        for (int i = 0; i < 8; i++)
+                            if ((vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00) vf[j][i >> 1] &= 0xFFFF << (16 * (~i & 1));
                 }
             }
         }
-        f16x8 p;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float e = __builtin_amdgcn_exp2f(v[i] - m_run);
-            l_run += e;
-            p[i] = (_Float16)e;
-        }
 #pragma unroll
         for (int j = 0; j < VB; j++)
-            if (FULL || 16 * j < a.dv) O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vf[j]), p, O[j], 0, 0, 0);
+            if (FULL || 16 * j < a.dv) {
+#pragma unroll
+                for (int x = 0; x < NQ; x++)
+                    O[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vf[j]), p[x], O[x][j], 0, 0, 0);
+            }
         if (more) load_v(next);
     }
-    l_run += __shfl_xor(l_run, 16, 64);
-    l_run += __shfl_xor(l_run, 32, 64);
 
     // merge the waves: [wave][row][LROW] outputs, then [wave][row] (max, sum)
     float *const Ol = reinterpret_cast<float *>(smem);
     f32x2 *const ml = reinterpret_cast<f32x2 *>(Ol + kWaves * R * LROW);
-    if (qok) {
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        l_run[x] += __shfl_xor(l_run[x], 16, 64);
+        l_run[x] += __shfl_xor(l_run[x], 32, 64);
+        if (!qok[x]) continue;
+        const int row = wave * R + 16 * x + c;
 #pragma unroll
         for (int j = 0; j < VB; j++)
-            if (FULL || 16 * j < a.dv) *reinterpret_cast<f32x4 *>(Ol + (wave * R + c) * LROW + 16 * j + 4 * q) = O[j];
-        if (q == 0) ml[wave * R + c] = f32x2{m_run, l_run};
+            if (FULL || 16 * j < a.dv) *reinterpret_cast<f32x4 *>(Ol + row * LROW + 16 * j + 4 * q) = O[x][j];
+        if (q == 0) ml[row] = f32x2{m_run[x], l_run[x]};
     }
     __syncthreads();
     const int dq = a.dv / 4;
@@ -353,25 +379,38 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
     }
 }
 
-template <int D, bool CAP, bool FULL, bool WIN> hipError_t launch_rows_f(const RowArgs &a, int kv_heads, hipStream_t s)
+template <int D, int NQ, bool CAP, bool FULL, bool WIN> hipError_t launch_rows_f(const RowArgs &a, int kv_heads, hipStream_t s)
 {
-    auto kern = k_fa_rows<D, CAP, FULL, WIN>;
+    auto kern = k_fa_rows<D, NQ, CAP, FULL, WIN>;
     const int R = a.gqa * a.T;
     const size_t lds = (size_t)kWaves * R * ((D + 4) * 4 + 8);
     if (lds > 64 * 1024) {
         static std::atomic<uint64_t> opted{0};
-        if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), 80 * 1024, opted)) return e;
+        constexpr int most = kWaves * 16 * NQ * ((D + 4) * 4 + 8);
+        static_assert(most <= 160 * 1024, "LDS budget");
+        if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), most, opted)) return e;
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)kv_heads, (unsigned)a.nsplit), dim3(kWaves * 64), lds, s, a);
     return hipGetLastError();
 }
 
-template <int D, bool WIN> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
+template <int D, int NQ, bool WIN> hipError_t launch_rows_q(const RowArgs &a, int kv_heads, hipStream_t s)
 {
     const bool cap = a.softcap != 0.f;
     if (a.dk == D && a.dv == D)
-        return cap ? launch_rows_f<D, true, true, WIN>(a, kv_heads, s) : launch_rows_f<D, false, true, WIN>(a, kv_heads, s);
-    return cap ? launch_rows_f<D, true, false, WIN>(a, kv_heads, s) : launch_rows_f<D, false, false, WIN>(a, kv_heads, s);
+        return cap ? launch_rows_f<D, NQ, true, true, WIN>(a, kv_heads, s) : launch_rows_f<D, NQ, false, true, WIN>(a, kv_heads, s);
+    return cap ? launch_rows_f<D, NQ, true, false, WIN>(a, kv_heads, s) : launch_rows_f<D, NQ, false, false, WIN>(a, kv_heads, s);
+}
+template <int D, bool WIN> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
+{
+    if constexpr (WIN) {
+        const int nq = (a.gqa * a.T + 15) / 16;
+        if constexpr (D <= 64) {
+            if (nq > 2) return launch_rows_q<D, 4, WIN>(a, kv_heads, s);
+        }
+        if (nq > 1) return launch_rows_q<D, 2, WIN>(a, kv_heads, s);
+    }
+    return launch_rows_q<D, 1, WIN>(a, kv_heads, s);
 }
 template <bool WIN> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
 {
@@ -413,8 +452,12 @@ void split_of(const FaLaunch &L, int *nsplit, int *cps)
 
 bool flash_attn_few_rows(const FaLaunch &L)
 {
-    if ((long)L.gqa * L.T > kRows || L.n_kv < 8 || L.dk % 32 || L.dv % 16) return false;
-    if (L.win) return true;
+    if (L.n_kv < 8 || L.dk % 32 || L.dv % 16) return false;
+    // Under a window up to 32 rows, of heads of up to 64 up to 64 (in tiles of 128 rows, one sequence: 20 rows of heads of
+    // 128, 4001 keys 15.9 us, here 12.4; 16000 keys 32.7 and 20.4; 24 rows of heads of 256, 4001 keys 23.1 and 19.2; 64 rows
+    // of heads of 64, 1000 keys 10.3 and 11.2, 16000 keys 26.3 and 13.2).
+    if (L.win) return (long)L.gqa * L.T <= (std::max(L.dk, L.dv) <= 64 ? 4 : 2) * kRows;
+    if ((long)L.gqa * L.T > kRows) return false;
     // One query head a KV head and long caches: the tiled kernel reads V^T in whole 128-byte lines (64
     // keys a tile, 32 here), and where its workgroups fill the CUs and nothing has to be padded it is the
     // faster one while the cache is not far larger than the memory-side cache (heads of 256, 16 x 8192

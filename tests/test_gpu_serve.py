@@ -256,6 +256,9 @@ WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
     (2, 2, 256, 256, 129, 1000, 1001, 0, 0, 20.0), (4, 2, 64, 64, 300, 1000, 1024, 129, 70, 0.0), (2, 1, 128, 64, 257, 900, 904, 64, 3, 0.0), (3, 1, 192, 192, 140, 1111, 1111, 100, 0, 0.0),
     (2, 1, 128, 128, 300, 310, 310, 64, 300, 0.0), (2, 1, 64, 48, 200, 90, 96, 0, 0, 0.0), (2, 1, 64, 64, 150, 100, 100, 20, 2, 0.0), (1, 1, 64, 64, 130, 4000, 4000, 17, 3, 0.0),
     (2, 1, 64, 64, 20, 70, 72, 2 ** 31 - 1, 2 ** 31 - 1, 0.0), (4, 1, 256, 256, 1, 4003, 4003, 1500, 33, 0.0), (2, 1, 128, 128, 40, 5, 7, 3, 1, 0.0), (2, 1, 64, 64, 20, 3000, 3000, 2000, 1, 0.0),
+    (4, 1, 64, 64, 9, 500, 500, 0, 0, 0.0), (8, 2, 128, 128, 8, 301, 301, 50, 3, 0.0), (4, 2, 96, 64, 16, 700, 700, 0, 0, 20.0), (2, 1, 64, 32, 24, 65, 70, 9, 2, 0.0),
+    (5, 1, 64, 64, 13, 400, 400, 100, 0, 0.0), (4, 2, 128, 80, 15, 333, 333, 300, 1, 0.0), (2, 1, 256, 256, 16, 200, 203, 40, 4, 0.0), (2, 1, 160, 176, 9, 13, 13, 5, 1, 0.0),
+    (2, 1, 128, 128, 70, 400, 401, 33, 5, 0.0), (4, 4, 256, 256, 33, 300, 300, 0, 0, 0.0),
     # V^T rows that end at every place of a chunk
     *((2, 1, 64, 48, 33, n, n, 0, 0, 0.0) for n in range(185, 201)), (4, 2, 128, 128, 40, 203, 205, 64, 2, 0.0), (2, 1, 256, 192, 40, 195, 195, 0, 0, 0.0), (2, 1, 64, 64, 40, 9, 9, 0, 0, 0.0),
 ]
@@ -298,10 +301,11 @@ def test_window_attn(lib, fd, case, kind):
     assert np.array_equal(*outs)
 
 
-@pytest.mark.parametrize("T,n,window,sinks", [(5, 200, 30, 2), (130, 400, 50, 3), (20, 333, 0, 0)])
-def test_window_attn_values_that_some_tokens_see(lib, fd, T, n, window, sinks):
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("T,n,window,sinks", [(5, 200, 30, 2), (130, 400, 50, 3), (130, 403, 50, 3), (16, 333, 0, 0), (30, 333, 100, 1)])
+def test_window_attn_values_that_some_tokens_see(lib, fd, T, n, window, sinks, d):
     """An infinite value reaches the tokens that see its key, and no other (0 times it would be NaN)."""
-    heads, kvh, d = 2, 1, 64
+    heads, kvh = 2, 1
     Q, K, V, see = win_case(21, heads, kvh, d, d, T, n, n, window, sinks)
     j = n - T + T // 2   # the middle token's own position
     V[0, 3, j] = np.inf
