@@ -39,11 +39,6 @@ constexpr int kAttnMaxHeadDim = 256;
 
 hipError_t flash_attn(const FaLaunch &L, hipStream_t s, uint64_t *blocks_out);
 
-// Merges key-axis splits: part holds [split][head][T][dv] fp16 outputs, each divided by its split's sum, then
-// [split][head][T] (max in log2 units, sum) fp32 pairs; up to 16 splits.
-hipError_t flash_attn_combine(const void *part, _Float16 *O, long o_hs, long o_rs, int n_head, int T, int dv, int nsplit, hipStream_t s,
-                              uint64_t *blocks_out);
-
 // Whether the tiled kernel's workgroups (128 queries of a head, a share of the keys) fill the CUs in
 // whole rounds.
 bool flash_attn_tiles_fill(const FaLaunch &L);

@@ -713,20 +713,17 @@ hipError_t flash_attn(const FaLaunch &L, hipStream_t s, uint64_t *blocks_out)
     if (blocks_out) *blocks_out = (uint64_t)wgs;
     const hipError_t e = launch_fa_dims(a, mvec, dhp, dvp, grid, s);
     if (e != hipSuccess || a.nsplit == 1) return e;
-    uint64_t blocks = 0;
-    const hipError_t ec = flash_attn_combine(a.part, L.O, L.o_hs, L.o_rs, L.n_head, L.T, L.dv, a.nsplit, s, &blocks);
-    if (blocks_out) *blocks_out += blocks;
-    return ec;
-}
-
-hipError_t flash_attn_combine(const void *part, _Float16 *O, long o_hs, long o_rs, int n_head, int T, int dv, int nsplit, hipStream_t s,
-                              uint64_t *blocks_out)
-{
-    const long n = (long)n_head * T * (dv / 8), blocks = (n + 255) / 256;
-    if (blocks > 0x7FFFFFFFL || nsplit > 16) return hipErrorInvalidValue;
-    auto *kern = nsplit <= 4 ? k_fa_combine<4> : nsplit <= 8 ? k_fa_combine<8> : k_fa_combine<16>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, part, O, o_hs, o_rs, n_head, T, dv, nsplit);
-    *blocks_out = (uint64_t)blocks;
+    const long n = (long)L.n_head * L.T * (L.dv / 8), blocks = (n + 255) / 256;
+    if (a.nsplit <= 4)
+        hipLaunchKernelGGL(k_fa_combine<4>, dim3((unsigned)blocks), dim3(256), 0, s, a.part, L.O, L.o_hs, L.o_rs,
+                           L.n_head, L.T, L.dv, a.nsplit);
+    else if (a.nsplit <= 8)
+        hipLaunchKernelGGL(k_fa_combine<8>, dim3((unsigned)blocks), dim3(256), 0, s, a.part, L.O, L.o_hs, L.o_rs,
+                           L.n_head, L.T, L.dv, a.nsplit);
+    else
+        hipLaunchKernelGGL(k_fa_combine<16>, dim3((unsigned)blocks), dim3(256), 0, s, a.part, L.O, L.o_hs, L.o_rs,
+                           L.n_head, L.T, L.dv, a.nsplit);
+    if (blocks_out) *blocks_out += (uint64_t)blocks;
     return hipGetLastError();
 }
 

@@ -12,7 +12,6 @@
 // them; K runs a tile ahead of V^T. Scores are transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so a lane
 // holds one row's scores and P stays in registers: rounded to fp16 and swapped between the half-waves
 // it is the second product's operand. O is rescaled only when some running maximum grows by more than 8.
-#include "attn.h"
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
@@ -26,6 +25,8 @@ namespace {
 
 typedef int      i32x2  __attribute__((ext_vector_type(2)));
 typedef int      i32x4  __attribute__((ext_vector_type(4)));
+typedef float    f32x2  __attribute__((ext_vector_type(2)));
+typedef float    f32x4  __attribute__((ext_vector_type(4)));
 typedef float    f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x4  __attribute__((ext_vector_type(4)));
 typedef __amdgpu_buffer_rsrc_t Rsrc;
@@ -52,7 +53,7 @@ struct TileArgs {
     ServeAttn a;
     int nsplit, nqb;   // shares of the key tiles; row blocks of a KV head
     int len, per;      // rows of a run that is cut into blocks of BQ: a head's T or all of a KV head's; blocks of a run
-    void *part;        // [split][row][dv] fp16 outputs (divided by the split's sum), then [split][row] (max, sum)
+    void *part;        // [split][row][dv] outputs (divided by the split's sum), then [split][row] (max, sum)
 };
 
 // D: 64, 128 or 256. 16-byte chunk c of an LDS row lies at slot c ^ x(row): the sixteen lanes that one
@@ -74,6 +75,13 @@ __device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T r
 // Where keys and values come from: fp16 rows by DMA; the same with V^T rows that are no whole 16-byte chunks, whose values
 // go through registers; codes.
 enum Src { kHalves, kRagged, kCodes };
+
+// Splits' outputs over fp16 keys are fp32: rounded to fp16 beside the weights and the result they would be a third rounding
+// (333 tokens under a window of 257: 2.9e-4 of the result, with it 3.4e-4). Over codes, whose widened values are rounded
+// already, they are fp16, at half the bytes (130 tokens over 1024 keys, heads of 256: 32.4 us with fp32, 25.7; 4.1e-4 and
+// 4.5e-4).
+template <Src SRC> struct Part { typedef float T; };
+template <> struct Part<kCodes> { typedef _Float16 T; };
 
 template <int D, Src SRC, bool CAP>
 __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1) void k_serve_tiles(const TileArgs ta)
@@ -581,30 +589,72 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     const float l = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing; NaN stays)
     if (!qok) return;
-    const size_t rows = (size_t)a.n_seq * a.n_head * T;
-    _Float16 *orow;
-    if (ta.nsplit > 1) {
-        orow = static_cast<_Float16 *>(ta.part) + (zs * rows + row0 + r) * a.dv;
-        if (hh == 0) {
-            float *pml = reinterpret_cast<float *>(static_cast<_Float16 *>(ta.part) + ta.nsplit * rows * a.dv) + 2 * (zs * rows + row0 + r);
-            pml[0] = m_run;
-            pml[1] = l;
-        }
-    } else {
-        orow = a.out + (row0 + r) * a.dv;
-    }
+    const size_t rows = (size_t)a.n_seq * a.n_head * T, prow = zs * rows + row0 + r;
+    typedef typename Part<SRC>::T P_;
+    typedef P_ P4 __attribute__((ext_vector_type(4)));
+    P_ *const part = static_cast<P_ *>(ta.part);
+    if (ta.nsplit > 1 && hh == 0) reinterpret_cast<f32x2 *>(part + ta.nsplit * rows * a.dv)[prow] = f32x2{m_run, l};
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             const int d0 = 32 * db + 8 * b + 4 * hh;
             if (32 * db + 8 * b < a.dv) {   // (dv is a multiple of 16: the same for both half-waves)
-                f16x4 v;
+                f32x4 v;
 #pragma unroll
-                for (int c = 0; c < 4; c++) v[c] = (_Float16)(O[db][4 * b + c] * inv);
-                *reinterpret_cast<f16x4 *>(orow + d0) = v;
+                for (int c = 0; c < 4; c++) v[c] = O[db][4 * b + c] * inv;
+                if (ta.nsplit > 1) {
+                    *reinterpret_cast<P4 *>(part + prow * a.dv + d0) = P4{(P_)v[0], (P_)v[1], (P_)v[2], (P_)v[3]};
+                } else {
+                    const f16x4 h = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+                    *reinterpret_cast<f16x4 *>(a.out + (row0 + r) * a.dv + d0) = h;
+                }
             }
         }
+}
+
+// Merges the splits: out = sum_s w_s O_s / sum_s w_s with w_s = 2^(m_s - m) l_s, m the largest of the m_s, for four output
+// dims of a row a thread; every split's pair and outputs are loaded before the first is used.
+template <typename P, int MAXS>
+__global__ __launch_bounds__(256) void k_serve_combine(const P *__restrict__ part, _Float16 *__restrict__ out, long rows, int dv, int nsplit)
+{
+    const int dq = dv / 4;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, row = i / dq;
+    if (row >= rows) return;
+    const int d0 = (int)(i - row * dq) * 4;
+    const f32x2 *const ml = reinterpret_cast<const f32x2 *>(part + nsplit * rows * dv);
+    typedef P P4 __attribute__((ext_vector_type(4)));
+    f32x2 x[MAXS];
+    P4 o[MAXS];
+#pragma unroll
+    for (int s = 0; s < MAXS; s++)
+        if (s < nsplit) {
+            x[s] = ml[s * rows + row];
+            o[s] = *reinterpret_cast<const P4 *>(part + (s * rows + row) * dv + d0);
+        }
+    float m = -1e30f;
+#pragma unroll
+    for (int s = 0; s < MAXS; s++)
+        if (s < nsplit) m = fmaxf(m, x[s][0]);
+    float l = 0.f;
+    f32x4 acc = {};
+#pragma unroll
+    for (int s = 0; s < MAXS; s++)
+        if (s < nsplit) {
+            const float w = __builtin_amdgcn_exp2f(x[s][0] - m) * x[s][1];
+            l += w;
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[c] += w * (float)o[s][c];
+        }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const f16x4 h = {(_Float16)(acc[0] * inv), (_Float16)(acc[1] * inv), (_Float16)(acc[2] * inv), (_Float16)(acc[3] * inv)};
+    *reinterpret_cast<f16x4 *>(out + row * dv + d0) = h;
+}
+
+template <typename P> void combine(const TileArgs &ta, long rows, long blocks, hipStream_t s)
+{
+    auto *kern = ta.nsplit <= 4 ? k_serve_combine<P, 4> : ta.nsplit <= 8 ? k_serve_combine<P, 8> : k_serve_combine<P, 16>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const P *>(ta.part), ta.a.out, rows, ta.a.dv, ta.nsplit);
 }
 
 template <int D, Src SRC, bool CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
@@ -655,7 +705,7 @@ int splits(const ServeAttn &a)
 size_t serve_tiles_ws(const ServeAttn &a)
 {
     const int ns = splits(a);
-    return ns > 1 ? (size_t)ns * a.n_seq * a.n_head * a.n_tokens * (a.dv * sizeof(_Float16) + 2 * sizeof(float)) : 0;
+    return ns > 1 ? (size_t)ns * a.n_seq * a.n_head * a.n_tokens * (a.dv * (a.Kf ? sizeof(float) : sizeof(_Float16)) + 2 * sizeof(float)) : 0;
 }
 
 hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
@@ -675,11 +725,11 @@ hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
     const hipError_t e = d <= 64 ? launch<64>(ta, (unsigned)wgs, s) : d <= 128 ? launch<128>(ta, (unsigned)wgs, s) : launch<256>(ta, (unsigned)wgs, s);
     *blocks = (uint64_t)wgs;
     if (e != hipSuccess || ta.nsplit == 1) return e;
-    uint64_t more = 0;
-    const int rows = a.n_seq * a.n_head * a.n_tokens;
-    const hipError_t e2 = flash_attn_combine(ta.part, a.out, 0, a.dv, 1, rows, a.dv, ta.nsplit, s, &more);
-    *blocks += more;
-    return e2;
+    const long rows = (long)a.n_seq * a.n_head * a.n_tokens, n = (rows * (a.dv / 4) + 255) / 256;
+    if (a.Kf) combine<float>(ta, rows, n, s);
+    else combine<_Float16>(ta, rows, n, s);
+    *blocks += (uint64_t)n;
+    return hipGetLastError();
 }
 
 }  // namespace rk
