@@ -66,7 +66,8 @@ int rocket_qk_norm_rope_f32in(int fd, int n_seq, int n_tokens, int n_head, int n
  * One buffer of rocket_kv4_bytes(shape) bytes of device memory, 16-byte aligned, that the caller
  * owns (host memory for fd < 0). It needs no initialisation. A group of 32 values of one key or
  * value row is stored as 4-bit codes c and an fp16 (scale, minimum):
- *     minimum = min(x),  scale = fp16((max(x) - min(x)) / 15),
+ *     minimum = min(x),  scale = fp16((max(x) - min(x)) / 15)  (the next lower fp16 where 15 * scale + minimum
+ *     would not be a finite fp16),
  *     c = clamp(rint((x - minimum) / scale), 0, 15)  (0 where scale is 0),  in fp32,
  *     value = fp16(c * scale + minimum), one rounding.
  * Inputs should be finite; an infinity is taken as the largest finite fp16 of its sign, a NaN as 0.

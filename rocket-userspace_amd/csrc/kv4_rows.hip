@@ -34,7 +34,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4RowArgs {
     ServeAttn a;
-    int nsplit, cps;   // workgroups a place and KV head, chunks a workgroup
+    int nsplit;   // workgroups a place and KV head, which share the chunks that its length has
     float *part;       // [place][split][head][token][dv] outputs, then (max, sum) pairs
 };
 
@@ -54,6 +54,9 @@ struct Chunks {
     __device__ int at(int v) const { return v < ns ? v : v + skip; }
 };
 
+// Chunks a workgroup: the length's own share, so that a long bound costs a short sequence nothing (one a wave at least).
+__device__ __forceinline__ int share(int count, int nsplit) { return max(kWaves, (count + nsplit - 1) / nsplit); }
+
 // D: head sizes up to this (64, 128, 256). NQ: blocks of 16 rows. FULL: dk and dv are D.
 template <int D, int NQ, bool CAP, bool FULL>
 __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
@@ -70,7 +73,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const bool served = n >= 1 && n <= a.max_kv;
     const Chunks list(a, served ? n : 1);
     const int count = served ? list.count : 0;
-    if (zs > 0 && zs * ra.cps >= count) return;   // (the merge knows)
+    const int cps = ra.nsplit > 1 ? share(count, ra.nsplit) : max(count, 1);
+    if (zs > 0 && zs * cps >= count) return;   // (the merge knows)
     // this lane's queries: row 16 x + c of the KV head's (head r / T, token r % T), and its position
     bool qok[NQ];
     int pos[NQ], behind[NQ];                      // (the last key behind its window)
@@ -153,8 +157,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
         for (int j = 0; j < VB; j++) O[x][j] = f32x4{};
     }
-    const int c1 = min(count, (zs + 1) * ra.cps);
-    int ch = zs * ra.cps + wave;
+    const int c1 = min(count, (zs + 1) * cps);
+    int ch = zs * cps + wave;
     if (ch < c1) {
         load_k(list.at(ch) * kChunk);
         load_v(list.at(ch) * kChunk);
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
     const int tid = threadIdx.x, row = blockIdx.x, s = blockIdx.y, dv = a.dv;
     const int n = a.seq_len[s];
     const int count = n >= 1 && n <= a.max_kv ? Chunks(a, n).count : 0;
-    const int nsplit = max(1, min(ra.nsplit, (count + ra.cps - 1) / ra.cps));
+    const int cps = share(count, ra.nsplit), nsplit = max(1, (count + cps - 1) / cps);
     const size_t rows = (size_t)a.n_head * a.n_tokens, base = (size_t)s * ra.nsplit * rows + row;
     const int dq = dv / 8, sg = tid / dq, d0 = (tid - sg * dq) * 8, ng = min(8, 256 / dq);   // dv <= 256: 8
     f32x4 os[8][2];
@@ -400,7 +404,7 @@ int most_chunks(const ServeAttn &a)
     return (int)std::min<long>(all, seen);
 }
 
-void split_of(const ServeAttn &a, int *nsplit, int *cps)
+int splits(const ServeAttn &a)
 {
     const int chunks = most_chunks(a);
     // As many workgroups as the CUs hold at once, a wave of each a SIMD: one more round, or a few workgroups of one, costs
@@ -409,9 +413,7 @@ void split_of(const ServeAttn &a, int *nsplit, int *cps)
     const int d = std::max(a.dk, a.dv), nq = row_blocks(a);
     const long resident = 256 * (nq == 1 ? (d <= 128 ? 4 : 2) : nq == 2 ? (d <= 64 ? 3 : d <= 128 ? 2 : 1) : d <= 64 ? 2 : 1);
     const long wgs = (long)a.c.heads * a.n_seq;
-    const int n = (int)std::max<long>(1, std::min<long>({(chunks + kWaves - 1) / kWaves, resident / wgs, kMaxSplit}));
-    *cps = (chunks + n - 1) / n;
-    *nsplit = (chunks + *cps - 1) / *cps;
+    return (int)std::max<long>(1, std::min<long>({(chunks + kWaves - 1) / kWaves, resident / wgs, kMaxSplit}));
 }
 
 }  // namespace
@@ -423,8 +425,7 @@ bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= (std:
 
 size_t kv4_rows_ws(const ServeAttn &a)
 {
-    int n, cps;
-    split_of(a, &n, &cps);
+    const int n = splits(a);
     return n > 1 ? (size_t)a.n_seq * n * a.n_head * a.n_tokens * (a.dv + 2) * sizeof(float) : 0;
 }
 
@@ -433,11 +434,7 @@ hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
     if (a.n_seq > 65535) return hipErrorInvalidValue;
     Kv4RowArgs ra;
     ra.a = a;
-    split_of(a, &ra.nsplit, &ra.cps);
-    if (ra.nsplit > 1 && (!a.ws || a.ws_bytes < kv4_rows_ws(a))) {
-        ra.nsplit = 1;
-        ra.cps = most_chunks(a);
-    }
+    ra.nsplit = a.ws && a.ws_bytes >= kv4_rows_ws(a) ? splits(a) : 1;
     ra.part = a.ws;
     const int d = std::max(a.dk, a.dv);
     const hipError_t e = d <= 64 ? launch<64>(ra, s) : d <= 128 ? launch<128>(ra, s) : launch<256>(ra, s);

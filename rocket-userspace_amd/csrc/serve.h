@@ -3,6 +3,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -27,7 +28,14 @@ __host__ __device__ inline float kv4_finite(float x)
 {
     return x != x ? 0.f : x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;
 }
-__host__ __device__ inline _Float16 kv4_scale(float lo, float hi) { return (_Float16)((hi - lo) / 15.f); }
+// (A scale that rounded up may carry code 15 past the largest fp16: then the next lower one, so that every value that a
+// cache stands for is finite.)
+__host__ __device__ inline _Float16 kv4_scale(float lo, float hi)
+{
+    const _Float16 s = (_Float16)((hi - lo) / 15.f);
+    if (fmaf(15.f, (float)s, lo) < 65520.f) return s;
+    return __builtin_bit_cast(_Float16, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
+}
 __host__ __device__ inline int kv4_code(float x, float lo, float scale)
 {
     if (!(scale > 0.f)) return 0;

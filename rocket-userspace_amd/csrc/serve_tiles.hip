@@ -77,9 +77,9 @@ __device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T r
 enum Src { kHalves, kRagged, kCodes };
 
 // Splits' outputs over fp16 keys are fp32: rounded to fp16 beside the weights and the result they would be a third rounding
-// (333 tokens under a window of 257: 2.9e-4 of the result, with it 3.4e-4). Over codes, whose widened values are rounded
-// already, they are fp16, at half the bytes (130 tokens over 1024 keys, heads of 256: 32.4 us with fp32, 25.7; 4.1e-4 and
-// 4.5e-4).
+// (333 tokens under a window of 257: 2.7e-4 of the result, with it 3.5e-4). Over codes, whose widened values are rounded
+// already, they are fp16, at half the bytes (130 tokens over 1024 keys, heads of 256: 32.4 us with fp32, 25.7; 3.9e-4 and
+// 4.4e-4).
 template <Src SRC> struct Part { typedef float T; };
 template <> struct Part<kCodes> { typedef _Float16 T; };
 

@@ -34,6 +34,7 @@ def quantise(x):
     g = x.astype(np.float32).reshape(*x.shape[:-1], -1, 32)
     lo, hi = g.min(-1, keepdims=True) + np.float32(0), g.max(-1, keepdims=True)
     s = ((hi - lo) / np.float32(15)).astype(np.float16)
+    s = np.where(s.astype(np.float64) * 15 + lo < 65520, s, (s.view(np.uint16) - 1).astype(np.uint16).view(np.float16))
     f = s.astype(np.float32)
     with np.errstate(divide="ignore", invalid="ignore"):
         c = np.where(f > 0, np.clip(np.rint((g - lo) / f), 0, 15), 0).astype(np.uint8)

@@ -92,7 +92,8 @@ def test_cache(lib, fd, n_seq, seq0, places, H, dk, dv, cap, T, lens):
         mem2 = dev(c.buf)
         assert put(fd, C.byref(sh), R.ptr(mem2), seq0, places, T, R.ptr(K), T * H * dk, dk, H * dk, R.ptr(V), H * T * dv, T * dv, dv, R.ptr(L)) == 0
         assert np.array_equal(mem2.cpu().numpy(), c.buf)
-    k, v = c.rows()
+    with np.errstate(all="ignore"):   # (unwritten scales are any bits)
+        k, v = c.rows()
     Ko, Vo = np.full((places, H, T, dk), 7, np.float16), np.full((places, H, T, dv), 7, np.float16)
     assert lib.rocket_kv4_read_fp16(fd, C.byref(sh), R.ptr(mem), seq0, places, T, R.ptr(L), R.ptr(Ko), R.ptr(Vo)) == 0
     for s in range(places):
@@ -100,9 +101,32 @@ def test_cache(lib, fd, n_seq, seq0, places, H, dk, dv, cap, T, lens):
         ok = (at >= 0) & (at < cap)
         assert np.array_equal(Ko[s][:, ok], F.f16(k[seq0 + s][:, at[ok]])) and np.array_equal(Vo[s][:, ok], F.f16(v[seq0 + s][:, at[ok]]))
         assert not Ko[s][:, ~ok].any() and not Vo[s][:, ~ok].any()
+        assert np.isfinite(Ko[s][:, ok]).all() and np.isfinite(Vo[s][:, ok]).all()
     V2 = np.full_like(Vo, 7)
     assert lib.rocket_kv4_read_fp16(fd, C.byref(sh), R.ptr(mem), seq0, places, T, R.ptr(L), None, R.ptr(V2)) == 0
     assert np.array_equal(V2, Vo)
+
+
+def test_cache_codes_at_halves(lib, fd):
+    """Quotients on and next to the halves between codes, where the reciprocal's code has to be the division's: multiples
+    of a half step, fp16 neighbours of them, scales of every exponent, subnormal ones among them."""
+    g = rng(4)
+    T, H, d = 64, 4, 256
+    x = g.integers(0, 31, (1, T, H, d)) / 2.0
+    x[..., 0::32], x[..., 1::32] = 0, 15
+    x = F.f16(x * 2.0 ** g.integers(-26, 12, (1, T, H, 1)))
+    near = (x.view(np.uint16) + g.integers(-1, 2, x.shape)).astype(np.uint16).view(np.float16)
+    K, V = x, F.f16(np.where(np.isfinite(near), near, x))
+    any_bits = g.integers(0, 1 << 16, x.shape).astype(np.uint16).view(np.float16)
+    for rows in (K, V, F.f16(np.where(np.isfinite(any_bits), any_bits, 1))):
+        c = F.Cache(1, H, d, d, T)
+        for t in range(T):
+            for h in range(H):
+                c.put(0, h, t, rows[0, t, h], rows[0, t, h])
+        sh, mem, L, dR = R.Kv4Shape(*c.dims), dev(c.buf * 0), dev(np.array([T], np.int32)), dev(rows)
+        assert lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, T, R.ptr(dR), 0, d, H * d, R.ptr(dR), 0, d, H * d, R.ptr(L)) == 0
+        assert np.array_equal(mem.cpu().numpy(), c.buf)
+        assert all(np.isfinite(F.f16(v)).all() for v in c.rows())
 
 
 def test_cache_lengths_past_the_capacity(lib, fd):
@@ -211,6 +235,21 @@ def test_kv4_attn_larger_bound_and_host_operands(lib, fd):
     for s, (want, tol) in list(enumerate(kv4_want(c, Q, lens, 0, 0, 0.1, 0.0)))[:2]:
         near(out[s], want, tol)
     assert first.any()
+
+
+@pytest.mark.parametrize("T", [1, 9, 40])
+def test_kv4_attn_short_lengths_under_a_long_bound(lib, fd, T):
+    """A bound of 40000 keys over sequences of a few: the work is shared out by the lengths themselves."""
+    lens = [1, 40, 700, 1500, 0]
+    c, Q = kv4_case(15, 4, 2, 64, 64, T, lens, spare=40000)
+    dQ, dL, sh, mem = dev(Q), dev(np.array(lens, np.int32)), R.Kv4Shape(*c.dims), dev(c.buf)
+    out = dev(np.full((len(lens), 4, T, 64), 7, np.float16))
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 1, len(lens), T, 40000, 4, 0.125, 0.0, 0, 0, R.ptr(dQ), R.ptr(dL), R.ptr(out)) == 0
+    got = out.cpu().numpy()
+    k, v = c.rows()
+    for s, n in enumerate(lens):
+        m = max(1, n)
+        near(got[s], *F.attend(Q[s], k[s + 1, :, :m], v[s + 1, :, :m], F.visible(n, T, 0, 0, m), 0.125, 0.0, True))
 
 
 def test_kv4_attn_large_scores(lib, fd):
