@@ -447,26 +447,25 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             char *vs = smem + slot * CF::STAGE + CF::KBYTES;
             // an exponent of all ones carries into the sign's place
             auto not_finite = [](unsigned w) __attribute__((always_inline)) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; };
+            // (a thread's chunks, 32 rows apart, hold the same eight keys)
+            const int key = key0 + 8 * ((tid & 7) ^ vx(tid >> 3));
+            unsigned live[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) live[i] = (dead(key + 2 * i) ? 0u : 0xFFFFu) | (dead(key + 2 * i + 1) ? 0u : 0xFFFF0000u);
+            const bool edge = (live[0] & live[1] & live[2] & live[3]) != 0xFFFFFFFFu;
             auto each = [&](bool finite) __attribute__((always_inline)) {
                 unsigned bad = 0;
-#pragma unroll 1
-                for (int g = tid; g < D * 8; g += 256) {
-                    const int d = g >> 3, key = key0 + 8 * ((g & 7) ^ vx(d));
-                    i32x4 *const p = reinterpret_cast<i32x4 *>(vs + g * 16);
+#pragma unroll
+                for (int g = 0; g < D / 32; g++) {
+                    i32x4 *const p = reinterpret_cast<i32x4 *>(vs + (tid + 256 * g) * 16);
                     i32x4 x = *p;
-                    const bool edge = key + 7 > p_hi || (key < first && key + 7 >= sinks);
-                    if (edge) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (dead(key + e)) x[e >> 1] &= 0xFFFF << (16 * (~e & 1));
+                    for (int i = 0; i < 4; i++) {
+                        x[i] &= (int)live[i];
+                        const unsigned nf = not_finite(x[i]);
+                        bad |= nf;
+                        if (finite) x[i] &= ~(int)((nf >> 15) * 0xFFFFu);
                     }
-                    unsigned nf[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) nf[i] = not_finite(x[i]);
-                    bad |= (nf[0] | nf[1]) | (nf[2] | nf[3]);
-                    if (finite)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) x[i] &= ~(int)((nf[i] >> 15) * 0xFFFFu);
                     if (edge || finite) *p = x;
                 }
                 return bad != 0;
