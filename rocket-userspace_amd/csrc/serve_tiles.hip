@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace rk {
 namespace {
@@ -587,29 +588,56 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     // lane holds dims 32 db + 8 b + 4 hh + c of its row
     const float l = l_run + __shfl_xor(l_run, 32, 64);
     const float inv = l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing; NaN stays)
-    if (!qok) return;
-    const size_t rows = (size_t)a.n_seq * a.n_head * T, prow = zs * rows + row0 + r;
-    typedef typename Part<SRC>::T P_;
-    typedef P_ P4 __attribute__((ext_vector_type(4)));
-    P_ *const part = static_cast<P_ *>(ta.part);
-    if (ta.nsplit > 1 && hh == 0) reinterpret_cast<f32x2 *>(part + ta.nsplit * rows * a.dv)[prow] = f32x2{m_run, l};
+    // Results go through LDS, a wave's 32 rows by themselves, so that they are stored as they lie, 16 bytes a lane side by
+    // side: lanes that store their own rows' pieces of 8 bytes took 6 us of a call's 21 (2048 rows of two tiles each,
+    // heads of 256). A pass takes as many dims as the tiles' room holds.
+    auto store_rows = [&](auto *base) __attribute__((always_inline)) {
+        typedef std::remove_reference_t<decltype(*base)> E;
+        typedef E E4 __attribute__((ext_vector_type(4)));
+        constexpr int EC = 16 / sizeof(E), DP = D * 2 / sizeof(E), RS = D * 2 + 16;   // (16 bytes of padding: rows start on other banks)
+        static_assert(NW * 32 * RS <= 2 * CF::STAGE, "the rows fit the tiles' room");
+        char *const mine = smem + wave * 32 * RS;
+        const int first_row = r0 + wave * 32, n_rows = min(32, r1 + 1 - first_row);
 #pragma unroll
-    for (int db = 0; db < DB; db++)
+        for (int d0 = 0; d0 < D; d0 += DP) {
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            const int d0 = 32 * db + 8 * b + 4 * hh;
-            if (32 * db + 8 * b < a.dv) {   // (dv is a multiple of 16: the same for both half-waves)
-                f32x4 v;
+            for (int db = d0 / 32; db < (d0 + DP) / 32; db++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) v[c] = O[db][4 * b + c] * inv;
-                if (ta.nsplit > 1) {
-                    *reinterpret_cast<P4 *>(part + prow * a.dv + d0) = P4{(P_)v[0], (P_)v[1], (P_)v[2], (P_)v[3]};
-                } else {
-                    const f16x4 h = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-                    *reinterpret_cast<f16x4 *>(a.out + (row0 + r) * a.dv + d0) = h;
+                for (int b = 0; b < 4; b++) {
+                    E4 v;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v[c] = (E)(O[db][4 * b + c] * inv);
+                    *reinterpret_cast<E4 *>(mine + l32 * RS + (32 * db + 8 * b + 4 * hh - d0) * (int)sizeof(E)) = v;
+                }
+            __builtin_amdgcn_wave_barrier();   // (a wave's LDS operations are served in order)
+            const int chunks = (min(a.dv, d0 + DP) - d0) / EC;   // of a row
+            if (chunks > 0) {
+                int row = lane / chunks, c = lane - row * chunks;
+                const int rows_on = 64 / chunks, c_on = 64 - rows_on * chunks;
+                while (row < n_rows) {
+                    *reinterpret_cast<i32x4 *>(base + (size_t)(first_row + row) * a.dv + d0 + c * EC) =
+                        *reinterpret_cast<const i32x4 *>(mine + row * RS + c * 16);
+                    row += rows_on;
+                    c += c_on;
+                    if (c >= chunks) {
+                        c -= chunks;
+                        row++;
+                    }
                 }
             }
+            __builtin_amdgcn_wave_barrier();
         }
+    };
+    lds_barrier();   // (the tiles are read no more)
+    if (ta.nsplit > 1) {
+        typedef typename Part<SRC>::T P_;
+        const size_t rows = (size_t)a.n_seq * a.n_head * T, prow = zs * rows + row0;
+        P_ *const part = static_cast<P_ *>(ta.part);
+        if (qok && hh == 0) reinterpret_cast<f32x2 *>(part + ta.nsplit * rows * a.dv)[prow + r] = f32x2{m_run, l};
+        store_rows(part + prow * a.dv);
+    } else {
+        store_rows(a.out + row0 * a.dv);
+    }
 }
 
 // Merges the splits: out = sum_s w_s O_s / sum_s w_s with w_s = 2^(m_s - m) l_s, m the largest of the m_s, for four output
