@@ -11,7 +11,7 @@
 // score arithmetic between them, then the next tile's QK products with this tile's exponentials between
 // them; K runs a tile ahead of V^T. Scores are transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so a lane
 // holds one row's scores and P stays in registers: rounded to fp16 and swapped between the half-waves
-// it is the second product's operand. O is rescaled only when some running maximum grows by more than 8.
+// it is the second product's operand. O is rescaled only when some running maximum grows by more than 5.5 (log2 units).
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
@@ -46,6 +46,12 @@ __device__ __forceinline__ void wait_vm0()
 #endif
 }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// (a wave's LDS operations are served in order: the compiler alone has to keep it)
+__device__ __forceinline__ void wave_lds_order()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // eight halves at any 2-byte address
 struct __attribute__((packed, aligned(2))) Halves8 { i32x4 v; };
@@ -382,12 +388,14 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             for (int e = 0; e < 16; e++) mloc = fmaxf(mloc, Sx[sb][e]);
         return fmaxf(mloc, __shfl_xor(mloc, 32, 64)) * unit;
     };
-    // the running maximum moves when some row's scores pass it by more than 8 (11.5 in log2 units: p stays far inside
-    // fp16); the division by the sum makes the result independent of it
+    // Weights are 2^(score - m_run), with m_run 10 (in log2 units) below the largest score, and it moves when some row's
+    // scores pass it by more than 15.5: then a weight stays inside fp16 and one is lost to it only below 2^-35 of the
+    // largest (around the maximum itself 2^-25, which 2^17 such keys made 2e-3 of a result). The division by the sum
+    // makes the result independent of m_run.
     auto grow = [&](float mloc) __attribute__((always_inline)) {
         float alpha = 1.f;
-        if (__builtin_expect(__any(mloc > m_run + 11.5f), 0)) {
-            const float m_new = fmaxf(m_run, mloc);
+        if (__builtin_expect(__any(mloc > m_run + 15.5f), 0)) {
+            const float m_new = fmaxf(m_run, mloc - 10.f);
             alpha = exp2f(m_run - m_new);
             m_run = m_new;
 #pragma unroll
@@ -609,7 +617,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     for (int c = 0; c < 4; c++) v[c] = (E)(O[db][4 * b + c] * inv);
                     *reinterpret_cast<E4 *>(mine + l32 * RS + (32 * db + 8 * b + 4 * hh - d0) * (int)sizeof(E)) = v;
                 }
-            __builtin_amdgcn_wave_barrier();   // (a wave's LDS operations are served in order)
+            wave_lds_order();
             const int chunks = (min(a.dv, d0 + DP) - d0) / EC;   // of a row
             if (chunks > 0) {
                 int row = lane / chunks, c = lane - row * chunks;
@@ -625,7 +633,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     }
                 }
             }
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_order();
         }
     };
     lds_barrier();   // (the tiles are read no more)

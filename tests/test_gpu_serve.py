@@ -269,6 +269,33 @@ def test_kv4_attn_large_scores(lib, fd):
             near(out[0], want, tol)
 
 
+@pytest.mark.parametrize("bits", [15.3, 20.5, 26.0])
+@pytest.mark.parametrize("T", [3, 70, 65600])
+def test_attn_many_small_weights(lib, fd, T, bits):
+    """One key outweighs each of 2^17 others by 2^bits: together those count, and no weight may be lost for being small
+    beside the largest; the prompt is so long that no workgroup's keys are split. Keys and values are exact in 4 bits. A
+    token that sees v keys gets ((v - 1) w - 1) / ((v - 1) w + 1), off by what attend() allows for exact keys and values
+    of 1: half a step of the result and of the weights, the scores' (within bits ln 2) fp32 steps, 2^-18."""
+    print("small weights", T, bits, flush=True)
+    n, d = 1 << 17, 32
+    K, V = np.zeros((1, n, d), np.float16), np.ones((1, n, d), np.float16)
+    K[0, 0, 0], V[0, 0] = 15, -1
+    Q = np.zeros((1, T, d), np.float16)
+    Q[..., 0] = 1
+    scale = float(np.float32(bits * np.log(2) / 15))
+    w = np.exp(-15 * scale) * (n - T + np.arange(T))
+    want = np.repeat(((w - 1) / (w + 1))[None, :, None], d, 2)
+    tol = np.abs(want) * F.U + 2 * np.expm1(2.0 ** -22 * 15 * scale + 2.0 ** -20) + F.U + 2.0 ** -18 + 2.0 ** -24
+    c = F.Cache(1, 1, d, d, n)
+    c.put_all(0, K, V)
+    sh, mem, dQ, L, out = R.Kv4Shape(*c.dims), dev(c.buf), dev(Q), dev(np.array([n], np.int32)), np.empty((1, T, d), np.float16)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, T, n, 1, scale, 0.0, 0, 0, R.ptr(dQ), R.ptr(L), R.ptr(out)) == 0
+    near(out, want, tol)
+    dK, dV, out = dev(K), dev(V.transpose(0, 2, 1)), np.empty((1, T, d), np.float16)
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, 1, 1, scale, 0.0, 0, 0, R.ptr(dQ), R.ptr(dK), R.ptr(dV), R.ptr(out)) == 0
+    near(out, want, tol)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, -0.0])
 @pytest.mark.parametrize("cap", [0.0, 5.0])
 @pytest.mark.parametrize("T", [2, 40])
