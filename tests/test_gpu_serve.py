@@ -571,3 +571,178 @@ def test_window_attn_captured(lib, T, n):
         near(out.cpu().numpy(), *win_want(Q, K, V, see, 0.1, 0.0))
     del graph
     lib.rocket_close(fd)
+
+
+def _calls(lib, seed):
+    """Every entry on device operands: name -> (call(fd), its results)."""
+    g = rng(seed)
+    heads, kvh, d, cap, n = 8, 2, 128, 2500, 2400
+    c = F.Cache(1, kvh, d, d, cap)
+    c.put_all(0, F.f16(g.standard_normal((kvh, n, d))), F.f16(g.standard_normal((kvh, n, d))))
+    sh, mem, L = R.Kv4Shape(*c.dims), dev(c.buf), dev(np.array([n], np.int32))
+    K, V = dev(F.f16(g.standard_normal((kvh, n, d)))), dev(F.f16(g.standard_normal((kvh, d, n))))
+    x, pos, freq = dev(F.f16(g.standard_normal((3, (heads + kvh) * d)))), dev(np.arange(3, dtype=np.int32)), dev(np.linspace(0.01, 1, d // 2, dtype=np.float32))
+    new = lambda *s: dev(np.zeros(s, np.float16))  # noqa: E731
+    q, k = new(heads, 3, d), new(kvh, 3, d)
+    calls = dict(rope=(lambda fd: lib.rocket_qk_norm_rope_fp16(fd, 1, 3, heads, kvh, d, d, 0, 1e-6, R.ptr(x), (heads + kvh) * d, R.ptr(x.data_ptr() + 2 * heads * d),
+                                                                    (heads + kvh) * d, None, None, R.ptr(freq), R.ptr(pos), R.ptr(q), R.ptr(k)), [q, k]),
+                 append=(lambda fd: lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, 3, R.ptr(K), 0, n * d, d, R.ptr(K), 0, n * d, d, R.ptr(L)), [mem]))
+    for T in (1, 90):
+        Q, a, b = dev(F.f16(g.standard_normal((heads, T, d)))), new(heads, T, d), new(heads, T, d)
+        calls[f"kv4 {T}"] = (lambda fd, T=T, Q=Q, a=a: lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, T, cap, heads, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(a)), [a])
+        calls[f"window {T}"] = (lambda fd, T=T, Q=Q, b=b: lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, 0.1, 0.0, 1500, 4, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(b)), [b])
+    return calls
+
+
+def _captured(fd, call, stream):
+    import torch
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        rc = call(fd)
+    assert rc == 0
+    return graph
+
+
+@pytest.mark.parametrize("name", ["rope", "append", "kv4 1", "kv4 90", "window 1", "window 90"])
+def test_serve_capture_on_a_fresh_handle(lib, name):
+    """A handle's first call is a captured one: it has no scratch to split keys on, and takes as many workgroups as it can
+    without. Up to the splits' order of sums the eager results."""
+    import torch
+    print("fresh handle", name, flush=True)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        call, outs = _calls(lib, 40)[name]
+    warm, fd = _handle(lib, stream), _handle(lib, stream)
+    with torch.cuda.stream(stream):
+        assert call(warm) == 0
+        want = [o.cpu().numpy() for o in outs]
+    graph = _captured(fd, call, stream)
+    for _ in range(3):
+        with torch.cuda.stream(stream):
+            if name != "append":
+                for o in outs:
+                    o.fill_(7)
+            graph.replay()
+            stream.synchronize()
+            for o, w in zip(outs, want):
+                if name in ("rope", "append"):
+                    assert np.array_equal(o.cpu().numpy(), w)
+                else:   # each side is off by its weights' and its result's rounding, of values up to 5
+                    assert np.abs(o.cpu().numpy().astype(np.float64) - w).max() <= 4 * 5 * F.U
+    del graph
+    for f in (warm, fd):
+        lib.rocket_close(f)
+
+
+def test_serve_graphs_of_one_handle(lib):
+    """Four attention calls captured one by one on one handle, replayed in turn, with an eager call between the replays that
+    makes the handle's scratch grow: the eager results, bit for bit."""
+    import torch
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        calls = {k: v for k, v in _calls(lib, 41).items() if " " in k}
+        big = F.Cache(1, 2, 256, 256, 9000, fill=0)
+        mem, L, Q, out = dev(big.buf), dev(np.array([9000], np.int32)), dev(np.zeros((2, 300, 256), np.float16)), dev(np.zeros((2, 300, 256), np.float16))
+    sh, fd = R.Kv4Shape(*big.dims), _handle(lib, stream)
+    want, graphs = {}, {}
+    with torch.cuda.stream(stream):
+        for k, (call, outs) in calls.items():
+            assert call(fd) == 0
+            want[k] = outs[0].cpu().numpy()
+    for k, (call, _) in calls.items():
+        graphs[k] = _captured(fd, call, stream)
+    with torch.cuda.stream(stream):
+        for rep in range(3):
+            for k in list(calls)[rep:] + list(calls)[:rep]:
+                calls[k][1][0].fill_(7)
+                graphs[k].replay()
+                assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, 100 * (rep + 1), 9000, 2, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+            stream.synchronize()
+            for k, (_, outs) in calls.items():
+                assert np.array_equal(outs[0].cpu().numpy(), want[k]), (rep, k)
+    graphs.clear()
+    lib.rocket_close(fd)
+
+
+def test_serve_from_two_threads(lib):
+    """Two threads with a handle each, and two that share one: every call's results are the first's, bit for bit."""
+    import threading
+
+    import torch
+    calls = [_calls(lib, 42 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    fds, wrong = [lib.rocket_open() for _ in range(3)], []
+    want = []
+    for cs in calls:
+        want.append({})
+        for k, (call, outs) in cs.items():
+            assert call(fds[0]) == 0
+            want[-1][k] = [o.cpu().numpy() for o in outs]
+
+    def work(i, fd):
+        for _ in range(5):
+            for k, (call, outs) in calls[i].items():
+                if call(fd) != 0 or any(not np.array_equal(o.cpu().numpy(), w) for o, w in zip(outs, want[i][k])):
+                    wrong.append((i, k))
+    for pair in ((fds[0], fds[1]), (fds[2], fds[2])):
+        ts = [threading.Thread(target=work, args=(i, pair[i])) for i in range(2)]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+    assert not wrong
+    for f in fds:
+        lib.rocket_close(f)
+
+
+# ---- the largest sizes -----------------------------------------------------------------
+
+def test_cache_past_32_bits(lib, fd):
+    """Parts of more than 4 GiB: the last two places' tokens, at the front of one and the end of the other."""
+    import torch
+    S, H, d, cap, new, window = 64, 8, 256, 1 << 16, 300, 200
+    sh = R.Kv4Shape(S, H, d, d, cap)
+    size = lib.rocket_kv4_bytes(C.byref(sh))
+    assert size >= 10 << 30
+    mem = torch.empty(size, dtype=torch.uint8, device=DEV)
+    g = rng(45)
+    lens = np.array([new, cap], np.int32)
+    K, V = F.f16(g.standard_normal((2, H, new, d))), F.f16(g.standard_normal((2, H, new, d)))
+    dK, dV, L = dev(K), dev(V), dev(lens)
+    ss, hs = H * new * d, new * d
+    assert lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), S - 2, 2, new, R.ptr(dK), ss, hs, d, R.ptr(dV), ss, hs, d, R.ptr(L)) == 0
+    c = F.Cache(2, H, d, d, new)
+    for s in range(2):
+        c.put_all(s, K[s], V[s])
+    k, v = c.rows()
+    a, b = np.empty((2, H, new, d), np.float16), np.empty((2, H, new, d), np.float16)
+    assert lib.rocket_kv4_read_fp16(fd, C.byref(sh), R.ptr(mem), S - 2, 2, new, R.ptr(L), R.ptr(a), R.ptr(b)) == 0
+    assert np.array_equal(a, F.f16(k[:, :, :new])) and np.array_equal(b, F.f16(v[:, :, :new]))
+    for T in (1, 40):
+        Q, out = F.f16(g.standard_normal((2, H, T, d))), np.empty((2, H, T, d), np.float16)
+        assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), S - 2, 2, T, cap, H, d ** -0.5, 0.0, window, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+        for s in range(2):   # (under the window the end of a long sequence is that of a short one)
+            near(out[s], *F.attend(Q[s], k[s, :, :new], v[s, :, :new], F.visible(new, T, window, 0, new), d ** -0.5, 0.0, True))
+
+
+@pytest.mark.parametrize("T", [2, 150])
+def test_window_longest(lib, fd, T):
+    """The longest keys and V^T rows that the call takes, NaN where no token sees them."""
+    import torch
+    stride, d, window, sinks, end = (1 << 22) - 64, 256, 300, 2, 600
+    n = stride - 3
+    g = rng(46)
+    at = np.concatenate([np.arange(sinks), np.arange(n - end, n)])
+    K, V, Q = F.f16(g.standard_normal((1, at.size, d))), F.f16(g.standard_normal((1, at.size, d))), F.f16(g.standard_normal((1, T, d)))
+    dK = torch.full((stride, d), float("nan"), dtype=torch.float16, device=DEV)
+    dV = torch.full((d, stride), float("nan"), dtype=torch.float16, device=DEV)
+    first = n - T - window + 1
+    seen = (at >= first) | (at < sinks)
+    i = dev(at[seen])
+    dK[i] = dev(K[0, seen])
+    dV[:, i] = dev(V[0, seen].T)
+    p = (n - T + np.arange(T))[:, None]
+    see = (at[None] <= p) & ((at[None] > p - window) | (at[None] < sinks))
+    dQ, out = dev(Q), np.empty((1, T, d), np.float16)
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, stride, d, d, 1, 1, d ** -0.5, 0.0, window, sinks, R.ptr(dQ), R.ptr(dK), R.ptr(dV), R.ptr(out)) == 0
+    near(out, *F.attend(Q, K.astype(np.float64), V.astype(np.float64), see, d ** -0.5, 0.0, False))
