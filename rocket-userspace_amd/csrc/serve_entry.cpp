@@ -61,7 +61,7 @@ int bad_fd(const char *who, int fd)
 int rope(const char *who, int fd, RopeLaunch L, int style)
 {
     if (L.n_seq < 1 || L.n_tokens < 1 || L.n_head < 1 || L.n_kv < 1 || L.n_seq > kDimMax || L.n_tokens > kDimMax || L.n_head > kDimMax ||
-        L.n_kv > kDimMax || (long)L.n_seq * L.n_tokens > kDimMax || (long)L.n_head + L.n_kv > 65535)
+        L.n_kv > kDimMax || (long)L.n_seq * L.n_tokens >= kDimMax || (long)L.n_head + L.n_kv > 65535)
         return bad(who, "a count is below 1 or too large");
     if (L.dim < 32 || L.dim % 32 || L.dim > kServeMaxDim || L.rot < 0 || L.rot % 8 || L.rot > L.dim)
         return bad(who, "head_dim is a multiple of 32 up to 256, rot_dim one of 8 up to head_dim");

@@ -65,6 +65,16 @@ def test_rope_refusals(lib, f32):
 
 
 @pytest.mark.parametrize("f32", [False, True])
+def test_rope_too_many_rows(lib, f32):
+    """2^24 rows, a workgroup each, are more threads than a launch takes: refused with the other bad counts, before the handle
+    is looked at (no such handle, and nothing behind the addresses)."""
+    fn = lib.rocket_qk_norm_rope_f32in if f32 else lib.rocket_qk_norm_rope_fp16
+    q, k, qo, ko, freq, pos = (R.ptr(i << 44) for i in range(1, 7))
+    call = lambda n: fn(200, 4096, n, 1, 1, 32, 32, 0, 1e-6, q, 32, k, 32, None, None, freq, pos, qo, ko)  # noqa: E731
+    assert call(4096) == S and call(4095) == R.ROCKET_E_DEVICE
+
+
+@pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("dim,rot,pairs,eps,weighted", [(32, 32, False, 1e-6, True), (96, 64, True, 1e-5, True), (256, 128, False, 0.0, False),
                                                         (128, 8, True, -1.0, False), (64, 0, False, 1e-6, True)])
 def test_rope_host(lib, f32, dim, rot, pairs, eps, weighted):
