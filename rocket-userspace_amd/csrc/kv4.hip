@@ -4,7 +4,8 @@
 // codes, and the group's scale. What bounds both is memory, so the lanes of a wave are laid out as the bytes lie: a key
 // row's groups end to end, and of values eight tokens of a group side by side, whose words the cache keeps together.
 // (A thread a group, which found its row by three 64-bit divisions and divided 32 times, took 25 us for the prompt below;
-// its reading 18.)
+// its reading 18.) 4096 tokens of 8 heads of 256, 44 MB each: append 13.9 us by trace (3.2 TB/s: the scale and the codes
+// are some 12 VALU operations a value), read 10.6 us (4.1 TB/s); one token of 32 sequences 3.7 and 2.8.
 #include "serve.h"
 
 namespace rk {

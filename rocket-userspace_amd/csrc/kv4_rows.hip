@@ -12,6 +12,12 @@
 // lane's sixteen bytes of a key share one scale. In O^T += V^T P^T the rows (dims) are free: lane c
 // takes a word of eight dims of each of its eight keys, product j their nibbles j, which a byte permute brings
 // side by side as pairs of keys.
+//
+// Roundings beside the result's: a widened value to fp16 (what rocket_kv4_read_fp16 gives, and what the MFMA takes) and a
+// weight to fp16; scores, maxima, sums and outputs are fp32. The result is within 4e-4 of its size (the rounded result alone
+// 2e-4). Measured by trace: 32 sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 47.5 us (5.2 TB/s, a
+// large copy's rate) and 4.8 for the merge; one sequence of 3000 keys, 16 / 8 heads of 256, 6.6 and 4.2: two launches, and a
+// wave's one chunk after another whose loads nothing else hides.
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"

@@ -12,6 +12,12 @@
 // them; K runs a tile ahead of V^T. Scores are transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so a lane
 // holds one row's scores and P stays in registers: rounded to fp16 and swapped between the half-waves
 // it is the second product's operand. O is rescaled only when some running maximum grows by more than 5.5 (log2 units).
+//
+// Roundings beside the result's: weights to fp16 (summed as rounded), codes' values to fp16 as the cache's reading gives them;
+// scores, maxima, sums and outputs are fp32. Measured: 2048 tokens under a window of 1024, 16 / 8 heads of 256, 60.0 us (575
+// TFLOP/s); 512 over 4096 codes 68.6 (469); 2048 over 8192 fp16 keys, 32 / 8 heads of 128, 289 (830). Heads of 256
+// have one wave a SIMD: a tile's MFMAs are 2048 of its 5700 cycles, bound by 256 KB of LDS reads (every wave reads
+// the whole tile) whose latency nothing else covers; over codes, 816 VALU operations a wave and tile (384 over halves) make it 7000.
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
