@@ -318,15 +318,13 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 
 // Merges the splits that a sequence's length has, one (head, token) row of a place a workgroup: out = sum_s
 // w_s On_s / sum_s w_s with w_s = 2^(m_s - m) l_s, outputs in fp32 (a rounding of each to fp16 would be a third
-// one beside the probabilities' and the result's).
+// one beside the probabilities' and the result's). Pairs and outputs of every split that there may be are loaded beside the
+// length, which then says how many count (the others' hold anything).
 __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
 {
     const ServeAttn &a = ra.a;
     __shared__ float wt[kMaxSplit], sum[8 * 256];
     const int tid = threadIdx.x, row = blockIdx.x, s = blockIdx.y, dv = a.dv;
-    const int n = a.seq_len[s];
-    const int count = n >= 1 && n <= a.max_kv ? Chunks(a, n).count : 0;
-    const int cps = share(count, ra.nsplit), nsplit = max(1, (count + cps - 1) / cps);
     const size_t rows = (size_t)a.n_head * a.n_tokens, base = (size_t)s * ra.nsplit * rows + row;
     const int dq = dv / 8, sg = tid / dq, d0 = (tid - sg * dq) * 8, ng = min(8, 256 / dq);   // dv <= 256: 8
     f32x4 os[8][2];
@@ -334,13 +332,16 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int sp = sg + i * ng;
-            if (sp < nsplit)
+            if (sp < ra.nsplit)
 #pragma unroll
                 for (int j = 0; j < 2; j++) os[i][j] = reinterpret_cast<const f32x4 *>(ra.part + (base + sp * rows) * dv + d0)[j];
         }
+    const f32x2 pair = reinterpret_cast<const f32x2 *>(ra.part + (size_t)a.n_seq * ra.nsplit * rows * dv)[base + min(tid & 63, ra.nsplit - 1) * rows];
+    const int n = a.seq_len[s];
+    const int count = n >= 1 && n <= a.max_kv ? Chunks(a, n).count : 0;
+    const int cps = share(count, ra.nsplit), nsplit = max(1, (count + cps - 1) / cps);
     if (tid < 64) {
-        const f32x2 x = tid < nsplit ? reinterpret_cast<const f32x2 *>(ra.part + (size_t)a.n_seq * ra.nsplit * rows * dv)[base + tid * rows]
-                                     : f32x2{-1e30f, 0.f};
+        const f32x2 x = tid < nsplit ? pair : f32x2{-1e30f, 0.f};
         float m = x[0];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
