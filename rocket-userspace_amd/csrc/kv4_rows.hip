@@ -79,6 +79,20 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const int hk = blockIdx.x, zs = blockIdx.y, s = blockIdx.z;
     const int T = a.n_tokens, R = a.gqa * T;
     const int n = a.seq_len[s];
+    const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;   // row of the first query
+    f16x8 qf[NQ][KS];
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        const _Float16 *qrow = a.Q + (head0 + min(16 * x + c, R - 1)) * a.dk;   // (rows behind the last repeat it)
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int d = D == 64 ? 16 * q + 8 * i : 128 * (i / 4) + 32 * q + 8 * (i % 4);
+            f16x8 y = *reinterpret_cast<const f16x8 *>(qrow + (FULL ? d : min(d, a.dk - 8)));
+            if (!FULL && d >= a.dk) y = f16x8{};
+            qf[x][i] = __builtin_shufflevector(y, y, 0, 4, 1, 5, 2, 6, 3, 7);
+        }
+    }
+    asm volatile("" ::: "memory");   // (the queries' loads are sent before the length is there)
     const bool served = n >= 1 && n <= a.max_kv;
     const Chunks list(a, served ? n : 1);
     const int count = served ? list.count : 0;
@@ -97,20 +111,6 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const int p_lo = n - T, p_hi = n - 1;
 
     const size_t hr = (size_t)s * a.c.heads + hk;
-    const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;   // row of the first query
-    f16x8 qf[NQ][KS];
-#pragma unroll
-    for (int x = 0; x < NQ; x++) {
-        const _Float16 *qrow = a.Q + (head0 + min(16 * x + c, R - 1)) * a.dk;   // (rows behind the last repeat it)
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-            const int d = D == 64 ? 16 * q + 8 * i : 128 * (i / 4) + 32 * q + 8 * (i % 4);
-            f16x8 y = *reinterpret_cast<const f16x8 *>(qrow + (FULL ? d : min(d, a.dk - 8)));
-            if (!FULL && d >= a.dk) y = f16x8{};
-            qf[x][i] = __builtin_shufflevector(y, y, 0, 4, 1, 5, 2, 6, 3, 7);
-        }
-    }
-
     const int dk = FULL ? D : a.dk, dv = FULL ? D : a.dv;
     const char *const kc = a.c.kc + hr * a.c.cap * (dk / 2), *const ks = a.c.ks + hr * a.c.cap * (dk / 8);
     const char *const vc = a.c.vc + hr * a.c.cap * (dv / 2), *const vs = a.c.vs + hr * a.c.cap * (dv / 8);
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
 {
     const ServeAttn &a = ra.a;
-    __shared__ float wt[kMaxSplit], sum[8 * 256];
+    __shared__ float sum[8 * 256];
     const int tid = threadIdx.x, row = blockIdx.x, s = blockIdx.y, dv = a.dv;
     const size_t rows = (size_t)a.n_head * a.n_tokens, base = (size_t)s * ra.nsplit * rows + row;
     const int dq = dv / 8, sg = tid / dq, d0 = (tid - sg * dq) * 8, ng = min(8, 256 / dq);   // dv <= 256: 8
@@ -340,18 +340,19 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
     const int n = a.seq_len[s];
     const int count = n >= 1 && n <= a.max_kv ? Chunks(a, n).count : 0;
     const int cps = share(count, ra.nsplit), nsplit = max(1, (count + cps - 1) / cps);
-    if (tid < 64) {
-        const f32x2 x = tid < nsplit ? pair : f32x2{-1e30f, 0.f};
-        float m = x[0];
+    // (every wave makes the weights, lane i split i's: that is shorter than one that hands them out)
+    const f32x2 x = (tid & 63) < nsplit ? pair : f32x2{-1e30f, 0.f};
+    float m = x[0];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        const float w = __builtin_amdgcn_exp2f(x[0] - m) * x[1];
-        float l = w;
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float w = __builtin_amdgcn_exp2f(x[0] - m) * x[1];
+    float l = w;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-        wt[tid] = l == 0.f ? 0.f : w / l;
-    }
-    __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    const float wt = l == 0.f ? 0.f : w / l;
+    float ws[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) ws[i] = __shfl(wt, sg + i * ng, 64);
     if (sg < ng) {
         float acc[8] = {};
 #pragma unroll
@@ -359,7 +360,7 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
             const int sp = sg + i * ng;
             if (sp < nsplit)
 #pragma unroll
-                for (int e = 0; e < 8; e++) acc[e] += wt[sp] * os[i][e >> 2][e & 3];
+                for (int e = 0; e < 8; e++) acc[e] += ws[i] * os[i][e >> 2][e & 3];
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) sum[sg * dv + d0 + e] = acc[e];
