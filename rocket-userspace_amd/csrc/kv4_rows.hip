@@ -2,8 +2,8 @@
 //
 // What bounds it is how fast the codes arrive, and then the VALU that widens them: about two
 // operations a value, whatever the number of query rows. So all rows of a KV head (its query heads'
-// tokens, at most 64, in blocks of 16) share one widening. A workgroup owns a place of the batch, a KV head and a range
-// of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
+// tokens, at most 64, in blocks of 16) share one widening (of heads above 128 each 32). A workgroup owns a place of the
+// batch, a KV head and a range of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
 // they lie in the cache, the next chunk's while this one's are widened.
 //
 // Scores are transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16, K the first operand): lane (c, q) =
@@ -76,10 +76,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x, zs = blockIdx.y, s = blockIdx.z;
-    const int T = a.n_tokens, R = a.gqa * T;
+    // the workgroup's R rows of the KV head's, from row0 on (heads above 128: blocks of 32 rows, a split's on one XCD where the
+    // heads are a multiple of 8, whose L2 gives the second block the codes)
+    constexpr bool BLOCKS = D == 256 && NQ == 2;
+    const int hk = blockIdx.x, zs = BLOCKS ? blockIdx.y % ra.nsplit : blockIdx.y, s = blockIdx.z;
+    const int T = a.n_tokens, row0 = BLOCKS ? blockIdx.y / ra.nsplit * 16 * NQ : 0;
+    const int R = BLOCKS ? min(16 * NQ, a.gqa * T - row0) : a.gqa * T;
     const int n = a.seq_len[s];
-    const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T;   // row of the first query
+    const size_t head0 = ((size_t)s * a.n_head + (size_t)hk * a.gqa) * T + row0;   // row of the first query
     f16x8 qf[NQ][KS];
 #pragma unroll
     for (int x = 0; x < NQ; x++) {
@@ -98,14 +102,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const int count = served ? list.count : 0;
     const int cps = ra.nsplit > 1 ? share(count, ra.nsplit) : max(count, 1);
     if (zs > 0 && zs * cps >= count) return;   // (the merge knows)
-    // this lane's queries: row 16 x + c of the KV head's (head r / T, token r % T), and its position
+    // this lane's queries: row 16 x + c of the workgroup's (a KV head's row r: head r / T of it, token r % T), and its position
     bool qok[NQ];
     int pos[NQ], behind[NQ];                      // (the last key behind its window)
 #pragma unroll
     for (int x = 0; x < NQ; x++) {
         const int r = 16 * x + c;
         qok[x] = r < R;
-        pos[x] = n - T + r % T;
+        pos[x] = n - T + (row0 + r) % T;
         behind[x] = a.window ? pos[x] - a.window : -1;
     }
     const int p_lo = n - T, p_hi = n - 1;
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;   // (a row that sees nothing; NaN stays)
         if (ra.nsplit > 1) {
-            const size_t row = ((size_t)s * ra.nsplit + zs) * a.n_head * T + (size_t)hk * R + r;
+            const size_t row = ((size_t)s * ra.nsplit + zs) * a.n_head * T + (size_t)hk * a.gqa * T + row0 + r;
             *reinterpret_cast<f32x4 *>(ra.part + row * dv + d0) = o * inv;
             if (d0 == 0) reinterpret_cast<f32x2 *>(ra.part + (size_t)a.n_seq * ra.nsplit * a.n_head * T * dv)[row] = f32x2{m, l};
         } else {
@@ -373,14 +377,16 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
     }
 }
 
-// Blocks of 16 rows that a KV head's queries make.
+// Blocks of 16 rows that a KV head's queries make; of heads above 128 a workgroup takes two at most, whose outputs its
+// registers hold.
 int row_blocks(const ServeAttn &a) { return (a.gqa * a.n_tokens + 15) / 16; }
+int row_groups(const ServeAttn &a) { return std::max(a.dk, a.dv) <= 128 ? 1 : (row_blocks(a) + 1) / 2; }
 
 template <int D, int NQ, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
 {
     auto kern = k_kv4_rows<D, NQ, CAP, FULL>;
     const ServeAttn &a = ra.a;
-    const int R = a.gqa * a.n_tokens;
+    const int R = std::min(16 * NQ, a.gqa * a.n_tokens);
     const size_t lds = (size_t)kWaves * R * ((D + 4) * 4 + 8);
     if (lds > 64 * 1024) {
         static std::atomic<uint64_t> opted{0};
@@ -388,7 +394,7 @@ template <int D, int NQ, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowAr
         static_assert(most <= 160 * 1024, "LDS budget");
         if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), most, opted)) return e;
     }
-    hipLaunchKernelGGL(kern, dim3((unsigned)a.c.heads, (unsigned)ra.nsplit, (unsigned)a.n_seq), dim3(kWaves * 64), lds, s, ra);
+    hipLaunchKernelGGL(kern, dim3((unsigned)a.c.heads, (unsigned)(ra.nsplit * row_groups(a)), (unsigned)a.n_seq), dim3(kWaves * 64), lds, s, ra);
     return hipGetLastError();
 }
 template <int D, int NQ> hipError_t launch_q(const Kv4RowArgs &ra, hipStream_t s)
@@ -423,16 +429,17 @@ int splits(const ServeAttn &a)
     // 66.9, 256 49.5; heads of 128, 20 rows 33.1, 512 29.3).
     const int d = std::max(a.dk, a.dv), nq = row_blocks(a);
     const long resident = 256 * (nq == 1 ? (d <= 128 ? 4 : 2) : nq == 2 ? (d <= 64 ? 3 : d <= 128 ? 2 : 1) : d <= 64 ? 2 : 1);
-    const long wgs = (long)a.c.heads * a.n_seq;
+    const long wgs = (long)a.c.heads * a.n_seq * row_groups(a);
     return (int)std::max<long>(1, std::min<long>({(chunks + kWaves - 1) / kWaves, resident / wgs, kMaxSplit}));
 }
 
 }  // namespace
 
-// Up to 64 rows (heads of more than 128, whose outputs do not fit the registers, 32). In tiles of 128 rows, at 16000 keys of
-// one sequence, heads of 128: 20 rows 28.1 us, here 16.3; 64 rows 38.8 and 24.9; at 16 sequences of 4000 keys 63.5 and 29.3,
-// 66.0 and 61.2. (Short sequences of narrow heads, 64 rows: 32 of 1000 keys, 2 heads of 64, 15.4 and 21.1.)
-bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= (std::max(a.dk, a.dv) <= 128 ? 64 : 32); }
+// Up to 64 rows. In tiles of 128 rows, at 16000 keys of one sequence, heads of 128: 20 rows 28.1 us, here 16.3; 64 rows 38.8
+// and 24.9; at 16 sequences of 4000 keys 63.5 and 29.3, 66.0 and 61.2. (Short sequences of narrow heads, 64 rows: 32 of
+// 1000 keys, 2 heads of 64, 15.4 and 21.1.) Heads of 256, 64 rows: 16000 keys of one sequence 58.5 and
+// 30.8, 8 sequences of 4000 59.9 and 53.6, 32 of 2000 99.0 and 78.4; a third block would lose there what it gains at one.
+bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= 64; }
 
 size_t kv4_rows_ws(const ServeAttn &a)
 {
@@ -449,7 +456,7 @@ hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
     ra.part = a.ws;
     const int d = std::max(a.dk, a.dv);
     const hipError_t e = d <= 64 ? launch<64>(ra, s) : d <= 128 ? launch<128>(ra, s) : launch<256>(ra, s);
-    *blocks = (uint64_t)a.c.heads * ra.nsplit * a.n_seq;
+    *blocks = (uint64_t)a.c.heads * ra.nsplit * row_groups(a) * a.n_seq;
     if (e != hipSuccess || ra.nsplit == 1) return e;
     const unsigned rows = (unsigned)(a.n_head * a.n_tokens);
     hipLaunchKernelGGL(k_kv4_merge, dim3(rows, (unsigned)a.n_seq), dim3(256), 0, s, ra);

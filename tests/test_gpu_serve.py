@@ -163,6 +163,9 @@ KV4 = [  # heads, kv heads, dk, dv, tokens, lengths (the largest is max_kv), win
     (6, 2, 96, 160, 200, [900], 0, 0, 50.0), (4, 1, 128, 128, 129, [64, 513], 0, 0, 0.0),
     (4, 1, 64, 64, 9, [500, 36, 35], 0, 0, 0.0), (8, 2, 128, 128, 16, [300, 15], 50, 3, 0.0), (4, 2, 96, 64, 32, [700], 0, 0, 20.0), (2, 1, 128, 32, 24, [65, 24, 7], 9, 2, 0.0),
     (2, 1, 64, 64, 33, [300, 60], 0, 0, 0.0), (5, 1, 128, 128, 13, [400], 100, 0, 0.0), (2, 1, 160, 160, 16, [200, 31], 0, 0, 0.0), (2, 1, 256, 256, 17, [200, 31], 40, 4, 0.0),
+    # two blocks of up to 32 rows of heads above 128
+    (3, 1, 192, 160, 11, [333, 5], 0, 0, 0.0), (5, 1, 160, 256, 12, [400, 0, 33], 0, 0, 0.0), (4, 2, 256, 96, 20, [70, 200, 19], 50, 3, 20.0),
+    (1, 1, 256, 256, 64, [64, 500], 0, 0, 0.0), (5, 1, 224, 224, 7, [2000], 0, 0, 0.0), (8, 2, 160, 160, 12, [5000, 700], 600, 9, 0.0),
     # windows: inside a chunk, across chunks, one key, more than the keys; sinks that meet the window, and that lie past it
     (4, 2, 64, 64, 1, [500, 20], 64, 4, 0.0), (4, 2, 128, 128, 5, [411, 3, 70], 33, 1, 0.0), (2, 2, 256, 128, 1, [1025], 1, 0, 0.0),
     (8, 2, 128, 128, 40, [600, 90], 100, 5, 0.0), (2, 1, 64, 64, 300, [1000], 129, 70, 0.0), (3, 1, 64, 64, 33, [200, 100], 1000, 1000, 20.0),
