@@ -296,8 +296,10 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
                 bool bad = false;
 #pragma unroll
                 for (int j = 0; j < VB; j++)
+                    if (FULL || 16 * j < a.dv) {   // (the others were not loaded)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) bad |= (vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
+                        for (int i = 0; i < 8; i++) bad |= (vf[j][i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
+                    }
                 if (__builtin_expect(__any(bad), 0)) {
                     const uint16_t *const vr = reinterpret_cast<const uint16_t *>(a.Vt + (size_t)hk * a.v_hs);
 #pragma unroll
