@@ -166,6 +166,7 @@ KV4 = [  # heads, kv heads, dk, dv, tokens, lengths (the largest is max_kv), win
     # two blocks of up to 32 rows of heads above 128
     (3, 1, 192, 160, 11, [333, 5], 0, 0, 0.0), (5, 1, 160, 256, 12, [400, 0, 33], 0, 0, 0.0), (4, 2, 256, 96, 20, [70, 200, 19], 50, 3, 20.0),
     (1, 1, 256, 256, 64, [64, 500], 0, 0, 0.0), (5, 1, 224, 224, 7, [2000], 0, 0, 0.0), (8, 2, 160, 160, 12, [5000, 700], 600, 9, 0.0),
+    (1, 1, 64, 64, 100, [9000, 40, 130], 0, 0, 0.0), (2, 1, 256, 160, 70, [9001], 0, 0, 0.0),   # tiles in 17 to 32 shares
     # windows: inside a chunk, across chunks, one key, more than the keys; sinks that meet the window, and that lie past it
     (4, 2, 64, 64, 1, [500, 20], 64, 4, 0.0), (4, 2, 128, 128, 5, [411, 3, 70], 33, 1, 0.0), (2, 2, 256, 128, 1, [1025], 1, 0, 0.0),
     (8, 2, 128, 128, 40, [600, 90], 100, 5, 0.0), (2, 1, 64, 64, 300, [1000], 129, 70, 0.0), (3, 1, 64, 64, 33, [200, 100], 1000, 1000, 20.0),
@@ -328,6 +329,7 @@ WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
     (4, 1, 64, 64, 9, 500, 500, 0, 0, 0.0), (8, 2, 128, 128, 8, 301, 301, 50, 3, 0.0), (4, 2, 96, 64, 16, 700, 700, 0, 0, 20.0), (2, 1, 64, 32, 24, 65, 70, 9, 2, 0.0),
     (5, 1, 64, 64, 13, 400, 400, 100, 0, 0.0), (4, 2, 128, 80, 15, 333, 333, 300, 1, 0.0), (2, 1, 256, 256, 16, 200, 203, 40, 4, 0.0), (2, 1, 160, 176, 9, 13, 13, 5, 1, 0.0),
     (2, 1, 128, 128, 70, 400, 401, 33, 5, 0.0), (4, 4, 256, 256, 33, 300, 300, 0, 0, 0.0),
+    (1, 1, 64, 64, 100, 9000, 9000, 0, 0, 0.0), (2, 1, 256, 160, 70, 9001, 9003, 7000, 4, 0.0),
     # V^T rows that end at every place of a chunk
     *((2, 1, 64, 48, 33, n, n, 0, 0, 0.0) for n in range(185, 201)), (4, 2, 128, 128, 40, 203, 205, 64, 2, 0.0), (2, 1, 256, 192, 40, 195, 195, 0, 0, 0.0), (2, 1, 64, 64, 40, 9, 9, 0, 0, 0.0),
 ]
