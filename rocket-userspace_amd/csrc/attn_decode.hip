@@ -446,7 +446,12 @@ void split_of(const FaLaunch &L, int *nsplit, int *cps)
     const int kvh = L.n_head / L.gqa, chunks = chunk_list(L, nullptr);
     const int d = std::max(L.dk, L.dv), odd = L.n_kv & 1;
     const int whole = d <= 64 ? (odd ? 10 : 16) : d <= 128 ? (odd ? 8 : 10) : odd ? 5 : 8;
-    const int n = chunks <= whole ? 1 : std::min({(chunks + kWaves - 1) / kWaves, std::max(1, 768 / kvh), 64});
+    // under a window no more than the CUs hold at once, where the registers leave room for fewer than three: a second round of
+    // them cost more than longer shares (8 KV heads of 256 over 6000 keys, 24 rows 28.8 us, here 19.1, one token of two heads
+    // each 18.1 and 13.9; 16 KV heads, 32 rows 47.8 and 28.5; 64 rows of 16 heads of 64 21.9 and 18.7)
+    const int nq = (L.gqa * L.T + 15) / 16;
+    const int resident = 256 * (!L.win ? 3 : d > 128 ? 1 : nq == 1 ? 3 : d > 64 ? 2 : nq == 2 ? 3 : 2);
+    const int n = chunks <= whole ? 1 : std::min({(chunks + kWaves - 1) / kWaves, std::max(1, resident / kvh), 64});
     *cps = (chunks + n - 1) / n;
     *nsplit = (chunks + *cps - 1) / *cps;
 }
@@ -456,9 +461,9 @@ void split_of(const FaLaunch &L, int *nsplit, int *cps)
 bool flash_attn_few_rows(const FaLaunch &L)
 {
     if (L.n_kv < 8 || L.dk % 32 || L.dv % 16) return false;
-    // Under a window up to 32 rows, of heads of up to 64 up to 64 (in tiles of 128 rows, one sequence: 20 rows of heads of
-    // 128, 4001 keys 15.9 us, here 12.4; 16000 keys 32.7 and 20.4; 24 rows of heads of 256, 4001 keys 23.1 and 19.2; 64 rows
-    // of heads of 64, 1000 keys 10.3 and 11.2, 16000 keys 26.3 and 13.2).
+    // Under a window up to 32 rows, of heads of up to 64 up to 64 (in tiles of 128 rows, 8 KV heads: 20 rows of heads of 128,
+    // 4001 keys 16.0 us, here 12.4, 16000 keys 24.1 and 20.0; 24 rows of heads of 256, 2000 keys 19.1 and 16.9, 16000 keys 36.2
+    // and 34.2; 64 rows of heads of 64, 1000 keys 11.0 and 11.5, 16000 keys 20.1 and 17.8).
     if (L.win) return (long)L.gqa * L.T <= (std::max(L.dk, L.dv) <= 64 ? 4 : 2) * kRows;
     if ((long)L.gqa * L.T > kRows) return false;
     // One query head a KV head and long caches: the tiled kernel reads V^T in whole 128-byte lines (64

@@ -435,10 +435,10 @@ int splits(const ServeAttn &a)
 
 }  // namespace
 
-// Up to 64 rows. In tiles of 128 rows, at 16000 keys of one sequence, heads of 128: 20 rows 28.1 us, here 16.3; 64 rows 38.8
-// and 24.9; at 16 sequences of 4000 keys 63.5 and 29.3, 66.0 and 61.2. (Short sequences of narrow heads, 64 rows: 32 of
-// 1000 keys, 2 heads of 64, 15.4 and 21.1.) Heads of 256, 64 rows: 16000 keys of one sequence 58.5 and
-// 30.8, 8 sequences of 4000 59.9 and 53.6, 32 of 2000 99.0 and 78.4; a third block would lose there what it gains at one.
+// Up to 64 rows. In tiles of 128 rows, at 16000 keys of one sequence, 8 KV heads of 128: 20 rows 26.9 us, here 15.8; 64 rows
+// 27.4 and 24.1; at 16 sequences of 4000 keys 64.2 and 27.8, 66.2 and 62.9. (Short sequences of narrow heads, 64 rows: 32 of
+// 1000 keys, 2 heads of 64, 15.6 and 21.7.) Heads of 256, 64 rows: 16000 keys of one sequence 39.6 and 30.8, 8
+// sequences of 4000 60.0 and 53.3, 32 of 2000 99.8 and 78.2; a third block would lose there what it gains at one.
 bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= 64; }
 
 size_t kv4_rows_ws(const ServeAttn &a)
