@@ -15,9 +15,9 @@
 //
 // Roundings beside the result's: a widened value to fp16 (what rocket_kv4_read_fp16 gives, and what the MFMA takes) and a
 // weight to fp16; scores, maxima, sums and outputs are fp32. The result is within 4e-4 of its size (the rounded result alone
-// 2e-4). Measured by trace: 32 sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 47.5 us (5.2 TB/s, a
-// large copy's rate) and 4.8 for the merge; one sequence of 3000 keys, 16 / 8 heads of 256, 6.6 and 4.2: two launches, and a
-// wave's one chunk after another whose loads nothing else hides.
+// 2e-4). Measured by trace: 32 sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 47.9 us (5.2 TB/s, a
+// large copy's rate) and 4.8 for the merge; one sequence of 3000 keys, 16 / 8 heads of 256, 6.2 and 3.8: two launches, each a
+// chain of loads that nothing else hides.
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
