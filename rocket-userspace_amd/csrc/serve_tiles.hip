@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     auto cap1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
         if constexpr (CAP) Sx[e >> 4][e & 15] = softcap_log2(Sx[e >> 4][e & 15], fabsf(a.scale), a.softcap);
     };
-    auto finish = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
+    auto mask = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
         const int key0 = key_of(kb);
         const int k0 = key0 + 4 * hh, after = pos - k0, before = behind - k0;
         auto hide = [&](auto &&hidden) __attribute__((always_inline)) {
@@ -387,28 +387,25 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             if (key0 >= a.sinks) hide([&](int k) __attribute__((always_inline)) { return k <= before; });
             else if (key0 + BK > a.sinks) hide([&](int k) __attribute__((always_inline)) { return ((k - before - 1) & (a.sinks - 1 - k0 - k)) < 0; });
         }
-        float mloc = -INFINITY;
-#pragma unroll
-        for (int sb = 0; sb < 2; sb++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) mloc = fmaxf(mloc, Sx[sb][e]);
-        return fmaxf(mloc, __shfl_xor(mloc, 32, 64)) * unit;
+    };
+    auto highest = [&](float mloc) __attribute__((always_inline)) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, mloc), __builtin_bit_cast(unsigned, mloc), false, false);
+        const unsigned x0 = x[0], x1 = x[1];
+        return fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1)) * unit;
     };
     // Weights are 2^(score - m_run), with m_run 10 (in log2 units) below the largest score, and it moves when some row's
     // scores pass it by more than 15.5: then a weight stays inside fp16 and one is lost to it only below 2^-35 of the
     // largest (around the maximum itself 2^-25, which 2^17 such keys made 2e-3 of a result). The division by the sum
     // makes the result independent of m_run.
-    auto grow = [&](float mloc) __attribute__((always_inline)) {
-        float alpha = 1.f;
-        if (__builtin_expect(__any(mloc > m_run + 15.5f), 0)) {
-            const float m_new = fmaxf(m_run, mloc - 10.f);
-            alpha = exp2f(m_run - m_new);
-            m_run = m_new;
+    auto rescale = [&](float m_new) __attribute__((always_inline)) {
+        const float alpha = exp2f(m_run - m_new);
+        m_run = m_new;
 #pragma unroll
-            for (int d = 0; d < DB; d++) O[d] *= alpha;
-        }
+        for (int d = 0; d < DB; d++) O[d] *= alpha;
         return alpha;
     };
+    auto grows = [&](float mloc) __attribute__((always_inline)) { return (bool)__any(mloc > m_run + 15.5f); };
+    auto raised = [&](float mloc) __attribute__((always_inline)) { return fmaxf(m_run, mloc - 10.f); };
     auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float m, float &psum, int e) __attribute__((always_inline)) {
         const int sb = e >> 4, i = e & 15;
         const float p = __builtin_amdgcn_exp2f(fmaf(Sx[sb][i], unit, -m));
@@ -509,13 +506,18 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
         }
     };
 
-    // Iteration kb: PV of tile kb - 1 beside the score arithmetic of tile kb, then QK of tile kb + 1 beside the
-    // exponentials of tile kb. K tile kb + 2 goes into the K slot that tile kb left, V^T tile kb into the V^T slot that tile
+    // Iteration kb: PV of tile kb - 1 beside the score arithmetic of tile kb (soft-caps, the maximum), then QK of tile kb + 1
+    // beside the exponentials of tile kb. K tile kb + 2 goes into the K slot that tile kb left, V^T tile kb into the V^T slot that tile
     // kb - 2 left; both are read an iteration on. The first iteration (kb0 - 1) has the first QK alone and the last
     // (kb1) the last PV, so that there is one copy of the products' code. Codes are loaded a whole iteration before they are
     // widened, keys beside PV and values beside QK (also where there is no such tile: into slots that nothing reads again
     // before they are written).
     constexpr int QKM = 2 * KC, PVM = 4 * DB;
+    // With one wave a SIMD a phase takes its instructions' issue or its MFMAs, whichever is longer: over halves of heads of 256
+    // QK's is the former and PV's the latter, so half of the exponentials go beside PV, whose first half then finds the
+    // maximum (512 tokens over 16384 keys 161 us, 155; 8 of the 32 159, 24 156). Over codes, whose widening fills PV, and at two
+    // waves a SIMD it was slower.
+    constexpr int EARLY = !CAP && !C4 && D == 256 ? 16 : 0, MXM = EARLY ? PVM / 2 : PVM;
     f32x16 S[2] = {};
     f16x8 P[2][2] = {};
     if (kb0 < kb1) {
@@ -532,6 +534,12 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 #pragma unroll 1
         for (int kb = kb0 - 1;; kb++) {
             const int cur = (kb - kb0) & 1;
+            // (Q in the accumulators' registers, where the MFMAs read it as well: else the compiler moves 70 others a tile, 3%.
+            // Over codes it is 5% slower.)
+            if constexpr (D == 256 && !C4) {
+#pragma unroll
+                for (int c = 0; c < KC; c++) asm volatile("" : "+a"(qf[c]));
+            }
             const bool tile = kb >= kb0 && kb < kb1;
             if constexpr (!C4) wait_vm0();
             lds_barrier();
@@ -544,11 +552,32 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     load_rv(kb + 1);
                 }
             }
+            if constexpr (!CAP) {
+                if (tile) mask(kb, S);
+            }
+            float mloc = -INFINITY, psum = 0.f;
+            [[maybe_unused]] float m_next = m_run;
+            [[maybe_unused]] bool up = false;
+            f16x8 Pm[2][2], (&Pn)[2][2] = EARLY > 0 ? Pm : P;
             if (kb > kb0) {
                 clean_v(kb - 1, cur ^ 1);
                 pv(cur ^ 1, P, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = m * 32 / PVM; e < (m + 1) * 32 / PVM; e++) cap1(S, e);
+                    for (int e = m * 32 / MXM; e < min(32, (m + 1) * 32 / MXM); e++) {
+                        cap1(S, e);
+                        if constexpr (!CAP) mloc = fmaxf(mloc, S[e >> 4][e & 15]);
+                    }
+                    if constexpr (EARLY > 0) {
+                        if (m == MXM) {
+                            mloc = highest(mloc);
+                            up = tile && grows(mloc);
+                            m_next = up ? raised(mloc) : m_run;
+                        }
+                        if (m >= MXM) {
+#pragma unroll
+                            for (int e = (m - MXM) * EARLY / (PVM - MXM); e < (m + 1 - MXM) * EARLY / (PVM - MXM); e++) prob1(S, Pn, m_next, psum, e);
+                        }
+                    }
                     if constexpr (C4) {
 #pragma unroll
                         for (int u = m * CF::KU / PVM; u < (m + 1) * CF::KU / PVM; u++) put_k(cur, u);
@@ -557,15 +586,35 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 if (kb == kb1) break;
             } else {
 #pragma unroll
-                for (int e = 0; e < 32; e++) cap1(S, e);
+                for (int e = 0; e < 32; e++) {
+                    cap1(S, e);
+                    if constexpr (!CAP) mloc = fmaxf(mloc, S[e >> 4][e & 15]);
+                }
+                if constexpr (EARLY > 0) {
+                    mloc = highest(mloc);
+                    up = tile && grows(mloc);
+                    m_next = up ? raised(mloc) : m_run;
+#pragma unroll
+                    for (int e = 0; e < EARLY; e++) prob1(S, Pn, m_next, psum, e);
+                }
                 if constexpr (C4) {
 #pragma unroll
                     for (int u = 0; u < CF::KU; u++) put_k(cur, u);
                 }
             }
-            float alpha = 1.f, psum = 0.f;
             if constexpr (C4) load_k(kb + 3);
-            if (tile) alpha = grow(finish(kb, S));
+            if constexpr (CAP) {
+                if (tile) mask(kb, S);
+#pragma unroll
+                for (int e = 0; e < 32; e++) mloc = fmaxf(mloc, S[e >> 4][e & 15]);
+            }
+            float alpha = 1.f;
+            if constexpr (EARLY > 0) {
+                if (__builtin_expect(up, 0)) alpha = rescale(m_next);
+            } else if (tile) {
+                mloc = highest(mloc);
+                if (__builtin_expect(grows(mloc), 0)) alpha = rescale(raised(mloc));
+            }
             if constexpr (C4) {
                 pair_v(max(kb, kb0));
                 load_v(kb + 1);
@@ -574,7 +623,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 f32x16 Sn[2];
                 qk(cur ^ 1, Sn, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = m * 32 / QKM; e < (m + 1) * 32 / QKM; e++) prob1(S, P, m_run, psum, e);
+                    for (int e = EARLY + m * (32 - EARLY) / QKM; e < EARLY + (m + 1) * (32 - EARLY) / QKM; e++) prob1(S, Pn, m_run, psum, e);
                     if constexpr (C4) {
 #pragma unroll
                         for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(cur, u);
@@ -586,14 +635,18 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 float m = m_run;
                 asm("" : "+v"(m));   // (or the compiler takes both branches' subtractions out in front of the products)
 #pragma unroll
-                for (int e = 0; e < 32; e++) prob1(S, P, m, psum, e);
+                for (int e = EARLY; e < 32; e++) prob1(S, Pn, m, psum, e);
                 if constexpr (C4) {
 #pragma unroll
                     for (int u = 0; u < CF::VU; u++) put_v(cur, u);
                 }
             }
             if (tile) {
-                reorder(P);
+                reorder(Pn);
+                if constexpr (EARLY > 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) P[i >> 1][i & 1] = Pn[i >> 1][i & 1];
+                }
                 l_run = l_run * alpha + psum;
             }
         }
