@@ -249,8 +249,8 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     [[maybe_unused]] int kw[CF::ITEMS][CF::KW];
     [[maybe_unused]] f16x2 ksm[CF::ITEMS];
     [[maybe_unused]] i32x4 vw[CF::ITEMS][2], vsm[CF::ITEMS][2];
-    [[maybe_unused]] unsigned vp[CF::ITEMS][4];      // pairs of keys, the thread's nibbles lowest
-    [[maybe_unused]] f16x2 vsc[CF::ITEMS][4], vmi[CF::ITEMS][4];
+    [[maybe_unused]] unsigned vp[4];                 // of one run: pairs of keys, the thread's nibbles lowest
+    [[maybe_unused]] f16x2 vsc[4], vmi[4];
     [[maybe_unused]] const int vpart = D == 64 ? (tid >> 3) & 3 : (tid >> 3) & 1, vword = D == 64 ? tid >> 5 : tid >> 4;
     [[maybe_unused]] const Widen widen;
     [[maybe_unused]] const size_t hr = C4 ? (size_t)s * a.c.heads + hk : 0;
@@ -275,18 +275,15 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             ksm[i] = *reinterpret_cast<const f16x2 *>(sms + d / 32 * 4);
         }
     };
-    auto load_v = [&](int kb) __attribute__((always_inline)) {
+    auto load_v = [&](int kb, int i) __attribute__((always_inline)) {
         const int key = min(key_of(min(kb, kb1 - 1)) + 8 * (tid & 7), a.c.cap - 8);
         const size_t block = hr * (a.c.cap / 8) + key / 8;
+        const int w = min(vword + 16 * i, a.dv / 8 - 1);
+        const char *p = a.c.vc + (block * (a.dv / 8) + w) * 32, *m = a.c.vs + (block * (a.dv / 32) + w / 4) * 32;
 #pragma unroll
-        for (int i = 0; i < CF::ITEMS; i++) {
-            const int w = min(vword + 16 * i, a.dv / 8 - 1);
-            const char *p = a.c.vc + (block * (a.dv / 8) + w) * 32, *m = a.c.vs + (block * (a.dv / 32) + w / 4) * 32;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                vw[i][e] = *reinterpret_cast<const i32x4 *>(p + 16 * e);
-                vsm[i][e] = *reinterpret_cast<const i32x4 *>(m + 16 * e);
-            }
+        for (int e = 0; e < 2; e++) {
+            vw[i][e] = *reinterpret_cast<const i32x4 *>(p + 16 * e);
+            vsm[i][e] = *reinterpret_cast<const i32x4 *>(m + 16 * e);
         }
     };
     // unit u of a thread's key words: eight dims of its key, one 16-byte write
@@ -296,36 +293,39 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
         const f16x8 x = widen.eight(kw[i][w], ksm[i]);
         *reinterpret_cast<f16x8 *>(smem + slot * CF::STAGE + key * (D * 2) + ((chunk ^ CF::kx(key)) << 4)) = x;
     };
-    // pairs of keys of the thread's value words; keys that no row sees get scale and minimum 0
-    auto pair_v = [&](int kb) __attribute__((always_inline)) {
+    // pairs of keys of run i of the thread's value words; keys that no row sees get scale and minimum 0
+    auto pair_v = [&](int kb, int i) __attribute__((always_inline)) {
         const int key0 = key_of(kb);
         if (!whole(key0)) {
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (dead(key0 + 8 * (tid & 7) + e))
-#pragma unroll
-                    for (int i = 0; i < CF::ITEMS; i++) vsm[i][e >> 2][e & 3] = 0;
+                if (dead(key0 + 8 * (tid & 7) + e)) vsm[i][e >> 2][e & 3] = 0;
         }
         const unsigned half = D == 64 ? vpart >> 1 : vpart;
         const unsigned sel = half ? 0x07060302u : 0x05040100u;
 #pragma unroll
-        for (int i = 0; i < CF::ITEMS; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const unsigned w0 = vw[i][k >> 1][2 * (k & 1)], w1 = vw[i][k >> 1][2 * (k & 1) + 1];
-                const unsigned s0 = vsm[i][k >> 1][2 * (k & 1)], s1 = vsm[i][k >> 1][2 * (k & 1) + 1];
-                vp[i][k] = __builtin_amdgcn_perm(w1, w0, sel) >> (D == 64 ? 8 * (vpart & 1) : 0);
-                vsc[i][k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
-                vmi[i][k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
-            }
+        for (int k = 0; k < 4; k++) {
+            const unsigned w0 = vw[i][k >> 1][2 * (k & 1)], w1 = vw[i][k >> 1][2 * (k & 1) + 1];
+            const unsigned s0 = vsm[i][k >> 1][2 * (k & 1)], s1 = vsm[i][k >> 1][2 * (k & 1) + 1];
+            vp[k] = __builtin_amdgcn_perm(w1, w0, sel) >> (D == 64 ? 8 * (vpart & 1) : 0);
+            vsc[k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x05040100u));
+            vmi[k] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(s1, s0, 0x07060302u));
+        }
+    };
+    // (Two runs, heads of 256: each where its first unit is written, so that the pairs of one take registers alone: 4% of
+    // 2048 tokens' time. One run: in front of QK, 6% of it for heads of 128, whose loads then have longer.)
+    auto next_v = [&](int kb, int i) __attribute__((always_inline)) {
+        pair_v(max(kb, kb0), i);
+        load_v(kb + 1, i);
     };
     // unit u: eight keys of one dim, one 16-byte write
-    auto put_v = [&](int slot, int u) __attribute__((always_inline)) {
+    auto put_v = [&](int kb, int slot, int u) __attribute__((always_inline)) {
         const int i = u / CF::VD, j = u % CF::VD, d = 8 * (vword + 16 * i) + CF::VD * vpart + j;
+        if (CF::ITEMS > 1 && j == 0) next_v(kb, i);
         f16x8 x;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const f16x2 y = widen.at(vp[i][k], j, vsc[i][k], vmi[i][k]);
+            const f16x2 y = widen.at(vp[k], j, vsc[k], vmi[k]);
             x[2 * k] = y[0];
             x[2 * k + 1] = y[1];
         }
@@ -523,7 +523,8 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     if (kb0 < kb1) {
         if constexpr (C4) {
             load_k(kb0);
-            load_v(kb0);
+#pragma unroll
+            for (int i = 0; i < CF::ITEMS; i++) load_v(kb0, i);
 #pragma unroll
             for (int u = 0; u < CF::KU; u++) put_k(0, u);
             load_k(kb0 + 1);
@@ -534,9 +535,8 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 #pragma unroll 1
         for (int kb = kb0 - 1;; kb++) {
             const int cur = (kb - kb0) & 1;
-            // (Q in the accumulators' registers, where the MFMAs read it as well: else the compiler moves 70 others a tile, 3%.
-            // Over codes it is 5% slower.)
-            if constexpr (D == 256 && !C4) {
+            // (Q in the accumulators' registers, where the MFMAs read it as well: else the compiler moves 70 others a tile, 3%)
+            if constexpr (D == 256) {
 #pragma unroll
                 for (int c = 0; c < KC; c++) asm volatile("" : "+a"(qf[c]));
             }
@@ -615,10 +615,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 mloc = highest(mloc);
                 if (__builtin_expect(grows(mloc), 0)) alpha = rescale(raised(mloc));
             }
-            if constexpr (C4) {
-                pair_v(max(kb, kb0));
-                load_v(kb + 1);
-            }
+            if constexpr (C4 && CF::ITEMS == 1) next_v(kb, 0);
             if (kb + 1 < kb1) {
                 f32x16 Sn[2];
                 qk(cur ^ 1, Sn, [&](int m) __attribute__((always_inline)) {
@@ -626,7 +623,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     for (int e = EARLY + m * (32 - EARLY) / QKM; e < EARLY + (m + 1) * (32 - EARLY) / QKM; e++) prob1(S, Pn, m_run, psum, e);
                     if constexpr (C4) {
 #pragma unroll
-                        for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(cur, u);
+                        for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(kb, cur, u);
                     }
                 });
                 S[0] = Sn[0];
@@ -638,7 +635,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 for (int e = EARLY; e < 32; e++) prob1(S, Pn, m, psum, e);
                 if constexpr (C4) {
 #pragma unroll
-                    for (int u = 0; u < CF::VU; u++) put_v(cur, u);
+                    for (int u = 0; u < CF::VU; u++) put_v(kb, cur, u);
                 }
             }
             if (tile) {
