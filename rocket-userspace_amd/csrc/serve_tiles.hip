@@ -14,10 +14,11 @@
 // it is the second product's operand. O is rescaled only when some running maximum grows by more than 5.5 (log2 units).
 //
 // Roundings beside the result's: weights to fp16 (summed as rounded), codes' values to fp16 as the cache's reading gives them;
-// scores, maxima, sums and outputs are fp32. Measured: 2048 tokens under a window of 1024, 16 / 8 heads of 256, 60.0 us (575
-// TFLOP/s); 512 over 4096 codes 68.6 (469); 2048 over 8192 fp16 keys, 32 / 8 heads of 128, 289 (830). Heads of 256
-// have one wave a SIMD: a tile's MFMAs are 2048 of its 5700 cycles, bound by 256 KB of LDS reads (every wave reads
-// the whole tile) whose latency nothing else covers; over codes, 816 VALU operations a wave and tile (384 over halves) make it 7000.
+// scores, maxima, sums and outputs are fp32. Measured: 2048 tokens under a window of 1024, 16 / 8 heads of 256, 54.6 us (630
+// TFLOP/s); 512 over 16384 fp16 keys of those heads 155 (870); 512 over 4096 codes 68 (475); 2048 over 8192 fp16 keys, 32 / 8
+// heads of 128, 274 (880). Heads of 256 have one wave a SIMD, which issues in order: a tile of halves is some 640
+// instructions of 4 cycles and 64 MFMAs of 32 in about 5200 cycles, of which a fifth waits for LDS, loads or the other waves
+// (LDS itself is busy a fifth of the time); over codes the widening makes it 6600 to 6900.
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
