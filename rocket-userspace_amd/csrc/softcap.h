@@ -1,4 +1,4 @@
-// softcap.h — a soft-capped score in log2 units, for the serving kernels.
+// softcap.h — a soft-capped score in log2 units, for the few-row serving kernels (the tiles leave out its constant).
 #pragma once
 
 #include <hip/hip_runtime.h>
