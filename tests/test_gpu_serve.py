@@ -317,6 +317,24 @@ def test_attn_scale_not_positive(lib, fd, T, cap, scale):
     near(out[0], *win_want(Q, K, V, see, scale, cap))
 
 
+@pytest.mark.parametrize("cap", [-30.0, -4.0, 1e-3, 1e4])
+@pytest.mark.parametrize("T,d", [(2, 64), (40, 64), (40, 256), (20, 160)])
+def test_attn_soft_caps(lib, fd, T, d, cap):
+    """c tanh(s / c) is even in c; caps that flatten every score, and that hardly bend one. (A cap's own bound: the
+    exponential's and the reciprocal's 2^-22 of it.)"""
+    heads, kvh, n, window, sinks, scale = 4, 2, 150, 70, 3, d ** -0.5
+    c, Q = kv4_case(15, heads, kvh, d, d, T, [n])
+    out, sh = np.full((1, heads, T, d), 7, np.float16), R.Kv4Shape(*c.dims)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, 1, T, n, heads, scale, cap, window, sinks, R.ptr(Q),
+                                    R.ptr(np.array([n], np.int32)), R.ptr(out)) == 0
+    (want, tol), = kv4_want(c, Q, [n], window, sinks, scale, cap)
+    near(out[0], want, tol + 2 * np.expm1(abs(cap) * 2.0 ** -22) * np.abs(c.rows()[1][1, :, :n]).max())
+    Q, K, V, see = win_case(16, heads, kvh, d, d, T, n, n, window, sinks)
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, cap, window, sinks, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(out)) == 0
+    want, tol = win_want(Q, K, V, see, scale, cap)
+    near(out[0], want, tol + 2 * np.expm1(abs(cap) * 2.0 ** -22) * np.abs(V.astype(np.float64)).max())
+
+
 # ---- windowed attention over fp16 keys -------------------------------------------------
 
 WIN = [  # heads, kv heads, dk, dv, tokens, keys, stride, window, sinks, softcap
@@ -592,7 +610,7 @@ def _calls(lib, seed):
     calls = dict(rope=(lambda fd: lib.rocket_qk_norm_rope_fp16(fd, 1, 3, heads, kvh, d, d, 0, 1e-6, R.ptr(x), (heads + kvh) * d, R.ptr(x.data_ptr() + 2 * heads * d),
                                                                     (heads + kvh) * d, None, None, R.ptr(freq), R.ptr(pos), R.ptr(q), R.ptr(k)), [q, k]),
                  append=(lambda fd: lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, 3, R.ptr(K), 0, n * d, d, R.ptr(K), 0, n * d, d, R.ptr(L)), [mem]))
-    for T in (1, 90):
+    for T in (1, 8, 12, 90):
         Q, a, b = dev(F.f16(g.standard_normal((heads, T, d)))), new(heads, T, d), new(heads, T, d)
         calls[f"kv4 {T}"] = (lambda fd, T=T, Q=Q, a=a: lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 0, 1, T, cap, heads, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(a)), [a])
         calls[f"window {T}"] = (lambda fd, T=T, Q=Q, b=b: lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, 0.1, 0.0, 1500, 4, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(b)), [b])
@@ -608,7 +626,7 @@ def _captured(fd, call, stream):
     return graph
 
 
-@pytest.mark.parametrize("name", ["rope", "append", "kv4 1", "kv4 90", "window 1", "window 90"])
+@pytest.mark.parametrize("name", ["rope", "append", "kv4 1", "kv4 12", "kv4 90", "window 1", "window 8", "window 90"])
 def test_serve_capture_on_a_fresh_handle(lib, name):
     """A handle's first call is a captured one: it has no scratch to split keys on, and takes as many workgroups as it can
     without. Up to the splits' order of sums the eager results."""
