@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void k_fa_merge(const float *__restrict__ part
 // lie in its window or among the sinks; no mask and no clamp. There a row may see nothing of a chunk (a
 // finite first maximum), and values of keys that a row does not see must not reach it as 0 times an infinity. NQ:
 // blocks of 16 rows that share a chunk's fragments.
-template <int D, int NQ, bool CAP, bool FULL, bool WIN>
+template <int D, int NQ, Cap CAP, bool FULL, bool WIN>
 __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 {
     constexpr int KS = D / 32, VB = D / 16, LROW = D + 4;   // score steps, output blocks, LDS row (floats)
@@ -257,8 +257,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float y = S[x][i >> 2][i & 3];
-                if constexpr (WIN) v[i] = CAP ? softcap_log2(y, a.scale, a.softcap) : y * (a.scale * kLog2e);
-                else if constexpr (CAP) v[i] = fmaxf(a.softcap * tanhf(y * a.scale / a.softcap) + (float)mv[i], -30000.f) * kLog2e;
+                if constexpr (WIN && CAP != kUncapped) v[i] = softcap_log2<CAP>(y, a.scale, a.softcap);
+                else if constexpr (WIN) v[i] = y * (a.scale * kLog2e);
+                else if constexpr (CAP != kUncapped) v[i] = fmaxf(a.softcap * tanhf(y * a.scale / a.softcap) + (float)mv[i], -30000.f) * kLog2e;
                 else v[i] = fmaxf(fmaf((float)mv[i], kLog2e, y * (a.scale * kLog2e)), -30000.f * kLog2e);
                 if constexpr (!WIN) {
                     if (key0 + 8 * q + i >= a.n_kv) v[i] = -INFINITY;   // weighs 0
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
     }
 }
 
-template <int D, int NQ, bool CAP, bool FULL, bool WIN> hipError_t launch_rows_f(const RowArgs &a, int kv_heads, hipStream_t s)
+template <int D, int NQ, Cap CAP, bool FULL, bool WIN> hipError_t launch_rows_f(const RowArgs &a, int kv_heads, hipStream_t s)
 {
     auto kern = k_fa_rows<D, NQ, CAP, FULL, WIN>;
     const int R = a.gqa * a.T;
@@ -399,10 +400,13 @@ template <int D, int NQ, bool CAP, bool FULL, bool WIN> hipError_t launch_rows_f
 
 template <int D, int NQ, bool WIN> hipError_t launch_rows_q(const RowArgs &a, int kv_heads, hipStream_t s)
 {
-    const bool cap = a.softcap != 0.f;
-    if (a.dk == D && a.dv == D)
-        return cap ? launch_rows_f<D, NQ, true, true, WIN>(a, kv_heads, s) : launch_rows_f<D, NQ, false, true, WIN>(a, kv_heads, s);
-    return cap ? launch_rows_f<D, NQ, true, false, WIN>(a, kv_heads, s) : launch_rows_f<D, NQ, false, false, WIN>(a, kv_heads, s);
+    const bool full = a.dk == D && a.dv == D;
+    const Cap cap = cap_of(a.softcap);
+    if (cap == kUncapped) return full ? launch_rows_f<D, NQ, kUncapped, true, WIN>(a, kv_heads, s) : launch_rows_f<D, NQ, kUncapped, false, WIN>(a, kv_heads, s);
+    if constexpr (WIN) {   // (without one, tanhf takes any cap)
+        if (cap == kWide) return launch_rows_f<D, NQ, kWide, false, WIN>(a, kv_heads, s);   // (rare: one kernel for all heads)
+    }
+    return full ? launch_rows_f<D, NQ, kNarrow, true, WIN>(a, kv_heads, s) : launch_rows_f<D, NQ, kNarrow, false, WIN>(a, kv_heads, s);
 }
 template <int D, bool WIN> hipError_t launch_rows(const RowArgs &a, int kv_heads, hipStream_t s)
 {

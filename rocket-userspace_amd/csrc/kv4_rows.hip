@@ -67,7 +67,7 @@ struct Chunks {
 __device__ __forceinline__ int share(int count, int nsplit) { return max(kWaves, (count + nsplit - 1) / nsplit); }
 
 // D: head sizes up to this (64, 128, 256). NQ: blocks of 16 rows. FULL: dk and dv are D.
-template <int D, int NQ, bool CAP, bool FULL>
+template <int D, int NQ, Cap CAP, bool FULL>
 __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 {
     const ServeAttn &a = ra.a;
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float y = S[x][i >> 2][i & 3];
-                if constexpr (CAP) v[i] = softcap_log2(y, a.scale, a.softcap);
+                if constexpr (CAP != kUncapped) v[i] = softcap_log2<CAP>(y, a.scale, a.softcap);
                 else v[i] = y * (a.scale * kLog2e);
             }
             if (!whole) {
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
 int row_blocks(const ServeAttn &a) { return (a.gqa * a.n_tokens + 15) / 16; }
 int row_groups(const ServeAttn &a) { return std::max(a.dk, a.dv) <= 128 ? 1 : (row_blocks(a) + 1) / 2; }
 
-template <int D, int NQ, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
+template <int D, int NQ, Cap CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
 {
     auto kern = k_kv4_rows<D, NQ, CAP, FULL>;
     const ServeAttn &a = ra.a;
@@ -399,9 +399,12 @@ template <int D, int NQ, bool CAP, bool FULL> hipError_t launch_f(const Kv4RowAr
 }
 template <int D, int NQ> hipError_t launch_q(const Kv4RowArgs &ra, hipStream_t s)
 {
-    const bool cap = ra.a.softcap != 0.f;
-    if (ra.a.dk == D && ra.a.dv == D) return cap ? launch_f<D, NQ, true, true>(ra, s) : launch_f<D, NQ, false, true>(ra, s);
-    return cap ? launch_f<D, NQ, true, false>(ra, s) : launch_f<D, NQ, false, false>(ra, s);
+    const bool full = ra.a.dk == D && ra.a.dv == D;
+    switch (cap_of(ra.a.softcap)) {
+    case kUncapped: return full ? launch_f<D, NQ, kUncapped, true>(ra, s) : launch_f<D, NQ, kUncapped, false>(ra, s);
+    case kNarrow: return full ? launch_f<D, NQ, kNarrow, true>(ra, s) : launch_f<D, NQ, kNarrow, false>(ra, s);
+    default: return launch_f<D, NQ, kWide, false>(ra, s);   // (rare: one kernel for all heads)
+    }
 }
 template <int D> hipError_t launch(const Kv4RowArgs &ra, hipStream_t s)
 {

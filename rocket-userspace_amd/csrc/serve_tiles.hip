@@ -22,6 +22,7 @@
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
+#include "softcap.h"
 
 #include <algorithm>
 #include <atomic>
@@ -96,10 +97,10 @@ enum Src { kHalves, kRagged, kCodes };
 template <Src SRC> struct Part { typedef float T; };
 template <> struct Part<kCodes> { typedef _Float16 T; };
 
-template <int D, Src SRC, bool CAP>
+template <int D, Src SRC, Cap CAP>
 __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1) void k_serve_tiles(const TileArgs ta)
 {
-    constexpr bool C4 = SRC == kCodes, RV = SRC == kRagged;
+    constexpr bool C4 = SRC == kCodes, RV = SRC == kRagged, CAPPED = CAP != kUncapped;
     const ServeAttn &a = ta.a;
     using CF = Cfg<D>;
     constexpr int KC = CF::KC, KCPR = CF::KCPR, DB = CF::DB;
@@ -368,13 +369,15 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     };
     // Scores stay products, and the factor to log2 units joins the exponential's subtraction (Q carries the scale's sign, so
     // that the largest product is the largest score; a scale of 0: Q is 0 and the factor 1, so that hidden keys'
-    // -infinity stays one). A soft-capped score, c tanh(y) = 2 c sigmoid(2 y) - c, is kept as its sigmoid: 2 c is the factor, and
-    // the constant leaves the softmax unchanged (hardware exponential and reciprocal: within c 2^-22 of the score; four
-    // operations for six, 2048 tokens over 8192 keys, heads of 128, 361 us, 342).
-    const float unit = CAP ? 2.f * 1.4426950408889634f * fabsf(a.softcap) : a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    // -infinity stays one). A score under a cap up to kNarrowCap, c tanh(y) = 2 c sigmoid(2 y) - c, is kept as its sigmoid: 2 c is
+    // the factor, and the constant leaves the softmax unchanged (hardware exponential and reciprocal: within c 2^-22 of the
+    // score; four operations for six, 2048 tokens over 8192 keys, heads of 128, 361 us, 342). One under a larger cap is
+    // kept as it is.
+    const float unit = CAP == kWide ? 1.4426950408889634f : CAP == kNarrow ? 2.f * 1.4426950408889634f * fabsf(a.softcap) : a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
     [[maybe_unused]] const float slope = -2.f * 1.4426950408889634f * fabsf(a.scale) / fabsf(a.softcap);
     auto cap1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
-        if constexpr (CAP) Sx[e >> 4][e & 15] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(Sx[e >> 4][e & 15] * slope));
+        if constexpr (CAP == kWide) Sx[e >> 4][e & 15] = softcap_wide(Sx[e >> 4][e & 15] * fabsf(a.scale), 1.f / a.softcap, a.softcap);
+        else if constexpr (CAP == kNarrow) Sx[e >> 4][e & 15] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(Sx[e >> 4][e & 15] * slope));
     };
     auto mask = [&](int kb, f32x16 (&Sx)[2]) __attribute__((always_inline)) {
         const int key0 = key_of(kb);
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     // QK's is the former and PV's the latter, so half of the exponentials go beside PV, whose first half then finds the
     // maximum (512 tokens over 16384 keys 161 us, 155; 8 of the 32 159, 24 156). Over codes, whose widening fills PV, and at two
     // waves a SIMD it was slower.
-    constexpr int EARLY = !CAP && !C4 && D == 256 ? 16 : 0, MXM = EARLY ? PVM / 2 : PVM;
+    constexpr int EARLY = !CAPPED && !C4 && D == 256 ? 16 : 0, MXM = EARLY ? PVM / 2 : PVM;
     f32x16 S[2] = {};
     f16x8 P[2][2] = {};
     if (kb0 < kb1) {
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     load_rv(kb + 1);
                 }
             }
-            if constexpr (!CAP) {
+            if constexpr (!CAPPED) {
                 if (tile) mask(kb, S);
             }
             float mloc = -INFINITY, psum = 0.f;
@@ -606,7 +609,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 }
             }
             if constexpr (C4) load_k(kb + 3);
-            if constexpr (CAP) {   // (a hidden key's sigmoid would not be -infinity: masks come behind it)
+            if constexpr (CAPPED) {   // (a hidden key's capped score would not be -infinity: masks come behind it)
                 if (tile && !whole(key_of(kb))) {
                     mask(kb, S);
                     mloc = -INFINITY;
@@ -754,7 +757,7 @@ template <typename P> void combine(const TileArgs &ta, long rows, long blocks, h
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const P *>(ta.part), ta.a.out, rows, ta.a.dv, ta.nsplit);
 }
 
-template <int D, Src SRC, bool CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
+template <int D, Src SRC, Cap CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
 {
     auto kern = k_serve_tiles<D, SRC, CAP>;
     static_assert(Cfg<D>::LDS <= 160 * 1024, "LDS budget");
@@ -763,12 +766,18 @@ template <int D, Src SRC, bool CAP> hipError_t launch_c(const TileArgs &ta, unsi
     hipLaunchKernelGGL(kern, dim3(wgs), dim3(256), Cfg<D>::LDS, s, ta);
     return hipGetLastError();
 }
+template <int D, Src SRC> hipError_t launch_s(const TileArgs &ta, unsigned wgs, hipStream_t s)
+{
+    switch (cap_of(ta.a.softcap)) {
+    case kUncapped: return launch_c<D, SRC, kUncapped>(ta, wgs, s);
+    case kNarrow: return launch_c<D, SRC, kNarrow>(ta, wgs, s);
+    default: return launch_c<D, SRC, kWide>(ta, wgs, s);
+    }
+}
 template <int D> hipError_t launch(const TileArgs &ta, unsigned wgs, hipStream_t s)
 {
-    const bool cap = ta.a.softcap != 0.f;
-    if (!ta.a.Kf) return cap ? launch_c<D, kCodes, true>(ta, wgs, s) : launch_c<D, kCodes, false>(ta, wgs, s);
-    if (ta.a.stride % 8) return cap ? launch_c<D, kRagged, true>(ta, wgs, s) : launch_c<D, kRagged, false>(ta, wgs, s);
-    return cap ? launch_c<D, kHalves, true>(ta, wgs, s) : launch_c<D, kHalves, false>(ta, wgs, s);
+    if (!ta.a.Kf) return launch_s<D, kCodes>(ta, wgs, s);
+    return ta.a.stride % 8 ? launch_s<D, kRagged>(ta, wgs, s) : launch_s<D, kHalves>(ta, wgs, s);
 }
 
 // Row blocks of a KV head: its rows in a row, or each head's tokens by themselves, which takes more blocks where the

@@ -424,6 +424,37 @@ def test_window_attn_is_the_masked_one(lib, fd):
     near(b, want, tol)
 
 
+# ---- soft-caps: every kernel that has them, and caps of any size -----------------------
+
+def tanh_slack(Q, K, V, scale, cap):
+    """What 2^-20 of the capped scores moves a result by: e^delta - 1 of the largest value, twice for the weights' sum."""
+    per = Q.shape[0] // K.shape[0]
+    s = max(np.abs(Q[i].astype(np.float64) @ K[i // per].astype(np.float64).T).max() for i in range(Q.shape[0]))
+    return 2 * np.expm1(2.0 ** -20 * min(abs(cap), s * abs(scale))) * np.abs(V.astype(np.float64)).max()
+
+
+@pytest.mark.parametrize("T,d,heads,kvh", [(1, 256, 4, 2), (5, 128, 8, 2), (20, 160, 4, 2), (40, 128, 4, 2), (70, 64, 4, 2), (70, 128, 2, 2), (66, 256, 2, 2), (65, 192, 2, 1)])
+@pytest.mark.parametrize("cap,scale", [(64.5, 1.0), (-300.0, 1.0), (1e4, 0.125), (-1e6, 0.125), (1e9, 0.125), (3e38, 0.125), (65.0, 20.0)])
+def test_attn_soft_caps_above_the_scores(lib, fd, T, d, heads, kvh, cap, scale):
+    """Caps far above the scores leave them as they are, up to one that means none; and scores of many times the cap. Beside the
+    bound of scores without a cap, 2^-20 of the capped score, for tanh's steps, and nothing that grows with the cap: y - y^3 / 3
+    + .. is off by a few 2^-24 of itself, and from y = 0.35 on 1 - 2 / (1 + e^2y), whose terms round to 1.7 2^-23, by 5 2^-23."""
+    n, window, sinks = 304, 150, 3
+    c, Q = kv4_case(17, heads, kvh, d, d, T, [n])
+    sh = R.Kv4Shape(*c.dims)
+    out = np.full((1, heads, T, d), 7, np.float16)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, 1, T, n, heads, scale, cap, window, sinks, R.ptr(Q), R.ptr(np.array([n], np.int32)),
+                                    R.ptr(out)) == 0
+    (want, tol), = kv4_want(c, Q, [n], window, sinks, scale, cap)
+    k, v = c.rows()
+    near(out[0], want, tol + tanh_slack(Q[0], k[1, :, :n], v[1, :, :n], scale, cap))
+    for stride in (n, n + 1):   # (V^T rows read by DMA, and through registers)
+        Q, K, V, see = win_case(18, heads, kvh, d, d, T, n, stride, window, sinks)
+        assert lib.rocket_flash_attn_window_fp16(fd, T, n, stride, d, d, heads, kvh, scale, cap, window, sinks, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(out)) == 0
+        want, tol = win_want(Q, K, V, see, scale, cap)
+        near(out[0], want, tol + tanh_slack(Q, K[:, :n], V, scale, cap))
+
+
 # ---- together, and as programs call them -----------------------------------------------
 
 def _handle(lib, stream):
