@@ -455,6 +455,37 @@ def test_attn_soft_caps_above_the_scores(lib, fd, T, d, heads, kvh, cap, scale):
         near(out[0], want, tol + tanh_slack(Q, K[:, :n], V, scale, cap))
 
 
+CAPPED_KV4 = [  # every soft-capped kernel over codes: rows of heads of up to 64, 128, 256, whole and narrower; tiles
+    (4, 2, 64, 64, 3, [300, 31, 0], 0, 0), (4, 2, 32, 64, 13, [300, 60], 100, 5), (2, 1, 64, 64, 32, [400], 50, 3),
+    (32, 8, 128, 128, 1, [700, 127, 128, 0], 0, 0), (8, 2, 128, 96, 7, [333, 70], 64, 3), (4, 1, 128, 128, 15, [300, 15], 0, 0), (8, 8, 96, 128, 1, [500], 0, 0),
+    (16, 8, 256, 256, 1, [1000, 33], 0, 0), (2, 1, 256, 256, 1, [2000], 700, 4), (4, 1, 256, 256, 6, [400, 31], 90, 2), (5, 1, 224, 256, 12, [500], 0, 0),
+    (4, 2, 64, 64, 70, [300, 90], 0, 0), (4, 2, 128, 128, 70, [500, 90], 0, 0), (6, 2, 96, 128, 40, [300, 77], 50, 3), (2, 1, 128, 128, 300, [900], 129, 70),
+    (2, 1, 256, 256, 70, [300, 200], 0, 0), (2, 1, 160, 224, 130, [700], 100, 5),
+]
+CAPPED_WIN = [  # the same over fp16 keys: rows; tiles of V^T rows that are whole chunks of eight keys, and ragged ones
+    (8, 2, 64, 64, 3, 300, 304, 0, 0), (2, 1, 64, 48, 12, 300, 301, 50, 3), (2, 1, 64, 64, 25, 400, 400, 100, 2), (16, 8, 128, 128, 1, 777, 784, 0, 0), (4, 2, 128, 112, 9, 333, 333, 60, 4),
+    (16, 8, 256, 256, 1, 777, 800, 0, 0), (2, 1, 256, 256, 1, 2001, 2001, 700, 4), (4, 2, 256, 256, 9, 600, 600, 100, 3), (2, 1, 160, 176, 9, 300, 303, 50, 1),
+    (4, 2, 64, 64, 70, 400, 400, 0, 0), (2, 1, 64, 64, 300, 1000, 1024, 129, 70), (2, 1, 96, 80, 90, 300, 304, 0, 0), (2, 1, 128, 128, 130, 512, 520, 100, 5),
+    (2, 2, 256, 256, 129, 1000, 1000, 200, 3), (2, 1, 160, 224, 70, 600, 600, 150, 4),
+    (2, 1, 64, 64, 90, 411, 411, 70, 4), (4, 2, 128, 128, 100, 411, 413, 90, 4), (2, 1, 256, 192, 70, 411, 413, 0, 0),
+]
+
+
+@pytest.mark.parametrize("cap", [30.0, -300.0])
+@pytest.mark.parametrize("uniform", [False, True])
+@pytest.mark.parametrize("case", CAPPED_KV4)
+def test_kv4_attn_capped(lib, fd, case, uniform, cap):
+    """The test of every attention call over the cache, for each soft-capped kernel."""
+    test_kv4_attn(lib, fd, case + (cap,), uniform)
+
+
+@pytest.mark.parametrize("cap", [30.0, -300.0])
+@pytest.mark.parametrize("kind", ["random", "uniform", "nan"])
+@pytest.mark.parametrize("case", CAPPED_WIN)
+def test_window_attn_capped(lib, fd, case, kind, cap):
+    test_window_attn(lib, fd, case + (cap,), kind)
+
+
 # ---- together, and as programs call them -----------------------------------------------
 
 def _handle(lib, stream):
