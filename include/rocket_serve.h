@@ -10,10 +10,12 @@
  *                                  and a few first keys that stay visible (sinks)
  *
  * As everywhere in this library: operands may be host or device pointers (the 4-bit cache alone must
- * be device memory), fd < 0 runs the fp64 host path (every operand host memory then), handles run
- * asynchronously where rocket_hip_set_mode says so, and a call returns 0 or a negative rocket_status:
- * -1 for a bad argument, before anything is launched. Results must not lie over a call's other
- * operands (-1). Strides count elements.
+ * be device memory); device memory is used in place where it is 16-byte aligned (seq_len and pos:
+ * 4-byte, so that a part of a batch's array is) and staged where it is not, which a captured call does
+ * not allow; fd < 0 runs the fp64 host path (every operand host memory then), handles run asynchronously
+ * where rocket_hip_set_mode says so, and a call returns 0 or a negative rocket_status: -1 for a bad
+ * argument, before anything is launched. Results must not lie over a call's other operands (-1).
+ * Strides count elements.
  *
  * Visibility. Token t of a call's n_tokens stands at position p = len - n_tokens + t of a sequence of
  * len keys. It sees key j when

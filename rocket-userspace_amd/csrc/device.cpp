@@ -213,15 +213,15 @@ Locked::~Locked()
 
 // ---- Call: operand staging for one entry-point invocation ----
 
-bool Call::direct_(const void *p) const
+bool Call::direct_(const void *p, size_t align) const
 {
-    if (!p || ((uintptr_t)p & 15u) != 0) return false;
+    if (!p || ((uintptr_t)p & (align - 1)) != 0) return false;
     return h_->trust_device || is_device_ptr(p, h_->device);
 }
 
-void Call::want(const void *p, size_t bytes)
+void Call::want(const void *p, size_t bytes, size_t align)
 {
-    if (!direct_(p)) need_ += round_(bytes);
+    if (!direct_(p, align)) need_ += round_(bytes);
 }
 
 bool stream_capturing(hipStream_t s)
@@ -287,9 +287,9 @@ void *Call::scratch(size_t bytes)
     return d;
 }
 
-void *Call::in(const void *p, size_t bytes)
+void *Call::in(const void *p, size_t bytes, size_t align)
 {
-    if (direct_(p)) return const_cast<void *>(p);
+    if (direct_(p, align)) return const_cast<void *>(p);
     PhaseTimer pt(t_stage_);
     host_io_ = true;
     void *d = scratch(bytes);

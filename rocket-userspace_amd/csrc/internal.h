@@ -52,7 +52,7 @@ void count_launch(uint64_t workgroups);
 bool is_device_ptr(const void *p, int device);
 
 // Stages one call's operands. in()/out() return the device address the kernel uses:
-// the caller's own pointer when it is 16-byte-aligned device memory, otherwise a slice
+// the caller's own pointer when it is aligned device memory (16 bytes but where a call says otherwise), otherwise a slice
 // of the handle's arena (inputs copied in, results copied back by finish()).
 // Whether the stream is being captured into a graph.
 bool stream_capturing(hipStream_t s);
@@ -60,8 +60,9 @@ bool stream_capturing(hipStream_t s);
 class Call {
 public:
     Call(Handle *h, const char *who) : h_(h), who_(who) {}
-    // Reserve arena space before in()/out(): sum of every host operand's bytes.
-    void want(const void *p, size_t bytes);
+    // Reserve arena space before in()/out(): sum of every host operand's bytes. `align`: what the kernels need to
+    // read a device operand in place (one that they read value by value: the value's size); the same for in().
+    void want(const void *p, size_t bytes, size_t align = 16);
     void want_scratch(size_t bytes) { need_ += round_(bytes); }
     // Scratch that the launch can do without (K slices' planes, key splits' partials, a padded mask):
     // `bytes`, reserved, or 0. While the handle's stream is being captured that is 0 where the arena would have
@@ -73,7 +74,7 @@ public:
     // Grows the arena if needed. One that a captured call has used is kept until the handle closes:
     // the graph replays on it (each at least 1.25 times the last, so all of them at most 5 times it).
     int  begin();
-    void *in(const void *p, size_t bytes);  // device view of an input
+    void *in(const void *p, size_t bytes, size_t align = 16);  // device view of an input
     void *out(void *p, size_t bytes);       // device view of an output
     void *scratch(size_t bytes);            // arena scratch (not copied)
     void *optional(size_t bytes) { return bytes && !opt_dropped_ ? scratch(bytes) : nullptr; }
@@ -85,7 +86,7 @@ public:
 
 private:
     static size_t round_(size_t b) { return (b + 255) & ~(size_t)255; }
-    bool direct_(const void *p) const;
+    bool direct_(const void *p, size_t align = 16) const;
     bool capturing_();
     int finish_();
     // ROCKET_MM_PROFILE: host milliseconds of this call's phases (staging copies and arena

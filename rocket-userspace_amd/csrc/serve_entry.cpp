@@ -15,6 +15,8 @@ using namespace rk;
 namespace {
 
 constexpr int64_t kMaxStride = (int64_t)1 << 40;
+// Lengths and positions are read one by one: a part of a batch's array (seq_len + seq0) is used in place.
+constexpr size_t kIntAlign = sizeof(int32_t);
 
 size_t h16(size_t n) { return n * sizeof(_Float16); }
 
@@ -78,7 +80,7 @@ int rope(const char *who, int fd, RopeLaunch L, int style)
     const size_t wb = h16((size_t)L.dim), fb = (size_t)L.rot / 2 * sizeof(float), pb = rows * sizeof(int32_t);
     const size_t qo = h16(rows * L.n_head * L.dim), ko = h16(rows * L.n_kv * L.dim);
     if (!L.rot) L.inv_freq = nullptr, L.pos = nullptr;
-    const struct { const void *p; size_t n; } in[] = {{L.q, qb}, {L.k, kb}, {L.wq, wb}, {L.wk, wb}, {L.inv_freq, fb}, {L.pos, pb}};
+    const struct { const void *p; size_t n, align; } in[] = {{L.q, qb, 16}, {L.k, kb, 16}, {L.wq, wb, 16}, {L.wk, wb, 16}, {L.inv_freq, fb, 16}, {L.pos, pb, kIntAlign}};
     for (const auto &i : in)
         if (overlap(i.p, i.n, L.q_out, qo) || overlap(i.p, i.n, L.k_out, ko)) return bad(who, "results over operands");
     if (overlap(L.q_out, qo, L.k_out, ko)) return bad(who, "results over each other");
@@ -87,13 +89,13 @@ int rope(const char *who, int fd, RopeLaunch L, int style)
     if (!lk.ok()) return bad_fd(who, fd);
     Call c(lk.h, who);
     for (const auto &i : in)
-        if (i.p) c.want(i.p, i.n);
+        if (i.p) c.want(i.p, i.n, i.align);
     c.want(L.q_out, qo);
     c.want(L.k_out, ko);
     if (int rc = c.begin()) return rc;
     const void *d[6];
     for (int i = 0; i < 6; i++) {
-        d[i] = in[i].p ? c.in(in[i].p, in[i].n) : nullptr;
+        d[i] = in[i].p ? c.in(in[i].p, in[i].n, in[i].align) : nullptr;
         if (in[i].p && !d[i]) return c.finish();
     }
     L.q = d[0];
@@ -216,11 +218,11 @@ int rocket_kv4_append_fp16(int fd, const rocket_kv4_shape *shape, void *cache, i
         Call c(lk.h, who);
         c.want(K, kb);
         c.want(V, vb);
-        c.want(seq_len, nb);
+        c.want(seq_len, nb, kIntAlign);
         if (int rc = c.begin()) return rc;
         r.K = static_cast<const _Float16 *>(c.in(K, kb));
         r.V = static_cast<const _Float16 *>(c.in(V, vb));
-        r.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb));
+        r.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb, kIntAlign));
         if (!r.K || !r.V || !r.seq_len) return c.finish();
         uint64_t blocks = 0;
         return launched(c, kv4_append(view, r, c.stream(), &blocks), blocks);
@@ -252,11 +254,11 @@ int rocket_kv4_read_fp16(int fd, const rocket_kv4_shape *shape, const void *cach
         if (!lk.ok()) return bad_fd(who, fd);
         if (!on_device(lk.h, cache)) return bad(who, "the cache is not memory of the handle's device");
         Call c(lk.h, who);
-        c.want(seq_len, nb);
+        c.want(seq_len, nb, kIntAlign);
         if (K) c.want(K, kb);
         if (V) c.want(V, vb);
         if (int rc = c.begin()) return rc;
-        r.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb));
+        r.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb, kIntAlign));
         r.Ko = K ? static_cast<_Float16 *>(c.out(K, kb)) : nullptr;
         r.Vo = V ? static_cast<_Float16 *>(c.out(V, vb)) : nullptr;
         if (!r.seq_len || (K && !r.Ko) || (V && !r.Vo)) return c.finish();
@@ -294,14 +296,14 @@ int rocket_kv4_attn_fp16(int fd, const rocket_kv4_shape *shape, const void *cach
         if (!lens_ok(lk.h, seq_len, n_seq, max_kv)) return bad(who, "a length above max_kv");
         Call c(lk.h, who);
         c.want(Q, qb);
-        c.want(seq_len, nb);
+        c.want(seq_len, nb, kIntAlign);
         c.want(out, ob);
         const size_t ws = c.want_optional(serve_attn_ws(a), max_kv >= 512);
         if (int rc = c.begin()) return rc;
         a.ws = static_cast<float *>(c.optional(ws));
         a.ws_bytes = a.ws ? ws : 0;
         a.Q = static_cast<const _Float16 *>(c.in(Q, qb));
-        a.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb));
+        a.seq_len = static_cast<const int32_t *>(c.in(seq_len, nb, kIntAlign));
         a.out = static_cast<_Float16 *>(c.out(out, ob));
         if (!a.Q || !a.seq_len || !a.out) return c.finish();
         uint64_t blocks = 0;

@@ -719,6 +719,56 @@ def test_serve_capture_on_a_fresh_handle(lib, name):
         lib.rocket_close(f)
 
 
+def test_serve_part_of_a_batch_captured(lib):
+    """Places 1 and 2 of four, their lengths and positions in the middle of the batch's arrays: a fresh handle's first calls
+    are captured ones, which only operands in place allow, and every replay takes the lengths of the day."""
+    import torch
+    stream, g = torch.cuda.Stream(), rng(47)
+    fd, heads, kvh, d, cap, T, window, sinks = _handle(lib, stream), 4, 2, 64, 200, 2, 40, 3
+    c = F.Cache(4, kvh, d, d, cap)
+    for s in range(4):
+        c.put_all(s, F.f16(g.standard_normal((kvh, cap, d))), F.f16(g.standard_normal((kvh, cap, d))))
+    sh, freq = R.Kv4Shape(*c.dims), np.linspace(0.01, 1, d // 2, dtype=np.float32)
+    W = (heads + 2 * kvh) * d
+    new = lambda *s: torch.zeros(s, dtype=torch.float16, device=DEV)  # noqa: E731
+    with torch.cuda.stream(stream):
+        mem, dfreq, x, q, k, out, back = dev(c.buf), dev(freq), new(2 * T, W), new(2, heads, T, d), new(2, kvh, T, d), new(2, heads, T, d), new(2, kvh, T, d)
+        lens, pos = torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(2 * T + 2, dtype=torch.int32, device=DEV)
+
+        def step():
+            L, at = R.ptr(lens.data_ptr() + 4), lambda h: R.ptr(x.data_ptr() + 2 * h * d)
+            return (lib.rocket_qk_norm_rope_fp16(fd, 2, T, heads, kvh, d, d, 0, 1e-6, at(0), W, at(heads), W, None, None, R.ptr(dfreq), R.ptr(pos.data_ptr() + 4), R.ptr(q), R.ptr(k)),
+                    lib.rocket_kv4_append_fp16(fd, C.byref(sh), R.ptr(mem), 1, 2, T, R.ptr(k), kvh * T * d, T * d, d, at(heads + kvh), T * W, d, W, L),
+                    lib.rocket_kv4_read_fp16(fd, C.byref(sh), R.ptr(mem), 1, 2, T, L, R.ptr(back), None),
+                    lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 1, 2, T, cap, heads, 0.125, 0.0, window, sinks, R.ptr(q), L, R.ptr(out)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        rcs = step()
+    assert rcs == (0, 0, 0, 0)
+    for day in ([150, 7, 99, 3], [1, 200, 64, 90], [5, 30, 2, 5]):
+        with torch.cuda.stream(stream):
+            X, P = F.f16(g.standard_normal((2 * T, W))), np.array(day[1:3])[:, None] - T + np.arange(T)
+            x.copy_(dev(X))
+            lens.copy_(dev(np.array(day, np.int32)))
+            pos[1:2 * T + 1].copy_(dev(P.reshape(-1).astype(np.int32)))
+            graph.replay()
+        stream.synchronize()
+        hq, hk, v = q.cpu().numpy(), k.cpu().numpy(), X[:, (heads + kvh) * d:].reshape(2, T, kvh, d)
+        near(hq, *F.rope(X, heads, d, d, False, 1e-6, None, freq, P.reshape(-1), 2))
+        near(hk, *F.rope(X[:, heads * d:], kvh, d, d, False, 1e-6, None, freq, P.reshape(-1), 2))
+        for s in range(2):
+            for t in range(T):
+                for h in range(kvh):
+                    c.put(s + 1, h, P[s, t], hk[s, h, t], v[s, t, h])
+        assert np.array_equal(mem.cpu().numpy(), c.buf)
+        K, V = c.rows()
+        for s, n in enumerate(day[1:3]):
+            assert np.array_equal(back.cpu().numpy()[s], F.f16(K[s + 1][:, P[s]]))
+            near(out.cpu().numpy()[s], *F.attend(hq[s], K[s + 1, :, :n], V[s + 1, :, :n], F.visible(n, T, window, sinks, n), 0.125, 0.0, True))
+    del graph
+    lib.rocket_close(fd)
+
+
 def test_serve_graphs_of_one_handle(lib):
     """Four attention calls captured one by one on one handle, replayed in turn, with an eager call between the replays that
     makes the handle's scratch grow: the eager results, bit for bit."""
