@@ -33,6 +33,7 @@ namespace {
 typedef int      i32x4  __attribute__((ext_vector_type(4)));
 typedef float    f32x2  __attribute__((ext_vector_type(2)));
 typedef float    f32x4  __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2  __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4  __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8  __attribute__((ext_vector_type(8)));
 typedef __amdgpu_buffer_rsrc_t Rsrc;
@@ -287,8 +288,10 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float e = __builtin_amdgcn_exp2f(v[i] - m_run[x]);
-                l_run[x] += e;
                 p[x][i] = (_Float16)e;
+                if constexpr (!WIN) l_run[x] += e;
+                // (under a window the sum of the rounded weights, two at a time: weights and their sum round alike)
+                else if (i & 1) l_run[x] = __builtin_amdgcn_fdot2(f16x2{p[x][i - 1], p[x][i]}, f16x2{(_Float16)1.f, (_Float16)1.f}, l_run[x], false);
             }
         }
         if constexpr (WIN) {

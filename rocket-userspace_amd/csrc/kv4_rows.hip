@@ -232,9 +232,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float e = __builtin_amdgcn_exp2f(v[i] - m_run[x]);
-                l_run[x] += e;
-                p[x][i] = (_Float16)e;
+                p[x][i] = (_Float16)__builtin_amdgcn_exp2f(v[i] - m_run[x]);
+                // the sum of the rounded weights, two at a time, in fp32: weights and their sum round alike
+                if (i & 1) l_run[x] = __builtin_amdgcn_fdot2(f16x2{p[x][i - 1], p[x][i]}, f16x2{(_Float16)1.f, (_Float16)1.f}, l_run[x], false);
             }
         }
 #pragma unroll

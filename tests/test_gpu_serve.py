@@ -300,6 +300,29 @@ def test_attn_many_small_weights(lib, fd, T, bits):
     near(out, want, tol)
 
 
+@pytest.mark.parametrize("T,heads", [(1, 2), (9, 4), (20, 4), (70, 2)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attn_of_equal_values(lib, fd, T, heads, d):
+    """Keys whose values are all the same give that value, whatever their weights: a weight and its share of the sum round
+    alike. In every 32 keys one weighs most and the others (1 + 0.98 2^-11) / 2 of it, which fp16 rounds down by nearly half a
+    step, and the value is the largest fp16 below 2, whose half step is 2^-12 of it: a sum of unrounded weights is off by
+    nearly twice that. With one of rounded weights 2^-18, for the fp32 steps, stands between the mean and the value, which is
+    the result."""
+    kvh, value = 2, 2047 / 1024
+    scale = float(np.float32((1 - np.log2(1 + 0.98 * 2.0 ** -11)) * np.log(2) / 15))
+    for n in (500, 3000):
+        K, V, Q = np.zeros((kvh, n, d), np.float16), np.full((kvh, n, d), value, np.float16), np.zeros((heads, T, d), np.float16)
+        K[:, ::32, 0], Q[..., 0] = 15, 1
+        c = F.Cache(1, kvh, d, d, n)
+        c.put_all(0, K, V)
+        sh, out, L = R.Kv4Shape(*c.dims), np.empty((heads, T, d), np.float16), np.array([n], np.int32)
+        assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 0, 1, T, n, heads, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+        assert (out == value).all()
+        Vt = np.ascontiguousarray(V.transpose(0, 2, 1))
+        assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(K), R.ptr(Vt), R.ptr(out)) == 0
+        assert (out == value).all()
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, -0.0])
 @pytest.mark.parametrize("cap", [0.0, 5.0])
 @pytest.mark.parametrize("T", [2, 40])
