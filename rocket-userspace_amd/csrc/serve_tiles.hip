@@ -67,7 +67,8 @@ struct TileArgs {
     ServeAttn a;
     int nsplit, nqb;   // shares of the key tiles; row blocks of a KV head
     int len, per;      // rows of a run that is cut into blocks of BQ: a head's T or all of a KV head's; blocks of a run
-    void *part;        // [split][row][dv] outputs (divided by the split's sum), then [split][row] (max, sum)
+    float *part;       // [split][row][dv] outputs (divided by the split's sum), then [split][row] (max, sum); rounded to fp16
+                       // they would be a third rounding beside the weights' and the result's
 };
 
 // D: 64, 128 or 256. 16-byte chunk c of an LDS row lies at slot c ^ x(row): the sixteen lanes that one
@@ -89,13 +90,6 @@ __device__ __forceinline__ int vx(int row) { return (row >> 1) & 7; }   // V^T r
 // Where keys and values come from: fp16 rows by DMA; the same with V^T rows that are no whole 16-byte chunks, whose values
 // go through registers; codes.
 enum Src { kHalves, kRagged, kCodes };
-
-// Splits' outputs over fp16 keys are fp32: rounded to fp16 beside the weights and the result they would be a third rounding
-// (333 tokens under a window of 257: 2.7e-4 of the result, with it 3.5e-4). Over codes, whose widened values are rounded
-// already, they are fp16, at half the bytes (130 tokens over 1024 keys, heads of 256: 32.4 us with fp32, 25.7; 3.9e-4 and
-// 4.4e-4).
-template <Src SRC> struct Part { typedef float T; };
-template <> struct Part<kCodes> { typedef _Float16 T; };
 
 template <int D, Src SRC, Cap CAP>
 __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1) void k_serve_tiles(const TileArgs ta)
@@ -703,11 +697,9 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     };
     lds_barrier();   // (the tiles are read no more)
     if (ta.nsplit > 1) {
-        typedef typename Part<SRC>::T P_;
         const size_t rows = (size_t)a.n_seq * a.n_head * T, prow = zs * rows + row0;
-        P_ *const part = static_cast<P_ *>(ta.part);
-        if (qok && hh == 0) reinterpret_cast<f32x2 *>(part + ta.nsplit * rows * a.dv)[prow + r] = f32x2{m_run, l};
-        store_rows(part + prow * a.dv);
+        if (qok && hh == 0) reinterpret_cast<f32x2 *>(ta.part + ta.nsplit * rows * a.dv)[prow + r] = f32x2{m_run, l};
+        store_rows(ta.part + prow * a.dv);
     } else {
         store_rows(a.out + row0 * a.dv);
     }
@@ -715,22 +707,21 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 
 // Merges the splits: out = sum_s w_s O_s / sum_s w_s with w_s = 2^(m_s - m) l_s, m the largest of the m_s, for four output
 // dims of a row a thread; every split's pair and outputs are loaded before the first is used.
-template <typename P, int MAXS>
-__global__ __launch_bounds__(256) void k_serve_combine(const P *__restrict__ part, _Float16 *__restrict__ out, long rows, int dv, int nsplit)
+template <int MAXS>
+__global__ __launch_bounds__(256) void k_serve_combine(const float *__restrict__ part, _Float16 *__restrict__ out, long rows, int dv, int nsplit)
 {
     const int dq = dv / 4;
     const long i = (long)blockIdx.x * 256 + threadIdx.x, row = i / dq;
     if (row >= rows) return;
     const int d0 = (int)(i - row * dq) * 4;
     const f32x2 *const ml = reinterpret_cast<const f32x2 *>(part + nsplit * rows * dv);
-    typedef P P4 __attribute__((ext_vector_type(4)));
     f32x2 x[MAXS];
-    P4 o[MAXS];
+    f32x4 o[MAXS];
 #pragma unroll
     for (int s = 0; s < MAXS; s++)
         if (s < nsplit) {
             x[s] = ml[s * rows + row];
-            o[s] = *reinterpret_cast<const P4 *>(part + (s * rows + row) * dv + d0);
+            o[s] = *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * dv + d0);
         }
     float m = -1e30f;
 #pragma unroll
@@ -744,17 +735,17 @@ __global__ __launch_bounds__(256) void k_serve_combine(const P *__restrict__ par
             const float w = __builtin_amdgcn_exp2f(x[s][0] - m) * x[s][1];
             l += w;
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[c] += w * (float)o[s][c];
+            for (int c = 0; c < 4; c++) acc[c] += w * o[s][c];
         }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const f16x4 h = {(_Float16)(acc[0] * inv), (_Float16)(acc[1] * inv), (_Float16)(acc[2] * inv), (_Float16)(acc[3] * inv)};
     *reinterpret_cast<f16x4 *>(out + row * dv + d0) = h;
 }
 
-template <typename P> void combine(const TileArgs &ta, long rows, long blocks, hipStream_t s)
+void combine(const TileArgs &ta, long rows, long blocks, hipStream_t s)
 {
-    auto *kern = ta.nsplit <= 4 ? k_serve_combine<P, 4> : ta.nsplit <= 8 ? k_serve_combine<P, 8> : ta.nsplit <= 16 ? k_serve_combine<P, 16> : k_serve_combine<P, 32>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const P *>(ta.part), ta.a.out, rows, ta.a.dv, ta.nsplit);
+    auto *kern = ta.nsplit <= 4 ? k_serve_combine<4> : ta.nsplit <= 8 ? k_serve_combine<8> : ta.nsplit <= 16 ? k_serve_combine<16> : k_serve_combine<32>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, s, ta.part, ta.a.out, rows, ta.a.dv, ta.nsplit);
 }
 
 template <int D, Src SRC, Cap CAP> hipError_t launch_c(const TileArgs &ta, unsigned wgs, hipStream_t s)
@@ -813,7 +804,7 @@ int splits(const ServeAttn &a)
 size_t serve_tiles_ws(const ServeAttn &a)
 {
     const int ns = splits(a);
-    return ns > 1 ? (size_t)ns * a.n_seq * a.n_head * a.n_tokens * (a.dv * (a.Kf ? sizeof(float) : sizeof(_Float16)) + 2 * sizeof(float)) : 0;
+    return ns > 1 ? (size_t)ns * a.n_seq * a.n_head * a.n_tokens * (a.dv + 2) * sizeof(float) : 0;
 }
 
 hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
@@ -834,8 +825,7 @@ hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks)
     *blocks = (uint64_t)wgs;
     if (e != hipSuccess || ta.nsplit == 1) return e;
     const long rows = (long)a.n_seq * a.n_head * a.n_tokens, n = (rows * (a.dv / 4) + 255) / 256;
-    if (a.Kf) combine<float>(ta, rows, n, s);
-    else combine<_Float16>(ta, rows, n, s);
+    combine(ta, rows, n, s);
     *blocks += (uint64_t)n;
     return hipGetLastError();
 }

@@ -323,6 +323,30 @@ def test_attn_of_equal_values(lib, fd, T, heads, d):
         assert (out == value).all()
 
 
+@pytest.mark.parametrize("T,heads", [(1, 2), (20, 4), (70, 2), (300, 2)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attn_sums_are_fp32(lib, fd, T, heads, d):
+    """Queries of zero weigh every key the same, with a power of two, so that results are plain means: half of one sequence's
+    values average 1 + 0.98 2^-11 and the others are -1, whose sum is what a rounding of any share's mean to fp16 would lose. Off by
+    half a step of the result and 2^-18 of the values, for fp32 sums over the keys and their shares."""
+    g, kvh, n = rng(49), 2, 4000
+    V = np.full((kvh, n, d), -1, np.float16)
+    V[:, :n // 2] = 1
+    V[:, g.permutation(n // 2)[:int(0.49 * (n // 2))]] = 1 + 2.0 ** -10
+    K, Q = F.f16(g.standard_normal((kvh, n, d))), np.zeros((heads, T, d), np.float16)
+    c = F.Cache(1, kvh, d, d, n)
+    c.put_all(0, K, V)
+    sh, out, L = R.Kv4Shape(*c.dims), np.empty((heads, T, d), np.float16), np.array([n], np.int32)
+    seen = n - T + 1 + np.arange(T)
+    want = (np.cumsum(V[0, :, 0].astype(np.float64))[seen - 1] / seen)[None, :, None]
+    tol = np.abs(want) * F.U + 2.0 ** -18
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 0, 1, T, n, heads, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+    near(out, np.broadcast_to(want, out.shape), np.broadcast_to(tol, out.shape))
+    Vt = np.ascontiguousarray(V.transpose(0, 2, 1))
+    assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, 0.1, 0.0, 0, 0, R.ptr(Q), R.ptr(K), R.ptr(Vt), R.ptr(out)) == 0
+    near(out, np.broadcast_to(want, out.shape), np.broadcast_to(tol, out.shape))
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, -0.0])
 @pytest.mark.parametrize("cap", [0.0, 5.0])
 @pytest.mark.parametrize("T", [2, 40])
