@@ -277,7 +277,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_fa_rows(const RowArgs a)
             }
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if constexpr (WIN) mx -= 15.f;   // weights up to 2^15: fp16 then loses those alone below 2^-40 of the largest
+            if constexpr (WIN) mx = lifted(mx);
             if (__any(mx > m_run[x])) {   // (a chunk has a key below n_kv, so without a window the new maximum is finite)
                 const float m_new = fmaxf(m_run[x], mx), alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
                 m_run[x] = m_new;

@@ -37,9 +37,6 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kChunk = 32, kWaves = 4, kMaxSplit = 64;
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights are 2^(score - (maximum - kLift)), up to 2^15: fp16 then loses those alone below 2^-40 of the largest. The
-// division by their sum makes the result independent of it.
-constexpr float kLift = 15.f;
 
 struct Kv4RowArgs {
     ServeAttn a;
@@ -222,7 +219,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) - kLift;
+            mx = lifted(fmaxf(mx, __shfl_xor(mx, 32, 64)));
             if (__any(mx > m_run[x])) {
                 const float m_new = fmaxf(m_run[x], mx), alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
                 m_run[x] = m_new;

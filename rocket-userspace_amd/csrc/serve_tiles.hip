@@ -391,12 +391,13 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     auto highest = [&](float mloc) __attribute__((always_inline)) {
         const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, mloc), __builtin_bit_cast(unsigned, mloc), false, false);
         const unsigned x0 = x[0], x1 = x[1];
-        return fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1)) * unit;
+        return fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1));
     };
     // Weights are 2^(score - m_run), with m_run 10 (in log2 units) below the largest score, and it moves when some row's
     // scores pass it by more than 15.5: then a weight stays inside fp16 and one is lost to it only below 2^-35 of the
     // largest (around the maximum itself 2^-25, which 2^17 such keys made 2e-3 of a result). The division by the sum
-    // makes the result independent of m_run.
+    // makes the result independent of m_run. Both go by the product that the exponential takes, unrounded, so that no
+    // rounding of a large score (2^27 is rounded by 4) carries a weight past fp16.
     auto rescale = [&](float m_new) __attribute__((always_inline)) {
         const float alpha = exp2f(m_run - m_new);
         m_run = m_new;
@@ -404,8 +405,8 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
         for (int d = 0; d < DB; d++) O[d] *= alpha;
         return alpha;
     };
-    auto grows = [&](float mloc) __attribute__((always_inline)) { return (bool)__any(mloc > m_run + 15.5f); };
-    auto raised = [&](float mloc) __attribute__((always_inline)) { return fmaxf(m_run, mloc - 10.f); };
+    auto grows = [&](float mloc) __attribute__((always_inline)) { return (bool)__any(fmaf(mloc, unit, -m_run) > 15.5f); };
+    auto raised = [&](float mloc) __attribute__((always_inline)) { return fmaxf(m_run, fmaf(mloc, unit, -10.f)); };
     auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float m, float &psum, int e) __attribute__((always_inline)) {
         const int sb = e >> 4, i = e & 15;
         const float p = __builtin_amdgcn_exp2f(fmaf(Sx[sb][i], unit, -m));

@@ -1,4 +1,4 @@
-// softcap.h — soft-capped scores of the serving kernels: softcap tanh(score / softcap).
+// softcap.h — scores of the serving kernels: soft-caps, softcap tanh(score / softcap), and what maxima are lifted by.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -32,6 +32,14 @@ template <Cap CAP> __device__ __forceinline__ float softcap_log2(float x, float 
     if constexpr (CAP == kWide) return softcap_wide(x * scale, 1.f / softcap, softcap) * kLog2e;
     const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e * scale / softcap));
     return (softcap * kLog2e) * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
+}
+
+// What a row's largest score, in log2 units, is taken down by so that its weight is 2^15: fp16 then loses those alone
+// below 2^-40 of the largest. (Not taken down where the difference would round to more, from scores of 2^24 on.)
+__device__ __forceinline__ float lifted(float mx)
+{
+    const float m = mx - 15.f;
+    return mx - m > 15.5f ? mx : m;
 }
 
 }  // namespace rk

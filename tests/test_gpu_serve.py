@@ -323,6 +323,42 @@ def test_attn_of_equal_values(lib, fd, T, heads, d):
         assert (out == value).all()
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size,step", [(20.0, 15.6), (21.5, 15.6), (22.3, 15.6), (23.5, 15.8), (24.2, 16.0), (24.7, 16.0), (25.5, 16.0), (25.5, 28.0), (26.4, 40.0)])
+def test_attn_scores_of_millions(lib, fd, size, step, sign):
+    """Scores of up to 2^26.4 (in log2 units), where fp32 rounds them by up to 4, in 16 levels that grow along the keys by about
+    what a weight may grow before the running maximum moves. Keys of a level are equal, so a token's result is the mean of the
+    last level's values that it sees. A level weighs 2^-(step - 3 ulp) of the next one (each score off by a sum's ulp and a
+    product's half), at most 1.6 of its keys to one of the last that a token sees; fp32 sums 2^-18."""
+    g, kvh, n, d = rng(50), 2, 4000, 64
+    level = np.arange(n) * 16 // n
+    K, V = np.zeros((kvh, n, d), np.float16), F.f16(g.integers(-7, 8, (kvh, n, d)) / 8.0)
+    K[:, :, 0], K[..., 32], K[..., 33] = 960, level, 15   # (exact in 4 bits)
+    ulp = 2.0 ** (np.floor(size) - 23)
+    tolerance = 2.0 ** -18 + 2 * 1.6 * 2.0 ** -(step - 3 * ulp)
+    for T, heads in ((1, 2), (20, 4), (70, 2)):
+        Q = np.zeros((heads, T, d), np.float16)
+        Q[..., 0], Q[..., 32] = sign * 1000, 1000 * 960 * step / 2.0 ** size
+        scale = float(np.float32(2.0 ** size * np.log(2) / (1000 * 960)))
+        c = F.Cache(1, kvh, d, d, n)
+        c.put_all(0, K, V)
+        k, v = c.rows()
+        assert np.array_equal(k[0, :, :n], K.astype(np.float64))
+        sh, out, L = R.Kv4Shape(*c.dims), np.empty((heads, T, d), np.float16), np.array([n], np.int32)
+        assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 0, 1, T, n, heads, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+        first = int(np.argmax(level == 15))
+
+        def check(values):
+            for h in range(heads):
+                top = values[h // (heads // kvh), first:]
+                want = (np.cumsum(top, 0) / np.arange(1, len(top) + 1)[:, None])[n - T - first:]
+                near(out[h], want, np.abs(want) * F.U + tolerance)
+        check(F.f16(v[0, :, :n]).astype(np.float64))
+        Vt = np.ascontiguousarray(V.transpose(0, 2, 1))
+        assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(K), R.ptr(Vt), R.ptr(out)) == 0
+        check(V.astype(np.float64))
+
+
 @pytest.mark.parametrize("T,heads", [(1, 2), (20, 4), (70, 2), (300, 2)])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attn_sums_are_fp32(lib, fd, T, heads, d):
