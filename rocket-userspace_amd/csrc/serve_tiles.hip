@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     // score; four operations for six, 2048 tokens over 8192 keys, heads of 128, 361 us, 342). One under a larger cap is
     // kept as it is.
     const float unit = CAP == kWide ? 1.4426950408889634f : CAP == kNarrow ? 2.f * 1.4426950408889634f * fabsf(a.softcap) : a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
-    [[maybe_unused]] const float slope = -2.f * 1.4426950408889634f * fabsf(a.scale) / fabsf(a.softcap);
+    [[maybe_unused]] const float slope = -cap_slope(fabsf(a.scale), fabsf(a.softcap));
     auto cap1 = [&](f32x16 (&Sx)[2], int e) __attribute__((always_inline)) {
         if constexpr (CAP == kWide) Sx[e >> 4][e & 15] = softcap_wide(Sx[e >> 4][e & 15] * fabsf(a.scale), 1.f / a.softcap, a.softcap);
         else if constexpr (CAP == kNarrow) Sx[e >> 4][e & 15] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(Sx[e >> 4][e & 15] * slope));

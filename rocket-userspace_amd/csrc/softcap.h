@@ -14,6 +14,13 @@ constexpr float kNarrowCap = 64.f;
 enum Cap { kUncapped, kNarrow, kWide };
 inline Cap cap_of(float softcap) { return softcap == 0.f ? kUncapped : fabsf(softcap) <= kNarrowCap ? kNarrow : kWide; }
 
+// What takes a product q . k to 2 y log2 e (finite, so that a product of 0 stays one under a cap next to 0).
+__device__ __forceinline__ float cap_slope(float scale, float softcap)
+{
+    const float k = 2.f * 1.4426950408889634f * scale / softcap;
+    return fmaxf(fminf(k, 3e38f), -3e38f);
+}
+
 // A scaled score under a cap above kNarrowCap (inv = 1 / cap), to 2^-20 of itself: below |y| = 0.35 by tanh's series,
 // y - y^3 / 3 + 2 y^5 / 15 - 17 y^7 / 315 + 62 y^9 / 2835 (the next term 2.5e-7 of it), which leaves a score far below its
 // cap as it is, and from there on by the form above (terms that round to 1.7 2^-23, of 0.336 or more).
@@ -30,7 +37,7 @@ template <Cap CAP> __device__ __forceinline__ float softcap_log2(float x, float 
 {
     constexpr float kLog2e = 1.4426950408889634f;
     if constexpr (CAP == kWide) return softcap_wide(x * scale, 1.f / softcap, softcap) * kLog2e;
-    const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e * scale / softcap));
+    const float e = __builtin_amdgcn_exp2f(x * cap_slope(scale, softcap));
     return (softcap * kLog2e) * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
 }
 

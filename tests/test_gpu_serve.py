@@ -509,6 +509,24 @@ def test_window_attn_is_the_masked_one(lib, fd):
 
 # ---- soft-caps: every kernel that has them, and caps of any size -----------------------
 
+@pytest.mark.parametrize("cap", [1e-38, -1e-40, 1.5e-45])
+@pytest.mark.parametrize("T,d", [(1, 128), (20, 64), (20, 160), (70, 64), (70, 256)])
+def test_attn_caps_next_to_none(lib, fd, T, d, cap):
+    """The smallest caps, by which a score's factor is past fp32: every score is within the cap of 0, one of a product of 0 as
+    well, and results are plain means."""
+    heads, kvh, n, window, sinks, scale = 4, 2, 150, 70, 3, 1.0
+    for uniform in (False, True):
+        c, Q = kv4_case(19, heads, kvh, d, d, T, [n], uniform)
+        out, sh = np.full((1, heads, T, d), 7, np.float16), R.Kv4Shape(*c.dims)
+        assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, 1, T, n, heads, scale, cap, window, sinks, R.ptr(Q), R.ptr(np.array([n], np.int32)),
+                                        R.ptr(out)) == 0
+        (want, tol), = kv4_want(c, Q * 0, [n], window, sinks, scale, 0.0)
+        near(out[0], want, tol)
+        Q, K, V, see = win_case(19, heads, kvh, d, d, T, n, n, window, sinks, uniform)
+        assert lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, cap, window, sinks, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(out)) == 0
+        near(out[0], *win_want(Q * 0, K, V, see, scale, 0.0))
+
+
 def tanh_slack(Q, K, V, scale, cap):
     """What 2^-20 of the capped scores moves a result by: e^delta - 1 of the largest value, twice for the weights' sum."""
     per = Q.shape[0] // K.shape[0]
