@@ -22,8 +22,9 @@
  *     0 <= j <= p  and  (window == 0  or  j > p - window  or  j < sinks).
  * With S = scale * (q . k), S = softcap * tanh(S / softcap) where softcap != 0, a token's result is
  * the softmax-weighted sum of the values of the keys it sees. A token that sees none (p < 0) gets
- * zeros. The GPU holds scores in fp32; they have to stay below 2^26 in size (where fp32 steps by 4). What keys that no token of a call sees hold (stale or not yet written memory, infinities,
- * NaN) does not reach any result.
+ * zeros. What keys that no token of a call sees hold (stale or not yet written memory, infinities,
+ * NaN) does not reach any result. scale and softcap are finite, |scale| at most 2^127. The GPU holds
+ * scores in fp32; they have to stay below 2^26 in size (where fp32 steps by 4).
  */
 #ifndef ROCKET_SERVE_H
 #define ROCKET_SERVE_H

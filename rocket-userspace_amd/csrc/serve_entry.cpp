@@ -149,7 +149,7 @@ int attn_args(const char *who, int n_tokens, int n_head, int kv_heads, float sca
 {
     if (n_head < 1 || n_head > 65535 || kv_heads < 1 || n_head % kv_heads) return bad(who, "n_head is not a multiple of the KV heads, or too large");
     if (window < 0 || sinks < 0 || (!window && sinks)) return bad(who, "window and sinks are not negative, and sinks need a window");
-    if (isnan(scale) || isnan(softcap)) return bad(who, "scale or softcap is NaN");
+    if (!(fabsf(scale) <= 0x1p127f) || !isfinite(softcap)) return bad(who, "scale or softcap is not finite, or scale above 2^127");
     if ((long)n_tokens * n_head > (long)1 << 30) return bad(who, "too many rows");
     return ROCKET_OK;
 }

@@ -271,3 +271,11 @@ def test_window_host(lib, T, n, window, sinks):
     assert lib.rocket_flash_attn_window_fp16(-1, T, n, stride, dk, dv, heads, kvh, 0.2, 0.0, window, sinks, R.ptr(Q), R.ptr(K), R.ptr(V), R.ptr(out)) == 0
     want, tol = F.attend(Q, K.astype(np.float64), V.astype(np.float64).transpose(0, 2, 1), see, 0.2, 0.0, False)
     assert (np.abs(out.astype(np.float64) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("x", [float("inf"), -float("inf"), 3e38])
+def test_attention_refuses_scales_and_caps_past_fp32(lib, x):
+    """An infinite scale or cap has no result but NaN; a scale whose log2 form is infinite has none on the GPU."""
+    assert kv4_call(lib, "attn", scale=x) == S and win_call(lib, scale=x) == S
+    want = 0 if x == 3e38 else S   # (a cap of that size is one that means none)
+    assert kv4_call(lib, "attn", cap=x) == want and win_call(lib, cap=x) == want
