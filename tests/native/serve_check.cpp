@@ -1,5 +1,6 @@
-// serve_check.cpp — which operands of rocket_serve.h's calls are used in place, on the fake runtime of fake_hip.h: a call
-// that stages one takes scratch of the handle and waits for its stream, which a captured call may not. Built and run by
+// serve_check.cpp — on the fake runtime of fake_hip.h: which operands of rocket_serve.h's calls are used in place (a call
+// that stages one takes scratch of the handle and waits for its stream, which a captured call may not), and which calls
+// over the cache split their keys. Built and run by
 // tests/test_serve_staging.py. Exit status 0 when every check passes.
 #include "fake_hip.h"
 
@@ -42,9 +43,27 @@ template <class F> static void in_place(const char *what, F call)
     rocket_close(fd);
 }
 
+// Launches of an eager attention call over the cache: 1, or 2 where its keys are split and merged.
+static size_t launches(int seqs, int heads, int dim, int rows, int max_kv)
+{
+    auto &f = fake::st();
+    const int fd = rocket_open();
+    CHECK(rocket_hip_set_mode(fd, ROCKET_HIP_ASYNC | ROCKET_HIP_DEVICE_OPERANDS) == 0);
+    const rocket_kv4_shape sh = {seqs, heads, dim, dim, max_kv};
+    f.launches.clear();
+    CHECK(rocket_kv4_attn_fp16(fd, &sh, at + ((size_t)1 << 36), 0, seqs, rows, max_kv, heads, 0.1f, 0.f, 0, 0, p<_Float16>(0), p<int32_t>((size_t)1 << 35),
+                               p<_Float16>((size_t)1 << 34)) == 0);
+    const size_t n = f.launches.size();
+    rocket_close(fd);
+    return n;
+}
+
 int main()
 {
     typedef _Float16 H;
+    // keys are split where that saves more than the merge costs: not many rows of short sequences
+    CHECK(launches(32, 8, 64, 64, 300) == 1 && launches(16, 8, 128, 24, 300) == 1 && launches(32, 8, 64, 64, 1000) == 1 && launches(1, 8, 64, 1, 300) == 1);
+    CHECK(launches(1, 8, 256, 1, 3000) == 2 && launches(1, 8, 128, 64, 2000) == 2 && launches(16, 8, 64, 24, 4000) == 2 && launches(32, 2, 64, 64, 3000) == 2);
     const rocket_kv4_shape sh = {8, 2, 64, 64, 400};
     H *const X = p<H>(0), *const Y = p<H>(1 << 20), *const Z = p<H>(2 << 20);
     char *const cache = at + (16 << 20);
