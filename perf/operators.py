@@ -293,15 +293,19 @@ _lib = {}
 
 
 def _session():
-    """The library, a handle and the stream that its calls are queued on."""
+    """The library, a handle and the stream that its calls are queued on. It becomes torch's current stream, as in a program
+    that queues its work on one stream: what reads a result, an event, a later input's allocation are all ordered with the
+    calls. (A handle cannot be bound to the default stream, and its own does not wait for that one.)"""
     if not _lib:
         sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rocket-userspace_amd"))
         import rocketnpu as R
         lib, stream = R.load(), torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
         fd = lib.rocket_open()
         assert fd >= 0, "no GPU"
         assert lib.rocket_hip_set_stream(fd, C.c_void_p(stream.cuda_stream)) == 0
         assert lib.rocket_hip_set_mode(fd, R.ROCKET_HIP_ASYNC | R.ROCKET_HIP_DEVICE_OPERANDS) == 0
+        torch.cuda.set_stream(stream)
         _lib.update(R=R, lib=lib, stream=stream, fd=fd)
     return _lib
 
@@ -339,6 +343,9 @@ def run(state):
         return _plain(c, t)
     if "calls" not in state:   # the arguments, as a program keeps them from step to step
         state["calls"], state["out"] = _calls(c, t)
+        for x in t.values():   # (made on another stream, maybe: their memory is not reused before the calls are through)
+            if torch.is_tensor(x):
+                x.record_stream(_lib["stream"])
     for fn, args in state["calls"]:
         rc = fn(*args)
         if rc:
