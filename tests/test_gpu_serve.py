@@ -931,6 +931,36 @@ def test_serve_from_two_threads(lib):
         lib.rocket_close(f)
 
 
+def test_measured_calls_are_on_the_current_stream(lib):
+    """perf/operators.py's calls are ordered with what torch does next: its stream is the one that they are queued on, and a
+    result may be read, and its state dropped, with no wait between."""
+    import importlib.util
+    import os
+
+    import torch
+    spec = importlib.util.spec_from_file_location("measured_operators", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "operators.py"))
+    M = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(M)
+    M.own, before = True, torch.cuda.current_stream()
+    case = next(c for c in M.listed() if c["name"] == "win_prefill")
+    try:
+        first = M.prepare(case, 1)   # (made on another stream than the calls')
+        M.run(first)
+        assert torch.cuda.current_stream().cuda_stream == lib.rocket_hip_stream(M._lib["fd"])
+        torch.cuda.synchronize()
+        want = first["out"].clone()
+        first["out"].zero_()
+        got = M.run(first).clone()
+        del first
+        M.prepare(case, 2)           # (takes the memory that the first state left)
+        assert torch.equal(got, want)
+    finally:
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(before)
+        if M._lib:
+            lib.rocket_close(M._lib["fd"])
+
+
 # ---- the largest sizes -----------------------------------------------------------------
 
 def test_cache_past_32_bits(lib, fd):
