@@ -820,6 +820,37 @@ def test_serve_capture_on_a_fresh_handle(lib, name):
         lib.rocket_close(f)
 
 
+@pytest.mark.parametrize("uniform", [False, True])
+@pytest.mark.parametrize("T", [1, 8, 12, 90])
+def test_serve_attn_captured_on_a_fresh_handle_counts_every_key(lib, T, uniform):
+    """A handle's first call, captured, over keys that it cannot split: against 64 bits, and for queries of zero, whose results
+    are plain means of the visible values, in which a key too many or too few shows."""
+    import torch
+    heads, kvh, d, n, window, sinks = 8, 2, 128, 2400, 1500, 4
+    stream = torch.cuda.Stream()
+    c, Q = kv4_case(51, heads, kvh, d, d, T, [n], uniform, spare=100)
+    Qw, K, V, see = win_case(52, heads, kvh, d, d, T, n, n, window, sinks, uniform)
+    sh, scale = R.Kv4Shape(*c.dims), d ** -0.5
+    with torch.cuda.stream(stream):
+        mem, L, dQ, dQw, dK, dV = dev(c.buf), dev(np.array([n], np.int32)), dev(Q), dev(Qw), dev(K), dev(V)
+        outs = [dev(np.zeros((heads, T, d), np.float16)) for _ in range(2)]
+    stream.synchronize()
+    calls = (lambda fd: lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(mem), 1, 1, T, n + 100, heads, scale, 0.0, 0, 0, R.ptr(dQ), R.ptr(L), R.ptr(outs[0])),
+             lambda fd: lib.rocket_flash_attn_window_fp16(fd, T, n, n, d, d, heads, kvh, scale, 0.0, window, sinks, R.ptr(dQw), R.ptr(dK), R.ptr(dV), R.ptr(outs[1])))
+    wants = (list(kv4_want(c, Q, [n], 0, 0, scale, 0.0))[0], win_want(Qw, K, V, see, scale, 0.0))
+    for call, out, want in zip(calls, outs, wants):
+        fd = _handle(lib, stream)
+        graph = _captured(fd, call, stream)
+        for _ in range(3):
+            with torch.cuda.stream(stream):
+                out.fill_(7)
+                graph.replay()
+            stream.synchronize()
+            near(out.cpu().numpy(), *want)
+        del graph
+        lib.rocket_close(fd)
+
+
 def test_serve_part_of_a_batch_captured(lib):
     """Places 1 and 2 of four, their lengths and positions in the middle of the batch's arrays: a fresh handle's first calls
     are captured ones, which only operands in place allow, and every replay takes the lengths of the day."""
