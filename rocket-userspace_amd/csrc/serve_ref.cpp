@@ -84,11 +84,11 @@ void store(const Group &x, const _Float16 *src)
     *x.sm = ScaleMin{s, (_Float16)lo};
 }
 
-// (a double holds code * scale + minimum exactly: one rounding)
-_Float16 value(const Group &x, int i)
+// (a double holds code * scale + minimum exactly)
+double value(const Group &x, int i)
 {
     const int byte = x.code[i / 8][i % 8 / 2];
-    return (_Float16)((double)(i & 1 ? byte >> 4 : byte & 15) * (double)x.sm->s + (double)x.sm->m);
+    return (double)(i & 1 ? byte >> 4 : byte & 15) * (double)x.sm->s + (double)x.sm->m;
 }
 
 }  // namespace
@@ -115,8 +115,8 @@ void kv4_read_ref(const Kv4View &c, const Kv4Rows &r)
                 const long j = (long)r.seq_len[s] - r.n_tokens + t;
                 const bool in = j >= 0 && j < c.capacity;
                 const size_t hr = (size_t)s * c.heads + h, row = hr * r.n_tokens + t;
-                for (int i = 0; r.Ko && i < c.dk; i++) r.Ko[row * c.dk + i] = in ? value(key_group(c, hr, j, i / 32), i % 32) : (_Float16)0.f;
-                for (int i = 0; r.Vo && i < c.dv; i++) r.Vo[row * c.dv + i] = in ? value(value_group(c, hr, j, i / 32), i % 32) : (_Float16)0.f;
+                for (int i = 0; r.Ko && i < c.dk; i++) r.Ko[row * c.dk + i] = in ? (_Float16)value(key_group(c, hr, j, i / 32), i % 32) : (_Float16)0.f;
+                for (int i = 0; r.Vo && i < c.dv; i++) r.Vo[row * c.dv + i] = in ? (_Float16)value(value_group(c, hr, j, i / 32), i % 32) : (_Float16)0.f;
             }
 }
 
@@ -173,7 +173,7 @@ try {
                     if (!sees(j)) continue;
                     double x = 0;
                     for (int i = 0; i < a.dk; i++)
-                        x += (double)q[i] * (a.Kf ? (double)a.Kf[(size_t)(h / a.gqa) * a.k_hs + (size_t)j * a.dk + i] : (double)value(key_group(a.c, hr, j, i / 32), i % 32));
+                        x += (double)q[i] * (a.Kf ? (double)a.Kf[(size_t)(h / a.gqa) * a.k_hs + (size_t)j * a.dk + i] : value(key_group(a.c, hr, j, i / 32), i % 32));
                     x *= (double)a.scale;
                     if (a.softcap != 0.f) x = (double)a.softcap * tanh(x / (double)a.softcap);
                     p[j] = x;
@@ -185,7 +185,7 @@ try {
                     const double w = exp(p[j] - mx);
                     sum += w;
                     for (int i = 0; i < a.dv; i++)
-                        o[i] += w * (a.Kf ? (double)a.Vf[((size_t)(h / a.gqa) * a.dv + i) * a.stride + j] : (double)value(value_group(a.c, hr, j, i / 32), i % 32));
+                        o[i] += w * (a.Kf ? (double)a.Vf[((size_t)(h / a.gqa) * a.dv + i) * a.stride + j] : value(value_group(a.c, hr, j, i / 32), i % 32));
                 }
                 for (int i = 0; i < a.dv; i++) a.out[row * a.dv + i] = (_Float16)(sum == 0 ? 0.0 : o[i] / sum);
             }

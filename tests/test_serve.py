@@ -214,26 +214,6 @@ def test_attention_host(lib, window, sinks, cap):
         assert not out[s][:, ~see.any(1)].any()
 
 
-def test_attention_host_multiplies_what_is_read_back(lib):
-    """fp16(code * scale + minimum), the values that the read gives, are what attention multiplies on the host as well: its results
-    are those of windowed attention over the read keys and values, bit for bit (the same steps in 64 bits)."""
-    g = rng(5)
-    H, dk, dv, n, heads, T = 2, 64, 32, 40, 4, 3
-    c = F.Cache(1, H, dk, dv, n)
-    c.put_all(0, F.f16(g.standard_normal((H, n, dk)) * 3), F.f16(g.standard_normal((H, n, dv))))
-    mem = np.zeros(c.buf.size + 16, np.uint8)
-    mem = mem[(-mem.ctypes.data) % 16:][:c.buf.size]
-    mem[:] = c.buf
-    sh, lens = R.Kv4Shape(*c.dims), np.array([n], np.int32)
-    K, V = np.empty((H, n, dk), np.float16), np.empty((H, n, dv), np.float16)
-    assert lib.rocket_kv4_read_fp16(-1, C.byref(sh), R.ptr(mem), 0, 1, n, R.ptr(lens), R.ptr(K), R.ptr(V)) == 0
-    Q, Vt = F.f16(g.standard_normal((heads, T, dk)) * 2), np.ascontiguousarray(V.transpose(0, 2, 1))
-    a, b = np.empty((heads, T, dv), np.float16), np.empty((heads, T, dv), np.float16)
-    assert lib.rocket_kv4_attn_fp16(-1, C.byref(sh), R.ptr(mem), 0, 1, T, n, heads, 0.125, 0.0, 9, 2, R.ptr(Q), R.ptr(lens), R.ptr(a)) == 0
-    assert lib.rocket_flash_attn_window_fp16(-1, T, n, n, dk, dv, heads, H, 0.125, 0.0, 9, 2, R.ptr(Q), R.ptr(K), R.ptr(Vt), R.ptr(b)) == 0
-    assert np.array_equal(a, b)
-
-
 WIN = dict(fd=-1, T=3, n=7, stride=9, dk=32, dv=16, heads=4, kvh=2, scale=0.2, cap=0.0, window=3, sinks=1)
 
 
