@@ -1,7 +1,7 @@
 // kv4_rows.hip — attention of few query rows (decode steps, drafts) over the 4-bit cache.
 //
 // What bounds it is how fast the codes arrive, and then the VALU that widens them: about two
-// operations a value, whatever the number of query rows. So all rows of a KV head (its query heads'
+// operations a value, whatever the number of query rows, and the MFMAs beside it. So all rows of a KV head (its query heads'
 // tokens, at most 64, in blocks of 16) share one widening (of heads above 128 each 32). A workgroup owns a place of the
 // batch, a KV head and a range of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
 // they lie in the cache, the next chunk's while this one's are widened.
@@ -13,9 +13,10 @@
 // takes a word of eight dims of each of its eight keys, product j their nibbles j, which a byte permute brings
 // side by side as pairs of keys.
 //
-// Roundings beside the result's: a widened value to fp16 (what rocket_kv4_read_fp16 gives, and what the MFMA takes) and a
-// weight to fp16; scores, maxima, sums and outputs are fp32. The result is within 4e-4 of its size (the rounded result alone
-// 2e-4). Measured by trace: 32 sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 47.9 us (5.2 TB/s, a
+// Keys and weights go into the products as two halves each (kv4_widen.h), so beside the result's there is one rounding: a widened
+// value's, to the half that rocket_kv4_read_fp16 gives; scores, maxima, sums and outputs are fp32. The result is within
+// 2.8e-4 of its size (the rounded result alone 2.1e-4). Of up to eight rows the weights' second halves take the product's other
+// eight columns (one token, 32 / 8 heads of 128: 52.6 us, with products of their own 58). Measured by trace: 32 sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 47.9 us (5.2 TB/s, a
 // large copy's rate) and 4.8 for the merge; one sequence of 3000 keys, 16 / 8 heads of 256, 6.2 and 3.8: two launches, each a
 // chain of loads that nothing else hides.
 #include "kv4_widen.h"
@@ -63,11 +64,13 @@ struct Chunks {
 // Chunks a workgroup: the length's own share, so that a long bound costs a short sequence nothing (one a wave at least).
 __device__ __forceinline__ int share(int count, int nsplit) { return max(kWaves, (count + nsplit - 1) / nsplit); }
 
-// D: head sizes up to this (64, 128, 256). NQ: blocks of 16 rows. FULL: dk and dv are D.
-template <int D, int NQ, Cap CAP, bool FULL>
-__global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
+// D: head sizes up to this (64, 128, 256). ROWS: at most this many (8, or blocks of 16). FULL: dk and dv are D.
+template <int D, int ROWS, Cap CAP, bool FULL>
+__global__ __launch_bounds__(kWaves * 64, D <= 128 && ROWS <= 16 ? 4 : D == 64 && ROWS == 64 ? 2 : 1) void k_kv4_rows(const Kv4RowArgs ra)
 {
     const ServeAttn &a = ra.a;
+    constexpr bool FOLD = ROWS == 8;
+    constexpr int NQ = FOLD ? 1 : ROWS / 16;
     constexpr int U = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4, KS = U * KW;   // key words of a lane: U runs of KW
     constexpr int NJ = D == 64 ? 4 : 8, VB = U * NJ, LROW = D + 4;          // output blocks of 16 dims; LDS row (floats)
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -84,16 +87,42 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     f16x8 qf[NQ][KS];
 #pragma unroll
     for (int x = 0; x < NQ; x++) {
-        const _Float16 *qrow = a.Q + (head0 + min(16 * x + c, R - 1)) * a.dk;   // (rows behind the last repeat it)
+        const _Float16 *qrow = a.Q + (head0 + min(FOLD ? c & 7 : 16 * x + c, R - 1)) * a.dk;   // (rows behind the last repeat it)
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             const int d = D == 64 ? 16 * q + 8 * i : 128 * (i / 4) + 32 * q + 8 * (i % 4);
             f16x8 y = *reinterpret_cast<const f16x8 *>(qrow + (FULL ? d : min(d, a.dk - 8)));
-            if (!FULL && d >= a.dk) y = f16x8{};
-            qf[x][i] = __builtin_shufflevector(y, y, 0, 4, 1, 5, 2, 6, 3, 7);
+            if ((!FULL && d >= a.dk) || (CAP == kUncapped && a.scale == 0.f)) y = f16x8{};
+            if (CAP == kUncapped && a.scale < 0.f) y = -y;
+            qf[x][i] = kv4_query_order(y);
         }
     }
     asm volatile("" ::: "memory");   // (the queries' loads are sent before the length is there)
+    // the sums of this lane's queries over its runs, a group's (D 64: half of one's) dims each, as the operand that meets the
+    // groups' minimums: halves 2 u and 2 u + 1 for run u
+    f16x4 qsum[NQ] = {};
+    float qback[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; x++) {
+        float sum[U], most = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            sum[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KW; i++) sum[u] = kv4_sum(qf[x][KW * u + i], sum[u]);
+            most = fmaxf(most, fabsf(sum[u]));
+        }
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const int e = kv4_sum_exponent(most);
+        qback[x] = __builtin_amdgcn_ldexpf(1.f, e);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const f16x2 h = kv4_sum_halves(sum[u], e);
+            qsum[x][2 * u] = h[0];
+            qsum[x][2 * u + 1] = h[1];
+        }
+    }
     const bool served = n >= 1 && n <= a.max_kv;
     const Chunks list(a, served ? n : 1);
     const int count = served ? list.count : 0;
@@ -104,8 +133,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     int pos[NQ], behind[NQ];                      // (the last key behind its window)
 #pragma unroll
     for (int x = 0; x < NQ; x++) {
-        const int r = 16 * x + c;
-        qok[x] = r < R;
+        const int r = FOLD ? c & 7 : 16 * x + c;
+        qok[x] = 16 * x + c < R;
         pos[x] = n - T + (row0 + r) % T;
         behind[x] = a.window ? pos[x] - a.window : -1;
     }
@@ -115,6 +144,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     const int dk = FULL ? D : a.dk, dv = FULL ? D : a.dv;
     const char *const kc = a.c.kc + hr * a.c.cap * (dk / 2), *const ks = a.c.ks + hr * a.c.cap * (dk / 8);
     const char *const vc = a.c.vc + hr * a.c.cap * (dv / 2), *const vs = a.c.vs + hr * a.c.cap * (dv / 8);
+    // (a head's part is 2^30 bytes at most: 32-bit offsets, which leave the addresses' upper halves in scalar registers)
     int kw[2][KS];        // block b's key of this lane: 8 (c / 4) + 4 b + c % 4
     f16x2 ksm[2][U];
     i32x4 vw[U][2];       // a word of each of the keys 8 q .. 8 q + 7
@@ -129,15 +159,15 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
                 // (past dk another run of the key: Q has those dims as 0)
                 const int run = FULL ? (D == 64 ? q : g) : D == 64 ? min(q, dk / 16 - 1) : min(g, dk / 32 - 1);
                 if constexpr (D == 64) {
-                    const i32x2 x = *reinterpret_cast<const i32x2 *>(kc + (size_t)key * (dk / 2) + 8 * run);
+                    const i32x2 x = *reinterpret_cast<const i32x2 *>(kc + (uint32_t)(key * (dk / 2) + 8 * run));
                     kw[b][0] = x[0];
                     kw[b][1] = x[1];
-                    ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (size_t)key * (dk / 8) + 4 * (run >> 1));
+                    ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (uint32_t)(key * (dk / 8) + 4 * (run >> 1)));
                 } else {
-                    const i32x4 x = *reinterpret_cast<const i32x4 *>(kc + (size_t)key * (dk / 2) + 16 * run);
+                    const i32x4 x = *reinterpret_cast<const i32x4 *>(kc + (uint32_t)(key * (dk / 2) + 16 * run));
 #pragma unroll
                     for (int i = 0; i < 4; i++) kw[b][4 * u + i] = x[i];
-                    ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (size_t)key * (dk / 8) + 4 * run);
+                    ksm[b][u] = *reinterpret_cast<const f16x2 *>(ks + (uint32_t)(key * (dk / 8) + 4 * run));
                 }
             }
         }
@@ -148,7 +178,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
         for (int u = 0; u < U; u++) {
             const int word = D == 64 ? c >> 1 : 16 * u + c;   // the lane's word: dims 8 w .. 8 w + 7
             const int w = FULL ? word : min(word, dv / 8 - 1);   // (results past dv are not stored)
-            const char *p = vc + ((size_t)block * (dv / 8) + w) * 32, *m = vs + ((size_t)block * (dv / 32) + w / 4) * 32;
+            const char *p = vc + (uint32_t)((block * (dv / 8) + w) * 32), *m = vs + (uint32_t)((block * (dv / 32) + w / 4) * 32);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 vw[u][i] = *reinterpret_cast<const i32x4 *>(p + 16 * i);
@@ -158,6 +188,11 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     };
 
     const Widen widen;
+    [[maybe_unused]] const float rest = c >= 8 ? 1.f : 0.f;   // (FOLD: this lane's column is of the weights' second halves)
+    // Uncapped scores stay products, and the factor to log2 units joins the exponential's subtraction. (Q carries the scale's
+    // sign, so that the largest product is the largest score; a scale of 0: Q is 0 and the factor 1, so that hidden keys'
+    // -infinity stays one.)
+    const float unit = CAP != kUncapped || a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
     float m_run[NQ], l_run[NQ];
     f32x4 O[NQ][VB];
 #pragma unroll
@@ -175,14 +210,24 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     }
     for (; ch < c1; ch += kWaves) {
         const int key0 = list.at(ch) * kChunk;
-        f32x4 S[NQ][2] = {};
+        f32x4 S[NQ][2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            f16x4 mf = {};
+#pragma unroll
+            for (int u = 0; u < U; u++) mf[2 * u] = mf[2 * u + 1] = ksm[b][u][1];
+#pragma unroll
+            for (int x = 0; x < NQ; x++) S[x][b] = __builtin_amdgcn_mfma_f32_16x16x16f16(mf, qsum[x], f32x4{}, 0, 0, 0) * qback[x];
+        }
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
             for (int b = 0; b < 2; b++) {
-                const f16x8 kf = widen.eight(kw[b][i], ksm[b][i / KW]);
+                const HiLo kf = kv4_keys(kw[b][i], KeyScale(ksm[b][i / KW][0]));
 #pragma unroll
-                for (int x = 0; x < NQ; x++) S[x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][i], S[x][b], 0, 0, 0);
+                for (int x = 0; x < NQ; x++) S[x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.hi, qf[x][i], S[x][b], 0, 0, 0);
+#pragma unroll
+                for (int x = 0; x < NQ; x++) S[x][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.lo, qf[x][i], S[x][b], 0, 0, 0);
             }
         const bool more = ch + kWaves < c1;
         const int next = list.at(more ? ch + kWaves : ch) * kChunk;
@@ -200,6 +245,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
                 }
         }
         f16x8 p[NQ];
+        [[maybe_unused]] f16x8 pl[NQ];
 #pragma unroll
         for (int x = 0; x < NQ; x++) {
             float v[8], mx = -INFINITY;
@@ -207,7 +253,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
             for (int i = 0; i < 8; i++) {
                 const float y = S[x][i >> 2][i & 3];
                 if constexpr (CAP != kUncapped) v[i] = softcap_log2<CAP>(y, a.scale, a.softcap);
-                else v[i] = y * (a.scale * kLog2e);
+                else v[i] = y;
             }
             if (!whole) {
 #pragma unroll
@@ -219,9 +265,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
 #pragma unroll
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = lifted(fmaxf(mx, __shfl_xor(mx, 32, 64)));
-            if (__any(mx > m_run[x])) {
-                const float m_new = fmaxf(m_run[x], mx), alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(fmaf(mx, unit, -m_run[x]) > 15.5f)) {
+                const float m_new = fmaxf(m_run[x], lifted(mx, unit)), alpha = __builtin_amdgcn_exp2f(m_run[x] - m_new);
                 m_run[x] = m_new;
                 l_run[x] *= alpha;
 #pragma unroll
@@ -229,9 +275,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                p[x][i] = (_Float16)__builtin_amdgcn_exp2f(v[i] - m_run[x]);
-                // the sum of the rounded weights, two at a time, in fp32: weights and their sum round alike
-                if (i & 1) l_run[x] = __builtin_amdgcn_fdot2(f16x2{p[x][i - 1], p[x][i]}, f16x2{(_Float16)1.f, (_Float16)1.f}, l_run[x], false);
+                const float e = __builtin_amdgcn_exp2f(fmaf(v[i], unit, -m_run[x]));
+                l_run[x] += e;
+                const _Float16 h = (_Float16)e;
+                if constexpr (FOLD) p[x][i] = (_Float16)fmaf(-(float)h, rest, e);
+                else {
+                    p[x][i] = h;
+                    pl[x][i] = (_Float16)(e - (float)h);
+                }
             }
         }
 #pragma unroll
@@ -261,8 +312,11 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
                     f[2 * k + 1] = y[1];
                 }
 #pragma unroll
-                for (int b = 0; b < NQ; b++)
-                    O[b][u * NJ + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[b], O[b][u * NJ + j], 0, 0, 0);
+                for (int b = 0; b < NQ; b++) O[b][u * NJ + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, p[b], O[b][u * NJ + j], 0, 0, 0);
+                if constexpr (!FOLD) {
+#pragma unroll
+                    for (int b = 0; b < NQ; b++) O[b][u * NJ + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, pl[b], O[b][u * NJ + j], 0, 0, 0);
+                }
             }
         }
         if (more) load_v(next);
@@ -275,6 +329,15 @@ __global__ __launch_bounds__(kWaves * 64) void k_kv4_rows(const Kv4RowArgs ra)
     for (int x = 0; x < NQ; x++) {
         l_run[x] += __shfl_xor(l_run[x], 16, 64);
         l_run[x] += __shfl_xor(l_run[x], 32, 64);
+        if constexpr (FOLD) {   // the columns of the second halves, eight lanes on
+#pragma unroll
+            for (int j = 0; j < VB; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y = O[x][j][e];   // (bit_cast of a vector's element itself takes the first)
+                    O[x][j][e] = y + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), 0x128, 0xF, 0xF, true));   // row_ror:8
+                }
+        }
         if (!qok[x]) continue;
         float *const row = Ol + (wave * R + 16 * x + c) * LROW;
 #pragma unroll
@@ -379,37 +442,38 @@ __global__ __launch_bounds__(256) void k_kv4_merge(const Kv4RowArgs ra)
 int row_blocks(const ServeAttn &a) { return (a.gqa * a.n_tokens + 15) / 16; }
 int row_groups(const ServeAttn &a) { return std::max(a.dk, a.dv) <= 128 ? 1 : (row_blocks(a) + 1) / 2; }
 
-template <int D, int NQ, Cap CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
+template <int D, int ROWS, Cap CAP, bool FULL> hipError_t launch_f(const Kv4RowArgs &ra, hipStream_t s)
 {
-    auto kern = k_kv4_rows<D, NQ, CAP, FULL>;
+    auto kern = k_kv4_rows<D, ROWS, CAP, FULL>;
     const ServeAttn &a = ra.a;
-    const int R = std::min(16 * NQ, a.gqa * a.n_tokens);
+    const int R = std::min(ROWS, a.gqa * a.n_tokens);
     const size_t lds = (size_t)kWaves * R * ((D + 4) * 4 + 8);
     if (lds > 64 * 1024) {
         static std::atomic<uint64_t> opted{0};
-        constexpr int most = kWaves * 16 * NQ * ((D + 4) * 4 + 8);
+        constexpr int most = kWaves * ROWS * ((D + 4) * 4 + 8);
         static_assert(most <= 160 * 1024, "LDS budget");
         if (const hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), most, opted)) return e;
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)a.c.heads, (unsigned)(ra.nsplit * row_groups(a)), (unsigned)a.n_seq), dim3(kWaves * 64), lds, s, ra);
     return hipGetLastError();
 }
-template <int D, int NQ> hipError_t launch_q(const Kv4RowArgs &ra, hipStream_t s)
+template <int D, int ROWS> hipError_t launch_q(const Kv4RowArgs &ra, hipStream_t s)
 {
     const bool full = ra.a.dk == D && ra.a.dv == D;
     switch (cap_of(ra.a.softcap)) {
-    case kUncapped: return full ? launch_f<D, NQ, kUncapped, true>(ra, s) : launch_f<D, NQ, kUncapped, false>(ra, s);
-    case kNarrow: return full ? launch_f<D, NQ, kNarrow, true>(ra, s) : launch_f<D, NQ, kNarrow, false>(ra, s);
-    default: return launch_f<D, NQ, kWide, false>(ra, s);   // (rare: one kernel for all heads)
+    case kUncapped: return full ? launch_f<D, ROWS, kUncapped, true>(ra, s) : launch_f<D, ROWS, kUncapped, false>(ra, s);
+    case kNarrow: return full ? launch_f<D, ROWS, kNarrow, true>(ra, s) : launch_f<D, ROWS, kNarrow, false>(ra, s);
+    default: return launch_f<D, ROWS, kWide, false>(ra, s);   // (rare: one kernel for all heads)
     }
 }
 template <int D> hipError_t launch(const Kv4RowArgs &ra, hipStream_t s)
 {
     const int nq = row_blocks(ra.a);
     if constexpr (D <= 128) {
-        if (nq > 2) return launch_q<D, 4>(ra, s);
+        if (nq > 2) return launch_q<D, 64>(ra, s);
     }
-    return nq == 1 ? launch_q<D, 1>(ra, s) : launch_q<D, 2>(ra, s);
+    if (ra.a.gqa * ra.a.n_tokens <= 8) return launch_q<D, 8>(ra, s);
+    return nq == 1 ? launch_q<D, 16>(ra, s) : launch_q<D, 32>(ra, s);
 }
 
 // Chunks that a sequence of up to max_kv keys may have to visit.

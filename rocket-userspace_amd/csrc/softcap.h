@@ -41,6 +41,18 @@ template <Cap CAP> __device__ __forceinline__ float softcap_log2(float x, float 
     return (softcap * kLog2e) * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
 }
 
+// The same for a row's largest product, times `unit` the score, by the product that the exponential takes, unrounded: 15 or 10
+// below it, whichever is within what a weight may grow to, or (from scores of 2^27 on, maybe) the score itself.
+__device__ __forceinline__ float lifted(float mx, float unit)
+{
+    float m = fmaf(mx, unit, -15.f);
+    if (fmaf(mx, unit, -m) > 15.25f) {
+        m = fmaf(mx, unit, -10.f);
+        if (fmaf(mx, unit, -m) > 15.25f) m = mx * unit;
+    }
+    return m;
+}
+
 // What a row's largest score, in log2 units, is taken down by so that its weight is 2^15: fp16 then loses those alone
 // below 2^-40 of the largest. (Not taken down where the difference would round to more, from scores of 2^24 on.)
 __device__ __forceinline__ float lifted(float mx)

@@ -359,6 +359,80 @@ def test_attn_scores_of_millions(lib, fd, size, step, sign):
         check(V.astype(np.float64))
 
 
+def exact_slack(c, s, n, Q, scale):
+    """What fp32 sums of codes and minimums add to the bound of exact keys: their magnitudes, 15 scales and a minimum, take the
+    place of the keys' and the values', 2^-21 of the scores' and 2^-20 of the values'."""
+    _, ks, _, vs = (p.astype(np.float64) for p in c.parts())
+    km = np.repeat(np.abs(ks[s, :, :n, :, 1]) + 15 * ks[s, :, :n, :, 0], 32, -1)
+    q = np.abs(Q.astype(np.float64)).reshape(km.shape[0], -1, Q.shape[-1]) @ km.transpose(0, 2, 1)
+    vm = (np.abs(vs[s, :, :n // 8, ..., 1]) + 15 * vs[s, :, :n // 8, ..., 0]).max()
+    return 2 * np.expm1(2.0 ** -21 * abs(scale) * q.max()) * np.abs(c.rows()[1][s, :, :n]).max() + 2.0 ** -20 * vm
+
+
+@pytest.mark.parametrize("T,heads,kvh", [(1, 16, 8), (5, 8, 2), (20, 4, 4), (40, 2, 2), (64, 2, 2)])
+@pytest.mark.parametrize("d", [64, 96, 128, 160, 256])
+def test_kv4_attn_multiplies_exact_keys_and_weights(lib, fd, T, heads, kvh, d):
+    """Of roundings to fp16 there are the result's and the values', not the keys' and not the weights'. One alone is off by
+    2^-11 sqrt(E[1 / m^2] / 3) = 2.07e-4 of its value (m, the mantissa, logarithmic in [1, 2): E = 3 / (8 ln 2)); two by sqrt 2
+    of it, over all results, and the others would make it 2. And every result is within the bound of exact keys, whose rounded
+    weights are rounded values here."""
+    lens = [700, 333, 2000]
+    c, Q = kv4_case(53, heads, kvh, d, d, T, lens)
+    sh, scale, out = R.Kv4Shape(*c.dims), d ** -0.5, np.full((len(lens), heads, T, d), 7, np.float16)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, len(lens), T, max(lens), heads, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(np.array(lens, np.int32)),
+                                    R.ptr(out)) == 0
+    K, V = c.rows()
+    off = size = 0.0
+    for s, n in enumerate(lens):
+        want, tol = F.attend(Q[s], K[s + 1, :, :n], V[s + 1, :, :n], F.visible(n, T, 0, 0, n), scale, 0.0, False)
+        g = out[s].astype(np.float64) - want
+        off, size = off + (g * g).sum(), size + (want * want).sum()
+        near(out[s], want, tol + exact_slack(c, s + 1, n, Q[s], scale))
+    assert np.sqrt(off / size) <= 1.05 * np.sqrt(2) * 2.07e-4
+
+
+@pytest.mark.parametrize("T,heads", [(1, 2), (12, 2), (30, 2), (60, 2)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("power,signed", [(-22, True), (-9, True), (12, True), (13, False)])
+def test_kv4_attn_queries_of_any_size(lib, fd, T, heads, d, power, signed):
+    """Queries of 2^-22 (subnormal ones) to 2^13, whose sums over a group's dims pass fp16 where they have one sign, under scales
+    that bring the scores back: the bound of exact keys."""
+    n, kvh = 300, 2
+    c, Q = kv4_case(54, heads, kvh, d, d, T, [n])
+    Q = F.f16((Q if signed else np.abs(Q)).astype(np.float64) * 2.0 ** power)
+    sh, scale, out = R.Kv4Shape(*c.dims), d ** -0.5 * 2.0 ** -power, np.full((1, heads, T, d), 7, np.float16)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 1, 1, T, n, heads, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(np.array([n], np.int32)), R.ptr(out)) == 0
+    K, V = c.rows()
+    want, tol = F.attend(Q[0], K[1, :, :n], V[1, :, :n], F.visible(n, T, 0, 0, n), scale, 0.0, False)
+    near(out[0], want, tol + exact_slack(c, 1, n, Q[0], scale))
+
+
+@pytest.mark.parametrize("T,heads", [(1, 2), (12, 2), (30, 2), (60, 2)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_kv4_attn_keys_and_values_over_the_whole_range(lib, fd, T, heads, d):
+    """Groups from -65504 to 65504, whose scale times 15 passes fp16, beside ordinary ones: there a key is off by up to half a
+    step of half its code's product, 7.5 scales (the scores by as much times the query), and everything stays finite."""
+    n, kvh, g = 300, 2, rng(55)
+    K, V = F.f16(g.standard_normal((kvh, n, d))), F.f16(g.standard_normal((kvh, n, d)))
+    wide = g.random((kvh, n, d // 32)) < 0.3
+    at = np.repeat(wide, 32, -1)
+    K[at] = F.f16(np.clip(g.standard_normal(at.sum()) * 30000, -65504, 65504))
+    K[:, ::7, 0], K[:, ::7, 1] = 65504, -65504
+    V[at] = F.f16(np.clip(g.standard_normal(at.sum()) * 30000, -65504, 65504))
+    V[:, ::5, 2], V[:, ::5, 3] = 65504, -65504
+    c = F.Cache(1, kvh, d, d, n)
+    c.put_all(0, K, V)
+    Q = F.f16(g.standard_normal((heads, T, d)) * 2.0 ** -4)
+    scale, L, out = 2.0 ** -13 * d ** -0.5, np.array([n], np.int32), np.full((heads, T, d), 7, np.float16)
+    sh = R.Kv4Shape(*c.dims)
+    assert lib.rocket_kv4_attn_fp16(fd, C.byref(sh), R.ptr(dev(c.buf)), 0, 1, T, n, heads, scale, 0.0, 0, 0, R.ptr(Q), R.ptr(L), R.ptr(out)) == 0
+    k, v = c.rows()
+    m = np.repeat(7.5 * c.parts()[1][0, :, :n, :, 0].astype(np.float64), 32, -1)
+    q = (np.abs(Q.astype(np.float64)).reshape(kvh, -1, d) @ m.transpose(0, 2, 1)).max()
+    want, tol = F.attend(Q, k[0, :, :n], v[0, :, :n], F.visible(n, T, 0, 0, n), scale, 0.0, True)
+    near(out, want, tol + exact_slack(c, 0, n, Q, scale) + 2 * np.expm1(F.U * scale * q) * np.abs(v).max())
+
+
 @pytest.mark.parametrize("T,heads", [(1, 2), (20, 4), (70, 2), (300, 2)])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attn_sums_are_fp32(lib, fd, T, heads, d):
