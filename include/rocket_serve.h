@@ -72,7 +72,8 @@ int rocket_qk_norm_rope_f32in(int fd, int n_seq, int n_tokens, int n_head, int n
  *     minimum = min(x),  scale = fp16((max(x) - min(x)) / 15)  (the next lower fp16 where 15 * scale + minimum
  *     would not be a finite fp16),
  *     c = clamp(rint((x - minimum) / scale), 0, 15)  (0 where scale is 0),  in fp32,
- *     value = fp16(c * scale + minimum), one rounding.
+ *     value = c * scale + minimum  (rocket_kv4_read_fp16 rounds it to fp16, once; attention on the GPU multiplies the
+ *     values of V so rounded and those of K as they are, the host path both as they are).
  * Inputs should be finite; an infinity is taken as the largest finite fp16 of its sign, a NaN as 0.
  * Parts, each starting at a multiple of 256 bytes, cap = capacity rounded up to 32:
  *     key codes    [n_seq][n_kv_heads][cap][head_dim / 2] bytes, value 2b in byte b's low nibble
@@ -97,8 +98,7 @@ int rocket_kv4_append_fp16(int fd, const rocket_kv4_shape *shape, void *cache, i
                            const _Float16 *K, int64_t k_ss, int64_t k_hs, int64_t k_rs,
                            const _Float16 *V, int64_t v_ss, int64_t v_hs, int64_t v_rs, const int32_t *seq_len);
 
-/* The values that the cache stands for: the last n_tokens positions of each sequence, in fp16 (what
- * attention multiplies), K[n_seq][n_kv_heads][n_tokens][head_dim], V[n_seq][n_kv_heads][n_tokens][dv].
+/* The values that the cache stands for: the last n_tokens positions of each sequence, in fp16, K[n_seq][n_kv_heads][n_tokens][head_dim], V[n_seq][n_kv_heads][n_tokens][dv].
  * Either may be NULL. Positions outside [0, capacity) read zeros. */
 int rocket_kv4_read_fp16(int fd, const rocket_kv4_shape *shape, const void *cache, int seq0, int n_seq, int n_tokens,
                          const int32_t *seq_len, _Float16 *K, _Float16 *V);

@@ -99,7 +99,8 @@ __global__ __launch_bounds__(kWaves * 64, D <= 128 && ROWS <= 16 ? 4 : D == 64 &
     }
     asm volatile("" ::: "memory");   // (the queries' loads are sent before the length is there)
     // the sums of this lane's queries over its runs, a group's (D 64: half of one's) dims each, as the operand that meets the
-    // groups' minimums: halves 2 u and 2 u + 1 for run u
+    // groups' minimums: halves 2 u and 2 u + 1 for run u. (Beside the length's load, as the queries: behind the first chunk's
+    // loads it was no faster, and took registers.)
     f16x4 qsum[NQ] = {};
     float qback[NQ];
 #pragma unroll

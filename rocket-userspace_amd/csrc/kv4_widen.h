@@ -38,19 +38,6 @@ struct Widen {
         const unsigned x = place & 2 ? w >> 8 : w;
         return place & 1 ? two<1>(x, s, m) : two<0>(x, s, m);
     }
-    // A word's eight codes in the order 0 4 1 5 2 6 3 7, with one scale and minimum.
-    __device__ __forceinline__ f16x8 eight(unsigned w, f16x2 sm) const
-    {
-        const f16x2 s = {sm[0], sm[0]}, m = {sm[1], sm[1]};
-        f16x8 r;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const f16x2 x = at(w, e, s, m);
-            r[2 * e] = x[0];
-            r[2 * e + 1] = x[1];
-        }
-        return r;
-    }
 };
 
 // ---- keys ----
@@ -84,15 +71,15 @@ __device__ __forceinline__ HiLo kv4_keys(unsigned w, const KeyScale &k)
 }
 __device__ __forceinline__ f16x8 kv4_query_order(f16x8 q) { return __builtin_shufflevector(q, q, 0, 2, 4, 6, 1, 3, 5, 7); }
 
-// A query's sums as two halves, for the products with the minimums: hi + lo = 2^-e sum to 2^-22 for an e with which none of the query's
-// sums, `most` the largest of their sizes, passes 2^14. The product is taken back by 2^e.
+// A query's sums as two halves, for the products with the minimums: hi + lo = 2^-e sum, to 2^-22 of `most`, the largest of their
+// sizes. e is 0 where halves hold them so, else it takes `most` to just below 2^14. The product is taken back by 2^e.
 __device__ __forceinline__ float kv4_sum(f16x8 q, float sum)
 {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) sum = __builtin_amdgcn_fdot2(f16x2{q[i], q[i + 1]}, f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
     return sum;
 }
-__device__ __forceinline__ int kv4_sum_exponent(float most) { return __builtin_amdgcn_frexp_expf(most) - 14; }
+__device__ __forceinline__ int kv4_sum_exponent(float most) { return most >= 0.125f && most < 16384.f ? 0 : __builtin_amdgcn_frexp_expf(most) - 14; }
 __device__ __forceinline__ f16x2 kv4_sum_halves(float sum, int e)
 {
     const float x = __builtin_amdgcn_ldexpf(sum, -e);

@@ -4,21 +4,24 @@
 // that they share each tile), a wave 32 rows. The key axis goes by tiles of 64 keys, those alone that some
 // row sees: the sinks' tiles, then from the first window's to the last token's. K tiles [64][D] and V^T
 // tiles [D][64] lie in LDS as halves, two of each. fp16 keys arrive by buffer-load DMA. Codes arrive in
-// registers a tile ahead and are widened between the MFMAs (under two VALU operations a value, shared by
-// the 128 rows), then written to LDS.
+// registers a tile ahead and are widened between the MFMAs (two VALU operations a value, shared by
+// the 128 rows), then written to LDS, a key as the two halves that hold it exactly (kv4_widen.h), one K tile of each.
 //
 // The loop is software-pipelined: an iteration runs the previous tile's PV products with this tile's
 // score arithmetic between them, then the next tile's QK products with this tile's exponentials between
 // them; K runs a tile ahead of V^T. Scores are transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so a lane
-// holds one row's scores and P stays in registers: rounded to fp16 and swapped between the half-waves
-// it is the second product's operand. O is rescaled only when some running maximum grows by more than 5.5 (log2 units).
+// holds one row's scores and P stays in registers: rounded to fp16 (over codes as two halves) and swapped between the
+// half-waves it is the second product's operand. O is rescaled only when some running maximum grows by more than 5.5 (log2
+// units).
 //
-// Roundings beside the result's: weights to fp16 (summed as rounded), codes' values to fp16 as the cache's reading gives them;
-// scores, maxima, sums and outputs are fp32. Measured: 2048 tokens under a window of 1024, 16 / 8 heads of 256, 54.6 us (630
-// TFLOP/s); 512 over 16384 fp16 keys of those heads 155 (870); 512 over 4096 codes 68 (475); 2048 over 8192 fp16 keys, 32 / 8
-// heads of 128, 274 (880). Heads of 256 have one wave a SIMD, which issues in order: a tile of halves is some 640
-// instructions of 4 cycles and 64 MFMAs of 32 in about 5200 cycles, of which a fifth waits for LDS, loads or the other waves
-// (LDS itself is busy a fifth of the time); over codes the widening makes it 6600 to 6900.
+// Roundings beside the result's: over halves the weights' to fp16 (summed as rounded); over codes the values', to the halves
+// that the cache's reading gives. Scores, maxima, sums, outputs and shares' outputs are fp32. Measured: 2048 tokens under a
+// window of 1024, 16 / 8 heads of 256, 55.0 us (630 TFLOP/s); 512 over 16384 fp16 keys of those heads 155 (870); 512 over 4096
+// codes 88 (365; with keys and weights rounded to one half each 69, and results 4.0e-4 of their size off, not 2.8e-4); 2048
+// over 8192 fp16 keys, 32 / 8 heads of 128, 274 (880). Heads of 256 have one wave a SIMD, which issues in order: by counters
+// a tile of halves is 240 VALU operations of 4 cycles and 64 MFMAs of 32 in 4900 cycles, an instruction issued in 46% of
+// them, 28% waiting to issue and 26% for LDS, loads or the other waves (LDS itself is busy a fifth of the time). Over codes
+// there are twice the products, and the widening.
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"
@@ -79,7 +82,8 @@ template <int D> struct Cfg {
     static constexpr int KINS = D / 32, VINS = D / 32;   // DMA instructions a wave and tile
     static constexpr int KBYTES = BK * D * 2, VBYTES = D * BK * 2, STAGE = KBYTES + VBYTES;
     static constexpr int DB = D / 32;            // 32-row blocks of output dims
-    static constexpr int LDS = 2 * STAGE + 16;   // + the flag of a tile with non-finite values
+    static constexpr int SUMS = BK * 16;         // 4-bit: the minimums of a tile's keys, eight groups each
+    static constexpr int LDS = 2 * STAGE + SUMS + 16;   // + the flag of a tile with non-finite values
     // 4-bit: a thread's runs of a tile's key codes and value codes, and the 16-byte writes they make
     static constexpr int ITEMS = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4, VD = D == 64 ? 2 : 4;
     static constexpr int KU = ITEMS * KW, VU = ITEMS * VD;
@@ -99,7 +103,12 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     using CF = Cfg<D>;
     constexpr int KC = CF::KC, KCPR = CF::KCPR, DB = CF::DB;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int *const bad_tile = reinterpret_cast<int *>(smem + 2 * CF::STAGE);
+    [[maybe_unused]] _Float16 *const mins = reinterpret_cast<_Float16 *>(smem + 2 * CF::STAGE);   // [key][8]
+    int *const bad_tile = reinterpret_cast<int *>(smem + 2 * CF::STAGE + CF::SUMS);
+    // Halves: two slots of a K tile and a V^T tile. Codes: one K tile as the halves that its products take first and second
+    // (kv4_widen.h), and two V^T tiles.
+    auto k_tile = [&](int slot) __attribute__((always_inline)) { return C4 ? smem + slot * CF::KBYTES : smem + slot * CF::STAGE; };
+    auto v_tile = [&](int slot) __attribute__((always_inline)) { return C4 ? smem + 2 * CF::KBYTES + slot * CF::VBYTES : smem + slot * CF::STAGE + CF::KBYTES; };
 
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -155,8 +164,31 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             f16x8 x = *reinterpret_cast<const f16x8 *>(qrow + min(16 * c, a.dk - 16));
             if (16 * c >= a.dk || a.scale == 0.f) x = f16x8{};
             if (a.scale < 0.f) x = -x;
-            qf[c] = C4 ? __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7) : x;
+            qf[c] = C4 ? kv4_query_order(x) : x;
         }
+    }
+    // 4-bit: the query's sums over the groups, first halves in half-wave 0 and second ones in 1, as the operand that meets the
+    // groups' minimums
+    [[maybe_unused]] f16x8 qsum = {};
+    [[maybe_unused]] float qback = 1.f;
+    [[maybe_unused]] bool back = false;
+    if constexpr (C4) {
+        float sum[D / 32], most = 0.f;
+#pragma unroll
+        for (int g = 0; g < D / 32; g++) {
+            const float own = kv4_sum(qf[2 * g + 1], kv4_sum(qf[2 * g], 0.f));
+            sum[g] = own + __shfl_xor(own, 32, 64);
+            most = fmaxf(most, fabsf(sum[g]));
+        }
+        const int e = kv4_sum_exponent(most);
+        qback = __builtin_amdgcn_ldexpf(1.f, e);
+        back = __any(e != 0);
+#pragma unroll
+        for (int g = 0; g < D / 32; g++) {
+            const f16x2 h = kv4_sum_halves(sum[g], e);
+            qsum[g] = hh ? h[1] : h[0];
+        }
+        if (D < 256 && tid < BK) *reinterpret_cast<i32x4 *>(mins + 8 * tid) = i32x4{0, 0, 0, 0};   // (groups that there are not)
     }
 
     // ---- tiles into LDS: K tile at smem + slot * STAGE, V^T tile right behind it ----
@@ -186,7 +218,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 #if defined(__HIP_DEVICE_COMPILE__)
         const int k0 = key_of(kb);
         const Rsrc rk = rsrc(Kh + (size_t)k0 * a.dk, (uint32_t)((long)max(n - k0, 0) * a.dk * 2));
-        char *ks = smem + slot * CF::STAGE;
+        char *ks = k_tile(slot);
 #pragma unroll
         for (int i = 0; i < CF::KINS; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void *)(ks + (i * NW + wave) * 1024), 16,
@@ -199,7 +231,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 #if defined(__HIP_DEVICE_COMPILE__)
         const int k0 = key_of(kb);
         const Rsrc rv = rsrc(Vh + k0, (uint32_t)((long)a.dv * a.stride * 2 - (long)k0 * 2));
-        char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+        char *vs = v_tile(slot);
         const uint32_t past = k0 + vkey < a.stride ? 0u : kOOB;   // past a row's end lies the next row
 #pragma unroll
         for (int i = 0; i < CF::VINS; i++)
@@ -220,7 +252,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     };
     auto put_rv = [&](int kb, int slot) __attribute__((always_inline)) {
         const int past = key_of(kb) + vkey + 8 - (int)a.stride;   // halves of the chunk behind the row's end
-        char *vs = smem + slot * CF::STAGE + CF::KBYTES + (wave * 64 + lane) * 16;
+        char *vs = v_tile(slot) + (wave * 64 + lane) * 16;
         if (key_of(kb) + BK > a.stride) {
 #pragma unroll
             for (int i = 0; i < CF::VINS; i++) {
@@ -281,12 +313,15 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             vsm[i][e] = *reinterpret_cast<const i32x4 *>(m + 16 * e);
         }
     };
-    // unit u of a thread's key words: eight dims of its key, one 16-byte write
-    auto put_k = [&](int slot, int u) __attribute__((always_inline)) {
+    // unit u of a thread's key words: eight dims of its key, a 16-byte write into each half's tile
+    auto put_k = [&](int u) __attribute__((always_inline)) {
         const int i = u / CF::KW, w = u % CF::KW, key = tid >> 2;
         const int chunk = D == 64 ? 2 * (tid & 3) + w : 4 * ((tid & 3) + 4 * i) + w;
-        const f16x8 x = widen.eight(kw[i][w], ksm[i]);
-        *reinterpret_cast<f16x8 *>(smem + slot * CF::STAGE + key * (D * 2) + ((chunk ^ CF::kx(key)) << 4)) = x;
+        const HiLo x = kv4_keys(kw[i][w], KeyScale(ksm[i][0]));
+        const int at = key * (D * 2) + ((chunk ^ CF::kx(key)) << 4);
+        *reinterpret_cast<f16x8 *>(k_tile(0) + at) = x.hi;
+        *reinterpret_cast<f16x8 *>(k_tile(1) + at) = x.lo;
+        if (w == 0) mins[8 * key + chunk / 4] = ksm[i][1];   // (D 64: two threads the same)
     };
     // pairs of keys of run i of the thread's value words; keys that no row sees get scale and minimum 0
     auto pair_v = [&](int kb, int i) __attribute__((always_inline)) {
@@ -324,39 +359,51 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             x[2 * k] = y[0];
             x[2 * k + 1] = y[1];
         }
-        *reinterpret_cast<f16x8 *>(smem + slot * CF::STAGE + CF::KBYTES + d * 128 + (((tid & 7) ^ vx(d)) << 4)) = x;
+        *reinterpret_cast<f16x8 *>(v_tile(slot) + d * 128 + (((tid & 7) ^ vx(d)) << 4)) = x;
     };
 
+    constexpr int PH = C4 ? 2 : 1;       // halves of a weight
     float m_run = -1e30f, l_run = 0.f;   // (finite: a row may see nothing of a tile)
     f32x16 O[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++) O[d] = f32x16{};
 
-    // S^T for the 64 keys of the K tile in slot `slot`: two 32-key blocks; fragments are read two steps ahead
+    // S^T for the 64 keys of the K tile in slot `slot`: two 32-key blocks; fragments are read two steps ahead. Codes: steps take
+    // first and second halves in turn, and the minimums' product stands in front.
+    constexpr int QKS = C4 ? 2 * KC : KC;
     auto qk = [&](int slot, f32x16 (&Sx)[2], auto &&beside) __attribute__((always_inline)) {
-        const char *ks = smem + slot * CF::STAGE;
-        Sx[0] = f32x16{};
-        Sx[1] = f32x16{};
-        auto kfrag = [&](int c, int sb) __attribute__((always_inline)) {
-            const int row = 32 * sb + l32, lc = 2 * c + hh;
-            return *reinterpret_cast<const f16x8 *>(ks + row * (D * 2) + ((lc ^ CF::kx(row)) << 4));
+        auto kfrag = [&](int t, int sb) __attribute__((always_inline)) {
+            const int row = 32 * sb + l32, lc = 2 * (C4 ? t / 2 : t) + hh;
+            return *reinterpret_cast<const f16x8 *>(k_tile(C4 ? t & 1 : slot) + row * (D * 2) + ((lc ^ CF::kx(row)) << 4));
         };
         f16x8 kf[3][2];
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            kf[c][0] = kfrag(c, 0);
-            kf[c][1] = kfrag(c, 1);
+        for (int t = 0; t < 2; t++) {
+            kf[t][0] = kfrag(t, 0);
+            kf[t][1] = kfrag(t, 1);
         }
 #pragma unroll
-        for (int c = 0; c < KC; c++) {
-            if (c + 2 < KC) {
-                kf[(c + 2) % 3][0] = kfrag(c + 2, 0);
-                kf[(c + 2) % 3][1] = kfrag(c + 2, 1);
+        for (int sb = 0; sb < 2; sb++) {
+            Sx[sb] = f32x16{};
+            if constexpr (C4)
+                Sx[sb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8 *>(mins + 8 * (32 * sb + l32)), qsum, Sx[sb], 0, 0, 0);
+        }
+        if constexpr (C4) {
+            if (__builtin_expect(back, 0)) {
+                Sx[0] *= qback;
+                Sx[1] *= qback;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < QKS; t++) {
+            if (t + 2 < QKS) {
+                kf[(t + 2) % 3][0] = kfrag(t + 2, 0);
+                kf[(t + 2) % 3][1] = kfrag(t + 2, 1);
             }
 #pragma unroll
             for (int sb = 0; sb < 2; sb++) {
-                Sx[sb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c % 3][sb], qf[c], Sx[sb], 0, 0, 0);
-                beside(2 * c + sb);
+                Sx[sb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t % 3][sb], qf[C4 ? t / 2 : t], Sx[sb], 0, 0, 0);
+                beside(2 * t + sb);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -407,32 +454,41 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
     };
     auto grows = [&](float mloc) __attribute__((always_inline)) { return (bool)__any(fmaf(mloc, unit, -m_run) > 15.5f); };
     auto raised = [&](float mloc) __attribute__((always_inline)) { return fmaxf(m_run, fmaf(mloc, unit, -10.f)); };
-    auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[2][2], float m, float &psum, int e) __attribute__((always_inline)) {
+    // Weights of halves are rounded to one, and the sum takes them as rounded, two at a time in fp32: weights and their sum round
+    // alike. Those of codes are two halves.
+    auto prob1 = [&](const f32x16 (&Sx)[2], f16x8 (&pb)[PH][2][2], float m, float &psum, int e) __attribute__((always_inline)) {
         const int sb = e >> 4, i = e & 15;
         const float p = __builtin_amdgcn_exp2f(fmaf(Sx[sb][i], unit, -m));
-        pb[sb][i >> 3][i & 7] = (_Float16)p;
-        // the sum of the rounded weights, two at a time, in fp32: weights and their sum round alike
-        if (i & 1) psum = __builtin_amdgcn_fdot2(f16x2{pb[sb][i >> 3][(i & 7) - 1], pb[sb][i >> 3][i & 7]}, f16x2{(_Float16)1.f, (_Float16)1.f}, psum, false);
+        const _Float16 h = (_Float16)p;
+        pb[0][sb][i >> 3][i & 7] = h;
+        if constexpr (C4) {
+            pb[PH - 1][sb][i >> 3][i & 7] = (_Float16)(p - (float)h);
+            psum += p;
+        } else if (i & 1) {
+            psum = __builtin_amdgcn_fdot2(f16x2{pb[0][sb][i >> 3][(i & 7) - 1], pb[0][sb][i >> 3][i & 7]}, f16x2{(_Float16)1.f, (_Float16)1.f}, psum, false);
+        }
     };
     // P to natural key order: of 16 keys, half-wave 0 holds 0-3 and 8-11 and takes 0-7
-    auto reorder = [&](f16x8 (&pb)[2][2]) __attribute__((always_inline)) {
+    auto reorder = [&](f16x8 (&pb)[PH][2][2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int sb = 0; sb < 2; sb++)
+        for (int h = 0; h < PH; h++)
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                i32x4 w = __builtin_bit_cast(i32x4, pb[sb][t]);
+            for (int sb = 0; sb < 2; sb++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const auto x = __builtin_amdgcn_permlane32_swap((unsigned)w[e], (unsigned)w[2 + e], false, false);
-                    w[e] = (int)x[0];
-                    w[2 + e] = (int)x[1];
+                for (int t = 0; t < 2; t++) {
+                    i32x4 w = __builtin_bit_cast(i32x4, pb[h][sb][t]);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const auto x = __builtin_amdgcn_permlane32_swap((unsigned)w[e], (unsigned)w[2 + e], false, false);
+                        w[e] = (int)x[0];
+                        w[2 + e] = (int)x[1];
+                    }
+                    pb[h][sb][t] = __builtin_bit_cast(f16x8, w);
                 }
-                pb[sb][t] = __builtin_bit_cast(f16x8, w);
-            }
     };
     // O^T += V^T P^T for the V^T tile in slot `slot`
-    auto pv = [&](int slot, const f16x8 (&pb)[2][2], auto &&beside) __attribute__((always_inline)) {
-        const char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+    auto pv = [&](int slot, const f16x8 (&pb)[PH][2][2], auto &&beside) __attribute__((always_inline)) {
+        const char *vs = v_tile(slot);
         auto vfrag = [&](int j, int db) __attribute__((always_inline)) {   // keys 16 j + 8 hh .. + 8
             const int d = 32 * db + l32;
             return *reinterpret_cast<const f16x8 *>(vs + d * 128 + (((2 * j + hh) ^ vx(d)) << 4));
@@ -445,9 +501,12 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 #pragma unroll
             for (int db = 0; db < DB; db++) {
                 if (j + 1 < 4) vf[(j + 1) & 1][db] = vfrag(j + 1, db);
-                O[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j & 1][db], pb[j >> 1][j & 1], O[db], 0, 0, 0);
-                beside(j * DB + db);
-                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int h = 0; h < PH; h++) {
+                    O[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j & 1][db], pb[h][j >> 1][j & 1], O[db], 0, 0, 0);
+                    beside((j * DB + db) * PH + h);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
     };
     // fp16 values of a tile that is not seen whole, before its products (0 times an infinity or a NaN would reach rows
@@ -457,7 +516,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
         if constexpr (!C4) {
             const int key0 = key_of(kb);
             if (whole(key0)) return;
-            char *vs = smem + slot * CF::STAGE + CF::KBYTES;
+            char *vs = v_tile(slot);
             // an exponent of all ones carries into the sign's place
             auto not_finite = [](unsigned w) __attribute__((always_inline)) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; };
             // (a thread's chunks, 32 rows apart, hold the same eight keys)
@@ -509,26 +568,24 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
 
     // Iteration kb: PV of tile kb - 1 beside the score arithmetic of tile kb (soft-caps, the maximum), then QK of tile kb + 1
     // beside the exponentials of tile kb. K tile kb + 2 goes into the K slot that tile kb left, V^T tile kb into the V^T slot that tile
-    // kb - 2 left; both are read an iteration on. The first iteration (kb0 - 1) has the first QK alone and the last
+    // kb - 2 left; both are read an iteration on. (Codes: K tile kb + 1 into the one slot that tile kb left, in front of its QK, with a
+    // barrier between.) The first iteration (kb0 - 1) has the first QK alone and the last
     // (kb1) the last PV, so that there is one copy of the products' code. Codes are loaded a whole iteration before they are
-    // widened, keys beside PV and values beside QK (also where there is no such tile: into slots that nothing reads again
+    // widened, keys beside PV and values beside QK, each beside its first half, so that the writes are through at the barrier (also where there is no such tile: into slots that nothing reads again
     // before they are written).
-    constexpr int QKM = 2 * KC, PVM = 4 * DB;
+    constexpr int QKM = 2 * QKS, PVM = 4 * DB * PH;
     // With one wave a SIMD a phase takes its instructions' issue or its MFMAs, whichever is longer: over halves of heads of 256
     // QK's is the former and PV's the latter, so half of the exponentials go beside PV, whose first half then finds the
     // maximum (512 tokens over 16384 keys 161 us, 155; 8 of the 32 159, 24 156). Over codes, whose widening fills PV, and at two
     // waves a SIMD it was slower.
     constexpr int EARLY = !CAPPED && !C4 && D == 256 ? 16 : 0, MXM = EARLY ? PVM / 2 : PVM;
     f32x16 S[2] = {};
-    f16x8 P[2][2] = {};
+    f16x8 P[PH][2][2] = {};
     if (kb0 < kb1) {
         if constexpr (C4) {
             load_k(kb0);
 #pragma unroll
             for (int i = 0; i < CF::ITEMS; i++) load_v(kb0, i);
-#pragma unroll
-            for (int u = 0; u < CF::KU; u++) put_k(0, u);
-            load_k(kb0 + 1);
         } else {
             dma_k(kb0, 0);
             if (tid == 0) *bad_tile = -1;
@@ -559,7 +616,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
             float mloc = -INFINITY, psum = 0.f;
             [[maybe_unused]] float m_next = m_run;
             [[maybe_unused]] bool up = false;
-            f16x8 Pm[2][2], (&Pn)[2][2] = EARLY > 0 ? Pm : P;
+            f16x8 Pm[PH][2][2], (&Pn)[PH][2][2] = EARLY > 0 ? Pm : P;
             if (kb > kb0) {
                 clean_v(kb - 1, cur ^ 1);
                 pv(cur ^ 1, P, [&](int m) __attribute__((always_inline)) {
@@ -581,7 +638,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     }
                     if constexpr (C4) {
 #pragma unroll
-                        for (int u = m * CF::KU / PVM; u < (m + 1) * CF::KU / PVM; u++) put_k(cur, u);
+                        for (int u = m * CF::KU / (PVM / 2); u < min(CF::KU, (m + 1) * CF::KU / (PVM / 2)); u++) put_k(u);
                     }
                 });
                 if (kb == kb1) break;
@@ -600,10 +657,10 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 }
                 if constexpr (C4) {
 #pragma unroll
-                    for (int u = 0; u < CF::KU; u++) put_k(cur, u);
+                    for (int u = 0; u < CF::KU; u++) put_k(u);
                 }
             }
-            if constexpr (C4) load_k(kb + 3);
+            if constexpr (C4) load_k(kb + 2);
             if constexpr (CAPPED) {   // (a hidden key's capped score would not be -infinity: masks come behind it)
                 if (tile && !whole(key_of(kb))) {
                     mask(kb, S);
@@ -620,6 +677,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 if (__builtin_expect(grows(mloc), 0)) alpha = rescale(raised(mloc));
             }
             if constexpr (C4 && CF::ITEMS == 1) next_v(kb, 0);
+            if constexpr (C4) lds_barrier();   // (the K tile is whole; the barrier above let it be written)
             if (kb + 1 < kb1) {
                 f32x16 Sn[2];
                 qk(cur ^ 1, Sn, [&](int m) __attribute__((always_inline)) {
@@ -627,7 +685,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                     for (int e = EARLY + m * (32 - EARLY) / QKM; e < EARLY + (m + 1) * (32 - EARLY) / QKM; e++) prob1(S, Pn, m_run, psum, e);
                     if constexpr (C4) {
 #pragma unroll
-                        for (int u = m * CF::VU / QKM; u < (m + 1) * CF::VU / QKM; u++) put_v(kb, cur, u);
+                        for (int u = m * CF::VU / (QKM / 2); u < min(CF::VU, (m + 1) * CF::VU / (QKM / 2)); u++) put_v(kb, cur, u);
                     }
                 });
                 S[0] = Sn[0];
@@ -646,7 +704,7 @@ __global__ __launch_bounds__(256, D <= 64 || (D == 128 && SRC != kCodes) ? 2 : 1
                 reorder(Pn);
                 if constexpr (EARLY > 0) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) P[i >> 1][i & 1] = Pn[i >> 1][i & 1];
+                    for (int i = 0; i < 4; i++) P[0][i >> 1][i & 1] = Pn[0][i >> 1][i & 1];
                 }
                 l_run = l_run * alpha + psum;
             }

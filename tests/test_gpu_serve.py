@@ -369,7 +369,7 @@ def exact_slack(c, s, n, Q, scale):
     return 2 * np.expm1(2.0 ** -21 * abs(scale) * q.max()) * np.abs(c.rows()[1][s, :, :n]).max() + 2.0 ** -20 * vm
 
 
-@pytest.mark.parametrize("T,heads,kvh", [(1, 16, 8), (5, 8, 2), (20, 4, 4), (40, 2, 2), (64, 2, 2)])
+@pytest.mark.parametrize("T,heads,kvh", [(1, 16, 8), (5, 8, 2), (20, 4, 4), (40, 2, 2), (64, 2, 2), (70, 2, 2), (130, 4, 2)])
 @pytest.mark.parametrize("d", [64, 96, 128, 160, 256])
 def test_kv4_attn_multiplies_exact_keys_and_weights(lib, fd, T, heads, kvh, d):
     """Of roundings to fp16 there are the result's and the values', not the keys' and not the weights'. One alone is off by
@@ -391,7 +391,7 @@ def test_kv4_attn_multiplies_exact_keys_and_weights(lib, fd, T, heads, kvh, d):
     assert np.sqrt(off / size) <= 1.05 * np.sqrt(2) * 2.07e-4
 
 
-@pytest.mark.parametrize("T,heads", [(1, 2), (12, 2), (30, 2), (60, 2)])
+@pytest.mark.parametrize("T,heads", [(1, 2), (12, 2), (30, 2), (60, 2), (70, 4)])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("power,signed", [(-22, True), (-9, True), (12, True), (13, False)])
 def test_kv4_attn_queries_of_any_size(lib, fd, T, heads, d, power, signed):
@@ -407,7 +407,7 @@ def test_kv4_attn_queries_of_any_size(lib, fd, T, heads, d, power, signed):
     near(out[0], want, tol + exact_slack(c, 1, n, Q[0], scale))
 
 
-@pytest.mark.parametrize("T,heads", [(1, 2), (12, 2), (30, 2), (60, 2)])
+@pytest.mark.parametrize("T,heads", [(1, 2), (12, 2), (30, 2), (60, 2), (70, 4)])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_kv4_attn_keys_and_values_over_the_whole_range(lib, fd, T, heads, d):
     """Groups from -65504 to 65504, whose scale times 15 passes fp16, beside ordinary ones: there a key is off by up to half a
