@@ -490,30 +490,31 @@ int splits(const ServeAttn &a)
 {
     const int chunks = most_chunks(a);
     // As many workgroups as the CUs hold at once, a wave of each a SIMD: one more round, or a few workgroups of one, costs
-    // more than longer shares (1024 for all: 16 sequences of 4000 keys, heads of 256, one row 34.8 us, 512 30.9; 24 rows
-    // 66.9, 256 49.5; heads of 128, 20 rows 33.1, 512 29.3).
+    // more than longer shares (1024 for all: 16 sequences of 4000 keys, heads of 256, one row 33.4 us, so 31.3; 24 rows
+    // 75.7, 59.8; heads of 128, 20 rows 34.7, 32.7).
     const int d = std::max(a.dk, a.dv), nq = row_blocks(a);
     const long resident = 256 * (nq == 1 ? (d <= 128 ? 4 : 2) : nq == 2 ? (d <= 64 ? 3 : d <= 128 ? 2 : 1) : d <= 64 ? 2 : 1);
     const long wgs = (long)a.c.heads * a.n_seq * row_groups(a), waves = (chunks + kWaves - 1) / kWaves;
     const long n = std::min<long>({waves, resident / wgs, kMaxSplit});
     if (n < 2) return 1;
     // Where that saves more than the merge costs: a wave's chunks less, at what one takes a wave (ns, measured unsplit), against
-    // a launch of some 3 us and 2 + dv / 100 ns a row of the batch, a workgroup each. (Over 250 shapes of 1 to 64 rows the better
-    // of the two but for 0.2% of the time, 14% at worst; always split 15%: 32 sequences of 300 keys, 8 heads of 64,
-    // 64 rows 44.5 us, unsplit 9.6; 16 of 1000, heads of 128, 24 rows 20.0 and 14.1; one token of one sequence of 300, heads of
-    // 64, 7.0 and 5.0, of 1000 7.0 and 8.1.)
-    static const long chunk_ns[3][3] = {{600, 900, 1400}, {900, 1100, 2000}, {1400, 1900, 1900}};
+    // a launch of some 3.5 us and 2 + dv / 100 ns a row of the batch, a workgroup each. (Over 250 shapes of 1 to 64 rows the better
+    // of the two but for 0.2% of the time, 20% at worst; always split 12%: 32 sequences of 300 keys, 8 heads of 64,
+    // 64 rows 46.1 us, unsplit 11.6; 16 of 1000, heads of 128, 24 rows 22.1 and 17.3; one token of one sequence of 300, heads
+    // of 64, 7.2 and 5.2, of 1000 7.2 and 8.7.)
+    static const long chunk_ns[3][3] = {{700, 1100, 1700}, {950, 1400, 2600}, {1600, 2400, 2400}};
     const long saved = (waves - (chunks + n * kWaves - 1) / (n * kWaves)) * chunk_ns[d <= 64 ? 0 : d <= 128 ? 1 : 2][std::min(nq, 3) - 1];
     const long rows = (long)a.n_seq * a.n_head * a.n_tokens;
-    return saved < 3000 + rows * (200 + a.dv) / 100 ? 1 : (int)n;
+    return saved < 3500 + rows * (200 + a.dv) / 100 ? 1 : (int)n;
 }
 
 }  // namespace
 
-// Up to 64 rows. In tiles of 128 rows, at 16000 keys of one sequence, 8 KV heads of 128: 20 rows 26.9 us, here 15.8; 64 rows
-// 27.4 and 24.1; at 16 sequences of 4000 keys 64.2 and 27.8, 66.2 and 62.9. (Closest where 64 rows of many short sequences leave
-// no room for splits: 32 of 1000 keys, 2 heads of 64, 17.5 and 16.8, of 128 20.3 and 24.6.) Heads of 256, 64 rows: 16000 keys of one sequence 39.6 and 30.8, 8
-// sequences of 4000 60.0 and 53.3, 32 of 2000 99.8 and 78.2; a third block would lose there what it gains at one.
+// Up to 64 rows. In tiles of 128 rows, at 16000 keys of one sequence, 8 KV heads of 128: 20 rows 31.8 us, here 16.9; 64 rows
+// 34.9 and 27.7; at 16 sequences of 4000 keys 80.7 and 32.7, 84.5 and 73.6. Heads of 256, 64 rows: 16000 keys of one sequence
+// 51.5 and 36.0, 8 sequences of 4000 81.5 and 63.3, 32 of 2000 137 and 97; a third block would lose there what it gains at
+// one. (64 rows of a few dozen short sequences are even, 32 of 1000 keys, 2 heads of 64, 20.4 and 20.7, or lose a little, heads
+// of 128 there 24.4 and 28.5.)
 bool kv4_few_rows(const ServeAttn &a) { return (long)a.gqa * a.n_tokens <= 64; }
 
 size_t kv4_rows_ws(const ServeAttn &a)
