@@ -1,7 +1,7 @@
 // attn_decode.hip — attention of few query rows (decode steps) for gfx950.
 //
-// A KV head's query rows, the tokens of every query head that reads it, are at most 16 here, so
-// the tiled kernel's 128-query workgroups (attn.hip) would be mostly padding; what bounds the
+// A KV head's query rows, the tokens of every query head that reads it, are at most 16 here (under
+// a window up to 64, in blocks of 16), so the tiled kernel's 128-query workgroups (attn.hip) would be mostly padding; what bounds the
 // call is how fast K and V arrive. A workgroup owns a KV head and a range of its keys; each of
 // its 4 waves takes chunks of 32 keys and loads their K rows and V^T columns straight into
 // registers as MFMA fragments, 32 KB of them in flight a wave at head size 256, next chunk's K

@@ -1,11 +1,12 @@
 // kv4.hip — new keys and values into the 4-bit cache, and the values that it stands for.
 //
 // Four lanes take a group of 32 values of one row, eight values each: 16 bytes in (or out) a lane, a word of
-// codes, and the group's scale. What bounds both is memory, so the lanes of a wave are laid out as the bytes lie: a key
-// row's groups end to end, and of values eight tokens of a group side by side, whose words the cache keeps together.
-// (A thread a group, which found its row by three 64-bit divisions and divided 32 times, took 25 us for the prompt below;
-// its reading 18.) 4096 tokens of 8 heads of 256, 44 MB each: append 13.9 us by trace (3.2 TB/s: the scale and the codes
-// are some 12 VALU operations a value), read 10.6 us (4.1 TB/s); one token of 32 sequences 3.7 and 2.8.
+// codes, and the group's scale. The lanes of a wave are laid out as the bytes lie: a key row's groups end to end, and of
+// values eight tokens of a group side by side, whose words the cache keeps together. (A thread a group, which found its row
+// by three 64-bit divisions and divided 32 times, took 25 us for the prompt below; its reading 18.) 4096 tokens of 8 heads of
+// 256, 44 MB each: append 14.0 us by trace (3.1 TB/s), read 10.5 us (4.2 TB/s); one token of 32 sequences 4.0 and 3.0.
+// The issue of VALU operations bounds append: by counters 210 a wave, 26 a value with the addresses, the extremes and the
+// scale, 26.8 thousand cycles of a SIMD, 11.2 us. Reading has 107 a wave, 5.7 us, and is bound by memory.
 #include "serve.h"
 
 namespace rk {

@@ -1,7 +1,7 @@
 // kv4_rows.hip — attention of few query rows (decode steps, drafts) over the 4-bit cache.
 //
-// What bounds it is how fast the codes arrive, and then the VALU that widens them: about two
-// operations a value, whatever the number of query rows, and the MFMAs beside it. So all rows of a KV head (its query heads'
+// What bounds it is how fast the codes arrive, and about as much the VALU that widens them: some three
+// operations a pair of values or keys, whatever the number of query rows, and the MFMAs beside it. So all rows of a KV head (its query heads'
 // tokens, at most 64, in blocks of 16) share one widening (of heads above 128 each 32). A workgroup owns a place of the
 // batch, a KV head and a range of its keys; each of its four waves takes chunks of 32 keys and loads them straight into registers as
 // they lie in the cache, the next chunk's while this one's are widened.
@@ -16,9 +16,10 @@
 // Keys and weights go into the products as two halves each (kv4_widen.h), so beside the result's there is one rounding: a widened
 // value's, to the half that rocket_kv4_read_fp16 gives; scores, maxima, sums and outputs are fp32. The result is within
 // 2.8e-4 of its size (the rounded result alone 2.1e-4). Of up to eight rows the weights' second halves take the product's other
-// eight columns (one token, 32 / 8 heads of 128: 52.6 us, with products of their own 58). Measured by trace: 32 sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 47.9 us (5.2 TB/s, a
-// large copy's rate) and 4.8 for the merge; one sequence of 3000 keys, 16 / 8 heads of 256, 6.2 and 3.8: two launches, each a
-// chain of loads that nothing else hides.
+// eight columns (32 / 8 heads of 128, one token of 32 sequences: 52.6 us, with products of their own 58). Measured by trace: 32
+// sequences of up to 8192 keys, 32 / 8 heads of 128, one token, 249 MB, 52.6 us (4.7 TB/s; a large copy's rate is 5.1, which keys
+// and weights of one half reached) and 4.7 for the merge; one sequence of 3000 keys, 16 / 8 heads of 256, 7.0 and 3.8: two
+// launches, each a chain of loads that nothing else hides.
 #include "kv4_widen.h"
 #include "lds_optin.h"
 #include "serve.h"

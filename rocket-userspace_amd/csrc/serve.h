@@ -97,7 +97,7 @@ bool kv4_few_rows(const ServeAttn &a);
 size_t kv4_rows_ws(const ServeAttn &a);
 hipError_t kv4_rows(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 
-// More rows, or fp16 keys (serve_tiles.hip).
+// More rows, over either (serve_tiles.hip); few over fp16 keys are fa_rows' (attn_decode.hip).
 size_t serve_tiles_ws(const ServeAttn &a);
 hipError_t serve_tiles(const ServeAttn &a, hipStream_t s, uint64_t *blocks);
 
