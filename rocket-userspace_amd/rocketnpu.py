@@ -200,6 +200,22 @@ PROTOS = {
     "rocket_kv4_read_fp16": (i32, [i32, C.POINTER(Kv4Shape), vp, i32, i32, i32, vp, vp, vp]),
     "rocket_kv4_attn_fp16": (i32, [i32, C.POINTER(Kv4Shape), vp] + [i32] * 5 + [fl, fl, i32, i32, vp, vp, vp]),
     "rocket_flash_attn_window_fp16": (i32, [i32] * 8 + [fl, fl, i32, i32] + [vp] * 4),
+    # rocket_fp8.h
+    "rocket_quantize_rows_fp8": (i32, [i32, i32, i32, vp, i64, vp, vp]),
+    "rocket_quantize_rows_fp8_fp16": (i32, [i32, i32, i32, vp, i64, vp, vp]),
+    "rocket_quantize_glu_fp8": (i32, [i32, i32, i32, vp, vp, i64, i32, vp, vp, vp]),
+    "rocket_quantize_glu_fp8_fp16": (i32, [i32, i32, i32, vp, vp, i64, i32, vp, vp, vp]),
+    "rocket_matmul_fp8_block": (i32, [i32] * 4 + [vp] * 5),
+    "rocket_matmul_fp8_block_f16out": (i32, [i32] * 4 + [vp] * 5),
+    "rocket_matmul_fp8_block_grouped": (i32, [i32] * 6 + [vp] * 7),
+    "rocket_matmul_fp8_block_grouped_f16out": (i32, [i32] * 6 + [vp] * 7),
+    # rocket_layer.h
+    "rocket_add_norm_fp16": (i32, [i32] * 3 + [vp, vp, i64, vp, fl, vp, i32, fl, vp, fl] + [vp] * 4),
+    "rocket_add_norm_f32": (i32, [i32] * 3 + [vp, vp, i64, vp, fl, vp, i32, fl, vp, fl] + [vp] * 4),
+    "rocket_moe_add_norm_fp16": (i32, [i32] * 3 + [vp, i32, i32] + [vp] * 5 + [fl, vp, i32, fl, vp, fl] + [vp] * 4),
+    "rocket_moe_add_norm_f32": (i32, [i32] * 3 + [vp, i32, i32] + [vp] * 5 + [fl, vp, i32, fl, vp, fl] + [vp] * 4),
+    "rocket_moe_route_f32": (i32, [i32] * 3 + [vp, i64, i32, vp] + [i32] * 5 + [fl] + [vp] * 6),
+    "rocket_moe_route_fp16": (i32, [i32] * 3 + [vp, i64, i32, vp] + [i32] * 5 + [fl] + [vp] * 6),
     # rocket_quant.h
     "rocket_quantize_rows_int8": (i32, [i32, i32, i32, vp, vp, vp]),
     "rocket_matmul_int4_prepacked_gw_f32in_noalloc": (i32, [vp, i32, i32, i32, vp, vp, vp, vp]),
@@ -217,6 +233,9 @@ ROCKET_ACTIVATION_SILU, ROCKET_ACTIVATION_TANH, ROCKET_ACTIVATION_GELU = 3, 4, 5
 
 # rocket_serve.h
 ROCKET_ROPE_HALVES, ROCKET_ROPE_PAIRS = 0, 1
+
+# rocket_layer.h
+ROCKET_ROUTE_SOFTMAX, ROCKET_ROUTE_SIGMOID = 0, 1
 
 # data objects exported by the headers (not functions)
 DATA_SYMBOLS = ("rocket_hw_mi355x", "rocket_hw_rk3588", "rocket_hw_rk3576")
