@@ -118,6 +118,10 @@ template <> struct Frag<true> {
         v[3] = w[1];
     }
 };
+// The same as it was loaded, which is kept where a widened one would take too many registers.
+struct Codes {
+    i32x4 lo, hi;
+};
 __device__ __forceinline__ f32x4 product(const Frag<false> &b, const Frag<false> &a)
 {
     const f32x4 z = {0.f, 0.f, 0.f, 0.f};

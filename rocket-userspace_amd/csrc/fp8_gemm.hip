@@ -32,24 +32,26 @@ namespace {
 [[maybe_unused]] __device__ constexpr int sw_a(int row) { return (row >> 1) & 7; }
 [[maybe_unused]] __device__ constexpr int sw_b(int row) { return ((row >> 1) & 1) | ((row >> 2) & 6); }
 
-template <int BM_, int BN_, int WGM_, int WGN_, int SLOTS_> struct Cfg {
-    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, SLOTS = SLOTS_;
+template <int BM_, int BN_, int WGM_, int WGN_, int SLOTS_, int WPE_, bool PIPE_> struct Cfg {
+    static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, SLOTS = SLOTS_, WPE = WPE_;
+    static constexpr bool PIPE = PIPE_;   // operands read a stage ahead
     static constexpr int NW = WGM * WGN, NT = 64 * NW, WTM = BM / WGM, WTN = BN / WGN, TM = WTM / 16, TN = WTN / 16;
     static constexpr int IA = BM / NW / 8, IB = BN / NW / 8;   // DMA instructions a wave and stage
-    static constexpr int RWS = BM / NW;                        // rows whose scales a wave loads
-    static constexpr int SLOT = (BM + BN) * 128 + NW * 256;
-    static constexpr int NVM = IA + IB + 1;
+    static constexpr int CH = 4 * NT / BM;                     // stages whose scales of A are loaded at once, four a lane
+    static constexpr int SLOT = (BM + BN) * 128;
+    static constexpr int NVM = IA + IB;
     static constexpr int SBN = (BN + 127) / 128;               // blocks of 128 columns
-    static_assert(IA >= 1 && IB >= 1 && RWS <= 64 && TN % 2 == 0 && (WTN == 128 || 128 % WTN == 0), "tile");
-    static constexpr int lds(int per) { return SLOTS * SLOT + SBN * per * 4; }
+    static_assert(IA >= 1 && IB >= 1 && TN % 2 == 0 && TM > 1 && (WTN == 128 || 128 % WTN == 0), "tile");
+    static_assert(NT % BM == 0, "whole lanes a row");
+    static constexpr int lds(int per) { return SLOTS * SLOT + 2 * BM * CH * 4 + SBN * per * 4; }
 };
 
-template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) void k_gemm_fp8(const Args a)
+template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __attribute__((amdgpu_waves_per_eu(CF::WPE))) void k_gemm_fp8(const Args a)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int BM = CF::BM, BN = CF::BN, TM = CF::TM, TN = CF::TN, SLOTS = CF::SLOTS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float *const sbl = reinterpret_cast<float *>(smem + SLOTS * CF::SLOT);
+    float *const sal = reinterpret_cast<float *>(smem + SLOTS * CF::SLOT), *const sbl = sal + 2 * BM * CF::CH;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / CF::WGN, wn = wave % CF::WGN;
 
@@ -90,21 +92,46 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) vo
         cb[i] = (uint32_t)((lane & 7) ^ sw_b(row)) * 16u;
         vb[i] = (uint32_t)row * (uint32_t)a.K + cb[i];
     }
+    constexpr int LR = CF::NT / BM;   // lanes that load a row's scales
     {
-        const int r = arow(wave * CF::RWS + lane % CF::RWS);
-        vs = r < 0 ? kOOB : (uint32_t)r * (uint32_t)a.nb * 4u;
+        const int r = arow(tid / LR);
+        vs = r < 0 ? kOOB : ((uint32_t)r * (uint32_t)a.nb + (uint32_t)(tid % LR) * 4u) * 4u;
     }
     typedef __attribute__((address_space(3))) void *Lds;
+    char *const pb0 = smem + SLOTS * BM * 128;   // A's slots, then B's
+    // The rows' scales of CH stages from stage CH c of the slice on, through registers (a DMA of four bytes a lane, once a
+    // stage, cost a fifth of the time), into the half of their LDS that the stages before do not read.
+    auto scales = [&](int c) __attribute__((always_inline)) {
+        return __builtin_bit_cast(f32x4, gk::ld16(rS, vs + (uint32_t)(kb0 + CF::CH * c) * 4u));   // (zeros past the last row's)
+    };
+    auto keep = [&](f32x4 v, int c) __attribute__((always_inline)) {
+        *reinterpret_cast<f32x4 *>(sal + (c & 1) * BM * CF::CH + tid * 4) = v;
+    };
+    // Loads of block b (past the slice's last: the last again, which nothing uses, so that the waits' counts stay). Where that
+    // is the last part of a block, the chunks past K read zeros, from then on.
+    const int part = a.K % 128 ? a.nb - 1 : -1;
+    auto block = [&](int b) __attribute__((always_inline)) {
+        b = min(b, kb1 - 1);
+        if (b == part) {
+            const uint32_t left = (uint32_t)a.K % 128u;
+#pragma unroll
+            for (int i = 0; i < CF::IA; i++) va[i] |= ca[i] < left ? 0u : kOOB;
+#pragma unroll
+            for (int i = 0; i < CF::IB; i++) vb[i] |= cb[i] < left ? 0u : kOOB;
+        }
+        return __builtin_amdgcn_readfirstlane(b * 128);
+    };
+    // Instruction i of the IA + IB that load a stage, whose codes start at byte k of a row.
+    auto load1 = [&](int i, int k, int slot) __attribute__((always_inline)) {
+        if (i < CF::IA)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (Lds)(smem + slot * BM * 128 + (wave * CF::IA + i) * 1024), 16, va[i], k, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (Lds)(pb0 + slot * BN * 128 + (wave * CF::IB + i - CF::IA) * 1024), 16, vb[i - CF::IA], k, 0, 0);
+    };
     auto load = [&](int b, int slot) __attribute__((always_inline)) {
-        char *const at = smem + slot * CF::SLOT;
-        const uint32_t k = (uint32_t)b * 128u, left = (uint32_t)a.K - k;
+        const int k = block(b);
 #pragma unroll
-        for (int i = 0; i < CF::IA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (Lds)(at + (wave * CF::IA + i) * 1024), 16, (va[i] + k) | (ca[i] < left ? 0u : kOOB), 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < CF::IB; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (Lds)(at + BM * 128 + (wave * CF::IB + i) * 1024), 16, (vb[i] + k) | (cb[i] < left ? 0u : kOOB), 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (Lds)(at + (BM + BN) * 128 + wave * 256), 4, vs + (uint32_t)b * 4u, 0, 0, 0);
+        for (int i = 0; i < CF::NVM; i++) load1(i, k, slot);
     };
 
     // the weights' scales of the tile's columns and the slice's blocks
@@ -112,6 +139,7 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) vo
         const int c = i / a.per, b = kb0 + i - c * a.per, n = n0 / 128 + c;
         sbl[i] = b < kb1 && n < (a.N + 127) / 128 ? a.sb[((size_t)e * ((a.N + 127) / 128) + n) * a.nb + b] : 0.f;
     }
+    keep(scales(0), 0);
     // (waited for before the ring starts: its waits count the DMA's loads alone)
     __syncthreads();
 
@@ -121,60 +149,176 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) vo
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-#pragma unroll
-    for (int s = 0; s < SLOTS - 1; s++) load(min(kb0 + s, kb1 - 1), s);
     const int ra = wm * CF::WTM + (lane & 15);
     const int q = lane >> 4, rb = wn * CF::WTN + 8 * ((lane & 15) >> 2) + (lane & 3);
-    const float *const sbw = sbl + (CF::SBN > 1 ? wn * CF::WTN / 128 * a.per : 0);
-    int slot = 0;
-    for (int b = kb0; b < kb1; b++) {
-        gk::wait_vm<(SLOTS - 2) * CF::NVM>();
+    const float *const sbw = sbl + (CF::SBN > 1 ? wn * CF::WTN / 128 * a.per : 0), *const saw = sal + ra * CF::CH;
+    auto codes = [&](const char *plane, int row, int sw) __attribute__((always_inline)) {
+        return Codes{*reinterpret_cast<const i32x4 *>(plane + row * 128 + ((q ^ sw) << 4)),
+                     *reinterpret_cast<const i32x4 *>(plane + row * 128 + (((4 + q) ^ sw) << 4))};
+    };
+    auto codes_a = [&](int slot, int i) __attribute__((always_inline)) { return codes(smem + slot * BM * 128, ra + 16 * i, sw_a(ra + 16 * i)); };
+    auto codes_b = [&](int slot, int j) __attribute__((always_inline)) {
+        const int row = rb + 32 * (j / 2) + 4 * (j % 2);
+        return codes(pb0 + slot * BN * 128, row, sw_b(row));
+    };
+    auto factors = [&](float (&sc)[TM], float &sb, unsigned u) __attribute__((always_inline)) {
+        const float *const ps = saw + (u / CF::CH % 2 * BM * CF::CH + u % CF::CH);
+        sb = sbw[u];
+#pragma unroll
+        for (int i = 0; i < TM; i++) sc[i] = ps[16 * i * CF::CH];
+    };
+    // A product is added kLag products later, when the matrix unit has it done. A stage's loads are issued between the
+    // products of its first half: at once they would hold the wave up, since a CU takes some 43 bytes a clock.
+    constexpr int NP = TM * TN, kLag = NP >= 8 ? 3 : 2;
+    constexpr int kEvery = NP >= 2 * CF::NVM ? NP / (2 * CF::NVM) : 1, kEach = (CF::NVM * kEvery + NP - 1) / NP;
+    auto spread = [&](int t, int k, int slot) __attribute__((always_inline)) {
+        if (t % kEvery) return;
+#pragma unroll
+        for (int e = 0; e < kEach; e++)
+            if (t / kEvery * kEach + e < CF::NVM) load1(t / kEvery * kEach + e, k, slot);
+    };
+    auto add = [&](f32x4 &c, const f32x4 &d, float s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) c[r] = fmaf(d[r], s, c[r]);
+    };
+    f32x4 next = {0.f, 0.f, 0.f, 0.f};
+    const unsigned n = (unsigned)(kb1 - kb0);
+    if constexpr (CF::PIPE) {
+        // A stage's operands are read from LDS while the stage before is multiplied from registers, so that the products
+        // wait for no read behind a barrier.
+        Codes xa[2][TM], xb[2][TN];
+        float sc[2][TM], sb[2];
+#pragma unroll
+        for (int s = 0; s < SLOTS; s++) load(kb0 + s, s);
+        gk::wait_vm<(SLOTS - 1) * CF::NVM>();
         gk::lds_barrier();
-        // (past the last block the ring loads it again, which nothing reads: the waits' counts stay)
-        load(min(b + SLOTS - 1, kb1 - 1), slot == 0 ? SLOTS - 1 : slot - 1);
-        const char *const pa = smem + slot * CF::SLOT, *const pb = pa + BM * 128;
-        const float *const ps = reinterpret_cast<const float *>(pb + BN * 128);
-        const float sb = sbw[b - kb0];
-        Frag<WIDE> fb[TN];
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-            const int row = rb + 32 * (j / 2) + 4 * (j % 2), f = sw_b(row);
-            fb[j].set(*reinterpret_cast<const i32x4 *>(pb + row * 128 + ((q ^ f) << 4)),
-                      *reinterpret_cast<const i32x4 *>(pb + row * 128 + (((4 + q) ^ f) << 4)));
-        }
+        for (int j = 0; j < TN; j++) xb[0][j] = codes_b(0, j);
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const int row = ra + 16 * i, f = sw_a(row);
-            Frag<WIDE> fa;
-            fa.set(*reinterpret_cast<const i32x4 *>(pa + row * 128 + ((q ^ f) << 4)),
-                   *reinterpret_cast<const i32x4 *>(pa + row * 128 + (((4 + q) ^ f) << 4)));
-            const float s = ps[row / CF::RWS * 64 + row % CF::RWS] * sb;
+        for (int i = 0; i < TM; i++) xa[0][i] = codes_a(0, i);
+        factors(sc[0], sb[0], 0);
+        auto stage = [&](auto S, unsigned u) __attribute__((always_inline)) {
+            constexpr int slot = S, after = (slot + 1) % SLOTS, now = slot % 2, then = 1 - now;
+            gk::wait_vm<(SLOTS - 2) * CF::NVM>();
+            if (u % CF::CH == CF::CH / 2) keep(next, (int)(u / CF::CH) + 1);
+            gk::lds_barrier();
+            if (u % CF::CH == 0) next = scales((int)(u / CF::CH) + 1);
+            const int k = block(kb0 + (int)u + SLOTS);
+            factors(sc[then], sb[then], min(u + 1, n - 1));
+            Frag<WIDE> fb[TN], fa;
 #pragma unroll
-            for (int j = 0; j < TN; j++) {
-                const f32x4 d = product(fb[j], fa);
+            for (int j = 0; j < TN; j++) fb[j].set(xb[now][j].lo, xb[now][j].hi);
+            f32x4 d[kLag + 1];
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(d[r], s, acc[i][j][r]);
+            for (int t = 0; t < NP + kLag; t++) {
+                if (t < NP) {
+                    if (t % TN == 0) fa.set(xa[now][t / TN].lo, xa[now][t / TN].hi);
+                    d[t % (kLag + 1)] = product(fb[t % TN], fa);
+                    spread(t, k, slot);
+                    if (t < TN) xb[then][t] = codes_b(after, t);
+                    else if (t < TN + TM) xa[then][t - TN] = codes_a(after, t - TN);
+                }
+                if (t >= kLag) {
+                    const int v = t - kLag;
+                    if (v % TN == 0) sc[now][v / TN] *= sb[now];
+                    add(acc[v / TN][v % TN], d[v % (kLag + 1)], sc[now][v / TN]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        slot = slot == SLOTS - 1 ? 0 : slot + 1;
+        };
+        static_assert(NP >= TN + TM && SLOTS % 2 == 0, "a stage has a product for each read of the next");
+        for (unsigned u = 0; u < n; u += SLOTS)
+            gk::static_for<SLOTS>([&](auto S) __attribute__((always_inline)) {
+                if (u + S < n) stage(S, u + S);
+            });
+    } else {
+#pragma unroll
+        for (int s = 0; s < SLOTS - 1; s++) load(kb0 + s, s);
+        auto stage = [&](auto S, unsigned u) __attribute__((always_inline)) {
+            constexpr int slot = S, free = (slot + SLOTS - 1) % SLOTS;
+            gk::wait_vm<(SLOTS - 2) * CF::NVM>();
+            if (u % CF::CH == CF::CH / 2) keep(next, (int)(u / CF::CH) + 1);
+            gk::lds_barrier();
+            if (u % CF::CH == 0) next = scales((int)(u / CF::CH) + 1);
+            const int k = block(kb0 + (int)u + SLOTS - 1);
+            Frag<WIDE> fa[2], fb[TN];
+            float sc[TM], sb;
+            auto set = [](Frag<WIDE> &f, const Codes &c) __attribute__((always_inline)) { f.set(c.lo, c.hi); };
+            set(fa[0], codes_a(slot, 0));
+#pragma unroll
+            for (int j = 0; j < TN; j++) set(fb[j], codes_b(slot, j));
+            factors(sc, sb, u);
+            f32x4 d[kLag + 1];
+#pragma unroll
+            for (int t = 0; t < NP + kLag; t++) {
+                if (t < NP) {
+                    const int i = t / TN, j = t % TN;
+                    if (j == 0 && i + 1 < TM) set(fa[(i + 1) & 1], codes_a(slot, i + 1));
+                    d[t % (kLag + 1)] = product(fb[j], fa[i & 1]);
+                    spread(t, k, free);
+                }
+                if (t >= kLag) {
+                    const int v = t - kLag;
+                    if (v % TN == 0) sc[v / TN] *= sb;
+                    add(acc[v / TN][v % TN], d[v % (kLag + 1)], sc[v / TN]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        for (unsigned u = 0; u < n; u += SLOTS)
+            gk::static_for<SLOTS>([&](auto S) __attribute__((always_inline)) {
+                if (u + S < n) stage(S, u + S);
+            });
     }
     gk::wait_vm<0>();   // (no DMA is in flight when the workgroup's LDS is given on)
 
     // ---- results ----
+    using T = std::conditional_t<F16, _Float16, float>;
+    const int n1 = n0 + wn * CF::WTN + 8 * q;
+    if (a.slices > 1) {
+        const int stride = (a.N + 3) & ~3;   // (columns from N on are zeros: the weights' rows there are)
+        float *const ws = a.ws + (size_t)slice * a.M * stride;
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+            if (m0 + ra + 16 * i < m1)
+#pragma unroll
+                for (int j = 0; j < TN; j++) store4(ws + (size_t)(m0 + ra + 16 * i) * stride, n1 + 32 * (j / 2) + 4 * (j % 2), a.N, true, acc[i][j]);
+        return;
+    }
     const bool wide = a.N % 4 == 0;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const int m = m0 + ra + 16 * i;
         if (m >= m1) continue;
-        using T = std::conditional_t<F16, _Float16, float>;
+        T *const row = static_cast<T *>(a.C) + (size_t)m * a.N;
+        if (wide) {
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-            const int n = n0 + wn * CF::WTN + 32 * (j / 2) + 8 * q + 4 * (j % 2);
-            if (a.slices > 1) store4(a.ws + ((size_t)slice * a.M + m) * a.N, n, a.N, wide, acc[i][j]);
-            else store4(static_cast<T *>(a.C) + (size_t)m * a.N, n, a.N, wide, acc[i][j]);
+            for (int j = 0; j < TN; j++) store4(row, n1 + 32 * (j / 2) + 4 * (j % 2), a.N, true, acc[i][j]);
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < 4 * TN; j++) {   // (any element of the sums by a chain of selects: no case that has to be fast)
+                float v = 0.f;
+#pragma unroll
+                for (int u = 0; u < 4 * TN; u++) v = j == u ? acc[i][u / 4][u % 4] : v;
+                const int n = n1 + 32 * (j / 8) + j % 8;
+                if (n < a.N) row[n] = (T)v;
+            }
         }
     }
 #endif
+}
+
+// The slices' sums, in order.
+template <bool F16> __global__ __launch_bounds__(256) void k_join_fp8(const Args a)
+{
+    const int stride = (a.N + 3) & ~3, quads = stride / 4;
+    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x, plane = (size_t)a.M * stride;
+    if (t >= (size_t)a.M * quads) return;
+    f32x4 v = *reinterpret_cast<const f32x4 *>(a.ws + 4 * t);
+    for (int s = 1; s < a.slices; s++) v += *reinterpret_cast<const f32x4 *>(a.ws + s * plane + 4 * t);
+    using T = std::conditional_t<F16, _Float16, float>;
+    const int m = (int)(t / quads), n = (int)(t - (size_t)m * quads) * 4;
+    store4(static_cast<T *>(a.C) + (size_t)m * a.N, n, a.N, a.N % 4 == 0, v);
 }
 
 template <class CF, bool WIDE, bool F16> hipError_t launch(Args a, const GemmF8 &L, hipStream_t s, uint64_t *blocks)
@@ -190,20 +334,97 @@ template <class CF, bool WIDE, bool F16> hipError_t launch(Args a, const GemmF8 
     if (hipError_t e = lds_opt_in(reinterpret_cast<const void *>(kern), CF::lds(kF8MaxK / kF8Block), opted)) return e;
     *blocks = (uint64_t)grid;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(CF::NT), lds, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (a.slices > 1) {
+        const size_t join = ((size_t)a.M * ((a.N + 3) / 4) + 255) / 256;
+        hipLaunchKernelGGL((k_join_fp8<F16>), dim3((unsigned)join), dim3(256), 0, s, a);
+        *blocks += join;
+    }
     return hipGetLastError();
 }
 
 }  // namespace
 }  // namespace f8
 
-size_t gemm_fp8_ws(const GemmF8 &L) { (void)L; return 0; }
+namespace {
 
-hipError_t gemm_fp8(const GemmF8 &L, hipStream_t s, uint64_t *blocks)
+using namespace f8;
+
+// The tiles, what a CU holds of one (cap), and what a stage takes in us: t1 with one workgroup a CU, tc with every CU full (cap 1: with
+// few workgroups, and with one a CU), measured at K = 4096 and 15360; `fixed` is the launch, the first loads and the results.
+struct Tile {
+    int bm, bn, cap;
+    float fixed, t1, tc;
+};
+enum Kind { kT256, kT128, kT128Deep, kT64x128, kT64x128Deep, kT64, kT32, kKinds, kRows = kKinds };
+constexpr Tile kNarrow[kKinds] = {{256, 256, 1, 9.f, 1.35f, 1.78f}, {128, 128, 2, 5.f, 0.66f, 1.15f}, {128, 128, 1, 5.f, 0.44f, 0.58f},
+                                  {64, 128, 2, 4.5f, 0.50f, 0.85f}, {64, 128, 1, 4.5f, 0.31f, 0.36f}, {64, 64, 2, 4.f, 0.23f, 0.40f},
+                                  {32, 64, 3, 3.5f, 0.20f, 0.36f}};
+// (widened: no tile of 256, whose codes' fp16 does not fit the registers, and none of 128 with four slots, which is no faster)
+constexpr Tile kWide[kKinds] = {{0, 0, 0, 0.f, 0.f, 0.f}, {128, 128, 2, 5.f, 0.98f, 1.78f}, {0, 0, 0, 0.f, 0.f, 0.f},
+                                {0, 0, 0, 0.f, 0.f, 0.f}, {64, 128, 1, 4.5f, 0.61f, 0.68f}, {64, 64, 2, 4.f, 0.41f, 0.66f},
+                                {32, 64, 3, 3.5f, 0.41f, 0.56f}};
+// Bytes a us: memory, what the CUs take out of the L2s, the slices' planes.
+constexpr float kCus = 256.f, kMem = 5.2e6f, kL2 = 14e6f, kJoin = 6e6f;
+
+// The kernel and the slices of K that are expected to take the least time.
+void plan(GemmF8 &L, bool split)
 {
-    using namespace f8;
-    const Args a = args(L);
-    using Base = Cfg<128, 128, 2, 2, 3>;
-    return L.f16 ? launch<Base, false, true>(a, L, s, blocks) : launch<Base, true, false>(a, L, s, blocks);
+    const Tile *const tiles = L.f16 ? kNarrow : kWide;
+    const int nb = f8_blocks(L.K);
+    const float used = L.off ? (float)std::min(L.n_expert, L.M) : 1.f, mean = (float)L.M / used;
+    const float mem = used * (float)L.N * (float)L.K / kMem;
+    float best = INFINITY;
+    for (int k = 0; k < kKinds; k++) {
+        const Tile &t = tiles[k];
+        if (!t.bm) continue;
+        const float rows = L.off ? used * std::max(1.f, mean / t.bm + 0.5f) : ceilf(mean / t.bm);
+        const float w1 = rows * (float)((L.N + t.bn - 1) / t.bn), room = kCus * t.cap;
+        for (int s : {1, 2, 3, 4, 6, 8}) {
+            if (s > 1 && (!split || L.off || nb < 3 * s || w1 * (s - 1) > room)) break;
+            const int per = (nb + s - 1) / s;
+            const float w = w1 * s, full = t.cap > 1 ? std::max(0.f, (std::min(w, room) / kCus - 1.f) / (t.cap - 1)) : std::min(1.f, w / kCus);
+            const float comp = std::max(ceilf(w / room) * per * (t.t1 + (t.tc - t.t1) * full), w * per * 128.f * (t.bm + t.bn) / kL2);
+            float us = t.fixed + sqrtf(comp * comp + mem * mem);
+            if (s > 1) us += 2.5f + 8.f * s * (float)L.M * (float)L.N / kJoin;
+            if (us < best) best = us, L.kind = k, L.slices = (nb + per - 1) / per;
+        }
+    }
+    const float rows = gemm_fp8_rows_us(L);
+    if (rows < best) L.kind = kRows, L.slices = 1;
+}
+
+template <class CF> hipError_t start(const Args &a, const GemmF8 &L, hipStream_t s, uint64_t *blocks)
+{
+    return L.f16 ? launch<CF, false, true>(a, L, s, blocks) : launch<CF, true, false>(a, L, s, blocks);
+}
+
+}  // namespace
+
+size_t gemm_fp8_plan(GemmF8 &L)
+{
+    plan(L, true);
+    return L.slices > 1 ? (size_t)L.slices * L.M * ((L.N + 3) & ~3) * sizeof(float) : 0;
+}
+
+hipError_t gemm_fp8(const GemmF8 &L0, hipStream_t s, uint64_t *blocks)
+{
+    GemmF8 L = L0;
+    if (L.slices > 1 && !L.ws) plan(L, false);
+    Args a = args(L);
+    a.ws = L.ws;
+    a.per = (a.nb + L.slices - 1) / L.slices;
+    a.slices = L.slices;
+    switch (L.kind) {
+    case kT256: return launch<Cfg<256, 256, 2, 4, 2, 2, false>, false, true>(a, L, s, blocks);
+    case kT128: return start<Cfg<128, 128, 2, 2, 2, 2, false>>(a, L, s, blocks);
+    case kT128Deep: return launch<Cfg<128, 128, 2, 2, 4, 1, true>, false, true>(a, L, s, blocks);
+    case kT64x128: return launch<Cfg<64, 128, 2, 2, 2, 2, true>, false, true>(a, L, s, blocks);
+    case kT64x128Deep: return start<Cfg<64, 128, 2, 2, 4, 2, true>>(a, L, s, blocks);
+    case kT64: return start<Cfg<64, 64, 2, 2, 4, 2, true>>(a, L, s, blocks);
+    case kT32: return start<Cfg<32, 64, 1, 2, 4, 2, true>>(a, L, s, blocks);
+    default: return gemm_fp8_rows(L, s, blocks);
+    }
 }
 
 }  // namespace rk

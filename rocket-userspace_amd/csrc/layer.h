@@ -41,15 +41,15 @@ struct GemmF8 {
     void *C = nullptr;
     bool f16 = false;
     int M = 0, K = 0, N = 0, n_expert = 1, a_rows = 0;   // M: rows of C
-    // workspace for slices of K (gemm_fp8_ws); without it a workgroup walks all of K
-    float *ws = nullptr;
-    size_t ws_bytes = 0;
+    int kind = 0, slices = 1;   // the kernel, and its slices of K (gemm_fp8_plan)
+    float *ws = nullptr;        // the slices' sums; without it a workgroup walks all of K
 };
-size_t gemm_fp8_ws(const GemmF8 &L);
+// Chooses the launch's kernel and slices. The bytes that `ws` has to have (0: no slices).
+size_t gemm_fp8_plan(GemmF8 &L);
 hipError_t gemm_fp8(const GemmF8 &L, hipStream_t s, uint64_t *blocks);
 
-// Few rows (fp8_rows.hip).
-bool gemm_fp8_few_rows(const GemmF8 &L);
+// Few rows (fp8_rows.hip): the time that they are expected to take (infinite: too many rows), and the launch.
+float gemm_fp8_rows_us(const GemmF8 &L);
 hipError_t gemm_fp8_rows(const GemmF8 &L, hipStream_t s, uint64_t *blocks);
 
 struct AddNorm {

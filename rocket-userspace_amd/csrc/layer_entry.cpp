@@ -108,7 +108,7 @@ int on_gpu(const char *who, int fd, const Operand (&in)[NI], const Operand (&out
     void *scratch = needed ? c.scratch(needed) : c.optional(opt);
     if (needed && !scratch) return c.finish();
     uint64_t blocks = 0;
-    const hipError_t e = go(scratch, scratch ? (needed ? needed : opt) : 0, c.stream(), &blocks);
+    const hipError_t e = go(scratch, c.stream(), &blocks);
     if (e != hipSuccess) {
         (void)hipGetLastError();
         ROCKET_LOGE("%s: kernel launch rejected: %s\n", who, hipGetErrorString(e));
@@ -136,7 +136,7 @@ int quantise(const char *who, int fd, QuantF8 L, bool gated)
         quant_fp8_ref(L);
         return ROCKET_OK;
     }
-    return on_gpu(who, fd, in, out, 0, 0, [&](void *, size_t, hipStream_t s, uint64_t *blocks) { return quant_fp8(L, s, blocks); });
+    return on_gpu(who, fd, in, out, 0, 0, [&](void *, hipStream_t s, uint64_t *blocks) { return quant_fp8(L, s, blocks); });
 }
 
 // ---- products ----
@@ -156,9 +156,9 @@ int product(const char *who, int fd, GemmF8 L, bool grouped)
     const Operand out[] = {in_part(L.C, (size_t)L.M * L.N * (L.f16 ? sizeof(_Float16) : sizeof(float)), grouped)};
     if (clash(in, out)) return bad(who, "results over operands");
     if (fd < 0) return gemm_fp8_ref(L) ? ROCKET_OK : ROCKET_E_NOMEM;
-    return on_gpu(who, fd, in, out, 0, gemm_fp8_ws(L), [&](void *ws, size_t bytes, hipStream_t s, uint64_t *blocks) {
+    const size_t ws_bytes = gemm_fp8_plan(L);
+    return on_gpu(who, fd, in, out, 0, ws_bytes, [&](void *ws, hipStream_t s, uint64_t *blocks) {
         L.ws = static_cast<float *>(ws);
-        L.ws_bytes = bytes;
         return gemm_fp8(L, s, blocks);
     });
 }
@@ -186,7 +186,7 @@ int norms(const char *who, int fd, AddNorm L, bool experts)
                            operand(L.x_scale, rows * nb * sizeof(float))};
     if (clash(in, out, L.h_out == L.h ? L.h : nullptr)) return bad(who, "results over operands or each other");
     if (fd < 0) return add_norm_ref(L) ? ROCKET_OK : ROCKET_E_NOMEM;
-    return on_gpu(who, fd, in, out, 0, 0, [&](void *, size_t, hipStream_t s, uint64_t *blocks) { return add_norm(L, s, blocks); });
+    return on_gpu(who, fd, in, out, 0, 0, [&](void *, hipStream_t s, uint64_t *blocks) { return add_norm(L, s, blocks); });
 }
 
 // ---- routing ----
@@ -208,7 +208,7 @@ int route(const char *who, int fd, Route L, int score)
                            in_part(L.src, kb), operand(L.slot, kb)};
     if (clash(in, out)) return bad(who, "results over operands or each other");
     if (fd < 0) return moe_route_ref(L) ? ROCKET_OK : ROCKET_E_NOMEM;
-    return on_gpu(who, fd, in, out, route_ws(L), 0, [&](void *ws, size_t, hipStream_t s, uint64_t *blocks) {
+    return on_gpu(who, fd, in, out, route_ws(L), 0, [&](void *ws, hipStream_t s, uint64_t *blocks) {
         L.counts = static_cast<int32_t *>(ws);
         return moe_route(L, s, blocks);
     });
