@@ -163,6 +163,22 @@ __device__ __forceinline__ void store4(float *row, int n, int N, bool wide, f32x
             if (n + r < N) row[n + r] = v[r];
     }
 }
+// Columns n .. n + 7 of one row (those below N, a multiple of 4): one store where the row is aligned to it.
+__device__ __forceinline__ void store8(_Float16 *row, int n, int N, f32x4 v, f32x4 w)
+{
+    const f16x8 o = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3], (_Float16)w[0], (_Float16)w[1], (_Float16)w[2], (_Float16)w[3]};
+    if (N % 8 == 0) {
+        if (n < N) *reinterpret_cast<f16x8 *>(row + n) = o;
+    } else {
+        store4(row, n, N, true, v);
+        store4(row, n + 4, N, true, w);
+    }
+}
+__device__ __forceinline__ void store8(float *row, int n, int N, f32x4 v, f32x4 w)
+{
+    store4(row, n, N, true, v);
+    store4(row, n + 4, N, true, w);
+}
 
 Args args(const GemmF8 &L);
 // The most tiles of bm rows that the launch's experts can have.

@@ -249,6 +249,8 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
             for (int j = 0; j < TN; j++) set(fb[j], codes_b(slot, j));
             factors(sc, sb, u);
             f32x4 d[kLag + 1];
+            // (ahead of a wave that still reads its operands: 1 to 2% at 256 x 256)
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int t = 0; t < NP + kLag; t++) {
                 if (t < NP) {
@@ -264,6 +266,7 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
         };
         for (unsigned u = 0; u < n; u += SLOTS)
             gk::static_for<SLOTS>([&](auto S) __attribute__((always_inline)) {
@@ -293,7 +296,7 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
         T *const row = static_cast<T *>(a.C) + (size_t)m * a.N;
         if (wide) {
 #pragma unroll
-            for (int j = 0; j < TN; j++) store4(row, n1 + 32 * (j / 2) + 4 * (j % 2), a.N, true, acc[i][j]);
+            for (int j = 0; j < TN; j += 2) store8(row, n1 + 16 * j, a.N, acc[i][j], acc[i][j + 1]);
         } else {
 #pragma unroll 1
             for (int j = 0; j < 4 * TN; j++) {   // (any element of the sums by a chain of selects: no case that has to be fast)
