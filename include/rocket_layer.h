@@ -27,7 +27,7 @@ extern "C" {
  *     z  = N(y[m]; w_post, eps_post)                               the block's result, y + m * y_rs
  *     h' = h[m] + alpha * gate[m / gate_every] * z                 (gate NULL: ones; y NULL: h' = h[m])
  *     x  = N(h'; w_pre, eps_pre)                                   of h' before it is rounded
- * Results, each of which may be NULL, but not all: h_out[M][H] (h' in h's type; it may be h itself), x[M][H] in fp16, and xq[M][H] with
+ * Results, each of which may be NULL, but not all: h_out[M][H] (h' in h's type; it may be h itself, if y is not), x[M][H] in fp16, and xq[M][H] with
  * x_scale[M][ceil(H / 128)] (both or neither), x's codes and scales as rocket_quantize_rows_fp8 makes them of the
  * unrounded x. h[M][H], gate[ceil(M / gate_every)][H]: gate_every 1 is a gate for each row, the tokens of a
  * sequence one for each sequence, M or more one for all. y_rs >= H, a multiple of 8, up to 2^40.
@@ -57,7 +57,7 @@ int rocket_moe_add_norm_f32(int fd, int M, int H, const float *h, int rows, int 
  * the largest finite float. With n_group > 1, the experts lie in n_group equal runs; a run's value is the sum of its
  * group_best (1 or 2) largest choices, and only candidates of the top_group runs of the largest values stay (of
  * equal ones the first). The top_k largest choices are a token's experts, in falling order, of equal ones the first
- * (without a bias they are compared as logits); weight = p of the expert, divided by the sum of the token's chosen p
+ * (without a bias they are compared as logits; numbers are compared up to 2^-42 of themselves); weight = p of the expert, divided by the sum of the token's chosen p
  * where renorm is not 0 (0 where that sum is 0), times scale, rounded to fp32 once. Where fewer candidates are
  * left, and for a token with active[m] == 0 (active NULL: all are active), the places left get id -1 and weight 0.
  * A NaN logit (or one that makes p NaN) ranks behind every number and its weights are NaN; ids stay in range.
@@ -67,8 +67,9 @@ int rocket_moe_add_norm_f32(int fd, int M, int H, const float *h, int rows, int 
  *     src_row[M * top_k]    the token of each row (places from expert_off[E] on are left as they were)
  *     slot[M][top_k]        the row of each choice, -1 where there is none
  * 1 <= E <= 1024, E % n_group == 0, 1 <= n_group <= 64, group_best 1 or 2, 1 <= top_group <= n_group,
- * 1 <= top_k <= min(32, E), M * top_k < 2^24, rs >= E. Tokens above 64 with a plan take scratch of the handle (a
- * captured call needs an eager one of the same size first). */
+ * 1 <= top_k <= min(32, E), M * top_k < 2^24, rs >= E. Results in device memory may be 4-byte aligned. More than 32
+ * tokens with a plan take scratch of the handle (a captured call needs an eager one of the same size first; graphs that
+ * hold scratch of one handle are replayed in the order of its stream). */
 #define ROCKET_ROUTE_SOFTMAX 0
 #define ROCKET_ROUTE_SIGMOID 1
 int rocket_moe_route_f32(int fd, int M, int E, const float *logits, int64_t rs, int score, const float *bias, int n_group, int group_best,

@@ -303,13 +303,13 @@ void *Call::in(const void *p, size_t bytes, size_t align)
     return d;
 }
 
-void *Call::out(void *p, size_t bytes)
+void *Call::out(void *p, size_t bytes, size_t align)
 {
-    if (direct_(p)) return p;
+    if (direct_(p, align)) return p;
     host_io_ = true;
     void *d = scratch(bytes);
     if (!d) return nullptr;
-    back_.push_back({p, d, bytes});
+    back_.push_back({p, d, bytes, is_device_ptr(p, h_->device)});
     return d;
 }
 
@@ -346,7 +346,7 @@ int Call::finish_()
     }
     if (!host_io_ && back_.empty() && h_->async) return ROCKET_OK;
     size_t total = 0;
-    for (const Back &b : back_) total += round_(b.bytes);
+    for (const Back &b : back_) total += b.device ? 0 : round_(b.bytes);
     {
         PhaseTimer pt(t_read_);
         if (total > h_->pin_cap) {
@@ -364,14 +364,16 @@ int Call::finish_()
         }
         size_t off = 0;
         for (const Back &b : back_) {
-            if (hipMemcpyAsync(static_cast<char *>(h_->pin) + off, b.src, b.bytes, hipMemcpyDeviceToHost,
-                               h_->stream) != hipSuccess) {
+            const hipError_t e = b.device ? hipMemcpyAsync(b.dst, b.src, b.bytes, hipMemcpyDeviceToDevice, h_->stream)
+                                          : hipMemcpyAsync(static_cast<char *>(h_->pin) + off, b.src, b.bytes,
+                                                           hipMemcpyDeviceToHost, h_->stream);
+            if (e != hipSuccess) {
                 (void)hipGetLastError();
                 ROCKET_LOGE("%s: device-to-host copy failed\n", who_);
                 (void)handle_wait(h_, who_);
                 return ROCKET_E_DEVICE;
             }
-            off += round_(b.bytes);
+            off += b.device ? 0 : round_(b.bytes);
         }
     }
     {
@@ -382,6 +384,7 @@ int Call::finish_()
     PhaseTimer pt(t_read_);
     size_t off = 0;
     for (const Back &b : back_) {
+        if (b.device) continue;
         memcpy(b.dst, static_cast<char *>(h_->pin) + off, b.bytes);
         off += round_(b.bytes);
     }

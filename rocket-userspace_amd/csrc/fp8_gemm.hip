@@ -363,9 +363,10 @@ enum Kind { kT256, kT128, kT128Deep, kT64x128, kT64x128Deep, kT64, kT32, kKinds,
 constexpr Tile kNarrow[kKinds] = {{256, 256, 1, 9.f, 1.35f, 1.78f}, {128, 128, 2, 5.f, 0.66f, 1.15f}, {128, 128, 1, 5.f, 0.44f, 0.58f},
                                   {64, 128, 2, 4.5f, 0.50f, 0.85f}, {64, 128, 1, 4.5f, 0.31f, 0.36f}, {64, 64, 2, 4.f, 0.23f, 0.40f},
                                   {32, 64, 3, 3.5f, 0.20f, 0.36f}};
-// (widened: no tile of 256, whose codes' fp16 does not fit the registers, and none of 128 with four slots, which is no faster)
+// (widened: no tile of 256, whose codes' fp16 does not fit the registers, none of 128 with four slots, which is no faster, and
+// none of 64 x 128, a stage of which takes 0.61 to 0.68: two workgroups of 64 x 64 on a CU have as much done in 0.66)
 constexpr Tile kWide[kKinds] = {{0, 0, 0, 0.f, 0.f, 0.f}, {128, 128, 2, 5.f, 0.98f, 1.78f}, {0, 0, 0, 0.f, 0.f, 0.f},
-                                {0, 0, 0, 0.f, 0.f, 0.f}, {64, 128, 1, 4.5f, 0.61f, 0.68f}, {64, 64, 2, 4.f, 0.41f, 0.66f},
+                                {0, 0, 0, 0.f, 0.f, 0.f}, {0, 0, 0, 0.f, 0.f, 0.f}, {64, 64, 2, 4.f, 0.41f, 0.66f},
                                 {32, 64, 3, 3.5f, 0.41f, 0.56f}};
 // Bytes a us: memory, what the CUs take out of the L2s, the slices' planes.
 constexpr float kCus = 256.f, kMem = 5.2e6f, kL2 = 14e6f, kJoin = 6e6f;
@@ -423,7 +424,7 @@ hipError_t gemm_fp8(const GemmF8 &L0, hipStream_t s, uint64_t *blocks)
     case kT128: return start<Cfg<128, 128, 2, 2, 2, 2, false>>(a, L, s, blocks);
     case kT128Deep: return launch<Cfg<128, 128, 2, 2, 4, 1, true>, false, true>(a, L, s, blocks);
     case kT64x128: return launch<Cfg<64, 128, 2, 2, 2, 2, true>, false, true>(a, L, s, blocks);
-    case kT64x128Deep: return start<Cfg<64, 128, 2, 2, 4, 2, true>>(a, L, s, blocks);
+    case kT64x128Deep: return launch<Cfg<64, 128, 2, 2, 4, 2, true>, false, true>(a, L, s, blocks);
     case kT64: return start<Cfg<64, 64, 2, 2, 4, 2, true>>(a, L, s, blocks);
     case kT32: return start<Cfg<32, 64, 1, 2, 4, 2, true>>(a, L, s, blocks);
     default: return gemm_fp8_rows(L, s, blocks);

@@ -75,7 +75,7 @@ public:
     // the graph replays on it (each at least 1.25 times the last, so all of them at most 5 times it).
     int  begin();
     void *in(const void *p, size_t bytes, size_t align = 16);  // device view of an input
-    void *out(void *p, size_t bytes);       // device view of an output
+    void *out(void *p, size_t bytes, size_t align = 16);       // device view of an output
     void *scratch(size_t bytes);            // arena scratch (not copied)
     void *optional(size_t bytes) { return bytes && !opt_dropped_ ? scratch(bytes) : nullptr; }
     int  launch(const Launch &L);           // enqueue one GEMM launch
@@ -99,7 +99,7 @@ private:
     bool opt_dropped_ = false;
     bool host_io_ = false;
     int err_ = 0;
-    struct Back { void *dst; const void *src; size_t bytes; };
+    struct Back { void *dst; const void *src; size_t bytes; bool device; };   // device: dst is (misaligned) device memory
     std::vector<Back> back_;
 };
 

@@ -47,9 +47,9 @@ template <class T> Operand operand(T *&p, size_t bytes, size_t align = 16)
 {
     return {p, bytes, const_cast<void *>(static_cast<const volatile void *>(&p)), align};
 }
-template <class T> Operand in_part(T *&p, size_t bytes, bool part = true)
+template <class T> Operand in_part(T *&p, size_t bytes, bool part = true, size_t align = 16)
 {
-    Operand o = operand(p, bytes);
+    Operand o = operand(p, bytes, align);
     o.part = part;
     return o;
 }
@@ -59,12 +59,12 @@ bool overlap(const void *a, size_t an, const void *b, size_t bn)
     return a && b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
 
-// Results over operands or each other; `in_place`: a result that may be the operand it names, whole.
-template <size_t NI, size_t NO> bool clash(const Operand (&in)[NI], const Operand (&out)[NO], const void *in_place = nullptr)
+// Results over operands or each other; `in_place`: the first result may be the first operand, whole.
+template <size_t NI, size_t NO> bool clash(const Operand (&in)[NI], const Operand (&out)[NO], bool in_place = false)
 {
     for (size_t o = 0; o < NO; o++) {
-        for (const Operand &i : in)
-            if (overlap(i.p, i.bytes, out[o].p, out[o].bytes) && !(out[o].p == in_place && i.p == in_place)) return true;
+        for (size_t i = 0; i < NI; i++)
+            if (overlap(in[i].p, in[i].bytes, out[o].p, out[o].bytes) && !(in_place && !o && !i && in[i].p == out[o].p)) return true;
         for (size_t u = 0; u < o; u++)
             if (overlap(out[o].p, out[o].bytes, out[u].p, out[u].bytes)) return true;
     }
@@ -85,7 +85,7 @@ int on_gpu(const char *who, int fd, const Operand (&in)[NI], const Operand (&out
     for (const Operand &i : in)
         if (i.p) c.want(i.p, i.bytes, i.align);
     for (const Operand &o : out)
-        if (o.p) c.want(o.p, o.bytes);
+        if (o.p) c.want(o.p, o.bytes, o.align);
     if (needed) c.want_scratch(needed);
     const size_t opt = optional ? c.want_optional(optional, true) : 0;
     if (int rc = c.begin()) return rc;
@@ -95,7 +95,7 @@ int on_gpu(const char *who, int fd, const Operand (&in)[NI], const Operand (&out
         i.set(at);
     }
     for (const Operand &o : out) {
-        const void *at = o.p ? c.out(const_cast<void *>(o.p), o.bytes) : nullptr;
+        const void *at = o.p ? c.out(const_cast<void *>(o.p), o.bytes, o.align) : nullptr;
         if (o.p && !at) return c.finish();
         if (o.part && at != o.p && hipMemcpyAsync(const_cast<void *>(at), o.p, o.bytes, hipMemcpyDefault, c.stream()) != hipSuccess) {
             (void)hipGetLastError();
@@ -184,7 +184,7 @@ int norms(const char *who, int fd, AddNorm L, bool experts)
                           operand(L.gate, gb), operand(L.slot, jb, kIntAlign), operand(L.weight, jb, kIntAlign)};
     const Operand out[] = {operand(L.h_out, hb), operand(L.x, rows * L.H * sizeof(_Float16)), operand(L.xq, rows * L.H),
                            operand(L.x_scale, rows * nb * sizeof(float))};
-    if (clash(in, out, L.h_out == L.h ? L.h : nullptr)) return bad(who, "results over operands or each other");
+    if (clash(in, out, true)) return bad(who, "results over operands or each other");
     if (fd < 0) return add_norm_ref(L) ? ROCKET_OK : ROCKET_E_NOMEM;
     return on_gpu(who, fd, in, out, 0, 0, [&](void *, hipStream_t s, uint64_t *blocks) { return add_norm(L, s, blocks); });
 }
@@ -204,8 +204,8 @@ int route(const char *who, int fd, Route L, int score)
     const size_t rows = (size_t)L.M, e = L.f32 ? sizeof(float) : sizeof(_Float16), kb = rows * L.top_k * 4;
     const Operand in[] = {operand(L.logits, ((rows - 1) * L.rs + L.E) * e, e), operand(L.bias, (size_t)L.E * sizeof(float), kIntAlign),
                           operand(L.active, rows, 1)};
-    const Operand out[] = {operand(L.ids, kb), operand(L.weight, kb), operand(L.off, ((size_t)L.E + 1) * sizeof(int32_t)),
-                           in_part(L.src, kb), operand(L.slot, kb)};
+    const Operand out[] = {operand(L.ids, kb, kIntAlign), operand(L.weight, kb, kIntAlign), operand(L.off, ((size_t)L.E + 1) * sizeof(int32_t), kIntAlign),
+                           in_part(L.src, kb, true, kIntAlign), operand(L.slot, kb, kIntAlign)};
     if (clash(in, out)) return bad(who, "results over operands or each other");
     if (fd < 0) return moe_route_ref(L) ? ROCKET_OK : ROCKET_E_NOMEM;
     return on_gpu(who, fd, in, out, route_ws(L), 0, [&](void *ws, hipStream_t s, uint64_t *blocks) {

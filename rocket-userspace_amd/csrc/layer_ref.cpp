@@ -157,7 +157,7 @@ bool moe_route_ref(const Route &L)
     } catch (const std::bad_alloc &) {
         return false;
     }
-    const auto rank = [](double v) { return v == v ? std::min(std::max(v, -1e300), 1e300) : -1e300; };
+    const auto rank = [](double v) { return v == v ? std::min(std::max(v, -1e300), 1e300) : -4e300; };   // (two -1e300 are a run's)
     const int run = L.E / L.n_group;
     for (int m = 0; m < L.M; m++) {
         int32_t *ids = L.ids + (size_t)m * L.top_k;
@@ -168,7 +168,7 @@ bool moe_route_ref(const Route &L)
         double most = -INFINITY, sum = 0.0;
         for (int e = 0; e < L.E; e++) {
             const float v = at(L.logits, L.f32, (size_t)m * L.rs + e);
-            s[e].key = v > 3.402823466e38f ? 3.402823466e38 : (double)v;
+            s[e].key = (double)(v > 3.402823466e38f ? 3.402823466e38f : v);
             most = fmax(most, s[e].key);
         }
         if (most == -INFINITY) most = 0.0;

@@ -4,9 +4,9 @@
 // 64-bit number of the choice's order whose last ten bits are the expert's, the first one's the largest. What bounds it is the
 // number of instructions a token: up to 256 experts a token is a row of 16 lanes, each with up to 16 neighbouring experts, four
 // tokens a wave, whose reductions stay in registers (DPP rotations within a row); more experts are a wave a token, where a lane
-// sorts its keys once and moves on where it has won. The sort by expert needs no order of atomics: a workgroup's tokens set their bit in one mask an expert, and a choice's place among them is the count of bits
-// below its own. Few tokens are one workgroup and one launch; more write their counts, which a second launch turns into starts and
-// a third into rows.
+// sorts its keys once and moves on where it has won. The sort by expert needs no order of atomics: a workgroup's tokens set their
+// bit in one mask an expert, and a choice's place among them is the count of bits below its own. Few tokens are one workgroup and
+// one launch; more write their counts, which a second launch turns into starts and a third into rows.
 #include "layer.h"
 
 #include <algorithm>
@@ -62,7 +62,7 @@ __device__ __forceinline__ uint64_t ordered(double v)
     const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);   // (-0 and 0 are one)
     return b >> 63 ? ~b : b | (uint64_t)1 << 63;
 }
-__device__ __forceinline__ double ranked(double v) { return v == v ? fmin(fmax(v, -1e300), 1e300) : -1e300; }
+__device__ __forceinline__ double ranked(double v) { return v == v ? fmin(fmax(v, -1e300), 1e300) : -4e300; }   // (two -1e300 are a run's)
 
 // The largest of keys that differ where they are not 0 (0: all are), in every lane.
 __device__ __forceinline__ uint64_t wave_best(uint64_t key)
@@ -433,14 +433,13 @@ template <int L_, int NE_> struct Form {
     static constexpr int L = L_, NE = NE_, WAVES = L == 16 || NE == 16 ? 8 : 16, E = L * NE;
 };
 
-// A workgroup's tokens. ONE: all tokens (up to 64), with the plan; otherwise kTokens of them, and their counts.
+// A workgroup's tokens. ONE: all tokens (up to kOne), with the plan; otherwise kTokens of them, and their counts.
 template <class F, bool ONE> __global__ __launch_bounds__(64 * F::WAVES) void k_route(const RArgs a)
 {
-    using Mask = std::conditional_t<ONE, unsigned long long, unsigned>;
-    constexpr int T = ONE ? 64 : kTokens;
+    constexpr int T = ONE ? kOne : kTokens;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int part[16], start[ONE ? F::E : 1], chosen[ONE ? T * kMaxTop : 1];
-    __shared__ Mask mask[F::E];
+    __shared__ unsigned mask[F::E];
     const int l = threadIdx.x % F::L, row = threadIdx.x / F::L, rows = blockDim.x / F::L, t0 = blockIdx.x * T;
     double *const keys = reinterpret_cast<double *>(smem) + (size_t)row * a.E;
     if (a.plan) {
@@ -460,7 +459,7 @@ template <class F, bool ONE> __global__ __launch_bounds__(64 * F::WAVES) void k_
                 a.ids[(size_t)m * a.top_k + j] = id[u];
                 a.weight[(size_t)m * a.top_k + j] = w[u];
                 if (ONE) chosen[t * a.top_k + j] = id[u];
-                if (a.plan && id[u] >= 0) atomicOr(&mask[id[u]], (Mask)1 << t);
+                if (a.plan && id[u] >= 0) atomicOr(&mask[id[u]], 1u << t);
             }
         }
     }
@@ -471,13 +470,13 @@ template <class F, bool ONE> __global__ __launch_bounds__(64 * F::WAVES) void k_
     } else {
         const int per = (a.E + blockDim.x - 1) / blockDim.x, e0 = threadIdx.x * per, e1 = min(a.E, e0 + per);   // experts a thread, neighbours
         int n = 0;
-        for (int e = e0; e < e1; e++) n += __popcll(mask[e]);
+        for (int e = e0; e < e1; e++) n += __popc(mask[e]);
         int all;
         int at = group_scan(n, part, all);
         for (int e = e0; e < e1; e++) {
             start[e] = at;
             a.off[e] = at;
-            at += __popcll(mask[e]);
+            at += __popc(mask[e]);
         }
         if (threadIdx.x == 0) a.off[a.E] = all;
         __syncthreads();
@@ -485,7 +484,7 @@ template <class F, bool ONE> __global__ __launch_bounds__(64 * F::WAVES) void k_
             const int t = i / a.top_k, id = chosen[i];
             int r = -1;
             if (id >= 0) {
-                r = start[id] + __popcll(mask[id] & (((Mask)1 << t) - 1));
+                r = start[id] + __popc(mask[id] & ((1u << t) - 1u));
                 a.src[r] = t;
             }
             a.slot[i] = r;

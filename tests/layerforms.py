@@ -184,7 +184,7 @@ def route(logits, k, sigmoid=False, bias=None, groups=1, best=1, top_groups=1, r
     M, n = logits.shape
     ids = torch.full((M, k), -1, dtype=torch.int64)
     weight = torch.zeros((M, k), dtype=torch.float64)
-    rank = lambda v: -1e300 if v != v else min(max(v, -1e300), 1e300)  # noqa: E731
+    rank = lambda v: -4e300 if v != v else min(max(v, -1e300), 1e300)  # noqa: E731
     for m in range(M):
         if active is not None and not active[m]:
             continue

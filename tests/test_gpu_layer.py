@@ -86,7 +86,11 @@ def test_quantise_gated(lib, fd, M, K, n, act, dtype):
 
 PRODUCTS = [(1, 16, 1), (1, 3840, 640), (2, 144, 7), (7, 4096, 130), (15, 272, 257), (16, 128, 128), (17, 1024, 100), (32, 640, 384), (33, 2080, 1000), (64, 16, 640),
             (65, 512, 129), (77, 2080, 1001), (128, 1152, 512), (129, 384, 255), (200, 4096, 256), (256, 256, 320), (257, 1040, 770), (300, 128, 2050), (512, 2048, 512),
-            (1030, 528, 516), (5, 65536, 33), (130, 65536, 17)]
+            (1030, 528, 516), (5, 65536, 33), (130, 65536, 17),
+            # the larger tiles and their slices of K, with rows and columns left over
+            (1030, 192, 4100), (2050, 384, 1000), (2050, 1232, 257), (1500, 656, 1000), (3000, 944, 770), (3000, 1120, 4100), (2900, 1136, 4099), (3000, 464, 1030),
+            (2050, 6832, 1000), (2050, 7520, 516), (1000, 7216, 513), (1500, 8608, 516), (2050, 3552, 257), (1000, 5152, 100), (17, 2432, 99), (700, 6960, 104),
+            (512, 15360, 640), (300, 16384, 1024), (16, 1024, 9000), (13, 400, 40000)]
 
 
 @pytest.mark.parametrize("dtype", [H16, F32])
@@ -150,6 +154,8 @@ def split(g, rows, E, empty=0.3):
 GROUPED = [  # experts, rows, rows of A (None: in order), K, N
     (1, 1, None, 128, 16), (8, 3, 2, 272, 40), (64, 96, 16, 512, 384), (64, 96, None, 400, 130), (5, 300, 70, 1024, 257), (16, 700, None, 144, 264),
     (1024, 64, 40, 128, 36), (130, 2000, 500, 256, 128), (3, 1500, 1500, 640, 516), (200, 40, 40, 2064, 64),
+    (3, 3000, None, 1056, 4100), (3, 3001, 900, 1136, 4099), (3, 2050, None, 176, 2050), (3, 3000, 700, 816, 770), (3, 2050, None, 352, 1030), (3, 3000, 2000, 944, 516),
+    (3, 2050, 300, 1296, 257), (9, 129, 50, 80, 1000), (40, 200, None, 112, 2050),
 ]
 
 
@@ -187,6 +193,74 @@ def test_grouped_offsets_out_of_range(lib, fd):
     want, tol = F.grouped(A, sa, None, off, B, sb, rows, F32)
     within(host[:11], want[:11].cpu(), tol[:11].cpu())
     assert (host[11:] == 7).all()
+
+
+def shifted(t, by):
+    """The tensor `by` bytes behind an aligned start, between guards."""
+    n = t.numel() * t.element_size()
+    mem = torch.full((by + n + 64,), 7, dtype=torch.uint8, device=DEV)
+    view = torch.as_strided(mem[by:by + n].view(t.dtype), t.shape, t.contiguous().stride())
+    view.copy_(t)
+    return mem, view
+
+
+@pytest.mark.parametrize("by", [4, 8, 12])
+def test_unaligned_device_memory(lib, fd, by):
+    """Operands and results in device memory at every multiple of four bytes, with nothing around a result touched."""
+    M, K, N = 40, 400, 72
+    A, sa, B, sb = operands(gen(30), M, K, N)
+    keep = [shifted(dev(t), by) for t in (A, sa, B, sb)]
+    A, sa, B, sb = (v for _, v in keep)
+    for dtype, fn in ((F32, lib.rocket_matmul_fp8_block), (H16, lib.rocket_matmul_fp8_block_f16out)):
+        mem, out = shifted(full((M, N), 0, dtype), by)
+        torch.cuda.synchronize()
+        assert fn(fd, M, K, N, p(A), p(sa), p(B), p(sb), p(out)) == 0
+        within(out, *F.product(A, sa, B, sb, dtype))
+        assert (mem[:by] == 7).all() and (mem[-64:] == 7).all()
+    x = odd_rows(gen(31), M, K, F32)
+    _, d = shifted(dev(x), by)
+    (mq, q), (ms, s) = shifted(full((M, K), 0, torch.uint8), by), shifted(full((M, F.blocks(K)), 0, F32), by)
+    torch.cuda.synchronize()
+    assert lib.rocket_quantize_rows_fp8(fd, M, K, p(d), K, p(q), p(s)) == 0
+    wq, ws = F.quantise(x)
+    assert torch.equal(s.cpu(), ws) and F.same_codes(q.cpu(), wq)
+    assert all((m[:by] == 7).all() and (m[-64:] == 7).all() for m in (mq, ms))
+
+
+@pytest.mark.parametrize("M,K,N", [(200, 4096, 256), (700, 6960, 104), (300, 16384, 1024)])
+def test_product_captured(lib, M, K, N):
+    """Products in slices of K: captured on a handle without scratch, then on one that has it, both replayed between eager calls."""
+    fd, stream = lib.rocket_open(), torch.cuda.Stream()
+    assert lib.rocket_hip_set_stream(fd, C.c_void_p(stream.cuda_stream)) == 0 and lib.rocket_hip_set_mode(fd, R.ROCKET_HIP_ASYNC | R.ROCKET_HIP_DEVICE_OPERANDS) == 0
+    try:
+        A, sa, B, sb = (dev(t) for t in operands(gen(32), M, K, N))
+        sa = sa * min(1.0, 300.0 / K)
+        outs = [full((M, N), 7, H16) for _ in range(3)]
+        call = lambda o: lib.rocket_matmul_fp8_block_f16out(fd, M, K, N, p(A), p(sa), p(B), p(sb), p(o))  # noqa: E731
+        graphs = []
+        for i in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                assert call(outs[i]) == 0
+            graphs.append(g)
+            assert call(outs[2]) == 0    # (eager: the handle's scratch from here on)
+            stream.synchronize()
+        want, tol = F.product(A, sa, B, sb, H16)
+        for _ in range(3):
+            for o in outs:
+                o.fill_(7)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for g in graphs:
+                    g.replay()
+            assert call(outs[2]) == 0
+            stream.synchronize()
+            for o in outs:
+                within(o, want, tol)
+            assert torch.equal(outs[1], outs[2])
+        del graphs, g
+    finally:
+        lib.rocket_close(fd)
 
 
 def test_weights_past_4_gib(lib, fd):
@@ -259,9 +333,27 @@ def test_route(lib, fd, case, dtype):
     route_check(o, x, k, plan=False, **kw)
 
 
+@pytest.mark.parametrize("M", [1, 16, 17, 32, 33, 70])
+@pytest.mark.parametrize("n", [1, 2, 16, 17, 64, 65, 128, 129, 250, 256, 257, 512, 513, 1024])
+def test_route_sizes(lib, fd, n, M):
+    """Every form of a token (rows of lanes, waves) at its smallest and largest count, results 4-byte aligned."""
+    print("route sizes", M, n, flush=True)
+    g, k = gen(33 + n), min(n, 7)
+    x = dev(logits_of(g, M, n, F32, 0.2))
+    groups = next(d for d in (8, 5, 3, 2, 1) if n % d == 0)
+    kw = dict(sigmoid=M % 2 == 0, bias=dev(torch.randn(n, generator=g) * 0.1), groups=groups, best=1 + (n > 2 * groups), top_groups=(groups + 1) // 2)
+    new = lambda *s, dtype: torch.full((math.prod(s) + 1,), 77, dtype=dtype, device=DEV)[1:].view(s)  # noqa: E731
+    o = dict(ids=new(M, k, dtype=torch.int32), weight=new(M, k, dtype=F32), off=new(n + 1, dtype=torch.int32), src=new(M * k, dtype=torch.int32), slot=new(M, k, dtype=torch.int32))
+    torch.cuda.synchronize()
+    assert lib.rocket_moe_route_f32(fd, M, n, p(x), x.stride(0), R.ROCKET_ROUTE_SIGMOID if kw["sigmoid"] else R.ROCKET_ROUTE_SOFTMAX, p(kw["bias"]), groups, kw["best"], kw["top_groups"], k, 1,
+                                    1.0, None, p(o["ids"]), p(o["weight"]), p(o["off"]), p(o["src"]), p(o["slot"])) == 0
+    route_check(o, x, k, **kw)
+
+
 @pytest.mark.parametrize("many", [1, 13])
 @pytest.mark.parametrize("kw", [dict(), dict(sigmoid=True), dict(sigmoid=True, bias=True), dict(bias=True), dict(groups=4, best=2, top_groups=2),
-                                dict(groups=2, best=1, top_groups=1, sigmoid=True, bias=True, renorm=False), dict(bias=math.nan), dict(bias=math.inf)])
+                                dict(groups=2, best=1, top_groups=1, sigmoid=True, bias=True, renorm=False), dict(bias=math.nan), dict(bias=math.inf), dict(bias=-math.inf),
+                                dict(groups=4, best=2, top_groups=2, sigmoid=True, bias=-math.inf)])
 def test_route_edges(lib, fd, kw, many):
     x = dev(torch.tensor(EDGES).repeat(many, 1))
     if "bias" in kw:

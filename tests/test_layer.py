@@ -243,7 +243,7 @@ def test_norm_refusals(lib):
     base = dict(M=4, H=128, h=x, y=x, rs=128, wp=w, ep=1e-6, g=w, ge=1, al=1.0, wq=w, eq=1e-6, ho=o[0], x=o[1], q=o[2], s=o[3], k=2, rows=8, slot=i, weight=wt, sh=x)
     both = [dict(M=0), dict(M=1 << 25), dict(H=0), dict(H=4), dict(H=132), dict(H=16392, rs=16392), dict(h=None), dict(ep=math.nan), dict(eq=math.nan),
             dict(al=math.inf), dict(al=math.nan), dict(ep=-1.0), dict(eq=-1.0), dict(ho=None, x=None, q=None, s=None), dict(q=None), dict(s=None), dict(ge=0),
-            dict(ho=o[1]), dict(x=o[2]), dict(x=x), dict(q=w), dict(s=x), dict(ho=w)]
+            dict(ho=o[1]), dict(x=o[2]), dict(x=x), dict(q=w), dict(s=x), dict(ho=w), dict(ho=x)]   # (the last: in place, but h is y too)
     near = x[8:]   # a result a few values behind the rows that it would replace
     for kw in both + [dict(ho=near), dict(rs=120), dict(rs=132), dict(rs=(1 << 40) + 8)]:
         a = dict(base, **kw)
@@ -319,12 +319,14 @@ def test_route_host(lib, case, dtype):
 
 EDGES = [  # a row of eight logits
     [0.0] * 8, [-math.inf] * 8, [-math.inf] * 5 + [1.0, 1.0, 0.5], [math.inf, 1, math.inf, 0, 0, 0, 0, 0], [math.nan, 1, 2, 3, -math.inf, 0, 0, 2],
-    [math.nan] * 8, [-3.4e38, 3.4e38, 0, -0.0, 0, 1e-45, -1e-45, 0], [-800.0, -801, -799, -800, -1e4, -1e5, -800, -799], [90.0, 91, 92, 40, 41, 42, 43, 90],
+    [math.nan] * 8, [0.5, 3.4028234663852886e38, math.inf, 3.4028234663852886e38, 0, 0, 0, 0], [math.nan, math.nan, 0, 1, 0, 0, 0, 0],
+    [-3.4e38, 3.4e38, 0, -0.0, 0, 1e-45, -1e-45, 0], [-800.0, -801, -799, -800, -1e4, -1e5, -800, -799], [90.0, 91, 92, 40, 41, 42, 43, 90],
 ]
 
 
 @pytest.mark.parametrize("kw", [dict(), dict(sigmoid=True), dict(sigmoid=True, bias=True), dict(bias=True), dict(groups=4, best=2, top_groups=2),
-                                dict(groups=2, best=1, top_groups=1, sigmoid=True, bias=True, renorm=False), dict(bias=math.nan), dict(bias=math.inf)])
+                                dict(groups=2, best=1, top_groups=1, sigmoid=True, bias=True, renorm=False), dict(bias=math.nan), dict(bias=math.inf), dict(bias=-math.inf),
+                                dict(groups=4, best=2, top_groups=2, sigmoid=True, bias=-math.inf)])
 def test_route_edges_host(lib, kw):
     x = torch.tensor(EDGES)
     if "bias" in kw:
