@@ -353,23 +353,24 @@ namespace {
 
 using namespace f8;
 
-// The tiles, what a CU holds of one (cap), and what a stage takes in us: t1 with one workgroup a CU, tc with every CU full (cap 1: with
-// few workgroups, and with one a CU), measured at K = 4096 and 15360; `fixed` is the launch, the first loads and the results.
+// The tiles, what a CU holds of one (cap), and what a stage takes in us: t1 with one workgroup a CU, tc with every CU full (cap 1:
+// with few workgroups, and with one a CU); `fixed` is the launch, the first loads and the results, `more` what each further round of
+// workgroups adds of these. Fitted to 390 products (17 to 8192 rows, and 8 to 128 experts', K and N from 512 to 15360) with every
+// tile and 1 to 8 slices: the chosen ones took 0.5% (fp32 results: 1%) longer than the fastest on average, 15% at most.
 struct Tile {
     int bm, bn, cap;
-    float fixed, t1, tc;
+    float fixed, more, t1, tc;
 };
 enum Kind { kT256, kT128, kT128Deep, kT64x128, kT64x128Deep, kT64, kT32, kKinds, kRows = kKinds };
-constexpr Tile kNarrow[kKinds] = {{256, 256, 1, 9.f, 1.35f, 1.78f}, {128, 128, 2, 5.f, 0.66f, 1.15f}, {128, 128, 1, 5.f, 0.44f, 0.58f},
-                                  {64, 128, 2, 4.5f, 0.50f, 0.85f}, {64, 128, 1, 4.5f, 0.31f, 0.36f}, {64, 64, 2, 4.f, 0.23f, 0.40f},
-                                  {32, 64, 3, 3.5f, 0.20f, 0.36f}};
+constexpr Tile kNarrow[kKinds] = {{256, 256, 1, 8.32f, 4.70f, 0.79f, 1.79f}, {128, 128, 2, 4.89f, 2.67f, 0.64f, 1.11f}, {128, 128, 1, 5.23f, 5.89f, 0.40f, 0.53f},
+                                  {64, 128, 2, 3.39f, 2.26f, 0.50f, 0.84f}, {64, 128, 1, 4.14f, 4.10f, 0.29f, 0.37f}, {64, 64, 2, 3.70f, 3.10f, 0.25f, 0.31f},
+                                  {32, 64, 3, 3.42f, 2.23f, 0.21f, 0.28f}};
 // (widened: no tile of 256, whose codes' fp16 does not fit the registers, none of 128 with four slots, which is no faster, and
-// none of 64 x 128, a stage of which takes 0.61 to 0.68: two workgroups of 64 x 64 on a CU have as much done in 0.66)
-constexpr Tile kWide[kKinds] = {{0, 0, 0, 0.f, 0.f, 0.f}, {128, 128, 2, 5.f, 0.98f, 1.78f}, {0, 0, 0, 0.f, 0.f, 0.f},
-                                {0, 0, 0, 0.f, 0.f, 0.f}, {0, 0, 0, 0.f, 0.f, 0.f}, {64, 64, 2, 4.f, 0.41f, 0.66f},
-                                {32, 64, 3, 3.5f, 0.41f, 0.56f}};
-// Bytes a us: memory, what the CUs take out of the L2s, the slices' planes.
-constexpr float kCus = 256.f, kMem = 5.2e6f, kL2 = 14e6f, kJoin = 6e6f;
+// none of 64 x 128, a stage of which takes 0.61 to 0.68: two workgroups of 64 x 64 on a CU have as much done in 0.65)
+constexpr Tile kWide[kKinds] = {{}, {128, 128, 2, 4.38f, 6.40f, 1.04f, 1.65f}, {}, {}, {}, {64, 64, 2, 3.51f, 3.01f, 0.41f, 0.67f}, {32, 64, 3, 4.05f, 3.14f, 0.35f, 0.64f}};
+// Bytes a us: memory, what the CUs take out of the L2s. What joining slices takes: us, and us a slice and value.
+constexpr float kCus = 256.f, kMem = 5.2e6f, kL2 = 14e6f;
+constexpr float kJoinFixed = 2.1f, kJoin = 1.7e-6f;
 
 // The kernel and the slices of K that are expected to take the least time.
 void plan(GemmF8 &L, bool split)
@@ -388,9 +389,10 @@ void plan(GemmF8 &L, bool split)
             if (s > 1 && (!split || L.off || nb < 3 * s || w1 * (s - 1) > room)) break;
             const int per = (nb + s - 1) / s;
             const float w = w1 * s, full = t.cap > 1 ? std::max(0.f, (std::min(w, room) / kCus - 1.f) / (t.cap - 1)) : std::min(1.f, w / kCus);
-            const float comp = std::max(ceilf(w / room) * per * (t.t1 + (t.tc - t.t1) * full), w * per * 128.f * (t.bm + t.bn) / kL2);
+            const float rounds = ceilf(w / room), stages = rounds * per * (t.t1 + (t.tc - t.t1) * full) + (rounds - 1.f) * t.more;
+            const float comp = std::max(stages, w * per * 128.f * (t.bm + t.bn) / kL2);
             float us = t.fixed + sqrtf(comp * comp + mem * mem);
-            if (s > 1) us += 2.5f + 8.f * s * (float)L.M * (float)L.N / kJoin;
+            if (s > 1) us += kJoinFixed + s * (float)L.M * (float)L.N * kJoin;
             if (us < best) best = us, L.kind = k, L.slices = (nb + per - 1) / per;
         }
     }

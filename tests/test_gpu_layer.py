@@ -90,7 +90,8 @@ PRODUCTS = [(1, 16, 1), (1, 3840, 640), (2, 144, 7), (7, 4096, 130), (15, 272, 2
             # the larger tiles and their slices of K, with rows and columns left over
             (1030, 192, 4100), (2050, 384, 1000), (2050, 1232, 257), (1500, 656, 1000), (3000, 944, 770), (3000, 1120, 4100), (2900, 1136, 4099), (3000, 464, 1030),
             (2050, 6832, 1000), (2050, 7520, 516), (1000, 7216, 513), (1500, 8608, 516), (2050, 3552, 257), (1000, 5152, 100), (17, 2432, 99), (700, 6960, 104),
-            (512, 15360, 640), (300, 16384, 1024), (16, 1024, 9000), (13, 400, 40000)]
+            (512, 15360, 640), (300, 16384, 1024), (3000, 928, 1030), (3000, 9360, 257), (2050, 7952, 260), (2050, 8672, 1000), (70, 9136, 2560), (16, 1024, 9000),
+            (13, 400, 40000)]
 
 
 @pytest.mark.parametrize("dtype", [H16, F32])
@@ -155,7 +156,7 @@ GROUPED = [  # experts, rows, rows of A (None: in order), K, N
     (1, 1, None, 128, 16), (8, 3, 2, 272, 40), (64, 96, 16, 512, 384), (64, 96, None, 400, 130), (5, 300, 70, 1024, 257), (16, 700, None, 144, 264),
     (1024, 64, 40, 128, 36), (130, 2000, 500, 256, 128), (3, 1500, 1500, 640, 516), (200, 40, 40, 2064, 64),
     (3, 3000, None, 1056, 4100), (3, 3001, 900, 1136, 4099), (3, 2050, None, 176, 2050), (3, 3000, 700, 816, 770), (3, 2050, None, 352, 1030), (3, 3000, 2000, 944, 516),
-    (3, 2050, 300, 1296, 257), (9, 129, 50, 80, 1000), (40, 200, None, 112, 2050),
+    (3, 2050, 300, 1296, 257), (3, 3000, 1500, 928, 1030), (3, 3000, None, 1264, 516), (9, 3000, 800, 160, 2560), (9, 129, 50, 80, 1000), (40, 200, None, 112, 2050),
 ]
 
 
