@@ -77,28 +77,60 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
     const uint32_t arows = a.src ? (uint32_t)a.a_rows : (uint32_t)(m1 - m0);
     const Rsrc rA = gk::rsrc_u(At, arows * (uint32_t)a.K), rB = gk::rsrc_u(Bt, (uint32_t)min(BN, a.N - n0) * (uint32_t)a.K);
     const Rsrc rS = gk::rsrc_u(sat, arows * (uint32_t)a.nb * 4u);
-    // (a row of the tile that C does not have, or that has no source, reads zeros)
-    auto arow = [&](int r) -> int { return m0 + r < m1 ? (a.src ? source(a, m0 + r) : r) : -1; };
+    constexpr int LR = CF::NT / BM;   // lanes that load a row's scales
+    // the weights' scales of the tile's columns and the slice's blocks
+    auto scale_b = [&](int i) __attribute__((always_inline)) {
+        const int c = i / a.per, b = kb0 + i - c * a.per, n = n0 / 128 + c;
+        return a.sb[((size_t)e * ((a.N + 127) / 128) + min(n, (a.N - 1) / 128)) * a.nb + min(b, kb1 - 1)];   // (past the last: not used)
+    };
+    for (int i = tid + CF::NT; i < CF::SBN * a.per; i += CF::NT) sbl[i] = scale_b(i);
+    // Where K ends inside its last block, the chunks past K read zeros from that block on.
+    const int part = a.K % 128 ? a.nb - 1 : -1;
+    const uint32_t left = (uint32_t)a.K % 128u;
     uint32_t va[CF::IA], vb[CF::IB], ca[CF::IA], cb[CF::IB], vs;
-#pragma unroll
-    for (int i = 0; i < CF::IA; i++) {
-        const int row = (wave * CF::IA + i) * 8 + (lane >> 3), r = arow(row);
-        ca[i] = (uint32_t)((lane & 7) ^ sw_a(row)) * 16u;
-        va[i] = r < 0 ? kOOB : (uint32_t)r * (uint32_t)a.K + ca[i];
-    }
 #pragma unroll
     for (int i = 0; i < CF::IB; i++) {
         const int row = (wave * CF::IB + i) * 8 + (lane >> 3);
         cb[i] = (uint32_t)((lane & 7) ^ sw_b(row)) * 16u;
-        vb[i] = (uint32_t)row * (uint32_t)a.K + cb[i];
-    }
-    constexpr int LR = CF::NT / BM;   // lanes that load a row's scales
-    {
-        const int r = arow(tid / LR);
-        vs = r < 0 ? kOOB : ((uint32_t)r * (uint32_t)a.nb + (uint32_t)(tid % LR) * 4u) * 4u;
+        vb[i] = ((uint32_t)row * (uint32_t)a.K + cb[i]) | (kb0 != part || cb[i] < left ? 0u : kOOB);
     }
     typedef __attribute__((address_space(3))) void *Lds;
     char *const pb0 = smem + SLOTS * BM * 128;   // A's slots, then B's
+    // Instruction i of the IA + IB that load a stage, whose codes start at byte k of a row.
+    auto load1 = [&](int i, int k, int slot) __attribute__((always_inline)) {
+        if (i < CF::IA)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (Lds)(smem + slot * BM * 128 + (wave * CF::IA + i) * 1024), 16, va[i], k, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (Lds)(pb0 + slot * BN * 128 + (wave * CF::IB + i - CF::IA) * 1024), 16, vb[i - CF::IA], k, 0, 0);
+    };
+    auto first_b = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = CF::IA; i < CF::NVM; i++) load1(i, __builtin_amdgcn_readfirstlane(kb0 * 128), 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Rows of A that the lane loads from, those of the tile's codes and the one of its scales; -1: a row of the tile that C does not have,
+    // or that has no source, which reads zeros. All loads of `src` are issued at once (each behind a condition of its own is
+    // waited for), and the first stage's weights are on their way behind them.
+    int ar[CF::IA + 1];
+    auto trow = [&](int i) __attribute__((always_inline)) { return i < CF::IA ? (wave * CF::IA + i) * 8 + (lane >> 3) : tid / LR; };
+    if (a.src) {
+#pragma unroll
+        for (int i = 0; i <= CF::IA; i++) ar[i] = a.src[min(m0 + trow(i), m1 - 1)];
+        __builtin_amdgcn_sched_barrier(0);
+        first_b();
+    } else {
+        first_b();
+#pragma unroll
+        for (int i = 0; i <= CF::IA; i++) ar[i] = trow(i);
+    }
+#pragma unroll
+    for (int i = 0; i <= CF::IA; i++) ar[i] = m0 + trow(i) < m1 && (unsigned)ar[i] < arows ? ar[i] : -1;
+#pragma unroll
+    for (int i = 0; i < CF::IA; i++) {
+        ca[i] = (uint32_t)((lane & 7) ^ sw_a(trow(i))) * 16u;
+        va[i] = ar[i] < 0 ? kOOB : (uint32_t)ar[i] * (uint32_t)a.K + ca[i];
+    }
+    vs = ar[CF::IA] < 0 ? kOOB : ((uint32_t)ar[CF::IA] * (uint32_t)a.nb + (uint32_t)(tid % LR) * 4u) * 4u;
     // The rows' scales of CH stages from stage CH c of the slice on, through registers (a DMA of four bytes a lane, once a
     // stage, cost a fifth of the time), into the half of their LDS that the stages before do not read.
     auto scales = [&](int c) __attribute__((always_inline)) {
@@ -107,13 +139,10 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
     auto keep = [&](f32x4 v, int c) __attribute__((always_inline)) {
         *reinterpret_cast<f32x4 *>(sal + (c & 1) * BM * CF::CH + tid * 4) = v;
     };
-    // Loads of block b (past the slice's last: the last again, which nothing uses, so that the waits' counts stay). Where that
-    // is the last part of a block, the chunks past K read zeros, from then on.
-    const int part = a.K % 128 ? a.nb - 1 : -1;
+    // Loads of block b (past the slice's last: the last again, which nothing uses, so that the waits' counts stay).
     auto block = [&](int b) __attribute__((always_inline)) {
         b = min(b, kb1 - 1);
         if (b == part) {
-            const uint32_t left = (uint32_t)a.K % 128u;
 #pragma unroll
             for (int i = 0; i < CF::IA; i++) va[i] |= ca[i] < left ? 0u : kOOB;
 #pragma unroll
@@ -121,27 +150,20 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
         }
         return __builtin_amdgcn_readfirstlane(b * 128);
     };
-    // Instruction i of the IA + IB that load a stage, whose codes start at byte k of a row.
-    auto load1 = [&](int i, int k, int slot) __attribute__((always_inline)) {
-        if (i < CF::IA)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (Lds)(smem + slot * BM * 128 + (wave * CF::IA + i) * 1024), 16, va[i], k, 0, 0);
-        else
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (Lds)(pb0 + slot * BN * 128 + (wave * CF::IB + i - CF::IA) * 1024), 16, vb[i - CF::IA], k, 0, 0);
-    };
-    auto load = [&](int b, int slot) __attribute__((always_inline)) {
-        const int k = block(b);
+    {
+        __builtin_amdgcn_sched_barrier(0);   // (addresses first: one computed behind the loads can wait for their registers)
+        const f32x4 s0 = scales(0);
+        const float b0 = scale_b(min(tid, CF::SBN * a.per - 1));
+        // the first stages; the scales' loads stand before theirs, so that a wait for the scales leaves them on their way
 #pragma unroll
-        for (int i = 0; i < CF::NVM; i++) load1(i, k, slot);
-    };
-
-    // the weights' scales of the tile's columns and the slice's blocks
-    for (int i = tid; i < CF::SBN * a.per; i += CF::NT) {
-        const int c = i / a.per, b = kb0 + i - c * a.per, n = n0 / 128 + c;
-        sbl[i] = b < kb1 && n < (a.N + 127) / 128 ? a.sb[((size_t)e * ((a.N + 127) / 128) + n) * a.nb + b] : 0.f;
+        for (int s = 0; s < (CF::PIPE ? SLOTS : SLOTS - 1); s++) {
+            const int k = block(kb0 + s);
+#pragma unroll
+            for (int i = 0; i < (s ? CF::NVM : CF::IA); i++) load1(i, k, s);
+        }
+        keep(s0, 0);
+        if (tid < CF::SBN * a.per) sbl[tid] = b0;
     }
-    keep(scales(0), 0);
-    // (waited for before the ring starts: its waits count the DMA's loads alone)
-    __syncthreads();
 
     f32x4 acc[TM][TN];
 #pragma unroll
@@ -188,8 +210,6 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
         // wait for no read behind a barrier.
         Codes xa[2][TM], xb[2][TN];
         float sc[2][TM], sb[2];
-#pragma unroll
-        for (int s = 0; s < SLOTS; s++) load(kb0 + s, s);
         gk::wait_vm<(SLOTS - 1) * CF::NVM>();
         gk::lds_barrier();
 #pragma unroll
@@ -232,8 +252,6 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
                 if (u + S < n) stage(S, u + S);
             });
     } else {
-#pragma unroll
-        for (int s = 0; s < SLOTS - 1; s++) load(kb0 + s, s);
         auto stage = [&](auto S, unsigned u) __attribute__((always_inline)) {
             constexpr int slot = S, free = (slot + SLOTS - 1) % SLOTS;
             gk::wait_vm<(SLOTS - 2) * CF::NVM>();
