@@ -32,7 +32,7 @@ struct Args {
     int M, K, N, nb, E, a_rows;
     int nbn, bm_tiles;    // column tiles; row tiles (experts: the most that there can be)
     int slices, per;      // slices of K and the blocks of one
-    int xcds, band;
+    int band;             // row tiles that neighbours in the launch share columns over
 };
 
 // The rows [m0, m1) of C that tile t has, and their expert; m0 == m1: none. Experts' tiles of BM rows are counted in order
