@@ -377,7 +377,7 @@ using namespace f8;
 // The tiles, what a CU holds of one (cap), and what a stage takes in us: t1 with one workgroup a CU, tc with every CU full (cap 1:
 // with few workgroups, and with one a CU); `fixed` is the launch, the first loads and the results, `more` what each further round of
 // workgroups adds of these. Fitted to 390 products (17 to 8192 rows, and 8 to 128 experts', K and N from 512 to 15360) with every
-// tile and 1 to 8 slices: the chosen ones took 0.5% (fp32 results: 1%) longer than the fastest on average, 15% at most.
+// tile and 1 to 8 slices: the chosen ones took 0.7% (fp32 results: 1.2%) longer than the fastest on average, 13% at most.
 struct Tile {
     int bm, bn, cap;
     float fixed, more, t1, tc;
