@@ -140,7 +140,9 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
         return __builtin_bit_cast(f32x4, gk::ld16(rS, vs + (uint32_t)(kb0 + CF::CH * c) * 4u));   // (zeros past the last row's)
     };
     auto keep = [&](f32x4 v, int c) __attribute__((always_inline)) {
-        *reinterpret_cast<f32x4 *>(sal + (c & 1) * BM * CF::CH + tid * 4) = v;
+        float *const at = sal + ((c & 1) * CF::CH + tid % LR * 4) * BM + tid / LR;   // ([stage][row]: sixteen rows are neighbours)
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[i * BM] = v[i];
     };
     // Loads of block b (past the slice's last: the last again, which nothing uses, so that the waits' counts stay).
     auto block = [&](int b) __attribute__((always_inline)) {
@@ -176,7 +178,7 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
 
     const int ra = wm * CF::WTM + (lane & 15);
     const int q = lane >> 4, rb = wn * CF::WTN + 8 * ((lane & 15) >> 2) + (lane & 3);
-    const float *const sbw = sbl + (CF::SBN > 1 ? wn * CF::WTN / 128 * a.per : 0), *const saw = sal + ra * CF::CH;
+    const float *const sbw = sbl + (CF::SBN > 1 ? wn * CF::WTN / 128 * a.per : 0), *const saw = sal + ra;
     auto codes = [&](const char *plane, int row, int sw) __attribute__((always_inline)) {
         return Codes{*reinterpret_cast<const i32x4 *>(plane + row * 128 + ((q ^ sw) << 4)),
                      *reinterpret_cast<const i32x4 *>(plane + row * 128 + (((4 + q) ^ sw) << 4))};
@@ -187,10 +189,10 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
         return codes(pb0 + slot * BN * 128, row, sw_b(row));
     };
     auto factors = [&](float (&sc)[TM], float &sb, unsigned u) __attribute__((always_inline)) {
-        const float *const ps = saw + (u / CF::CH % 2 * BM * CF::CH + u % CF::CH);
+        const float *const ps = saw + u % (2 * CF::CH) * BM;
         sb = sbw[u];
 #pragma unroll
-        for (int i = 0; i < TM; i++) sc[i] = ps[16 * i * CF::CH];
+        for (int i = 0; i < TM; i++) sc[i] = ps[16 * i];
     };
     // A product is added kLag products later, when the matrix unit has it done. A stage's loads are issued between the
     // products of its first half: at once they would hold the wave up, since a CU takes some 43 bytes a clock.
