@@ -2,7 +2,8 @@
 //
 // A group of 128 is 16 lanes of eight values: two wide loads a lane, the maximum a shuffle over 16 lanes, eight
 // codes one 8-byte store. Groups are counted through all rows, so that no size of row leaves lanes idle but in a last
-// part of a group. Memory bounds it.
+// part of a group. Memory bounds it: 512 fp32 rows of 15360 take 7.6 us (5.2 TB/s, as a large copy), 24576 gated fp16 rows of 1408
+// 34 us (5.1 TB/s).
 #include "f8codes.h"
 #include "gemm_impl.h"
 
