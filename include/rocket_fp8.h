@@ -18,8 +18,9 @@
  * does not allow; fd < 0 runs the host path (every operand host memory then), whose products are fp64; handles run
  * asynchronously where rocket_hip_set_mode says so, and a call returns 0 or a negative rocket_status: -1 for a bad
  * argument, before anything is launched. Results must not lie over a call's other operands or each other (-1).
- * Strides count elements. A product of few rows and a long K may be summed in slices of K that lie in scratch of the handle: a captured
- * one on a handle that has none yet takes none, and graphs that hold it are replayed in the order of the handle's stream.
+ * Strides count elements. A product of few rows and a long K may be summed in slices of K that lie in scratch of the handle:
+ * a captured one on a handle that has none yet takes none, and graphs that hold it are replayed in the order of the
+ * handle's stream.
  */
 #ifndef ROCKET_FP8_H
 #define ROCKET_FP8_H
@@ -41,7 +42,7 @@ extern "C" {
  * A NaN gives a NaN code (0x7f or 0xff) and does not count in the maximum; an infinity makes its group's scale infinite,
  * so that products with the group are NaN.
  * Row m of A begins at A + m * a_rs. Results are dense: Aq[M][K], a_scale[M][ceil(K / 128)].
- * K and the strides are multiples of 8, 8 <= K <= 65536, K <= stride <= 2^40. */
+ * K and the strides are multiples of 8, 8 <= K <= 65536, K <= stride, M * stride <= 2^40. */
 int rocket_quantize_rows_fp8(int fd, int M, int K, const float *A, int64_t a_rs, uint8_t *Aq, float *a_scale);
 int rocket_quantize_rows_fp8_fp16(int fd, int M, int K, const _Float16 *A, int64_t a_rs, uint8_t *Aq, float *a_scale);
 

@@ -30,7 +30,7 @@ extern "C" {
  * Results, each of which may be NULL, but not all: h_out[M][H] (h' in h's type; it may be h itself, if y is not), x[M][H] in fp16, and xq[M][H] with
  * x_scale[M][ceil(H / 128)] (both or neither), x's codes and scales as rocket_quantize_rows_fp8 makes them of the
  * unrounded x. h[M][H], gate[ceil(M / gate_every)][H]: gate_every 1 is a gate for each row, the tokens of a
- * sequence one for each sequence, M or more one for all. y_rs >= H, a multiple of 8, up to 2^40.
+ * sequence one for each sequence, M or more one for all. y_rs >= H, a multiple of 8, M * y_rs <= 2^40.
  * H a multiple of 8, 8 <= H <= 16384; eps not NaN, alpha finite. An fp16 h' past fp16's range is an infinity. */
 int rocket_add_norm_fp16(int fd, int M, int H, const _Float16 *h, const _Float16 *y, int64_t y_rs, const _Float16 *w_post, float eps_post,
                          const _Float16 *gate, int gate_every, float alpha, const _Float16 *w_pre, float eps_pre, _Float16 *h_out,
@@ -67,7 +67,7 @@ int rocket_moe_add_norm_f32(int fd, int M, int H, const float *h, int rows, int 
  *     src_row[M * top_k]    the token of each row (places from expert_off[E] on are left as they were)
  *     slot[M][top_k]        the row of each choice, -1 where there is none
  * 1 <= E <= 1024, E % n_group == 0, 1 <= n_group <= 64, group_best 1 or 2, 1 <= top_group <= n_group,
- * 1 <= top_k <= min(32, E), M * top_k < 2^24, rs >= E. Results in device memory may be 4-byte aligned. More than 32
+ * 1 <= top_k <= min(32, E), M * top_k < 2^24, rs >= E, M * rs <= 2^40. Results in device memory may be 4-byte aligned. More than 32
  * tokens with a plan take scratch of the handle (a captured call needs an eager one of the same size first; graphs that
  * hold scratch of one handle are replayed in the order of its stream). */
 #define ROCKET_ROUTE_SOFTMAX 0

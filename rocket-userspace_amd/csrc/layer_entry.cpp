@@ -13,7 +13,7 @@ using namespace rk;
 
 namespace {
 
-constexpr int64_t kMaxStride = (int64_t)1 << 40;
+constexpr int64_t kMaxSpan = (int64_t)1 << 40;   // elements of strided rows
 constexpr size_t kIntAlign = sizeof(int32_t);
 
 // Nothing may throw across the C ABI (the staging lists allocate).
@@ -123,7 +123,7 @@ int on_gpu(const char *who, int fd, const Operand (&in)[NI], const Operand (&out
 int quantise(const char *who, int fd, QuantF8 L, bool gated)
 {
     if (L.M < 1 || L.M > kDimMax || L.K < 8 || L.K % 8 || L.K > kF8MaxK) return bad(who, "M below 1 or too large, or K no multiple of 8 up to 65536");
-    if (L.rs < L.K || L.rs % 8 || L.rs > kMaxStride) return bad(who, "a row stride is a multiple of 8 and holds the row");
+    if (L.rs < L.K || L.rs % 8 || L.rs > kMaxSpan / L.M) return bad(who, "a row stride is a multiple of 8 and holds the row, and all rows are up to 2^40 values");
     if (gated && L.act != kActSilu && L.act != kActGelu) return bad(who, "the activation is neither SiLU nor GELU");
     if (!L.a || (gated && !L.up) || !L.q || !L.scale) return bad(who, "null operand");
     const int nb = f8_blocks(L.K);
@@ -174,8 +174,8 @@ int norms(const char *who, int fd, AddNorm L, bool experts)
     if (experts) {
         if (L.top_k < 1 || L.top_k > kMaxTop || L.rows < 1 || L.rows > kDimMax) return bad(who, "top_k outside [1, 32], or rows below 1 or too large");
         if (!L.y || !L.slot || !L.weight) return bad(who, "null operand");
-    } else if (L.y && (L.y_rs < L.H || L.y_rs % 8 || L.y_rs > kMaxStride)) {
-        return bad(who, "a row stride is a multiple of 8 and holds the row");
+    } else if (L.y && (L.y_rs < L.H || L.y_rs % 8 || L.y_rs > kMaxSpan / L.M)) {
+        return bad(who, "a row stride is a multiple of 8 and holds the row, and all rows are up to 2^40 values");
     }
     const size_t e = L.f32 ? sizeof(float) : sizeof(_Float16), rows = (size_t)L.M, hb = rows * L.H * e, wb = (size_t)L.H * sizeof(_Float16);
     const size_t yb = !L.y ? 0 : experts ? (size_t)L.rows * L.H * e : ((rows - 1) * L.y_rs + L.H) * e;
@@ -197,7 +197,7 @@ int route(const char *who, int fd, Route L, int score)
     if (L.n_group < 1 || L.n_group > kMaxGroups || L.E % L.n_group || L.top_group < 1 || L.top_group > L.n_group || L.group_best < 1 || L.group_best > 2)
         return bad(who, "n_group outside [1, 64] or no divisor of E, top_group outside [1, n_group], or group_best neither 1 nor 2");
     if (score != ROCKET_ROUTE_SOFTMAX && score != ROCKET_ROUTE_SIGMOID) return bad(who, "unknown score");
-    if (L.rs < L.E || L.rs > kMaxStride) return bad(who, "a row stride below E or too large");
+    if (L.rs < L.E || L.rs > kMaxSpan / L.M) return bad(who, "a row stride below E or too large");
     if (!isfinite(L.scale)) return bad(who, "scale is not finite");
     if (!L.logits || !L.ids || !L.weight || !L.off != !L.src || !L.off != !L.slot) return bad(who, "null operand, or a part of the plan");
     L.sigmoid = score == ROCKET_ROUTE_SIGMOID;

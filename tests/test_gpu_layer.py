@@ -89,7 +89,7 @@ PRODUCTS = [(1, 16, 1), (1, 3840, 640), (2, 144, 7), (7, 4096, 130), (15, 272, 2
             (1030, 528, 516), (5, 65536, 33), (130, 65536, 17),
             # the larger tiles and their slices of K, with rows and columns left over
             (1030, 192, 4100), (2050, 384, 1000), (2050, 1232, 257), (1500, 656, 1000), (3000, 944, 770), (3000, 1120, 4100), (2900, 1136, 4099), (3000, 464, 1030),
-            (2050, 6832, 1000), (2050, 7520, 516), (1000, 7216, 513), (1500, 8608, 516), (2050, 3552, 257), (1000, 5152, 100), (17, 2432, 99), (700, 6960, 104),
+            (2050, 6832, 1000), (2050, 7520, 516), (1000, 7216, 513), (1500, 8608, 516), (2050, 3552, 257), (1000, 5152, 100), (17, 2432, 99), (700, 6960, 104), (200, 3088, 256), (24, 3088, 100),
             (512, 15360, 640), (300, 16384, 1024), (3000, 928, 1030), (3000, 9360, 257), (2050, 7952, 260), (2050, 8672, 1000), (70, 9136, 2560), (16, 1024, 9000),
             (13, 400, 40000)]
 
@@ -179,6 +179,26 @@ def test_grouped(lib, fd, case, dtype):
     n = int(off[-1])
     within(out[:n], want[:n], tol[:n])
     assert out[n:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [H16, F32])
+@pytest.mark.parametrize("E,rows,K,N", [(64, 500, 512, 96), (8, 1500, 640, 516), (9, 3000, 160, 2560)])
+def test_grouped_one_expert(lib, fd, E, rows, K, N, dtype):
+    """All rows are one expert's, the same row of A again and again; sizes where an even share would be a few rows, and many."""
+    g = gen(34)
+    A, sa, B, sb = (dev(t) for t in operands(g, 3, K, N, E))
+    if dtype == H16:
+        sa = sa * min(1.0, 300.0 / K)
+    for e in (0, E - 1):
+        off = torch.tensor([0] * (e + 1) + [rows - 1] * (E - e), dtype=torch.int32)
+        src = torch.full((rows,), 1, dtype=torch.int32)
+        out = full((rows, N), math.nan, dtype)
+        fn = lib.rocket_matmul_fp8_block_grouped_f16out if dtype == H16 else lib.rocket_matmul_fp8_block_grouped
+        doff, dsrc = dev(off), dev(src)
+        assert fn(fd, E, rows, 3, K, N, p(A), p(sa), p(dsrc), p(doff), p(B), p(sb), p(out)) == 0
+        want, tol = F.product(A[1:2], sa[1:2], B[e], sb[e], dtype)
+        within(out[:rows - 1], want.expand(rows - 1, N), tol.expand(rows - 1, N))
+        assert out[rows - 1].isnan().all() and torch.equal(out[0].expand(rows - 1, N), out[:rows - 1])
 
 
 def test_grouped_offsets_out_of_range(lib, fd):
@@ -450,6 +470,37 @@ def test_layer_of_experts(lib, fd, M):
     first = a.x2.clone()
     a.call(lib, fd)                      # no order of anything changes a bit
     assert torch.equal(first, a.x2)
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_dense_layer(lib, fd, M):
+    """A layer without experts: norm to codes, gate and up, gated rows, down, and the norm behind in place; device and host memory."""
+    K, I, H, g = 496, 384, 520, gen(35)
+    (B1, s1), (B2, s2) = (F.quantise_weights(torch.randn(s, generator=g) * 0.05) for s in ((2 * I, K), (H, I)))
+    w = (1 + 0.2 * torch.randn(K, generator=g)).half()
+    h0, back = (torch.randn((M, K), generator=g) * 2).half(), torch.randn((M, H), generator=g).half()
+    for put in (dev, lambda t: t.clone()):
+        new = lambda *s, dtype: put(torch.zeros(s, dtype=dtype))  # noqa: E731
+        b1, t1, b2, t2, wd, h, hb = (put(t) for t in (B1, s1, B2, s2, w, h0, back))
+        xq, xs, gu = new(M, K, dtype=torch.uint8), new(M, F.blocks(K), dtype=F32), new(M, 2 * I, dtype=H16)
+        aq, as_, y, x2 = new(M, I, dtype=torch.uint8), new(M, F.blocks(I), dtype=F32), new(M, H, dtype=H16), new(M, H, dtype=H16)
+        torch.cuda.synchronize()
+        up = C.c_void_p(gu.data_ptr() + 2 * I)
+        assert lib.rocket_add_norm_fp16(fd, M, K, p(h), None, K, None, -1.0, None, 1, 1.0, p(wd), 1e-6, None, None, p(xq), p(xs)) == 0
+        assert lib.rocket_matmul_fp8_block_f16out(fd, M, K, 2 * I, p(xq), p(xs), p(b1), p(t1), p(gu)) == 0
+        assert lib.rocket_quantize_glu_fp8_fp16(fd, M, I, p(gu), up, 2 * I, R.ROCKET_ACTIVATION_GELU, None, p(aq), p(as_)) == 0
+        assert lib.rocket_matmul_fp8_block_f16out(fd, M, I, H, p(aq), p(as_), p(b2), p(t2), p(y)) == 0
+        assert lib.rocket_add_norm_fp16(fd, M, H, p(hb), p(y), H, None, -1.0, None, 1, 0.5, None, 1e-5, p(hb), p(x2), None, None) == 0
+        xq, xs, gu, aq, as_, y, hb, x2 = (dev(t) for t in (xq, xs, gu, aq, as_, y, hb, x2))
+        _, _, x, ex = F.add_norm(dev(h0), None, None, -1.0, None, 1, 1.0, dev(w), 1e-6)
+        assert F.near_codes(xq, xs, x, ex)
+        within(gu, *F.product(xq, xs, dev(B1), dev(s1), H16))
+        want, tol = F.gated("gelu", gu[:, :I], gu[:, I:])
+        assert F.near_codes(aq, as_, want, tol + F.e32 * want.abs())
+        within(y, *F.product(aq, as_, dev(B2), dev(s2), H16))
+        hn, eh, x, ex = F.add_norm(dev(back), y, None, -1.0, None, 1, 0.5, None, 1e-5)
+        within(hb, hn, F.rounded(hn, eh, H16))
+        within(x2, x, F.rounded(x, ex, H16))
 
 
 @pytest.mark.parametrize("M", [8, 128])

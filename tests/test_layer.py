@@ -86,7 +86,7 @@ def test_quantise_gated_host(lib, act):
 def test_quantise_refusals(lib):
     x, q, s, n = torch.ones(4096), torch.full((4096,), 7, dtype=torch.uint8), torch.full((64,), 7.0), torch.ones(1, dtype=torch.int32)
     base = dict(fd=-1, M=2, K=256, a=x, rs=256, q=q, s=s)
-    for kw in (dict(M=0), dict(M=1 << 25), dict(K=0), dict(K=4), dict(K=12), dict(K=65544, rs=65544), dict(rs=248), dict(rs=260), dict(rs=(1 << 40) + 8), dict(rs=-256),
+    for kw in (dict(M=0), dict(M=1 << 25), dict(K=0), dict(K=4), dict(K=12), dict(K=65544, rs=65544), dict(rs=248), dict(rs=260), dict(rs=(1 << 39) + 8), dict(rs=-256), dict(M=1 << 20, rs=1 << 40),
                dict(a=None), dict(q=None), dict(s=None), dict(M=1 << 24, K=65536, rs=65536)):
         a = dict(base, **kw)
         for fn in (lib.rocket_quantize_rows_fp8, lib.rocket_quantize_rows_fp8_fp16):
@@ -245,7 +245,7 @@ def test_norm_refusals(lib):
             dict(al=math.inf), dict(al=math.nan), dict(ep=-1.0), dict(eq=-1.0), dict(ho=None, x=None, q=None, s=None), dict(q=None), dict(s=None), dict(ge=0),
             dict(ho=o[1]), dict(x=o[2]), dict(x=x), dict(q=w), dict(s=x), dict(ho=w), dict(ho=x)]   # (the last: in place, but h is y too)
     near = x[8:]   # a result a few values behind the rows that it would replace
-    for kw in both + [dict(ho=near), dict(rs=120), dict(rs=132), dict(rs=(1 << 40) + 8)]:
+    for kw in both + [dict(ho=near), dict(rs=120), dict(rs=132), dict(rs=(1 << 38) + 8), dict(M=1 << 20, rs=1 << 40)]:
         a = dict(base, **kw)
         for fn in (lib.rocket_add_norm_fp16, lib.rocket_add_norm_f32):
             assert fn(-1, a["M"], a["H"], p(a["h"]), p(a["y"]), a["rs"], p(a["wp"]), a["ep"], p(a["g"]), a["ge"], a["al"], p(a["wq"]), a["eq"], p(a["ho"]),
@@ -345,7 +345,7 @@ def test_route_refusals(lib):
     x, b, act = torch.ones(4096), torch.ones(64), torch.ones(8, dtype=torch.uint8)
     o = [torch.full((4096,), 7, dtype=torch.int32) for _ in range(5)]
     base = dict(M=8, E=64, x=x, rs=64, score=0, b=b, g=8, best=2, tg=4, k=6, scale=1.0, act=act, ids=o[0], w=o[1], off=o[2], src=o[3], slot=o[4])
-    for kw in (dict(M=0), dict(M=1 << 25), dict(M=(1 << 24) // 6 + 1), dict(E=0), dict(E=1025, rs=1025), dict(E=60), dict(rs=63), dict(rs=(1 << 40) + 1), dict(score=2), dict(score=-1),
+    for kw in (dict(M=0), dict(M=1 << 25), dict(M=(1 << 24) // 6 + 1), dict(E=0), dict(E=1025, rs=1025), dict(E=60), dict(rs=63), dict(rs=(1 << 37) + 1), dict(M=1 << 20, k=1, rs=1 << 40), dict(score=2), dict(score=-1),
                dict(g=0), dict(g=65), dict(best=0), dict(best=3), dict(tg=0), dict(tg=9), dict(k=0), dict(k=33), dict(E=4, g=1, tg=1, k=5), dict(scale=math.nan),
                dict(scale=math.inf), dict(x=None), dict(ids=None), dict(w=None), dict(off=None), dict(src=None), dict(slot=None), dict(ids=o[1]), dict(w=x), dict(src=b),
                dict(slot=act), dict(off=o[4])):
