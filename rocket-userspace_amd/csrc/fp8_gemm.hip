@@ -68,7 +68,9 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
     // there are not, the last ones, left XCDs idle, and 4096 tokens of 6 of 64 experts took 243 us, not 216; 4096 x 3840 x 15360 232, not 227.)
     constexpr int kNear = 16, kRun = 8 * kNear;
     const int run0 = (int)blockIdx.x / kRun * kRun, id = run0 + gk::xcd_remap((int)blockIdx.x - run0, min(kRun, (int)gridDim.x - run0), 8);
-    const int slice = id % a.slices, tile = id / a.slices;
+    // (a slice's tiles are neighbours, which share rows of A and B; a tile's slices share nothing: 128 x 15360 x 3840 in four slices
+    // 18.9 us so, 19.8 with a tile's slices side by side)
+    const int tiles = (int)gridDim.x / a.slices, slice = id / tiles, tile = id - slice * tiles;
     int bm, bn;
     {   // bands of `band` row tiles, rows fastest
         const int full = a.band * a.nbn, band = tile / full, r = tile - band * full, rows = min(a.band, a.bm_tiles - band * a.band);
@@ -397,8 +399,9 @@ constexpr Tile kNarrow[kKinds] = {{256, 256, 1, 8.32f, 4.70f, 0.79f, 1.79f}, {12
                                   {64, 128, 2, 3.39f, 2.26f, 0.50f, 0.84f}, {64, 128, 1, 4.14f, 4.10f, 0.29f, 0.37f}, {64, 64, 2, 3.70f, 3.10f, 0.25f, 0.31f},
                                   {32, 64, 3, 3.42f, 2.23f, 0.21f, 0.28f}};
 // (widened: no tile of 256, whose codes' fp16 does not fit the registers, none of 128 with four slots, which is no faster, and
-// none of 64 x 128, a stage of which takes 0.61 to 0.68: two workgroups of 64 x 64 on a CU have as much done in 0.65)
-constexpr Tile kWide[kKinds] = {{}, {128, 128, 2, 4.38f, 6.40f, 1.04f, 1.65f}, {}, {}, {}, {64, 64, 2, 3.51f, 3.01f, 0.41f, 0.67f}, {32, 64, 3, 4.05f, 3.14f, 0.35f, 0.64f}};
+// none of 64 x 128, a stage of which takes 0.61 to 0.68: two workgroups of 64 x 64 on a CU have as much done in 0.67)
+constexpr Tile kWide[kKinds] = {{}, {128, 128, 2, 4.38f, 6.40f, 1.04f, 1.65f}, {}, {}, {}, {64, 64, 2, 3.51f, 3.01f, 0.41f, 0.67f},
+                                {32, 64, 3, 4.05f, 3.14f, 0.35f, 0.64f}};
 // Bytes a us: memory, what the CUs take out of the L2s. What joining slices takes: us, and us a slice and value.
 constexpr float kCus = 256.f, kMem = 5.2e6f, kL2 = 14e6f;
 constexpr float kJoinFixed = 2.1f, kJoin = 1.7e-6f;
