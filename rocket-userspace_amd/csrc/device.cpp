@@ -174,7 +174,7 @@ bool is_device_ptr(const void *p, int device)
         return false;
     }
     if (a.type == hipMemoryTypeManaged || a.isManaged) return true;
-    return a.type == hipMemoryTypeDevice && a.device == device;
+    return a.type == hipMemoryTypeDevice && (device < 0 || a.device == device);
 }
 
 void *dev_alloc(size_t bytes, const char *who)
@@ -309,7 +309,7 @@ void *Call::out(void *p, size_t bytes, size_t align)
     host_io_ = true;
     void *d = scratch(bytes);
     if (!d) return nullptr;
-    back_.push_back({p, d, bytes, is_device_ptr(p, h_->device)});
+    back_.push_back({p, d, bytes, is_device_ptr(p, -1)});
     return d;
 }
 
@@ -364,7 +364,7 @@ int Call::finish_()
         }
         size_t off = 0;
         for (const Back &b : back_) {
-            const hipError_t e = b.device ? hipMemcpyAsync(b.dst, b.src, b.bytes, hipMemcpyDeviceToDevice, h_->stream)
+            const hipError_t e = b.device ? hipMemcpyAsync(b.dst, b.src, b.bytes, hipMemcpyDefault, h_->stream)
                                           : hipMemcpyAsync(static_cast<char *>(h_->pin) + off, b.src, b.bytes,
                                                            hipMemcpyDeviceToHost, h_->stream);
             if (e != hipSuccess) {

@@ -99,7 +99,7 @@ private:
     bool opt_dropped_ = false;
     bool host_io_ = false;
     int err_ = 0;
-    struct Back { void *dst; const void *src; size_t bytes; bool device; };   // device: dst is (misaligned) device memory
+    struct Back { void *dst; const void *src; size_t bytes; bool device; };   // device: dst is device memory, misaligned or another device's
     std::vector<Back> back_;
 };
 
