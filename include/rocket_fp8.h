@@ -71,7 +71,7 @@ int rocket_matmul_fp8_block_f16out(int fd, int M, int K, int N, const uint8_t *A
  * expert_off[n_expert + 1], ascending from 0: rows [expert_off[e], expert_off[e + 1]) of C[rows][N] are expert e's;
  * rows from expert_off[n_expert] on are left as they were. `rows` sizes the launch: offsets count as if cut to [0, rows],
  * and a call whose offsets descend gives no defined result (it stays inside its operands). Row r of C is made of
- * row src_row[r] of A[a_rows] (a row outside [0, a_rows) gives zeros), or, src_row NULL, of row r (a_rows >= rows then).
+ * row src_row[r] of A[a_rows] (a row outside [0, a_rows) gives zeros, whatever the weights hold), or, src_row NULL, of row r (a_rows >= rows then).
  * expert_off and src_row may be device memory that an earlier call of the stream writes, so that nothing waits
  * for the host and a captured call is replayed with other counts. 1 <= n_expert <= 1024; a_rows * K < 2^31.
  * n_expert * N * K may be past 2^32. */

@@ -87,6 +87,7 @@ template <int NB, bool F16> __global__ __launch_bounds__(512) void k_rows_fp8(co
     for (int t = threadIdx.x; t < NB * 64; t += blockDim.x) {
         f32x4 v = part[t];
         for (int w = 1; w < waves; w++) v += part[w * NB * 64 + t];
+        if (r < 0) v = f32x4{0.f, 0.f, 0.f, 0.f};   // (row t & 15 is the lane's own c; without a source its sums are zeros times the weights)
         const int m = m0 + (t & 15), n = n0 + 16 * (t >> 6) + 4 * (t >> 4 & 3);
         using T = std::conditional_t<F16, _Float16, float>;
         if (m < m1) store4(static_cast<T *>(a.C) + (size_t)m * a.N, n, a.N, a.N % 4 == 0, v);
