@@ -31,7 +31,9 @@ extern "C" {
  * x_scale[M][ceil(H / 128)] (both or neither), x's codes and scales as rocket_quantize_rows_fp8 makes them of the
  * unrounded x. h[M][H], gate[ceil(M / gate_every)][H]: gate_every 1 is a gate for each row, the tokens of a
  * sequence one for each sequence, M or more one for all. y_rs >= H, a multiple of 8, M * y_rs <= 2^40.
- * H a multiple of 8, 8 <= H <= 16384; eps not NaN, alpha finite. An fp16 h' past fp16's range is an infinity. */
+ * H a multiple of 8, 8 <= H <= 16384; eps not NaN, alpha finite. An fp16 h' past fp16's range is an infinity.
+ * A norm holds for rows of any finite size, also where their squares pass fp32's range; 0 / 0 (a row of zeros under eps 0) is NaN. A row with an
+ * infinity is NaN there and 0 elsewhere, a row with a NaN is NaN. */
 int rocket_add_norm_fp16(int fd, int M, int H, const _Float16 *h, const _Float16 *y, int64_t y_rs, const _Float16 *w_post, float eps_post,
                          const _Float16 *gate, int gate_every, float alpha, const _Float16 *w_pre, float eps_pre, _Float16 *h_out,
                          _Float16 *x, uint8_t *xq, float *x_scale);

@@ -42,8 +42,8 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8])
     *reinterpret_cast<f32x4 *>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
 }
 
-// 1 / sqrt(mean of squares + eps) of the row whose values the workgroup holds. `part`: a word a wave.
-template <int V> __device__ __forceinline__ float row_rsqrt(const float (&v)[V][8], float rH, float eps, float *part)
+// The sum of squares of the row whose values the workgroup holds, the same in every thread. `part`: a word a wave.
+template <int V> __device__ __forceinline__ float row_squares(const float (&v)[V][8], float *part)
 {
     float q = 0.f;
 #pragma unroll
@@ -59,7 +59,25 @@ template <int V> __device__ __forceinline__ float row_rsqrt(const float (&v)[V][
         q = 0.f;
         for (int w = 0; w < waves; w++) q += part[w];
     }
-    return 1.f / sqrtf(fmaf(q, rH, eps));
+    return q;
+}
+
+// 1 / sqrt(mean of squares + eps) of the row, for its values as the call leaves them: where the squares pass fp32's range, or lie so low in
+// it that they lose bits, the values are scaled by a power of two, which the norm does not see. Scaled down (2^48 is the largest then, and
+// the row's mean square at least 2^-46), a value loses bits only where its norm is below 2^-103; scaled up, none does.
+template <int V> __device__ __forceinline__ float row_rsqrt(float (&v)[V][8], float rH, float eps, float *part)
+{
+    float d = fmaf(row_squares<V>(v, part), rH, eps);
+    if (!(d >= 0x1p-96f && d <= 3.402823466e38f)) {   // (a NaN too; the same in every thread)
+        const float s = d < 1.f ? 0x1p100f : 0x1p-80f;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[i][e] *= s;
+        __syncthreads();   // (all have read `part`)
+        d = fmaf(row_squares<V>(v, part), rH, eps * s * s);
+    }
+    return 1.f / sqrtf(d);
 }
 
 template <bool F16, bool MOE, int V> __global__ __launch_bounds__(1024) void k_add_norm(const NArgs a)
