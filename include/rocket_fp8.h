@@ -58,6 +58,8 @@ int rocket_quantize_glu_fp8_fp16(int fd, int M, int K, const _Float16 *gate, con
 /* ---- products ----
  * C[m][n] = sum over blocks b of a_scale[m][b] * b_scale[n / 128][b] * (sum over k in b of A[m][k] * B[n][k]).
  * A [M][K] and B [N][K] codes, dense; M, N >= 1, K a multiple of 16, 16 <= K <= 65536.
+ * A block's two scales are multiplied first, in fp32 (fd < 0: in fp64), and have to keep their product from 2^-126 up to 2^128: a smaller one
+ * loses bits of its block's sum (none where that is 0, as of a group of zeros), a larger one is an infinity, which makes a sum of 0 a NaN.
  * The entries with fp32 results widen the codes, so that products and sums are fp32's. Those with fp16 results
  * (rounded once; an fp32 sum past fp16 is an infinity) may use the matrix unit's 8-bit products, twice as fast: of each
  * eight neighbouring k (8 i .. 8 i + 7) it cuts every product at 2^-13 of the largest one's power of two and sums the rest in
