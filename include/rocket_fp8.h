@@ -19,7 +19,7 @@
  * asynchronously where rocket_hip_set_mode says so, and a call returns 0 or a negative rocket_status: -1 for a bad
  * argument, before anything is launched. Results must not lie over a call's other operands or each other (-1).
  * Strides count elements. A product of few rows and a long K may be summed in slices of K that lie in scratch of the handle:
- * a captured one on a handle that has none yet takes none, and graphs that hold it are replayed in the order of the
+ * a captured one on a handle that has none yet takes none (its sums are in another order then), and graphs that hold it are replayed in the order of the
  * handle's stream.
  */
 #ifndef ROCKET_FP8_H

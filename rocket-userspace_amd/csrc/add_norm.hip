@@ -3,8 +3,8 @@
 //
 // A workgroup is a row, a lane eight neighbours of it (two such runs above 8192 values), so a row is read once and kept in
 // registers through both norms; each square sum is a shuffle over the wave and one exchange through LDS. Sixteen lanes
-// hold a group of 128, whose maximum is a shuffle. Memory bounds long calls: 4096 fp32 rows of 3840 with codes 43.6 us, 4.7 TB/s.
-// Two exchanges and the loads' latency bound short ones: 16 rows of 2048, six experts' rows each, 5.3 us, of which a launch is some
+// hold a group of 128, whose maximum is a shuffle. Memory bounds long calls: 4096 fp32 rows of 3840 with codes 44.0 us, 4.7 TB/s.
+// Two exchanges and the loads' latency bound short ones: 16 rows of 2048, six experts' rows each, 5.4 us, of which a launch is some
 // 4. (Four experts' rows in flight instead of one: 5.7 us, and 38.9 instead of 37.6 for 4096 tokens.)
 #include "f8codes.h"
 #include "gemm_impl.h"

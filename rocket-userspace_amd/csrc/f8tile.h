@@ -28,7 +28,7 @@ struct Args {
     const float *sa, *sb;
     const int32_t *src, *off;
     void *C;
-    float *ws;            // slices of K: [slice][M][N]
+    float *ws;            // slices of K: [slice][M][N rounded up to 4]
     int M, K, N, nb, E, a_rows;
     int nbn, bm_tiles;    // column tiles; row tiles (experts: the most that there can be)
     int slices, per;      // slices of K and the blocks of one

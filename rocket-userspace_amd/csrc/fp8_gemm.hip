@@ -337,7 +337,7 @@ template <class CF, bool WIDE, bool F16> __global__ __launch_bounds__(CF::NT) __
             for (int j = 0; j < TN; j += 2) store8(row, n1 + 16 * j, a.N, acc[i][j], acc[i][j + 1]);
         } else {
 #pragma unroll 1
-            for (int j = 0; j < 4 * TN; j++) {   // (any element of the sums by a chain of selects: no case that has to be fast)
+            for (int j = 0; j < 4 * TN; j++) {   // (any element of the sums by a chain of selects: 4096 x 3840 x 15359 327 us, x 15360 225)
                 float v = 0.f;
 #pragma unroll
                 for (int u = 0; u < 4 * TN; u++) v = j == u ? acc[i][u / 4][u % 4] : v;
@@ -409,7 +409,8 @@ using namespace f8;
 // The tiles, what a CU holds of one (cap), and what a stage takes in us: t1 with one workgroup a CU, tc with every CU full (cap 1:
 // with few workgroups, and with one a CU); `fixed` is the launch, the first loads and the results, `more` what each further round of
 // workgroups adds of these. Fitted to 390 products (17 to 8192 rows, and 8 to 128 experts', K and N from 512 to 15360) with every
-// tile and 1 to 8 slices: the chosen ones took 0.7% (fp32 results: 1.2%) longer than the fastest on average, 13% at most.
+// tile and 1 to 8 slices; of 394 timed with the kernels as they are, the chosen ones took 0.9% (fp32 results: 1.1%) longer than the fastest on average,
+// 21% at most.
 struct Tile {
     int bm, bn, cap;
     float fixed, more, t1, tc;
